@@ -296,6 +296,80 @@ int w4a16_gemm_silu_mul_config(const uint16_t* x, const int32_t* packed, const i
  * enough for every wave layout).  No reference counterpart. */
 size_t w4a16_workspace_bytes_config(int M, int N, int regime, int p0, int split);
 
+/* ---------------------------------------------------------------------------
+ * Attention over a key/value cache held in 4 bits.  The reference keeps its cache in bf16 and
+ * calls flash-attn (attention.py:21-133); these entry points take the place of that store and
+ * attention, and of the slot maps and block tables that its model runner builds on the host.
+ *
+ * Cache: bytes [num_blocks, KV, block_size * (D + 8)], one page per (block, kv head), D in
+ * {64, 128}, block_size a power of two in 16 .. 256.  A row (one token of one kv head) is D
+ * codes c in 0 .. 15 with one bf16 scale s and one zero point z in 0 .. 15; a channel's value is
+ * s * (c - z).  A page holds, in 32-bit words of eight channels (AutoAWQ's nibble order), the
+ * tokens' keys [token][word], then their values [token / 4][word][token % 4], then one word a
+ * token for the keys and one for the values: bf16(s) in the high half, bf16(128 + z) in the low.
+ * A slot is block * block_size + token; slots outside the cache name no row.  Tables, slots and
+ * lengths are int32 on the device and are never trusted: an id or length that points outside
+ * the cache, the tables or the packed rows reads and writes nothing there.
+ * ------------------------------------------------------------------------- */
+
+/* One step's bookkeeping from the request lengths.  Request r has context_lens[r] tokens in the
+ * cache and brings query_lens[r] new ones (0 for a padded request; negative lengths count as 0);
+ * its cached tokens' blocks are the first ones of tables[r].  Writes cu_query_lens [R + 1] (the
+ * requests' offsets among the packed rows), seq_lens [R] = context + query, and, for each of T
+ * packed rows, its position in its sequence and its cache slot; rows behind the last request
+ * get position 0 and slot -1.  Blocks that new tokens open are taken from free_blocks
+ * [num_free], in order of request and position, and entered in tables (row stride table_stride
+ * elements); blocks_used [1] receives how many are needed.  A token whose block the free list or
+ * the table's width lacks gets slot -1 (and -1 in the table).  The lists are not consumed: the
+ * same call again gives the same result.  R <= 4096, T <= 2^18; T < sum(query_lens) drops the
+ * last rows.  Replaces the host loops of prepare_prefill / prepare_decode (model_runner.py:
+ * 279-333). */
+int w4a16_kv_step(const int32_t* query_lens, const int32_t* context_lens, int32_t* tables,
+                  int64_t table_stride, const int32_t* free_blocks, int32_t* cu_query_lens,
+                  int32_t* seq_lens, int32_t* positions, int32_t* slots, int32_t* blocks_used, int R,
+                  int width, int num_free, int block_size, int T, void* stream);
+
+/* Quantize rows k, v [T, KV, D] (bf16, unit stride along D, the other strides in elements and
+ * multiples of 8, 16-byte aligned) into the cache at slots [T]; rows of a slot outside the cache
+ * are skipped, live slots must differ.  Per row: the range [min(x, 0), max(x, 0)] in 15 steps,
+ * s = bf16(range / 15), z = min(round(-min / s), 15), c = clamp(round(x / s) + z, 0, 15), round
+ * half to even.  A row with a NaN or infinity is stored as NaN; one whose scale rounds to zero
+ * as zeros.  Replaces store_kvcache (attention.py:21-57). */
+int w4a16_kv_store(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v,
+                   int64_t v_stride_t, int64_t v_stride_h, uint8_t* cache, const int32_t* slots, int T,
+                   int KV, int D, int num_blocks, int block_size, void* stream);
+
+/* The rows at slots [T] as bf16(s * (c - z)), k and v [T, KV, D] contiguous and 16-byte aligned;
+ * zeros for a slot outside the cache.  No reference counterpart (its cache is bf16). */
+int w4a16_kv_load(const uint8_t* cache, const int32_t* slots, uint16_t* k, uint16_t* v, int T, int KV,
+                  int D, int num_blocks, int block_size, void* stream);
+
+/* Bytes of workspace w4a16_kv_attention needs (its contents need no initialization and are not
+ * kept; calls in flight at the same time must not share one). */
+size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int block_size, int width,
+                                    int max_query_len);
+
+/* Causal attention of packed query rows q [T, H, D] (bf16, strides as in w4a16_kv_store) over
+ * their sequences' cached keys and values, those of the rows themselves included (store first):
+ * request r owns rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1, the last tokens of its
+ * seq_lens[r] (at most width * block_size are reached) on the pages of tables[r]; query head h
+ * reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v with
+ * fp32 scores, statistics and sums; the weights enter the second product as bf16(p * s_v).
+ * tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of the
+ * earlier new ones, those new ones j < 64 whose bit j is set.  A row that sees no key gives
+ * zeros; keys on a page id outside the cache are not seen; NaN and infinities in keys that a
+ * row does not see have no effect on it.  Rows behind cu_query_lens[R] are set to zero if
+ * zero_tail, else left as they are.  max_query_len (>= 1) is a hint that chooses kernels and
+ * grid: the longest query of the batch; results are right for any.  scale > 0 and finite;
+ * H % KV == 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache
+ * (attention.py:118-132). */
+int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
+                       const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
+                       const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale,
+                       int T, int R, int H, int KV, int D, int num_blocks, int block_size, int width,
+                       int max_query_len, int zero_tail, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,6 +6,15 @@ The package directory name contains a hyphen; import it with
 owns device memory through torch, and mirrors the reference's operator interface.
 """
 from ._lib import REGIME_DECODE, REGIME_NONE, REGIME_TILE, W4A16Error, W4A16Library, lib
+from .layers.attention import (
+    Attention,
+    KVStep,
+    attention_int4,
+    kv_step,
+    load_kv_int4,
+    new_kv_cache_int4,
+    store_kv_int4,
+)
 from .layers.quantization.awq import (
     AWQLinearMethod,
     AWQRuntimeConfig,
@@ -27,7 +36,9 @@ from .layers.quantization.awq import (
 __all__ = (
     "AWQLinearMethod",
     "AWQRuntimeConfig",
+    "Attention",
     "FUSED_NORM_MAX_M",
+    "KVStep",
     "NormInput",
     "REGIME_DECODE",
     "REGIME_NONE",
@@ -35,6 +46,7 @@ __all__ = (
     "W4A16Error",
     "W4A16Library",
     "add_rms_norm",
+    "attention_int4",
     "awq_linear",
     "awq_linear_residual",
     "awq_linear_residual_stats",
@@ -43,7 +55,11 @@ __all__ = (
     "awq_linear_silu_mul",
     "awq_regime",
     "dequantize_awq_gemm",
+    "kv_step",
     "lib",
+    "load_kv_int4",
+    "new_kv_cache_int4",
     "repack_awq_qweight",
+    "store_kv_int4",
     "unpack_awq_int4",
 )

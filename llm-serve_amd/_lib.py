@@ -21,6 +21,7 @@ REGIME_TILE = 2
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_ptr = ctypes.c_void_p
+_c_i64 = ctypes.c_int64
 
 # name -> (restype, argtypes); mirrors include/w4a16.h
 _SIGNATURES = {
@@ -60,6 +61,15 @@ _SIGNATURES = {
                                            _c_int, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
     "w4a16_gemm_rmsnorm_stats": (_c_int, [_c_ptr, _c_ptr, _c_ptr, ctypes.c_float, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                           _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
+    "w4a16_kv_step": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int,
+                               _c_int, _c_int, _c_int, _c_int, _c_ptr]),
+    "w4a16_kv_store": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_int, _c_int, _c_int,
+                                _c_int, _c_int, _c_ptr]),
+    "w4a16_kv_load": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr]),
+    "w4a16_kv_attention_workspace": (_c_size, [_c_int] * 8),
+    "w4a16_kv_attention": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                    ctypes.c_float, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                                    _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
 }
 ABI_VERSION = 5
 
@@ -289,6 +299,39 @@ class W4A16Library:
                      packed.data_ptr(), qzeros.data_ptr(), scales.data_ptr(), y.data_ptr(), m, k, n, group_size,
                      regime, p0, p1, p2, split, ws_ptr, ws_len)
         return y
+
+    def kv_step(self, query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions, slots,
+                blocks_used, block_size: int) -> None:
+        self._launch(self.dll.w4a16_kv_step, "w4a16_kv_step", query_lens, query_lens.data_ptr(),
+                     context_lens.data_ptr(), tables.data_ptr(), tables.stride(0), free_blocks.data_ptr(),
+                     cu_query_lens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(),
+                     blocks_used.data_ptr(), query_lens.shape[0], tables.shape[1], free_blocks.shape[0], block_size,
+                     positions.shape[0])
+
+    def kv_store(self, k, v, cache, slots, head_dim: int, block_size: int) -> None:
+        """Rows k, v [T, KV, D] quantized into the cache's slots."""
+        self._launch(self.dll.w4a16_kv_store, "w4a16_kv_store", cache, k.data_ptr(), k.stride(0), k.stride(1),
+                     v.data_ptr(), v.stride(0), v.stride(1), cache.data_ptr(), slots.data_ptr(), k.shape[0],
+                     cache.shape[1], head_dim, cache.shape[0], block_size)
+
+    def kv_load(self, cache, slots, k, v, head_dim: int, block_size: int) -> None:
+        """The cache's rows at the slots into k, v [T, KV, D]."""
+        self._launch(self.dll.w4a16_kv_load, "w4a16_kv_load", cache, cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
+                     v.data_ptr(), slots.shape[0], cache.shape[1], head_dim, cache.shape[0], block_size)
+
+    def kv_attention_workspace(self, t: int, r: int, h: int, kv: int, head_dim: int, block_size: int, width: int,
+                               max_query_len: int) -> int:
+        return int(self.dll.w4a16_kv_attention_workspace(t, r, h, kv, head_dim, block_size, width, max_query_len))
+
+    def kv_attention(self, q, cache, tables, seq_lens, cu_query_lens, tree_mask, out, scale: float, block_size: int,
+                     max_query_len: int, zero_tail: bool, workspace) -> None:
+        """out [T, H, D] = attention of the packed rows q over the cache's pages."""
+        t, h, d = q.shape
+        self._launch(self.dll.w4a16_kv_attention, "w4a16_kv_attention", cache, q.data_ptr(), q.stride(0), q.stride(1),
+                     cache.data_ptr(), tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(),
+                     cu_query_lens.data_ptr(), _ptr(tree_mask), out.data_ptr(), scale, t, seq_lens.shape[0], h,
+                     cache.shape[1], d, cache.shape[0], block_size, tables.shape[1], max_query_len, int(zero_tail),
+                     workspace.data_ptr(), workspace.numel())
 
 
 _LOCK = threading.Lock()

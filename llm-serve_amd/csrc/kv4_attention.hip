@@ -1,0 +1,563 @@
+// Attention over the 4-bit paged cache.
+//
+// For a row q of a kv head and its visible keys t,
+//   S_t = scale s_k (q . (c_k - z_k)),  P = softmax(S),  out = sum_t P_t s_v (c_v - z_v).
+// Codes and zero points enter the matrix instructions as they are: (128 + c) is an exact bf16
+// value (kv4_common.h), and
+//   q . (c - z)          = q . (128 + c) - (128 + z) sum(q)
+//   sum P' (c - z)       = sum P' (128 + c) - sum P' (128 + z),   P' = bf16(P s_v),
+// so no code is ever scaled: the key's offset is the accumulator's initial value and its scale
+// one multiplication a score, and the values' offset is one more matrix tile whose operand is
+// the meta words' low halves.  Scores, statistics and sums are fp32; the one rounding is P' to
+// bf16, the matrix instruction's operand type.
+#include "kv4_common.h"
+#include "kv4_launch.h"
+
+namespace w4a16 {
+namespace {
+
+constexpr int kUnit = 128;      // keys of one work unit: 32 a wave
+constexpr int kWaves = 4;
+constexpr int kThreads = 64 * kWaves;
+
+// What a combine needs to join one row tile's partial results.
+struct KvSplit {
+  int request, head, tile;
+  int count;        // partial results (0: this entry joins nothing)
+  int first, next;  // slot of the first one, and of the second
+  int stride;       // between slots from the second on
+  int pad;
+};
+
+struct KvPartials {
+  float* out;      // [slots][rows][D], unnormalized
+  float* stats;    // [slots][rows][2]: maximum (raw score) and sum
+  KvSplit* split;  // one a worker
+};
+
+// One request as the kernels see it, all lengths safe whatever the tensors hold.
+struct KvRequest {
+  int row;   // its first packed row
+  int n;     // its packed rows
+  int cached;  // sequence length before them
+  int keys;  // keys that its block table can hold of the sequence
+};
+
+__device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r) {
+  KvRequest q;
+  const int lo = a.cu_query_lens[r], hi = a.cu_query_lens[r + 1];
+  q.row = min(max(lo, 0), a.T);
+  q.n = max(min(hi, a.T) - q.row, 0);
+  const int seq = max(a.seq_lens[r], 0);
+  q.cached = seq - (hi - lo);
+  const int64_t room = static_cast<int64_t>(a.width) << a.log2_block;
+  q.keys = seq < room ? seq : static_cast<int>(room);
+  return q;
+}
+
+__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// Work of a request in units (a request whose rows see nothing still has its zeros to write).
+__device__ __forceinline__ int64_t kv_units(const KvAttentionArgs& a, const KvRequest& q, int tile_rows) {
+  const int tiles = ceil_div(q.n * (a.H / a.KV), tile_rows);
+  return static_cast<int64_t>(tiles) * a.KV * max(ceil_div(q.keys, kUnit), 1);
+}
+
+// out[row, h, ch ..] = o / sum, rounded; a row that saw nothing (or only scores of -inf) is zero.
+template <int N>
+__device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int h, int ch, float sum, const float (&o)[N]) {
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  uint16_t* p = a.out + (static_cast<size_t>(row) * a.H + h) * a.D + ch;
+  if constexpr (N == 8) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                                              pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
+  } else if constexpr (N == 2) {
+    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(o[0] * inv, o[1] * inv);
+  } else {
+    *p = f32_to_bf16_bits(o[0] * inv);
+  }
+}
+
+// One slice of 32 keys of a wave, in registers: two 16-key tiles.
+template <int D>
+struct KvSlice {
+  uint32_t k[2][D / 32];  // K words of key lane % 16: D / 4 channels from (D / 4) (lane / 16)
+  uint32_t v[2][4];       // V word of four keys 4 (lane / 16) ..
+  uint32_t km[2][4], vm[2][4];  // their meta words
+  bool ok[2];             // the tile's page is in the cache (wave-uniform)
+};
+
+template <int D>
+__device__ __forceinline__ void load_slice(KvSlice<D>& s, const KvAttentionArgs& a, const int32_t* table, int head,
+                                           int key, int keys, int lane) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int k0 = key + 16 * t;
+    const int id = k0 < keys ? __builtin_amdgcn_readfirstlane(table[k0 >> a.log2_block]) : -1;
+    s.ok[t] = id >= 0 && id < a.num_blocks;
+    if (!s.ok[t]) {
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) s.k[t][i] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.v[t][i] = s.km[t][i] = s.vm[t][i] = 0;
+      continue;
+    }
+    const uint32_t* page = reinterpret_cast<const uint32_t*>(
+        a.cache + (static_cast<size_t>(id) * a.KV + head) * kv_page_bytes<D>(a.log2_block));
+    const int token = k0 & ((1 << a.log2_block) - 1);
+    const int part = (D / 8) << a.log2_block;
+    const uint32_t* kp = page + (token + r) * (D / 8) + g * (D / 32);
+    if (D == 128) {
+      const uint4 w = *reinterpret_cast<const uint4*>(kp);
+      s.k[t][0] = w.x, s.k[t][1] = w.y, s.k[t][D / 32 - 2] = w.z, s.k[t][D / 32 - 1] = w.w;
+    } else {
+      const uint2 w = *reinterpret_cast<const uint2*>(kp);
+      s.k[t][0] = w.x, s.k[t][1] = w.y;
+    }
+    const uint4 v = *reinterpret_cast<const uint4*>(page + part + kv_v_word<D>(token + 4 * g, r % (D / 8)));
+    s.v[t][0] = v.x, s.v[t][1] = v.y, s.v[t][2] = v.z, s.v[t][3] = v.w;
+    const uint4 km = *reinterpret_cast<const uint4*>(page + 2 * part + token + 4 * g);
+    s.km[t][0] = km.x, s.km[t][1] = km.y, s.km[t][2] = km.z, s.km[t][3] = km.w;
+    const uint4 vm = *reinterpret_cast<const uint4*>(page + 2 * part + (1 << a.log2_block) + token + 4 * g);
+    s.vm[t][0] = vm.x, s.vm[t][1] = vm.y, s.vm[t][2] = vm.z, s.vm[t][3] = vm.w;
+  }
+}
+
+// Split attention.  A row tile is up to 16 MT rows (tokens x heads of the group) of one request
+// and kv head; its keys are cut into units of 128.  All units of all tiles, in order, are dealt
+// to the grid's workgroups in equal contiguous shares, so that a batch of any lengths loads them
+// alike; a share that covers a tile's keys only in part leaves a partial result, joined in a
+// fixed order by kv_combine_kernel.  Inside a unit each of the 4 waves takes 32 keys and keeps
+// its own running maximum and sum; the waves are joined through LDS at the end of a tile.
+template <int D, int MT>
+__global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {
+  constexpr int kRows = 16 * MT, kSteps = D / 32, kTiles = D / 16, kPitch = D + 4;
+  __shared__ __align__(16) float s_out[kWaves][kRows][kPitch];
+  __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
+  __shared__ int64_t s_part[kWaves];
+  __shared__ int64_t s_base;
+  __shared__ int s_request;
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int group = a.H / a.KV;
+
+  // This workgroup's share: a scan of the requests' units, and the request where it begins.
+  const int per = (a.R + kThreads - 1) / kThreads;
+  const int r0 = tid * per, r1 = min(a.R, r0 + per);
+  int64_t mine = 0;
+  for (int r = r0; r < r1; ++r) mine += kv_units(a, kv_request(a, r), kRows);
+  int64_t upto = mine;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t u = __shfl_up(upto, d);
+    if (lane >= d) upto += u;
+  }
+  if (lane == 63) s_part[wave] = upto;
+  __syncthreads();
+  int64_t total = 0;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    if (w < wave) upto += s_part[w];
+    total += s_part[w];
+  }
+  const int64_t workers = total < gridDim.x ? total : gridDim.x;
+  const int64_t me = blockIdx.x;
+  KvSplit* split = out.split + blockIdx.x;
+
+  if (a.zero_tail) {
+    const int end = min(max(a.cu_query_lens[a.R], 0), a.T);
+    const int chunks = a.H * D / 8;
+    for (int row = end + blockIdx.x; row < a.T; row += gridDim.x)
+      for (int c = tid; c < chunks; c += kThreads)
+        reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
+  }
+  if (me >= workers) {
+    if (tid == 0) split->count = 0;
+    return;
+  }
+  const int64_t begin = total * me / workers, end = total * (me + 1) / workers;
+  if (begin >= upto - mine && begin < upto) {
+    int64_t base = upto - mine;
+    int r = r0;
+    for (;; ++r) {
+      const int64_t u = kv_units(a, kv_request(a, r), kRows);
+      if (begin < base + u) break;
+      base += u;
+    }
+    s_base = base;
+    s_request = r;
+  }
+  __syncthreads();
+  int r = __builtin_amdgcn_readfirstlane(s_request);
+  int64_t base = s_base;
+  KvRequest q = kv_request(a, r);
+  int64_t units = kv_units(a, q, kRows);
+  bool left = false;  // whether this workgroup left the first part of a tile
+
+  const NibbleConsts nc = nibble_consts();
+  const int col = lane & 15, g = lane >> 4;
+  const float scale = a.scale_log2e;
+
+  for (int64_t u = begin; u < end;) {
+    while (u >= base + units) {
+      base += units;
+      q = kv_request(a, ++r);
+      units = kv_units(a, q, kRows);
+    }
+    const int tiles = ceil_div(q.n * group, kRows);
+    const int span = max(ceil_div(q.keys, kUnit), 1);
+    const int64_t local = u - base;
+    const int seg = static_cast<int>(local / span), k0 = static_cast<int>(local - static_cast<int64_t>(seg) * span);
+    const int head = seg / tiles, tile = seg - head * tiles;
+    const int n = static_cast<int>(min(static_cast<int64_t>(span - k0), end - u));
+    const int row0 = tile * kRows, rows = min(kRows, q.n * group - row0);
+    const int32_t* table = a.tables + static_cast<int64_t>(r) * a.table_stride;
+
+    // The queries as the second operand: column = row of the tile, channels as K's words have them.
+    bf16x8_t qf[MT][kSteps];
+    float neg_sum[MT];
+    int sees[MT];       // leading keys that the lane's row sees
+    uint64_t bits[MT];  // and which of the request's new ones behind them
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const int row = row0 + 16 * m + col;
+      const int token = row / group, h = head * group + row - token * group;
+      const bool live = 16 * m + col < rows;
+      float sum = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (live)
+          w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + h * a.q_stride_h + (D / 4) * g +
+                                              8 * s);
+        float f[8];
+        unpack_bf16x8(w, f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += f[i];
+        qf[m][s] = __builtin_bit_cast(bf16x8_t, w);
+      }
+      neg_sum[m] = -column_sum(sum);
+      const bool tree = a.tree_mask != nullptr;
+      bits[m] = tree && live ? a.tree_mask[q.row + token] : 0;
+      sees[m] = live ? min(tree ? q.cached : q.cached + token + 1, q.keys) : 0;
+    }
+    const int all_see = min(a.tree_mask ? q.cached : q.cached + row0 / group + 1, q.keys);
+
+    f32x4_t acc_o[MT][kTiles], acc_z[MT];
+    float row_max[MT], row_sum[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c) acc_o[m][c] = f32x4_t{0, 0, 0, 0};
+      acc_z[m] = f32x4_t{0, 0, 0, 0};
+      row_max[m] = -INFINITY;
+      row_sum[m] = 0.0f;
+    }
+
+    const int key_end = min((k0 + n) * kUnit, q.keys);
+    KvSlice<D> now;
+    int key = k0 * kUnit + 32 * wave;
+    if (key < key_end) load_slice<D>(now, a, table, head, key, key_end, lane);
+    for (; key < key_end; key += kUnit) {
+      KvSlice<D> ahead;
+      if (key + kUnit < key_end) load_slice<D>(ahead, a, table, head, key + kUnit, key_end, lane);
+
+      f32x4_t sc[MT][2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[m][t][i] = kv_meta_zero128(now.km[t][i]) * neg_sum[m];
+#pragma unroll
+        for (int s = 0; s < kSteps; ++s) {
+          const bf16x8_t kf = unpack_codes(now.k[t][s], nc);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) sc[m][t] = mfma16(kf, qf[m][s], sc[m][t]);
+        }
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[m][t][i] *= kv_meta_scale(now.km[t][i]);
+      }
+
+      const bool whole = key + 32 <= all_see && now.ok[0] && now.ok[1];
+      u32x4_t zf;  // the keys' 128 + z as the first operand of the offset tile
+      bf16x8_t pf[MT];
+      bool grew = false;
+      float top[MT];
+      uint32_t seen[MT];
+      if (!whole) {
+        // A lane's keys are 16 t + 4 g + i.  Keys outside the sequence, or on no page, hold
+        // anything: their score becomes -inf, their scale 0 and their zero point 0.  Keys that
+        // only this row does not see keep their zero point (the offset tile's operand serves
+        // all rows), and their scale is taken as 0 for this row.
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          seen[m] = 0;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = key + 16 * t + 4 * g + i;
+              const unsigned fresh = static_cast<unsigned>(k - q.cached);
+              const bool visible = now.ok[t] && k < q.keys &&
+                                   (k < sees[m] || (fresh < 64u && ((bits[m] >> fresh) & 1)));
+              if (visible) seen[m] |= 1u << (4 * t + i);
+              else sc[m][t][i] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!now.ok[t] || key + 16 * t + 4 * g + i >= q.keys) now.vm[t][i] = 0x00004300u, now.v[t][i] = 0;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          zf[2 * t + i] = __builtin_amdgcn_perm(now.vm[t][2 * i + 1], now.vm[t][2 * i], 0x05040100u);
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        float mx = fmaxf(fmaxf(fmaxf(sc[m][0][0], sc[m][0][1]), fmaxf(sc[m][0][2], sc[m][0][3])),
+                         fmaxf(fmaxf(sc[m][1][0], sc[m][1][1]), fmaxf(sc[m][1][2], sc[m][1][3])));
+        top[m] = fmaxf(row_max[m], column_max(mx));
+        grew |= top[m] > row_max[m];
+      }
+      if (__any(grew)) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          const float ref = top[m] == -INFINITY ? 0.0f : top[m];
+          const float f = __builtin_amdgcn_exp2f((row_max[m] - ref) * scale);
+          row_max[m] = top[m];
+          row_sum[m] *= f;
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc_o[m][c][i] *= f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc_z[m][i] *= f;
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        const float ref = (row_max[m] == -INFINITY ? 0.0f : row_max[m]) * scale;
+        u32x4_t w;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          float p[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][t][i], scale, -ref));
+            row_sum[m] += p[i];
+            float s = kv_meta_scale(now.vm[t][i]);
+            if (!whole) s = (seen[m] >> (4 * t + i)) & 1 ? s : 0.0f;
+            p[i] *= s;
+          }
+          w[2 * t] = pack_bf16x2(p[0], p[1]);
+          w[2 * t + 1] = pack_bf16x2(p[2], p[3]);
+        }
+        pf[m] = __builtin_bit_cast(bf16x8_t, w);
+        acc_z[m] = mfma16(__builtin_bit_cast(bf16x8_t, zf), pf[m], acc_z[m]);
+      }
+
+      // V: words of tokens paired into halves with 4 channels each (even ones, then odd ones);
+      // nibble i of the halves is one channel of two tokens.  A 64-channel row has 8 words, and
+      // lanes 8 .. 15 of a row of 16 take the same words' odd channels.
+#pragma unroll
+      for (int half = 0; half < (D == 128 ? 2 : 1); ++half) {
+        uint32_t pair[4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t select = half ? 0x07060302u : 0x05040100u;
+            if (D == 64) select = col & 8 ? 0x07060302u : 0x05040100u;
+            pair[2 * t + i] = __builtin_amdgcn_perm(now.v[t][2 * i + 1], now.v[t][2 * i], select);
+          }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          u32x4_t f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) f[i] = ((pair[i] >> (4 * c)) & nc.mask) | nc.bias;
+          const int ch = D == 128 ? 2 * c + half : c;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+            acc_o[m][ch] = mfma16(__builtin_bit_cast(bf16x8_t, f), pf[m], acc_o[m][ch]);
+        }
+      }
+      now = ahead;
+    }
+
+    // Join the waves.  Accumulator register i of a lane is operand row 4 g + i: the word (D =
+    // 128) or word and half (D = 64) whose channels the tiles c count.
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      const float sum = column_sum(row_sum[m]);
+      if (g == 0) {
+        s_max[wave][16 * m + col] = row_max[m];
+        s_sum[wave][16 * m + col] = sum;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float* o = s_out[wave][16 * m + col];
+        if (D == 128) {
+#pragma unroll
+          for (int c = 0; c < 8; c += 4) {
+            const f32x4_t v = {acc_o[m][c][i] - acc_z[m][i], acc_o[m][c + 1][i] - acc_z[m][i],
+                               acc_o[m][c + 2][i] - acc_z[m][i], acc_o[m][c + 3][i] - acc_z[m][i]};
+            *reinterpret_cast<f32x4_t*>(o + 8 * (4 * g + i) + c) = v;
+          }
+        } else {
+          const int word = (4 * g + i) & 7, odd = g >> 1;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[8 * word + 2 * c + odd] = acc_o[m][c][i] - acc_z[m][i];
+        }
+      }
+    }
+    __syncthreads();
+    const bool complete = k0 == 0 && n == span;
+    // A partial result's slot: 2 w for a tile begun before this share, 2 w + 1 for one begun in it.
+    const int slot = 2 * blockIdx.x + (k0 == 0);
+    constexpr int kChunks = D / 8;
+    for (int e = tid; e < rows * kChunks; e += kThreads) {
+      const int row = e / kChunks, ch = e % kChunks * 8;
+      float top = s_max[0][row];
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[w][row]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      float sum = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const float f = __builtin_amdgcn_exp2f((s_max[w][row] - ref) * scale);
+        sum += f * s_sum[w][row];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] += f * s_out[w][row][ch + i];
+      }
+      if (complete) {
+        const int token = (row0 + row) / group;
+        kv_write(a, q.row + token, head * group + row0 + row - token * group, ch, sum, o);
+      } else {
+        float* p = out.out + (static_cast<size_t>(slot) * kRows + row) * D + ch;
+        *reinterpret_cast<f32x4_t*>(p) = f32x4_t{o[0], o[1], o[2], o[3]};
+        *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{o[4], o[5], o[6], o[7]};
+        if (ch == 0) {
+          float* st = out.stats + (static_cast<size_t>(slot) * kRows + row) * 2;
+          st[0] = top;
+          st[1] = sum;
+        }
+      }
+    }
+    if (!complete && k0 == 0) {
+      // This share begins the tile: the workgroup with unit x has number ((x + 1) workers - 1) / total.
+      left = true;
+      if (tid == 0) {
+        const int64_t last = u + span - 1;
+        const int64_t owner = ((last + 1) * workers - 1) / total;
+        *split = KvSplit{r, head, tile, static_cast<int>(owner - me) + 1, slot, 2 * (static_cast<int>(me) + 1), 2, 0};
+      }
+    }
+    u += n;
+    __syncthreads();
+  }
+  if (!left && tid == 0) split->count = 0;
+}
+
+// Joins the partial results of the tile that worker blockIdx.x begins and others end, in the
+// workers' order: a wave a row, its lanes over the channels (and, for the statistics, over the
+// parts).
+template <int D, int MT>
+__global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a, KvPartials part) {
+  constexpr int kRows = 16 * MT, kPer = D / 64;
+  const KvSplit s = part.split[blockIdx.x];
+  if (s.count <= 0) return;
+  const int lane = threadIdx.x & 63;
+  const int group = a.H / a.KV;
+  const KvRequest q = kv_request(a, s.request);
+  const int row0 = s.tile * kRows, rows = min(kRows, q.n * group - row0);
+  for (int row = wave_id() + kWaves * blockIdx.y; row < rows; row += kWaves * gridDim.y) {
+    auto at = [&](int i) { return static_cast<size_t>(i == 0 ? s.first : s.next + s.stride * (i - 1)) * kRows + row; };
+    float top = -INFINITY;
+    for (int i = lane; i < s.count; i += 64) top = fmaxf(top, part.stats[at(i) * 2]);
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float ref = top == -INFINITY ? 0.0f : top;
+    float sum = 0.0f, o[kPer] = {};
+    for (int b = 0; b < s.count; b += 64) {
+      float f = 0.0f;
+      if (b + lane < s.count) {
+        const float* st = part.stats + at(b + lane) * 2;
+        f = __builtin_amdgcn_exp2f((st[0] - ref) * a.scale_log2e);
+        sum += f * st[1];
+      }
+      const int n = min(64, s.count - b);
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) {
+        const float fj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), j));
+        const float* p = part.out + at(b + j) * D + lane * kPer;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) o[i] += fj * p[i];
+      }
+    }
+    sum = wave_sum64(sum);
+    const int token = (row0 + row) / group;
+    kv_write(a, q.row + token, s.head * group + row0 + row - token * group, lane * kPer, sum, o);
+  }
+}
+
+struct KvPlan {
+  int mt;       // 16-row tiles of a workgroup
+  int workers;  // grid
+};
+
+KvPlan kv_plan(const KvAttentionArgs& a) {
+  KvPlan p;
+  const int64_t rows = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
+  p.mt = rows <= 16 ? 1 : 2;
+  const int64_t tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
+  const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
+  const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
+  const int64_t fill = p.mt == 1 ? 1024 : 512;
+  p.workers = static_cast<int>(most < fill ? most : fill);
+  return p;
+}
+
+size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+template <int D, int MT>
+hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, const KvPartials& part, hipStream_t stream) {
+  kv_attention_kernel<D, MT><<<p.workers, kThreads, 0, stream>>>(a, part);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  const int64_t rows = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
+  const int y = static_cast<int>(((rows < 16 * MT ? rows : 16 * MT) + kWaves - 1) / kWaves);
+  kv_combine_kernel<D, MT><<<dim3(p.workers, y > 0 ? y : 1), kThreads, 0, stream>>>(a, part);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t kv_attention_workspace(const KvAttentionArgs& a) {
+  const KvPlan p = kv_plan(a);
+  const size_t rows = static_cast<size_t>(2) * p.workers * 16 * p.mt;
+  return align256(rows * a.D * sizeof(float)) + align256(rows * 2 * sizeof(float)) +
+         align256(p.workers * sizeof(KvSplit));
+}
+
+hipError_t launch_kv_attention(const KvAttentionArgs& a, void* workspace, hipStream_t stream) {
+  const KvPlan p = kv_plan(a);
+  const size_t rows = static_cast<size_t>(2) * p.workers * 16 * p.mt;
+  char* ws = static_cast<char*>(workspace);
+  KvPartials part;
+  part.out = reinterpret_cast<float*>(ws);
+  ws += align256(rows * a.D * sizeof(float));
+  part.stats = reinterpret_cast<float*>(ws);
+  ws += align256(rows * 2 * sizeof(float));
+  part.split = reinterpret_cast<KvSplit*>(ws);
+  if (a.D == 64) return p.mt == 1 ? launch<64, 1>(a, p, part, stream) : launch<64, 2>(a, p, part, stream);
+  return p.mt == 1 ? launch<128, 1>(a, p, part, stream) : launch<128, 2>(a, p, part, stream);
+}
+
+}  // namespace w4a16

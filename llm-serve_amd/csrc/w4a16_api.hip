@@ -6,6 +6,7 @@
 #include <mutex>
 
 #include "../../include/w4a16.h"
+#include "kv4_launch.h"
 #include "w4a16_common.h"
 #include "w4a16_launch.h"
 
@@ -1214,6 +1215,160 @@ size_t w4a16_workspace_bytes_config(int M, int N, int regime, int p0, int split)
     most = b > most ? b : most;
   }
   return most;
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ 4-bit key/value cache
+namespace {
+
+// log2 of a cache's block size, or -1.
+int kv_log2_block(int block_size) {
+  for (int i = 4; i <= 8; ++i)
+    if (block_size == 1 << i) return i;
+  return -1;
+}
+
+int validate_kv_cache(const void* cache, int KV, int D, int num_blocks, int block_size, int* log2_block) {
+  if (!cache) return fail(W4A16_ERR_ARG, "the KV cache pointer is null");
+  if (KV <= 0 || num_blocks <= 0) return fail(W4A16_ERR_ARG, "kv heads (%d) and num_blocks (%d) must be positive", KV, num_blocks);
+  if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
+  *log2_block = kv_log2_block(block_size);
+  if (*log2_block < 0)
+    return fail(W4A16_ERR_SHAPE, "block_size must be a power of two in 16 .. 256 (got %d)", block_size);
+  if (static_cast<int64_t>(num_blocks) << *log2_block > 0x7FFFFFFF)
+    return fail(W4A16_ERR_SHAPE, "the cache's slots must stay below 2^31 (%d blocks of %d)", num_blocks, block_size);
+  if (!aligned(cache, 16)) return fail(W4A16_ERR_ALIGN, "the KV cache must be 16-byte aligned");
+  return W4A16_OK;
+}
+
+int validate_kv_rows(const char* name, const void* p, int64_t stride_t, int64_t stride_h) {
+  if (!p) return fail(W4A16_ERR_ARG, "%s is null", name);
+  if (!aligned(p, 16) || stride_t % 8 || stride_h % 8)
+    return fail(W4A16_ERR_ALIGN, "%s must be 16-byte aligned with strides that are multiples of 8 elements", name);
+  return W4A16_OK;
+}
+
+int kv_rows(w4a16::KvRowsArgs* a, int T, int KV, int D, int num_blocks, int log2_block) {
+  if (static_cast<int64_t>(T) * KV * D / 64 > 0x3FFFFFFF)
+    return fail(W4A16_ERR_SHAPE, "%d rows of %d kv heads are too many for one call", T, KV);
+  a->T = T, a->KV = KV, a->D = D, a->num_blocks = num_blocks, a->log2_block = log2_block;
+  return W4A16_OK;
+}
+
+int validate_kv_heads(int T, int R, int H, int KV, int D, int width, int max_query_len) {
+  if (T < 0 || R < 0) return fail(W4A16_ERR_ARG, "T (%d) and R (%d) must not be negative", T, R);
+  if (H <= 0 || KV <= 0 || H % KV) return fail(W4A16_ERR_SHAPE, "query heads (%d) must be a multiple of kv heads (%d)", H, KV);
+  if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
+  if (width <= 0) return fail(W4A16_ERR_ARG, "the block tables' width must be positive (got %d)", width);
+  if (max_query_len < 1) return fail(W4A16_ERR_ARG, "max_query_len must be at least 1 (got %d)", max_query_len);
+  if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
+    return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
+  return W4A16_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int w4a16_kv_step(const int32_t* query_lens, const int32_t* context_lens, int32_t* tables, int64_t table_stride,
+                  const int32_t* free_blocks, int32_t* cu_query_lens, int32_t* seq_lens, int32_t* positions,
+                  int32_t* slots, int32_t* blocks_used, int R, int width, int num_free, int block_size, int T,
+                  void* stream) {
+  if (R < 0 || T < 0 || num_free < 0) return fail(W4A16_ERR_ARG, "R (%d), T (%d) and num_free (%d) must not be negative", R, T, num_free);
+  if (R > w4a16::kKvStepMaxRequests || T > w4a16::kKvStepMaxTokens)
+    return fail(W4A16_ERR_SHAPE, "a step takes at most %d requests and %d rows (got %d, %d)", w4a16::kKvStepMaxRequests,
+                w4a16::kKvStepMaxTokens, R, T);
+  if (!cu_query_lens || !blocks_used || (R && (!query_lens || !context_lens || !tables || !seq_lens)) ||
+      (T && (!positions || !slots)) || (num_free && !free_blocks))
+    return fail(W4A16_ERR_ARG, "a step pointer is null");
+  if (R && (width <= 0 || table_stride < width))
+    return fail(W4A16_ERR_ARG, "the block tables need a positive width (%d) and rows at least that far apart", width);
+  const int log2_block = kv_log2_block(block_size);
+  if (log2_block < 0)
+    return fail(W4A16_ERR_SHAPE, "block_size must be a power of two in 16 .. 256 (got %d)", block_size);
+  const w4a16::KvStepArgs a{query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions, slots,
+                            blocks_used, table_stride, R, width, num_free, log2_block, T};
+  return check_launch(w4a16::launch_kv_step(a, static_cast<hipStream_t>(stream)), "kv step");
+}
+
+int w4a16_kv_store(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
+                   int64_t v_stride_h, uint8_t* cache, const int32_t* slots, int T, int KV, int D, int num_blocks,
+                   int block_size, void* stream) {
+  if (T < 0) return fail(W4A16_ERR_ARG, "T must not be negative (got %d)", T);
+  int log2_block = 0;
+  int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block);
+  if (e != W4A16_OK) return e;
+  if (T == 0) return ok();
+  if (!slots) return fail(W4A16_ERR_ARG, "slots is null");
+  if ((e = validate_kv_rows("k", k, k_stride_t, k_stride_h)) != W4A16_OK) return e;
+  if ((e = validate_kv_rows("v", v, v_stride_t, v_stride_h)) != W4A16_OK) return e;
+  w4a16::KvRowsArgs a{};
+  if ((e = kv_rows(&a, T, KV, D, num_blocks, log2_block)) != W4A16_OK) return e;
+  a.k = const_cast<uint16_t*>(k), a.k_stride_t = k_stride_t, a.k_stride_h = k_stride_h;
+  a.v = const_cast<uint16_t*>(v), a.v_stride_t = v_stride_t, a.v_stride_h = v_stride_h;
+  a.cache = cache, a.slots = slots;
+  return check_launch(w4a16::launch_kv_store(a, static_cast<hipStream_t>(stream)), "kv store");
+}
+
+int w4a16_kv_load(const uint8_t* cache, const int32_t* slots, uint16_t* k, uint16_t* v, int T, int KV, int D,
+                  int num_blocks, int block_size, void* stream) {
+  if (T < 0) return fail(W4A16_ERR_ARG, "T must not be negative (got %d)", T);
+  int log2_block = 0;
+  int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block);
+  if (e != W4A16_OK) return e;
+  if (T == 0) return ok();
+  if (!slots) return fail(W4A16_ERR_ARG, "slots is null");
+  if ((e = validate_kv_rows("k", k, 0, 0)) != W4A16_OK) return e;
+  if ((e = validate_kv_rows("v", v, 0, 0)) != W4A16_OK) return e;
+  w4a16::KvRowsArgs a{};
+  if ((e = kv_rows(&a, T, KV, D, num_blocks, log2_block)) != W4A16_OK) return e;
+  a.k = k, a.v = v;
+  a.k_stride_t = a.v_stride_t = static_cast<int64_t>(KV) * D;
+  a.k_stride_h = a.v_stride_h = D;
+  a.cache = const_cast<uint8_t*>(cache), a.slots = slots;
+  return check_launch(w4a16::launch_kv_load(a, static_cast<hipStream_t>(stream)), "kv load");
+}
+
+size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int block_size, int width, int max_query_len) {
+  if (validate_kv_heads(T, R, H, KV, D, width, max_query_len) != W4A16_OK || kv_log2_block(block_size) < 0) return 0;
+  if (T == 0 || R == 0) return 0;
+  w4a16::KvAttentionArgs a{};
+  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.width = width;
+  a.log2_block = kv_log2_block(block_size);
+  a.max_query_len = max_query_len < T ? max_query_len : T;
+  return w4a16::kv_attention_workspace(a);
+}
+
+int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
+                       const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
+                       const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale, int T,
+                       int R, int H, int KV, int D, int num_blocks, int block_size, int width, int max_query_len,
+                       int zero_tail, void* workspace, size_t workspace_bytes, void* stream) {
+  int log2_block = 0;
+  int e = validate_kv_heads(T, R, H, KV, D, width, max_query_len);
+  if (e != W4A16_OK) return e;
+  if ((e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block)) != W4A16_OK) return e;
+  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(W4A16_ERR_ARG, "scale must be positive and finite (got %g)", static_cast<double>(scale));
+  if (T == 0) return ok();
+  if (R == 0) return fail(W4A16_ERR_ARG, "%d rows of no request", T);
+  if (!tables || !seq_lens || !cu_query_lens || !out) return fail(W4A16_ERR_ARG, "an attention pointer is null");
+  if (table_stride < width) return fail(W4A16_ERR_ARG, "the block tables' rows must be at least %d apart", width);
+  if ((e = validate_kv_rows("q", q, q_stride_t, q_stride_h)) != W4A16_OK) return e;
+  if (!aligned(out, 16)) return fail(W4A16_ERR_ALIGN, "out must be 16-byte aligned");
+  w4a16::KvAttentionArgs a{};
+  a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
+  a.cache = cache, a.tables = tables, a.table_stride = table_stride;
+  a.seq_lens = seq_lens, a.cu_query_lens = cu_query_lens, a.tree_mask = tree_mask, a.out = out;
+  a.scale_log2e = scale * 1.44269504088896341f;
+  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.num_blocks = num_blocks, a.log2_block = log2_block, a.width = width;
+  a.max_query_len = max_query_len < T ? max_query_len : T;
+  a.zero_tail = zero_tail != 0;
+  const size_t need = w4a16::kv_attention_workspace(a);
+  if (!workspace || workspace_bytes < need)
+    return fail(W4A16_ERR_WORKSPACE, "attention needs %zu bytes of workspace (got %zu)", need, workspace ? workspace_bytes : size_t(0));
+  if (!aligned(workspace, 16)) return fail(W4A16_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  return check_launch(w4a16::launch_kv_attention(a, workspace, static_cast<hipStream_t>(stream)), "kv attention");
 }
 
 }  // extern "C"
