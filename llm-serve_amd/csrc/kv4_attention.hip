@@ -37,10 +37,10 @@ struct KvPartials {
 
 // One request as the kernels see it, all lengths safe whatever the tensors hold.
 struct KvRequest {
-  int row;   // its first packed row
-  int n;     // its packed rows
+  int row;     // its first packed row
+  int n;       // its packed rows
   int cached;  // sequence length before them
-  int keys;  // keys that its block table can hold of the sequence
+  int keys;    // keys that its block table can hold of the sequence
 };
 
 __device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r) {
@@ -57,11 +57,36 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r)
 
 __device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
-// Work of a request in units (a request whose rows see nothing still has its zeros to write).
-__device__ __forceinline__ int64_t kv_units(const KvAttentionArgs& a, const KvRequest& q, int tile_rows) {
-  const int tiles = ceil_div(q.n * (a.H / a.KV), tile_rows);
-  return static_cast<int64_t>(tiles) * a.KV * max(ceil_div(q.keys, kUnit), 1);
+// Units of one row tile (a tile whose rows see nothing still has its zeros to write).
+__device__ __forceinline__ int kv_span(const KvRequest& q) { return max((q.keys + kUnit - 1) / kUnit, 1); }
+
+// Units of a request.
+template <int ROWS>
+__device__ __forceinline__ int kv_units(const KvAttentionArgs& a, const KvRequest& q, int group) {
+  return (q.n * group + ROWS - 1) / ROWS * a.KV * kv_span(q);
 }
+
+// Inclusive sum over the lanes up to this one: DPP moves within rows of 16, then the row totals.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row 0 -> 1, row 2 -> 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 -> rows 2, 3
+  return v;
+}
+
+// Equal contiguous shares of `total` units for `workers` workgroups: the first `rest` take one
+// more than the others.
+struct KvShares {
+  int each, rest;
+  __device__ __forceinline__ int begin(int w) const { return w * each + min(w, rest); }
+  __device__ __forceinline__ int owner(int unit) const {
+    const int head = rest * (each + 1);
+    return unit < head ? unit / (each + 1) : rest + (unit - head) / each;
+  }
+};
 
 // out[row, h, ch ..] = o / sum, rounded; a row that saw nothing (or only scores of -inf) is zero.
 template <int N>
@@ -78,50 +103,75 @@ __device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int 
   }
 }
 
-// One slice of 32 keys of a wave, in registers: two 16-key tiles.
+// One slice of 32 keys of a wave, in registers: two 16-key tiles, each inside one page.
 template <int D>
 struct KvSlice {
-  uint32_t k[2][D / 32];  // K words of key lane % 16: D / 4 channels from (D / 4) (lane / 16)
-  uint32_t v[2][4];       // V word of four keys 4 (lane / 16) ..
-  uint32_t km[2][4], vm[2][4];  // their meta words
-  bool ok[2];             // the tile's page is in the cache (wave-uniform)
+  uint32_t k[2][D / 32];        // K words of key lane % 16: D / 4 channels from (D / 4) (lane / 16)
+  uint32_t v[2][4];             // one V word of four keys 4 (lane / 16) ..
+  uint32_t km[2][4], vm[2][4];  // those keys' meta words
+};
+
+// Where a slice's tiles are: wave-uniform page addresses.
+struct KvPlace {
+  const char* page[2];  // the tile's page, moved to the tile's K rows
+  int token[2];
+  bool ok[2];  // the page is in the cache (else the first page's rows are read, and masked)
+};
+
+// Lane offsets into a page, in bytes.
+struct KvLane {
+  uint32_t k, v, meta;
 };
 
 template <int D>
-__device__ __forceinline__ void load_slice(KvSlice<D>& s, const KvAttentionArgs& a, const int32_t* table, int head,
-                                           int key, int keys, int lane) {
-  const int r = lane & 15, g = lane >> 4;
+__device__ __forceinline__ KvPlace kv_place(const KvAttentionArgs& a, const int (&id)[2], int head, int key) {
+  KvPlace p;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int k0 = key + 16 * t;
-    const int id = k0 < keys ? __builtin_amdgcn_readfirstlane(table[k0 >> a.log2_block]) : -1;
-    s.ok[t] = id >= 0 && id < a.num_blocks;
-    if (!s.ok[t]) {
+    p.ok[t] = static_cast<unsigned>(id[t]) < static_cast<unsigned>(a.num_blocks);
+    p.token[t] = (key + 16 * t) & ((1 << a.log2_block) - 1);
+    p.page[t] = reinterpret_cast<const char*>(a.cache) +
+                (static_cast<size_t>(p.ok[t] ? id[t] : 0) * a.KV + head) * kv_page_bytes<D>(a.log2_block);
+  }
+  return p;
+}
+
+template <int D>
+__device__ __forceinline__ void load_keys(KvSlice<D>& s, const KvPlace& p, const KvLane& o, int log2_block) {
 #pragma unroll
-      for (int i = 0; i < D / 32; ++i) s.k[t][i] = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s.v[t][i] = s.km[t][i] = s.vm[t][i] = 0;
-      continue;
-    }
-    const uint32_t* page = reinterpret_cast<const uint32_t*>(
-        a.cache + (static_cast<size_t>(id) * a.KV + head) * kv_page_bytes<D>(a.log2_block));
-    const int token = k0 & ((1 << a.log2_block) - 1);
-    const int part = (D / 8) << a.log2_block;
-    const uint32_t* kp = page + (token + r) * (D / 8) + g * (D / 32);
-    if (D == 128) {
-      const uint4 w = *reinterpret_cast<const uint4*>(kp);
-      s.k[t][0] = w.x, s.k[t][1] = w.y, s.k[t][D / 32 - 2] = w.z, s.k[t][D / 32 - 1] = w.w;
+  for (int t = 0; t < 2; ++t) {
+    const char* k = p.page[t] + p.token[t] * (D / 2);
+    if constexpr (D == 128) {
+      const uint4 w = *reinterpret_cast<const uint4*>(k + o.k);
+      s.k[t][0] = w.x, s.k[t][1] = w.y, s.k[t][2] = w.z, s.k[t][3] = w.w;
     } else {
-      const uint2 w = *reinterpret_cast<const uint2*>(kp);
+      const uint2 w = *reinterpret_cast<const uint2*>(k + o.k);
       s.k[t][0] = w.x, s.k[t][1] = w.y;
     }
-    const uint4 v = *reinterpret_cast<const uint4*>(page + part + kv_v_word<D>(token + 4 * g, r % (D / 8)));
-    s.v[t][0] = v.x, s.v[t][1] = v.y, s.v[t][2] = v.z, s.v[t][3] = v.w;
-    const uint4 km = *reinterpret_cast<const uint4*>(page + 2 * part + token + 4 * g);
-    s.km[t][0] = km.x, s.km[t][1] = km.y, s.km[t][2] = km.z, s.km[t][3] = km.w;
-    const uint4 vm = *reinterpret_cast<const uint4*>(page + 2 * part + (1 << a.log2_block) + token + 4 * g);
-    s.vm[t][0] = vm.x, s.vm[t][1] = vm.y, s.vm[t][2] = vm.z, s.vm[t][3] = vm.w;
+    const char* m = p.page[t] + (D << log2_block) + p.token[t] * 4;
+    const uint4 w = *reinterpret_cast<const uint4*>(m + o.meta);
+    s.km[t][0] = w.x, s.km[t][1] = w.y, s.km[t][2] = w.z, s.km[t][3] = w.w;
   }
+}
+
+template <int D>
+__device__ __forceinline__ void load_values(KvSlice<D>& s, const KvPlace& p, const KvLane& o, int log2_block) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const char* v = p.page[t] + ((D / 2) << log2_block) + p.token[t] * (D / 2);
+    const uint4 w = *reinterpret_cast<const uint4*>(v + o.v);
+    s.v[t][0] = w.x, s.v[t][1] = w.y, s.v[t][2] = w.z, s.v[t][3] = w.w;
+    const char* m = p.page[t] + ((D + 4) << log2_block) + p.token[t] * 4;
+    const uint4 x = *reinterpret_cast<const uint4*>(m + o.meta);
+    s.vm[t][0] = x.x, s.vm[t][1] = x.y, s.vm[t][2] = x.z, s.vm[t][3] = x.w;
+  }
+}
+
+// The page ids of the tiles at key and key + 16; keys behind the last one repeat its page.
+__device__ __forceinline__ void kv_ids(int (&id)[2], const int32_t* __restrict__ table, int key, int last, int log2_block) {
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+    id[t] = __builtin_amdgcn_readfirstlane(table[min(key + 16 * t, last) >> log2_block]);
 }
 
 // Split attention.  A row tile is up to 16 MT rows (tokens x heads of the group) of one request
@@ -130,45 +180,34 @@ __device__ __forceinline__ void load_slice(KvSlice<D>& s, const KvAttentionArgs&
 // alike; a share that covers a tile's keys only in part leaves a partial result, joined in a
 // fixed order by kv_combine_kernel.  Inside a unit each of the 4 waves takes 32 keys and keeps
 // its own running maximum and sum; the waves are joined through LDS at the end of a tile.
+//
+// The next slice's keys are loaded into the registers that the scores have just consumed, and
+// its values into those that the second product has, so a wave has loads in flight throughout
+// without a second set of registers, and three waves fit a SIMD (MT = 1; two with MT = 2).  A
+// fourth would cost spills inside the loop: 128 sequences of up to 8192 keys took 255 us with
+// four, 149 us with three.
 template <int D, int MT>
-__global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {
+__global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {
   constexpr int kRows = 16 * MT, kSteps = D / 32, kTiles = D / 16, kPitch = D + 4;
   __shared__ __align__(16) float s_out[kWaves][kRows][kPitch];
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
-  __shared__ int64_t s_part[kWaves];
-  __shared__ int64_t s_base;
-  __shared__ int s_request;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int group = a.H / a.KV;
 
-  // This workgroup's share: a scan of the requests' units, and the request where it begins.
-  const int per = (a.R + kThreads - 1) / kThreads;
-  const int r0 = tid * per, r1 = min(a.R, r0 + per);
-  int64_t mine = 0;
-  for (int r = r0; r < r1; ++r) mine += kv_units(a, kv_request(a, r), kRows);
-  int64_t upto = mine;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t u = __shfl_up(upto, d);
-    if (lane >= d) upto += u;
-  }
-  if (lane == 63) s_part[wave] = upto;
-  __syncthreads();
-  int64_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) upto += s_part[w];
-    total += s_part[w];
-  }
-  const int64_t workers = total < gridDim.x ? total : gridDim.x;
-  const int64_t me = blockIdx.x;
-  KvSplit* split = out.split + blockIdx.x;
+  // This workgroup's share.  Every wave sums the requests' units (64 requests at a time, a lane
+  // each), then scans them to the request where the share begins.
+  int sum = 0;
+  for (int r = lane; r < a.R; r += 64) sum += kv_units<kRows>(a, kv_request(a, r), group);
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int workers = min(total, static_cast<int>(gridDim.x));
+  const int me = blockIdx.x;
+  KvSplit* split = out.split + me;
 
   if (a.zero_tail) {
     const int end = min(max(a.cu_query_lens[a.R], 0), a.T);
     const int chunks = a.H * D / 8;
-    for (int row = end + blockIdx.x; row < a.T; row += gridDim.x)
+    for (int row = end + me; row < a.T; row += gridDim.x)
       for (int c = tid; c < chunks; c += kThreads)
         reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
   }
@@ -176,43 +215,56 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
     if (tid == 0) split->count = 0;
     return;
   }
-  const int64_t begin = total * me / workers, end = total * (me + 1) / workers;
-  if (begin >= upto - mine && begin < upto) {
-    int64_t base = upto - mine;
-    int r = r0;
-    for (;; ++r) {
-      const int64_t u = kv_units(a, kv_request(a, r), kRows);
-      if (begin < base + u) break;
-      base += u;
+  const KvShares shares{total / workers, total % workers};
+  const int begin = shares.begin(me), end = shares.begin(me + 1);
+  int r = 0, base = 0;  // the share's first request, and the units before it
+  for (;; r += 64) {
+    const int units = r + lane < a.R ? kv_units<kRows>(a, kv_request(a, r + lane), group) : 0;
+    const int upto = wave_scan(units);
+    const uint64_t past = __ballot(base + upto > begin);
+    if (past || r + 64 >= a.R) {
+      const int first = past ? __builtin_ctzll(past) : 0;
+      base += __builtin_amdgcn_readlane(upto - units, first);
+      r += first;
+      break;
     }
-    s_base = base;
-    s_request = r;
+    base += __builtin_amdgcn_readlane(upto, 63);
   }
-  __syncthreads();
-  int r = __builtin_amdgcn_readfirstlane(s_request);
-  int64_t base = s_base;
   KvRequest q = kv_request(a, r);
-  int64_t units = kv_units(a, q, kRows);
+  int units = kv_units<kRows>(a, q, group);
   bool left = false;  // whether this workgroup left the first part of a tile
 
   const NibbleConsts nc = nibble_consts();
   const int col = lane & 15, g = lane >> 4;
   const float scale = a.scale_log2e;
+  const KvLane offset{static_cast<uint32_t>(col * (D / 2) + g * (D / 8)),
+                      static_cast<uint32_t>((g * (D / 8) + col % (D / 8)) * 16), static_cast<uint32_t>(g * 16)};
 
-  for (int64_t u = begin; u < end;) {
+  for (int u = begin; u < end;) {
     while (u >= base + units) {
       base += units;
       q = kv_request(a, ++r);
-      units = kv_units(a, q, kRows);
+      units = kv_units<kRows>(a, q, group);
     }
-    const int tiles = ceil_div(q.n * group, kRows);
-    const int span = max(ceil_div(q.keys, kUnit), 1);
-    const int64_t local = u - base;
-    const int seg = static_cast<int>(local / span), k0 = static_cast<int>(local - static_cast<int64_t>(seg) * span);
+    const int tiles = (q.n * group + kRows - 1) / kRows, span = kv_span(q);
+    const int seg = (u - base) / span, k0 = u - base - seg * span;
     const int head = seg / tiles, tile = seg - head * tiles;
-    const int n = static_cast<int>(min(static_cast<int64_t>(span - k0), end - u));
+    const int n = min(span - k0, end - u);
     const int row0 = tile * kRows, rows = min(kRows, q.n * group - row0);
     const int32_t* table = a.tables + static_cast<int64_t>(r) * a.table_stride;
+
+    const int key_end = min((k0 + n) * kUnit, q.keys);
+    int key = k0 * kUnit + 32 * wave;
+    KvSlice<D> s;
+    KvPlace place;
+    int id[2];
+    if (key < key_end) {
+      kv_ids(id, table, key, key_end - 1, a.log2_block);
+      place = kv_place<D>(a, id, head, key);
+      load_keys<D>(s, place, offset, a.log2_block);
+      load_values<D>(s, place, offset, a.log2_block);
+      if (key + kUnit < key_end) kv_ids(id, table, key + kUnit, key_end - 1, a.log2_block);
+    }
 
     // The queries as the second operand: column = row of the tile, channels as K's words have them.
     bf16x8_t qf[MT][kSteps];
@@ -224,20 +276,20 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
       const int row = row0 + 16 * m + col;
       const int token = row / group, h = head * group + row - token * group;
       const bool live = 16 * m + col < rows;
-      float sum = 0.0f;
+      float total_q = 0.0f;
 #pragma unroll
-      for (int s = 0; s < kSteps; ++s) {
+      for (int i = 0; i < kSteps; ++i) {
         uint4 w = make_uint4(0, 0, 0, 0);
         if (live)
           w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + h * a.q_stride_h + (D / 4) * g +
-                                              8 * s);
+                                              8 * i);
         float f[8];
         unpack_bf16x8(w, f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += f[i];
-        qf[m][s] = __builtin_bit_cast(bf16x8_t, w);
+        for (int j = 0; j < 8; ++j) total_q += f[j];
+        qf[m][i] = __builtin_bit_cast(bf16x8_t, w);
       }
-      neg_sum[m] = -column_sum(sum);
+      neg_sum[m] = -column_sum(total_q);
       const bool tree = a.tree_mask != nullptr;
       bits[m] = tree && live ? a.tree_mask[q.row + token] : 0;
       sees[m] = live ? min(tree ? q.cached : q.cached + token + 1, q.keys) : 0;
@@ -255,13 +307,10 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
       row_sum[m] = 0.0f;
     }
 
-    const int key_end = min((k0 + n) * kUnit, q.keys);
-    KvSlice<D> now;
-    int key = k0 * kUnit + 32 * wave;
-    if (key < key_end) load_slice<D>(now, a, table, head, key, key_end, lane);
     for (; key < key_end; key += kUnit) {
-      KvSlice<D> ahead;
-      if (key + kUnit < key_end) load_slice<D>(ahead, a, table, head, key + kUnit, key_end, lane);
+      const bool more = key + kUnit < key_end;
+      const bool whole = key + 32 <= all_see && place.ok[0] && place.ok[1];
+      const bool ok[2] = {place.ok[0], place.ok[1]};
 
       f32x4_t sc[MT][2];
 #pragma unroll
@@ -269,60 +318,68 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[m][t][i] = kv_meta_zero128(now.km[t][i]) * neg_sum[m];
+          for (int i = 0; i < 4; ++i) sc[m][t][i] = kv_meta_zero128(s.km[t][i]) * neg_sum[m];
 #pragma unroll
-        for (int s = 0; s < kSteps; ++s) {
-          const bf16x8_t kf = unpack_codes(now.k[t][s], nc);
+        for (int i = 0; i < kSteps; ++i) {
+          const bf16x8_t kf = unpack_codes(s.k[t][i], nc);
 #pragma unroll
-          for (int m = 0; m < MT; ++m) sc[m][t] = mfma16(kf, qf[m][s], sc[m][t]);
+          for (int m = 0; m < MT; ++m) sc[m][t] = mfma16(kf, qf[m][i], sc[m][t]);
         }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[m][t][i] *= kv_meta_scale(now.km[t][i]);
+          for (int i = 0; i < 4; ++i) sc[m][t][i] *= kv_meta_scale(s.km[t][i]);
+      }
+      if (more) {
+        place = kv_place<D>(a, id, head, key + kUnit);
+        load_keys<D>(s, place, offset, a.log2_block);
+        if (key + 2 * kUnit < key_end) kv_ids(id, table, key + 2 * kUnit, key_end - 1, a.log2_block);
       }
 
-      const bool whole = key + 32 <= all_see && now.ok[0] && now.ok[1];
-      u32x4_t zf;  // the keys' 128 + z as the first operand of the offset tile
-      bf16x8_t pf[MT];
-      bool grew = false;
-      float top[MT];
-      uint32_t seen[MT];
+      float vs[MT][2][4];  // the values' scales as the rows see them
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) vs[m][t][i] = kv_meta_scale(s.vm[t][i]);
       if (!whole) {
         // A lane's keys are 16 t + 4 g + i.  Keys outside the sequence, or on no page, hold
         // anything: their score becomes -inf, their scale 0 and their zero point 0.  Keys that
         // only this row does not see keep their zero point (the offset tile's operand serves
         // all rows), and their scale is taken as 0 for this row.
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          seen[m] = 0;
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int k = key + 16 * t + 4 * g + i;
-              const unsigned fresh = static_cast<unsigned>(k - q.cached);
-              const bool visible = now.ok[t] && k < q.keys &&
-                                   (k < sees[m] || (fresh < 64u && ((bits[m] >> fresh) & 1)));
-              if (visible) seen[m] |= 1u << (4 * t + i);
-              else sc[m][t][i] = -INFINITY;
-            }
-        }
-#pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (!now.ok[t] || key + 16 * t + 4 * g + i >= q.keys) now.vm[t][i] = 0x00004300u, now.v[t][i] = 0;
+          for (int i = 0; i < 4; ++i) {
+            const int k = key + 16 * t + 4 * g + i;
+            // selections, not branches, one scalar at a time
+            const bool held = ok[t] & (k < q.keys);
+            const unsigned fresh = static_cast<unsigned>(k - q.cached);
+            s.vm[t][i] = held ? s.vm[t][i] : 0x00004300u;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+              const uint32_t word = fresh & 32u ? static_cast<uint32_t>(bits[m] >> 32) : static_cast<uint32_t>(bits[m]);
+              const uint32_t named = fresh < 64u ? word >> (fresh & 31u) : 0u;
+              const bool visible = held & ((k < sees[m]) | ((named & 1u) != 0));
+              const float x = sc[m][t][i];
+              sc[m][t][i] = visible ? x : -INFINITY;
+              vs[m][t][i] = visible ? vs[m][t][i] : 0.0f;
+            }
+          }
       }
+      u32x4_t zf;  // the keys' 128 + z as the first operand of the offset tile
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-          zf[2 * t + i] = __builtin_amdgcn_perm(now.vm[t][2 * i + 1], now.vm[t][2 * i], 0x05040100u);
+          zf[2 * t + i] = __builtin_amdgcn_perm(s.vm[t][2 * i + 1], s.vm[t][2 * i], 0x05040100u);
+      bool grew = false;
+      float top[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
-        float mx = fmaxf(fmaxf(fmaxf(sc[m][0][0], sc[m][0][1]), fmaxf(sc[m][0][2], sc[m][0][3])),
-                         fmaxf(fmaxf(sc[m][1][0], sc[m][1][1]), fmaxf(sc[m][1][2], sc[m][1][3])));
+        const float mx = fmaxf(fmaxf(fmaxf(sc[m][0][0], sc[m][0][1]), fmaxf(sc[m][0][2], sc[m][0][3])),
+                               fmaxf(fmaxf(sc[m][1][0], sc[m][1][1]), fmaxf(sc[m][1][2], sc[m][1][3])));
         top[m] = fmaxf(row_max[m], column_max(mx));
         grew |= top[m] > row_max[m];
       }
@@ -341,6 +398,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
           for (int i = 0; i < 4; ++i) acc_z[m][i] *= f;
         }
       }
+      bf16x8_t pf[MT];
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         const float ref = (row_max[m] == -INFINITY ? 0.0f : row_max[m]) * scale;
@@ -352,9 +410,7 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
           for (int i = 0; i < 4; ++i) {
             p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][t][i], scale, -ref));
             row_sum[m] += p[i];
-            float s = kv_meta_scale(now.vm[t][i]);
-            if (!whole) s = (seen[m] >> (4 * t + i)) & 1 ? s : 0.0f;
-            p[i] *= s;
+            p[i] *= vs[m][t][i];
           }
           w[2 * t] = pack_bf16x2(p[0], p[1]);
           w[2 * t + 1] = pack_bf16x2(p[2], p[3]);
@@ -369,14 +425,12 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
 #pragma unroll
       for (int half = 0; half < (D == 128 ? 2 : 1); ++half) {
         uint32_t pair[4];
+        const uint32_t select = (D == 128 ? half != 0 : (col & 8) != 0) ? 0x07060302u : 0x05040100u;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            uint32_t select = half ? 0x07060302u : 0x05040100u;
-            if (D == 64) select = col & 8 ? 0x07060302u : 0x05040100u;
-            pair[2 * t + i] = __builtin_amdgcn_perm(now.v[t][2 * i + 1], now.v[t][2 * i], select);
-          }
+          for (int i = 0; i < 2; ++i)
+            pair[2 * t + i] = __builtin_amdgcn_perm(s.v[t][2 * i + 1], s.v[t][2 * i], select);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           u32x4_t f;
@@ -388,22 +442,22 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
             acc_o[m][ch] = mfma16(__builtin_bit_cast(bf16x8_t, f), pf[m], acc_o[m][ch]);
         }
       }
-      now = ahead;
+      if (more) load_values<D>(s, place, offset, a.log2_block);
     }
 
     // Join the waves.  Accumulator register i of a lane is operand row 4 g + i: the word (D =
     // 128) or word and half (D = 64) whose channels the tiles c count.
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
-      const float sum = column_sum(row_sum[m]);
+      const float row_total = column_sum(row_sum[m]);
       if (g == 0) {
         s_max[wave][16 * m + col] = row_max[m];
-        s_sum[wave][16 * m + col] = sum;
+        s_sum[wave][16 * m + col] = row_total;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float* o = s_out[wave][16 * m + col];
-        if (D == 128) {
+        if constexpr (D == 128) {
 #pragma unroll
           for (int c = 0; c < 8; c += 4) {
             const f32x4_t v = {acc_o[m][c][i] - acc_z[m][i], acc_o[m][c + 1][i] - acc_z[m][i],
@@ -420,47 +474,43 @@ __global__ __launch_bounds__(kThreads) void kv_attention_kernel(KvAttentionArgs 
     __syncthreads();
     const bool complete = k0 == 0 && n == span;
     // A partial result's slot: 2 w for a tile begun before this share, 2 w + 1 for one begun in it.
-    const int slot = 2 * blockIdx.x + (k0 == 0);
+    const int slot = 2 * me + (k0 == 0);
     constexpr int kChunks = D / 8;
     for (int e = tid; e < rows * kChunks; e += kThreads) {
       const int row = e / kChunks, ch = e % kChunks * 8;
-      float top = s_max[0][row];
+      float high = s_max[0][row];
 #pragma unroll
-      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, s_max[w][row]);
-      const float ref = top == -INFINITY ? 0.0f : top;
-      float sum = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      for (int w = 1; w < kWaves; ++w) high = fmaxf(high, s_max[w][row]);
+      const float ref = high == -INFINITY ? 0.0f : high;
+      float all = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f((s_max[w][row] - ref) * scale);
-        sum += f * s_sum[w][row];
+        all += f * s_sum[w][row];
 #pragma unroll
         for (int i = 0; i < 8; ++i) o[i] += f * s_out[w][row][ch + i];
       }
       if (complete) {
         const int token = (row0 + row) / group;
-        kv_write(a, q.row + token, head * group + row0 + row - token * group, ch, sum, o);
+        kv_write(a, q.row + token, head * group + row0 + row - token * group, ch, all, o);
       } else {
         float* p = out.out + (static_cast<size_t>(slot) * kRows + row) * D + ch;
         *reinterpret_cast<f32x4_t*>(p) = f32x4_t{o[0], o[1], o[2], o[3]};
         *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{o[4], o[5], o[6], o[7]};
         if (ch == 0) {
           float* st = out.stats + (static_cast<size_t>(slot) * kRows + row) * 2;
-          st[0] = top;
-          st[1] = sum;
+          st[0] = high;
+          st[1] = all;
         }
       }
     }
     if (!complete && k0 == 0) {
-      // This share begins the tile: the workgroup with unit x has number ((x + 1) workers - 1) / total.
       left = true;
-      if (tid == 0) {
-        const int64_t last = u + span - 1;
-        const int64_t owner = ((last + 1) * workers - 1) / total;
-        *split = KvSplit{r, head, tile, static_cast<int>(owner - me) + 1, slot, 2 * (static_cast<int>(me) + 1), 2, 0};
-      }
+      if (tid == 0)
+        *split = KvSplit{r, head, tile, shares.owner(u + span - 1) - me + 1, slot, 2 * (me + 1), 2, 0};
     }
     u += n;
-    __syncthreads();
+    if (u < end) __syncthreads();
   }
   if (!left && tid == 0) split->count = 0;
 }
@@ -493,7 +543,6 @@ __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a,
         sum += f * st[1];
       }
       const int n = min(64, s.count - b);
-#pragma unroll 8
       for (int j = 0; j < n; ++j) {
         const float fj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), j));
         const float* p = part.out + at(b + j) * D + lane * kPer;
@@ -519,7 +568,7 @@ KvPlan kv_plan(const KvAttentionArgs& a) {
   const int64_t tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
   const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
-  const int64_t fill = p.mt == 1 ? 1024 : 512;
+  const int64_t fill = p.mt == 1 ? 768 : 512;
   p.workers = static_cast<int>(most < fill ? most : fill);
   return p;
 }
