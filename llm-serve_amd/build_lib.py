@@ -16,7 +16,7 @@ BUILD_DIR = os.path.join(CSRC, "_build")
 LIB_NAME = "libw4a16.so"
 LIB_PATH = os.path.join(CSRC, LIB_NAME)
 SOURCES = ("w4a16_format.hip", "w4a16_quant.hip", "w4a16_decode.hip", "w4a16_tile.hip", "w4a16_norm.hip",
-           "kv4_cache.hip", "kv4_attention.hip", "w4a16_api.hip")
+           "kv4_cache.hip", "kv4_attention.hip", "kv4_prompt.hip", "w4a16_api.hip")
 ARCH = "gfx950"
 
 COMPILE_FLAGS = [

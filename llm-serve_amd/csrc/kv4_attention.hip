@@ -10,8 +10,7 @@
 // one multiplication a score, and the values' offset is one more matrix tile whose operand is
 // the meta words' low halves.  Scores, statistics and sums are fp32; the one rounding is P' to
 // bf16, the matrix instruction's operand type.
-#include "kv4_common.h"
-#include "kv4_launch.h"
+#include "kv4_attention.h"
 
 namespace w4a16 {
 namespace {
@@ -20,87 +19,14 @@ constexpr int kUnit = 128;      // keys of one work unit: 32 a wave
 constexpr int kWaves = 4;
 constexpr int kThreads = 64 * kWaves;
 
-// What a combine needs to join one row tile's partial results.
-struct KvSplit {
-  int request, head, tile;
-  int count;        // partial results (0: this entry joins nothing)
-  int first, next;  // slot of the first one, and of the second
-  int stride;       // between slots from the second on
-  int pad;
-};
-
-struct KvPartials {
-  float* out;      // [slots][rows][D], unnormalized
-  float* stats;    // [slots][rows][2]: maximum (raw score) and sum
-  KvSplit* split;  // one a worker
-};
-
-// One request as the kernels see it, all lengths safe whatever the tensors hold.
-struct KvRequest {
-  int row;     // its first packed row
-  int n;       // its packed rows
-  int cached;  // sequence length before them
-  int keys;    // keys that its block table can hold of the sequence
-};
-
-__device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r) {
-  KvRequest q;
-  const int lo = a.cu_query_lens[r], hi = a.cu_query_lens[r + 1];
-  q.row = min(max(lo, 0), a.T);
-  q.n = max(min(hi, a.T) - q.row, 0);
-  const int seq = max(a.seq_lens[r], 0);
-  q.cached = seq - (hi - lo);
-  const int64_t room = static_cast<int64_t>(a.width) << a.log2_block;
-  q.keys = seq < room ? seq : static_cast<int>(room);
-  return q;
-}
-
-__device__ __forceinline__ int ceil_div(int a, int b) { return (a + b - 1) / b; }
-
 // Units of one row tile (a tile whose rows see nothing still has its zeros to write).
 __device__ __forceinline__ int kv_span(const KvRequest& q) { return max((q.keys + kUnit - 1) / kUnit, 1); }
 
-// Units of a request.
+// Units of a request (none if the prompt kernel takes it).
 template <int ROWS>
 __device__ __forceinline__ int kv_units(const KvAttentionArgs& a, const KvRequest& q, int group) {
+  if (q.n * group > a.split_rows) return 0;
   return (q.n * group + ROWS - 1) / ROWS * a.KV * kv_span(q);
-}
-
-// Inclusive sum over the lanes up to this one: DPP moves within rows of 16, then the row totals.
-__device__ __forceinline__ int wave_scan(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row 0 -> 1, row 2 -> 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // lane 31 -> rows 2, 3
-  return v;
-}
-
-// Equal contiguous shares of `total` units for `workers` workgroups: the first `rest` take one
-// more than the others.
-struct KvShares {
-  int each, rest;
-  __device__ __forceinline__ int begin(int w) const { return w * each + min(w, rest); }
-  __device__ __forceinline__ int owner(int unit) const {
-    const int head = rest * (each + 1);
-    return unit < head ? unit / (each + 1) : rest + (unit - head) / each;
-  }
-};
-
-// out[row, h, ch ..] = o / sum, rounded; a row that saw nothing (or only scores of -inf) is zero.
-template <int N>
-__device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int h, int ch, float sum, const float (&o)[N]) {
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* p = a.out + (static_cast<size_t>(row) * a.H + h) * a.D + ch;
-  if constexpr (N == 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
-                                              pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-  } else if constexpr (N == 2) {
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(o[0] * inv, o[1] * inv);
-  } else {
-    *p = f32_to_bf16_bits(o[0] * inv);
-  }
 }
 
 // One slice of 32 keys of a wave, in registers: two 16-key tiles, each inside one page.
@@ -507,7 +433,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
     if (!complete && k0 == 0) {
       left = true;
       if (tid == 0)
-        *split = KvSplit{r, head, tile, shares.owner(u + span - 1) - me + 1, slot, 2 * (me + 1), 2, 0};
+        *split = KvSplit{r, head, tile, shares.owner(u + span - 1) - me + 1, slot, 2 * (me + 1)};
     }
     u += n;
     if (u < end) __syncthreads();
@@ -518,17 +444,19 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
 // Joins the partial results of the tile that worker blockIdx.x begins and others end, in the
 // workers' order: a wave a row, its lanes over the channels (and, for the statistics, over the
 // parts).
-template <int D, int MT>
-__global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a, KvPartials part) {
-  constexpr int kRows = 16 * MT, kPer = D / 64;
+template <int D>
+__global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a, KvPartials part, int tile_rows) {
+  constexpr int kPer = D / 64;
   const KvSplit s = part.split[blockIdx.x];
   if (s.count <= 0) return;
   const int lane = threadIdx.x & 63;
   const int group = a.H / a.KV;
   const KvRequest q = kv_request(a, s.request);
-  const int row0 = s.tile * kRows, rows = min(kRows, q.n * group - row0);
+  const int row0 = s.tile * tile_rows, rows = min(tile_rows, q.n * group - row0);
   for (int row = wave_id() + kWaves * blockIdx.y; row < rows; row += kWaves * gridDim.y) {
-    auto at = [&](int i) { return static_cast<size_t>(i == 0 ? s.first : s.next + s.stride * (i - 1)) * kRows + row; };
+    auto at = [&](int i) {
+      return static_cast<size_t>(i == 0 ? s.first : s.next + 2 * (i - 1)) * tile_rows + row;
+    };
     float top = -INFINITY;
     for (int i = lane; i < s.count; i += 64) top = fmaxf(top, part.stats[at(i) * 2]);
 #pragma unroll
@@ -556,33 +484,70 @@ __global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a,
   }
 }
 
+// Kernels and grids of a call, by sizes alone (lengths are on the device, and every choice is
+// right for any).  Requests of at most split_rows rows (tokens x heads of a group) go to the
+// split kernel, longer ones to the prompt kernel, which is launched only if the longest query
+// may be that long.
 struct KvPlan {
-  int mt;       // 16-row tiles of a workgroup
-  int workers;  // grid
+  int mt;             // split kernel: 16-row tiles of a workgroup
+  int split_workers;  // its grid
+  int split_rows;
+  int prompt_workers;  // the prompt kernel's grid (0: not launched)
 };
 
 KvPlan kv_plan(const KvAttentionArgs& a) {
   KvPlan p;
   const int64_t rows = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
-  p.mt = rows <= 16 ? 1 : 2;
-  const int64_t tiles = (rows + 16 * p.mt - 1) / (16 * p.mt);
+  const bool prompts = rows > kKvSplitMaxRows;
+  p.mt = rows <= 16 || prompts ? 1 : 2;
+  p.split_rows = prompts ? kKvMixedMaxRows : 0x7FFFFFFF;
+  const int64_t tile_rows = prompts ? kKvMixedMaxRows : rows;
+  const int64_t tiles = (tile_rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
   const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
   const int64_t fill = p.mt == 1 ? 768 : 512;
-  p.workers = static_cast<int>(most < fill ? most : fill);
+  p.split_workers = static_cast<int>(most < fill ? most : fill);
+  p.prompt_workers = prompts ? kKvPromptWorkers : 0;
   return p;
 }
 
 size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 
-template <int D, int MT>
-hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, const KvPartials& part, hipStream_t stream) {
-  kv_attention_kernel<D, MT><<<p.workers, kThreads, 0, stream>>>(a, part);
+// A kernel's part of the workspace: partial results of 2 tiles of `rows` rows a worker.
+size_t partials_bytes(int workers, int rows, int D) {
+  const size_t n = static_cast<size_t>(2) * workers * rows;
+  return align256(n * D * sizeof(float)) + align256(n * 2 * sizeof(float)) + align256(workers * sizeof(KvSplit));
+}
+
+KvPartials partials_at(char* ws, int workers, int rows, int D) {
+  const size_t n = static_cast<size_t>(2) * workers * rows;
+  KvPartials part;
+  part.out = reinterpret_cast<float*>(ws);
+  ws += align256(n * D * sizeof(float));
+  part.stats = reinterpret_cast<float*>(ws);
+  ws += align256(n * 2 * sizeof(float));
+  part.split = reinterpret_cast<KvSplit*>(ws);
+  return part;
+}
+
+template <int D>
+hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, hipStream_t stream) {
+  const int rows = 16 * p.mt;
+  const KvPartials split = partials_at(ws, p.split_workers, rows, D);
+  if (p.mt == 1)
+    kv_attention_kernel<D, 1><<<p.split_workers, kThreads, 0, stream>>>(a, split);
+  else
+    kv_attention_kernel<D, 2><<<p.split_workers, kThreads, 0, stream>>>(a, split);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  const int64_t rows = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
-  const int y = static_cast<int>(((rows < 16 * MT ? rows : 16 * MT) + kWaves - 1) / kWaves);
-  kv_combine_kernel<D, MT><<<dim3(p.workers, y > 0 ? y : 1), kThreads, 0, stream>>>(a, part);
+  const int64_t most = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
+  const int y = static_cast<int>(((most < rows ? most : rows) + kWaves - 1) / kWaves);
+  kv_combine_kernel<D><<<dim3(p.split_workers, y > 0 ? y : 1), kThreads, 0, stream>>>(a, split, rows);
+  if ((e = hipGetLastError()) != hipSuccess || p.prompt_workers == 0) return e;
+  const KvPartials prompt =
+      partials_at(ws + partials_bytes(p.split_workers, rows, D), p.prompt_workers, kKvPromptRows, D);
+  if ((e = launch_kv_prompt(a, prompt, p.prompt_workers, stream)) != hipSuccess) return e;
+  kv_combine_kernel<D><<<dim3(p.prompt_workers, kKvPromptRows / kWaves), kThreads, 0, stream>>>(a, prompt, kKvPromptRows);
   return hipGetLastError();
 }
 
@@ -590,23 +555,16 @@ hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, const KvPartials& p
 
 size_t kv_attention_workspace(const KvAttentionArgs& a) {
   const KvPlan p = kv_plan(a);
-  const size_t rows = static_cast<size_t>(2) * p.workers * 16 * p.mt;
-  return align256(rows * a.D * sizeof(float)) + align256(rows * 2 * sizeof(float)) +
-         align256(p.workers * sizeof(KvSplit));
+  return partials_bytes(p.split_workers, 16 * p.mt, a.D) +
+         (p.prompt_workers ? partials_bytes(p.prompt_workers, kKvPromptRows, a.D) : 0);
 }
 
-hipError_t launch_kv_attention(const KvAttentionArgs& a, void* workspace, hipStream_t stream) {
-  const KvPlan p = kv_plan(a);
-  const size_t rows = static_cast<size_t>(2) * p.workers * 16 * p.mt;
+hipError_t launch_kv_attention(const KvAttentionArgs& args, void* workspace, hipStream_t stream) {
+  const KvPlan p = kv_plan(args);
+  KvAttentionArgs a = args;
+  a.split_rows = p.split_rows;
   char* ws = static_cast<char*>(workspace);
-  KvPartials part;
-  part.out = reinterpret_cast<float*>(ws);
-  ws += align256(rows * a.D * sizeof(float));
-  part.stats = reinterpret_cast<float*>(ws);
-  ws += align256(rows * 2 * sizeof(float));
-  part.split = reinterpret_cast<KvSplit*>(ws);
-  if (a.D == 64) return p.mt == 1 ? launch<64, 1>(a, p, part, stream) : launch<64, 2>(a, p, part, stream);
-  return p.mt == 1 ? launch<128, 1>(a, p, part, stream) : launch<128, 2>(a, p, part, stream);
+  return a.D == 64 ? launch<64>(a, p, ws, stream) : launch<128>(a, p, ws, stream);
 }
 
 }  // namespace w4a16

@@ -52,6 +52,7 @@ struct KvAttentionArgs {
   float scale_log2e;
   int T, R, H, KV, D, num_blocks, log2_block, width;
   int max_query_len;
+  int split_rows;  // requests of more rows (tokens x heads of a group) are the prompt kernel's
   bool zero_tail;
 };
 size_t kv_attention_workspace(const KvAttentionArgs& a);

@@ -1,0 +1,418 @@
+// Attention of long queries over the 4-bit paged cache: prompts, and chunks of them.
+//
+// The same mathematics as kv4_attention.hip in the shape of a matrix kernel.  A workgroup takes
+// 256 rows (tokens x heads of a kv head's group) of a request, 32 a wave, and walks their keys in
+// tiles of 64.  Eight waves would each have to unpack the same codes, and unpacking costs more
+// vector instructions than the softmax, so a tile is dequantized once for all of them: the first
+// four waves turn the K codes of the next tile into bf16 rows in LDS while the other four turn
+// the V codes into bf16 columns, into the buffer that is not being read.  Keys and values are
+// therefore bf16(s (c - z)) here, the values that kv_load_kernel returns.
+//
+// Scores are formed transposed, S^T = K Q^T, so that a lane holds 16 keys' scores of one row in
+// the accumulator layout, and P^T is the second product's operand as it stands: its 16 contraction
+// slots 8 h + j of a lane half h are the keys 16 s + 4 h + j (j < 4) and 16 s + 8 + 4 h + j - 4,
+// and V's columns are written in that order.  The output is O^T = V^T P^T: every statistic of a
+// row sits in the two lanes that hold it.
+#include "kv4_attention.h"
+
+namespace w4a16 {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int kPromptThreads = 512;
+constexpr int kKeys = 64;      // keys of a tile
+constexpr int kTileCost = 16;  // cost units of a tile of keys
+constexpr int kMinShare = 4 * kTileCost;
+
+__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+__device__ __forceinline__ int64_t wave_scan64(int64_t v, int lane) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t u = __shfl_up(v, d);
+    if (lane >= d) v += u;
+  }
+  return v;
+}
+
+// Cost of a request's row tiles in sixteenths of a key tile: tile j of a head costs first +
+// step j, its keys growing with its last token (all keys under a tree mask), plus one key tile
+// for its own set-up.
+struct KvTileCosts {
+  int tiles;
+  int64_t first, step;
+  __device__ __forceinline__ int64_t before(int j) const { return j * first + step * j * (j - 1) / 2; }
+  __device__ __forceinline__ int64_t of(int j) const { return first + step * j; }
+};
+
+__device__ __forceinline__ KvTileCosts kv_costs(const KvAttentionArgs& a, const KvRequest& q, int group) {
+  KvTileCosts c;
+  const int rows = q.n * group;
+  c.tiles = rows > a.split_rows ? (rows + kKvPromptRows - 1) / kKvPromptRows : 0;
+  c.step = a.tree_mask ? 0 : (kKvPromptRows / 4 + group - 1) / group;
+  c.first = (a.tree_mask ? q.keys : max(q.cached, 0)) / (kKeys / kTileCost) + c.step + kTileCost;
+  return c;
+}
+
+__device__ __forceinline__ int64_t kv_request_cost(const KvAttentionArgs& a, const KvRequest& q, int group) {
+  const KvTileCosts c = kv_costs(a, q, group);
+  return c.before(c.tiles) * a.KV;
+}
+
+// Share w of `total` cost units.
+__device__ __forceinline__ int64_t share(int64_t total, int workers, int w) { return total * w / workers; }
+
+// Byte b of the shifted word holds nibble 2 b + odd of a code word: its channel.
+__device__ __forceinline__ constexpr int byte_channel(int b, int odd) { return (b == 0 ? 0 : b == 1 ? 4 : b == 2 ? 1 : 5) + 2 * odd; }
+
+template <int B>
+__device__ __forceinline__ float byte_f32(uint32_t w) {
+  return static_cast<float>((w >> (8 * B)) & 0xFFu);  // v_cvt_f32_ubyteB
+}
+
+template <int D>
+__global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentionArgs a, KvPartials out) {
+  constexpr int kPitchK = D + 8, kPitchV = kKeys + 8;  // bf16 elements; 16-byte reads of 16 lanes meet all banks
+  constexpr int kSteps = D / 16, kTiles = D / 32;
+  __shared__ __align__(16) uint16_t s_k[2][kKeys][kPitchK];
+  __shared__ __align__(16) uint16_t s_v[2][D][kPitchV];
+  __shared__ uint64_t s_held[2][4];  // 4 bits a key: whether it is in the sequence and on a page
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int group = a.H / a.KV;
+  // Workers of one XCD (workgroups go to the 8 XCDs in turn) take neighbouring shares, mostly of
+  // the same kv heads, whose pages then stay in that XCD's L2.
+  const int per_xcd = gridDim.x / 8;
+  const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
+  KvSplit* split = out.split + me;
+
+  int64_t sum = 0;
+  for (int r = lane; r < a.R; r += 64) sum += kv_request_cost(a, kv_request(a, r), group);
+  const int64_t total = __shfl(wave_scan64(sum, lane), 63);
+  const int64_t fit = (total + kMinShare - 1) / kMinShare;
+  const int workers = fit < gridDim.x ? static_cast<int>(fit) : gridDim.x;
+  if (me >= workers) {
+    if (tid == 0) split->count = 0;
+    return;
+  }
+  const int64_t begin = share(total, workers, me), end = share(total, workers, me + 1);
+  int r = 0;
+  int64_t base = 0;
+  for (;; r += 64) {
+    const int64_t cost = r + lane < a.R ? kv_request_cost(a, kv_request(a, r + lane), group) : 0;
+    const int64_t upto = wave_scan64(cost, lane);
+    const uint64_t past = __ballot(base + upto > begin);
+    if (past || r + 64 >= a.R) {
+      const int first = past ? __builtin_ctzll(past) : 0;
+      base += __shfl(upto - cost, first);
+      r += first;
+      break;
+    }
+    base += __shfl(upto, 63);
+  }
+  r = __builtin_amdgcn_readfirstlane(r);
+  KvRequest q = kv_request(a, r);
+  bool left = false;
+
+  const int col = lane & 31, h = lane >> 5;
+  const float scale = a.scale_log2e;
+
+  for (int64_t u = begin; u < end;) {
+    KvTileCosts costs = kv_costs(a, q, group);
+    while (u >= base + costs.before(costs.tiles) * a.KV) {
+      base += costs.before(costs.tiles) * a.KV;
+      q = kv_request(a, ++r);
+      costs = kv_costs(a, q, group);
+    }
+    const int64_t a_head = costs.before(costs.tiles);
+    const int head = static_cast<int>((u - base) / a_head);
+    const int64_t x = u - base - head * a_head;
+    int tile = 0, over = costs.tiles;  // the last tile that begins at or before x
+    while (over - tile > 1) {
+      const int mid = (tile + over) >> 1;
+      if (costs.before(mid) <= x) tile = mid; else over = mid;
+    }
+    const int64_t cost = costs.of(tile), x0 = x - costs.before(tile);
+    const int64_t x1 = min(cost, x0 + end - u);
+    const int row0 = tile * kKvPromptRows, rows = min(kKvPromptRows, q.n * group - row0);
+    const int key_end = a.tree_mask ? q.keys : max(min(q.cached + (row0 + rows - 1) / group + 1, q.keys), 0);
+    const int key_tiles = (key_end + kKeys - 1) / kKeys;
+    // The share's part of the tile's keys, in proportion to the cost.
+    const int t0 = static_cast<int>(x0 * key_tiles / cost), t1 = static_cast<int>(x1 * key_tiles / cost);
+    const bool complete = x0 == 0 && x1 == cost;
+    const int32_t* table = a.tables + static_cast<int64_t>(r) * a.table_stride;
+
+    // This thread's part of a key tile.  K (waves 0 .. 3): D / 4 channels of one key.  V (waves 4
+    // .. 7): D / 32 channels of the 8 keys of one lane half and contraction step, two quads.
+    const bool converts_v = wave >= 4;
+    const int t = tid & 255;
+    const int chunk = t & 3;                       // K: channels (D / 4) chunk ..
+    const int vgroup = t & 7, word = (t >> 3) & (D / 8 - 1), part = t / D;  // V: keys, word, bytes of it
+    const int quad = 4 * (vgroup >> 1) + (vgroup & 1);
+    const int my_key = converts_v ? 4 * quad : t >> 2;
+    const int last_key = max(key_end - 1, 0);
+    int id = 0;
+    uint32_t raw[8], meta[8];
+    bool held = false;
+    auto fetch_id = [&](int key_tile) { id = table[min(key_tile * kKeys + my_key, last_key) >> a.log2_block]; };
+    auto fetch = [&](int key_tile) {
+      const int key = key_tile * kKeys + my_key;
+      const bool page_ok = static_cast<unsigned>(id) < static_cast<unsigned>(a.num_blocks);
+      const char* page = reinterpret_cast<const char*>(a.cache) +
+                         (static_cast<size_t>(page_ok ? id : 0) * a.KV + head) * kv_page_bytes<D>(a.log2_block);
+      const int token = key & ((1 << a.log2_block) - 1);
+      held = page_ok;
+      if (converts_v) {
+        const char* v = page + ((D / 2) << a.log2_block) + token * (D / 2) + word * 16;
+        const char* m = page + ((D + 4) << a.log2_block) + token * 4;
+        const uint4 v0 = *reinterpret_cast<const uint4*>(v), v1 = *reinterpret_cast<const uint4*>(v + 4 * D);
+        const uint4 m0 = *reinterpret_cast<const uint4*>(m), m1 = *reinterpret_cast<const uint4*>(m + 32);
+        raw[0] = v0.x, raw[1] = v0.y, raw[2] = v0.z, raw[3] = v0.w;
+        raw[4] = v1.x, raw[5] = v1.y, raw[6] = v1.z, raw[7] = v1.w;
+        meta[0] = m0.x, meta[1] = m0.y, meta[2] = m0.z, meta[3] = m0.w;
+        meta[4] = m1.x, meta[5] = m1.y, meta[6] = m1.z, meta[7] = m1.w;
+      } else {
+        const char* k = page + token * (D / 2) + chunk * (D / 8);
+        if constexpr (D == 128) {
+          const uint4 w = *reinterpret_cast<const uint4*>(k);
+          raw[0] = w.x, raw[1] = w.y, raw[2] = w.z, raw[3] = w.w;
+        } else {
+          const uint2 w = *reinterpret_cast<const uint2*>(k);
+          raw[0] = w.x, raw[1] = w.y;
+        }
+        const char* m = page + (D << a.log2_block) + token * 4;
+        meta[0] = *reinterpret_cast<const uint32_t*>(m);
+        meta[1] = *reinterpret_cast<const uint32_t*>(m + (4 << a.log2_block));
+      }
+    };
+    // Fetched codes -> bf16(s (c - z)) in LDS.  Keys outside the sequence or on no page become
+    // zeros (they hold anything) and are masked by s_held.  A key whose value row is NaN would
+    // reach rows that do not see it (0 * NaN in the second product): its values become zeros and
+    // its scores NaN, which masks hide from those rows, and which make every row that sees it NaN.
+    auto convert = [&](int key_tile, int buf) {
+      const int key = key_tile * kKeys + my_key;
+      if (converts_v) {
+        float s[8], zs[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int k = key + (i < 4 ? i : i + 4);
+          const float scale_v = kv_meta_scale(meta[i]);
+          const bool use = held & (k < q.keys) & (fabsf(scale_v) < INFINITY);
+          s[i] = use ? scale_v : 0.0f;
+          zs[i] = use ? -scale_v * (kv_meta_zero128(meta[i]) - 128.0f) : 0.0f;
+        }
+        // bytes of the word: four nibbles (D = 128, a thread takes 4 channels) or two (D = 64)
+        const int odd = part & 1, shift = 4 * odd + (D == 64 ? 16 * (part >> 1) : 0);
+#pragma unroll
+        for (int b = 0; b < D / 32; ++b) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = (raw[2 * i] >> shift) & 0x0F0F0F0Fu, hi = (raw[2 * i + 1] >> shift) & 0x0F0F0F0Fu;
+            const float f0 = static_cast<float>((lo >> (8 * b)) & 0xFFu), f1 = static_cast<float>((hi >> (8 * b)) & 0xFFu);
+            w[i] = pack_bf16x2(__builtin_fmaf(f0, s[2 * i], zs[2 * i]), __builtin_fmaf(f1, s[2 * i + 1], zs[2 * i + 1]));
+          }
+          const int ch = 8 * word + (D == 64 ? byte_channel(b, 0) + 2 * odd + (part >> 1) : byte_channel(b, 0) + 2 * odd);
+          *reinterpret_cast<uint4*>(&s_v[buf][ch][8 * vgroup]) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      } else {
+        const bool use = held & (key < q.keys);
+        const uint64_t all = __ballot(use);
+        if (lane == 0) s_held[buf][wave] = all;
+        const float value_scale = kv_meta_scale(meta[1]);
+        const float s = use ? (fabsf(value_scale) < INFINITY ? kv_meta_scale(meta[0]) : __builtin_nanf("")) : 0.0f;
+        const float zs = use ? -s * (kv_meta_zero128(meta[0]) - 128.0f) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+          float f[8];
+#pragma unroll
+          for (int odd = 0; odd < 2; ++odd) {
+            const uint32_t w = (raw[i] >> (4 * odd)) & 0x0F0F0F0Fu;
+            f[byte_channel(0, odd)] = __builtin_fmaf(byte_f32<0>(w), s, zs);
+            f[byte_channel(1, odd)] = __builtin_fmaf(byte_f32<1>(w), s, zs);
+            f[byte_channel(2, odd)] = __builtin_fmaf(byte_f32<2>(w), s, zs);
+            f[byte_channel(3, odd)] = __builtin_fmaf(byte_f32<3>(w), s, zs);
+          }
+          *reinterpret_cast<uint4*>(&s_k[buf][t >> 2][(D / 4) * chunk + 8 * i]) = pack_bf16x8(f);
+        }
+      }
+    };
+
+    if (t0 < t1) {
+      fetch_id(t0);
+      fetch(t0);
+      fetch_id(min(t0 + 1, t1 - 1));
+    }
+
+    // The wave's 32 rows: queries as the second operand, and what they see.
+    const int first_row = row0 + 32 * wave;
+    const int row = first_row + col;
+    const int token = row / group, qh = head * group + row - token * group;
+    const bool live = 32 * wave + col < rows;
+    bf16x8_t qf[kSteps];
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (live)
+        w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + qh * a.q_stride_h + 16 * i + 8 * h);
+      qf[i] = __builtin_bit_cast(bf16x8_t, w);
+    }
+    const bool tree = a.tree_mask != nullptr;
+    const uint64_t bits = tree && live ? a.tree_mask[q.row + token] : 0;
+    const int sees = live ? min(tree ? q.cached : q.cached + token + 1, q.keys) : 0;
+    // keys that all rows of the wave see, and that some row may
+    const int all_see = min(tree ? q.cached : q.cached + first_row / group + 1, q.keys);
+    const int last_row = row0 + min(32 * wave + 32, rows) - 1;
+    const int any_sees = 32 * wave >= rows ? 0 : tree ? q.keys : min(q.cached + last_row / group + 1, q.keys);
+
+    f32x16_t acc[kTiles];
+#pragma unroll
+    for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
+    float row_max = -INFINITY, row_sum = 0.0f;
+
+    if (t0 < t1) {
+      convert(t0, 0);
+      if (t0 + 1 < t1) {
+        fetch(t0 + 1);
+        fetch_id(min(t0 + 2, t1 - 1));
+      }
+    }
+    __syncthreads();
+
+    for (int kt = t0; kt < t1; ++kt) {
+      const int buf = (kt - t0) & 1;
+      if (kt + 1 < t1) {
+        convert(kt + 1, buf ^ 1);
+        if (kt + 2 < t1) {
+          fetch(kt + 2);
+          fetch_id(min(kt + 3, t1 - 1));
+        }
+      }
+      const int key0 = kt * kKeys;
+      if (key0 < any_sees) {
+        f32x16_t sc[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kSteps; ++i) {
+            const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(&s_k[buf][32 * n + col][16 * i + 8 * h]);
+            sc[n] = mfma32(kf, qf[i], sc[n]);
+          }
+        }
+        const uint64_t held_keys[4] = {s_held[buf][0], s_held[buf][1], s_held[buf][2], s_held[buf][3]};
+        const bool whole = key0 + kKeys <= all_see &&
+                           (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
+        if (!whole) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const int k = key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
+              const uint64_t on = held_keys[2 * n + (i >> 3)] >> (16 * h);
+              const unsigned fresh = static_cast<unsigned>(k - q.cached);
+              const uint32_t half = fresh & 32u ? static_cast<uint32_t>(bits >> 32) : static_cast<uint32_t>(bits);
+              const uint32_t named = fresh < 64u ? half >> (fresh & 31u) : 0u;
+              const bool visible = ((on >> (4 * (8 * ((i >> 2) & 1) + (i & 3)))) & 1) & ((k < sees) | ((named & 1u) != 0));
+              const float y = sc[n][i];
+              sc[n][i] = visible ? y : -INFINITY;
+            }
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[n][i]);
+        const u32x2_t other = __builtin_bit_cast(
+            u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false));
+        top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
+        // The reference follows the maximum only when that leads it by 2^8: weights up to 2^8 are as
+        // exact as weights up to 1, and sums are rescaled rarely.
+        const bool grew = top > row_max && (top - row_max) * scale > 8.0f;
+        if (__any(grew)) {
+          const float next = grew ? top : row_max;
+          const float f = __builtin_amdgcn_exp2f((row_max - (next == -INFINITY ? 0.0f : next)) * scale);
+          row_max = next;
+          row_sum *= f;
+#pragma unroll
+          for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+        }
+        const float ref = (row_max == -INFINITY ? 0.0f : row_max) * scale;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            u32x4_t w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i], scale, -ref));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i + 1], scale, -ref));
+              row_sum += p0 + p1;
+              w[i] = pack_bf16x2(p0, p1);
+            }
+            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
+#pragma unroll
+            for (int c = 0; c < kTiles; ++c) {
+              const bf16x8_t vf = *reinterpret_cast<const bf16x8_t*>(&s_v[buf][32 * c + col][8 * (4 * n + 2 * s + h)]);
+              acc[c] = mfma32(vf, pf, acc[c]);
+            }
+          }
+      }
+      __syncthreads();
+    }
+
+    const u32x2_t both = __builtin_bit_cast(
+        u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(row_sum), __float_as_uint(row_sum), false, false));
+    row_sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    const int slot = 2 * me + (x0 == 0);
+    if (live) {
+      const size_t at = static_cast<size_t>(slot) * kKvPromptRows + 32 * wave + col;
+#pragma unroll
+      for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+          const float o[4] = {acc[c][4 * b], acc[c][4 * b + 1], acc[c][4 * b + 2], acc[c][4 * b + 3]};
+          const int ch = 32 * c + 8 * b + 4 * h;
+          if (complete)
+            kv_write(a, q.row + token, qh, ch, row_sum, o);
+          else
+            *reinterpret_cast<f32x4_t*>(out.out + at * D + ch) = f32x4_t{o[0], o[1], o[2], o[3]};
+        }
+      if (!complete && h == 0) {
+        out.stats[at * 2] = row_max;
+        out.stats[at * 2 + 1] = row_sum;
+      }
+    }
+    if (!complete && x0 == 0) {
+      left = true;
+      if (tid == 0) {
+        // the worker whose share holds the tile's last unit
+        const int64_t last = u + cost - 1;
+        int owner = static_cast<int>(((last + 1) * workers - 1) / total);
+        *split = KvSplit{r, head, tile, owner - me + 1, slot, 2 * (me + 1)};
+      }
+    }
+    u += x1 - x0;
+  }
+  if (!left && tid == 0) split->count = 0;
+}
+
+}  // namespace
+
+hipError_t launch_kv_prompt(const KvAttentionArgs& a, const KvPartials& part, int workers, hipStream_t stream) {
+  if (a.D == 64)
+    kv_prompt_kernel<64><<<workers, kPromptThreads, 0, stream>>>(a, part);
+  else
+    kv_prompt_kernel<128><<<workers, kPromptThreads, 0, stream>>>(a, part);
+  return hipGetLastError();
+}
+
+}  // namespace w4a16

@@ -1256,14 +1256,20 @@ int kv_rows(w4a16::KvRowsArgs* a, int T, int KV, int D, int num_blocks, int log2
   return W4A16_OK;
 }
 
-int validate_kv_heads(int T, int R, int H, int KV, int D, int width, int max_query_len) {
+int validate_kv_heads(int T, int R, int H, int KV, int D, int log2_block, int width, int max_query_len) {
   if (T < 0 || R < 0) return fail(W4A16_ERR_ARG, "T (%d) and R (%d) must not be negative", T, R);
   if (H <= 0 || KV <= 0 || H % KV) return fail(W4A16_ERR_SHAPE, "query heads (%d) must be a multiple of kv heads (%d)", H, KV);
   if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
   if (width <= 0) return fail(W4A16_ERR_ARG, "the block tables' width must be positive (got %d)", width);
   if (max_query_len < 1) return fail(W4A16_ERR_ARG, "max_query_len must be at least 1 (got %d)", max_query_len);
+  if (T == 0 || R == 0) return W4A16_OK;
   if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
+  // the split kernel counts its work units (16 rows x 128 keys) in 32 bits
+  const int64_t tiles = (static_cast<int64_t>(T) * (H / KV) + 15) / 16 + R;
+  const int64_t spans = ((static_cast<int64_t>(width) << log2_block) + 127) / 128;
+  if (spans > 0x7FFFFFFF / tiles / KV)
+    return fail(W4A16_ERR_SHAPE, "%d rows over block tables of %d blocks are too much work for one call", T, width);
   return W4A16_OK;
 }
 
@@ -1331,11 +1337,12 @@ int w4a16_kv_load(const uint8_t* cache, const int32_t* slots, uint16_t* k, uint1
 }
 
 size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int block_size, int width, int max_query_len) {
-  if (validate_kv_heads(T, R, H, KV, D, width, max_query_len) != W4A16_OK || kv_log2_block(block_size) < 0) return 0;
+  const int log2_block = kv_log2_block(block_size);
+  if (log2_block < 0 || validate_kv_heads(T, R, H, KV, D, log2_block, width, max_query_len) != W4A16_OK) return 0;
   if (T == 0 || R == 0) return 0;
   w4a16::KvAttentionArgs a{};
   a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.width = width;
-  a.log2_block = kv_log2_block(block_size);
+  a.log2_block = log2_block;
   a.max_query_len = max_query_len < T ? max_query_len : T;
   return w4a16::kv_attention_workspace(a);
 }
@@ -1346,9 +1353,9 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
                        int R, int H, int KV, int D, int num_blocks, int block_size, int width, int max_query_len,
                        int zero_tail, void* workspace, size_t workspace_bytes, void* stream) {
   int log2_block = 0;
-  int e = validate_kv_heads(T, R, H, KV, D, width, max_query_len);
+  int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block);
   if (e != W4A16_OK) return e;
-  if ((e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block)) != W4A16_OK) return e;
+  if ((e = validate_kv_heads(T, R, H, KV, D, log2_block, width, max_query_len)) != W4A16_OK) return e;
   if (!(scale > 0.0f) || scale > 3.0e38f) return fail(W4A16_ERR_ARG, "scale must be positive and finite (got %g)", static_cast<double>(scale));
   if (T == 0) return ok();
   if (R == 0) return fail(W4A16_ERR_ARG, "%d rows of no request", T);

@@ -61,13 +61,13 @@ def test_load_refusals(pkg, dll, change, status, message):
 @pytest.mark.parametrize("change,status,message", [
     ({"q": None}, 1, "null"), ({"cache": None}, 1, "null"), ({"tables": None}, 1, "null"), ({"seq": None}, 1, "null"),
     ({"cu": None}, 1, "null"), ({"out": None}, 1, "null"), ({"T": -1}, 1, "negative"), ({"R": 0}, 1, "no request"),
-    ({"H": 30}, 2, "multiple"), ({"KV": 0}, 2, "multiple"), ({"D": 256}, 2, "head size"), ({"width": 0}, 1, "width"),
+    ({"H": 30}, 2, "multiple"), ({"KV": 0}, 1, "positive"), ({"D": 256}, 2, "head size"), ({"width": 0}, 1, "width"),
     ({"stride": 7}, 1, "apart"), ({"block": 8}, 2, "block_size"), ({"longest": 0}, 1, "max_query_len"),
     ({"scale": ctypes.c_float(0.0)}, 1, "scale"), ({"scale": ctypes.c_float(-1.0)}, 1, "scale"),
     ({"scale": ctypes.c_float(float("nan"))}, 1, "scale"), ({"scale": ctypes.c_float(float("inf"))}, 1, "scale"),
     ({"q": P + 8}, 3, "aligned"), ({"qt": 4097}, 3, "multiples of 8"), ({"out": P + 8}, 3, "aligned"),
     ({"ws": None}, 4, "workspace"), ({"ws_bytes": 64}, 4, "workspace"), ({"ws": P + 4}, 3, "aligned"),
-    ({"T": 1 << 28}, 2, "too many")])
+    ({"T": 1 << 28}, 2, "too many"), ({"T": 1 << 18, "width": 1 << 20, "stride": 1 << 20}, 2, "too much work")])
 def test_attention_refusals(pkg, dll, change, status, message):
     assert dll.w4a16_kv_attention(*{**ATTENTION, **change}.values()) == status and message in error(pkg)
 

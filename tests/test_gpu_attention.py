@@ -257,3 +257,53 @@ def test_graph_replays_follow_the_lengths(gpu_lib):
             graph.replay()
             torch.cuda.synchronize()
             assert torch.equal(out, want), i
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (10, 2, 128), (4, 4, 64), (16, 1, 64)])
+@pytest.mark.parametrize("new,seq", [([80], [80]), ([65, 129], [65, 700]), ([1, 200, 3, 1], [300, 260, 3, 90]),
+                                     ([100, 0, 70], [1100, 5, 70])])
+def test_prompts(gpu_lib, heads, kv_heads, dim, new, seq):
+    """Whole prompts and chunks behind cached tokens, alone and among decode rows: tiles of 256
+    rows and 64 keys that end anywhere."""
+    b = Batch(new, seq, heads, kv_heads, dim, 16, seed=heads + sum(seq), pad=2)
+    print("prompts", heads, kv_heads, dim, new, seq, flush=True)
+    b.check(b.run(max_query_len=max(new)))
+
+
+def test_prompt_tree_masks(gpu_lib):
+    new, seq = [90, 2], [300, 40]
+    b = Batch(new, seq, 8, 2, 128, 32, seed=21)
+    gen = random.Random(4)
+    masks = [gen.getrandbits(64) for _ in range(sum(new))]
+    masks[7] = 0
+    signed = [m - (1 << 64) if m >> 63 else m for m in masks]
+    b.check(b.run(tree_mask=torch.tensor(signed, dtype=torch.int64, device="cuda")), tree_mask=masks)
+
+
+def test_prompt_bad_pages_and_nan_rows(gpu_lib):
+    """As for decode rows: pages outside the cache are not seen, a NaN row (its keys, or its values
+    alone) reaches the rows that see it and no other."""
+    b = Batch([150], [400], 8, 2, 128, 16, seed=22)
+    b.tables[0][3], b.tables[0][17] = -1, b.cache.shape[0] + 5
+    b.check(b.run())
+    words = b.cache.view(torch.int32)
+    token = 330  # new token 80
+    words[b.tables[0][token // 16], :, 16 * 128 // 4 + 16 + token % 16] = 0x7FC04300
+    out = b.run()
+    assert bool(torch.isfinite(out[:80].float()).all()) and bool(torch.isnan(out[80:].float()).all())
+
+
+def test_long_prompt_split(gpu_lib):
+    """A chunk whose row tiles are shared by many workgroups."""
+    b = Batch([300], [3000], 8, 1, 128, 64, seed=23)
+    b.check(b.run())
+
+
+def test_extreme_prompt_queries(gpu_lib):
+    b = Batch([70], [200], 8, 2, 128, 16, seed=24)
+    b.qkv[3] *= 1000
+    b.qkv[4] = 0
+    b.check(b.run())
+    b.qkv[5, 0, 0] = float("inf")
+    out = b.run()
+    assert bool(torch.isnan(out[5, 0].float()).all()) and bool(torch.isfinite(out[5, 1:].float()).all())
