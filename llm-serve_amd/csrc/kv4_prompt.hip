@@ -65,12 +65,43 @@ __device__ __forceinline__ int64_t kv_request_cost(const KvAttentionArgs& a, con
 // Share w of `total` cost units.
 __device__ __forceinline__ int64_t share(int64_t total, int workers, int w) { return total * w / workers; }
 
-// Byte b of the shifted word holds nibble 2 b + odd of a code word: its channel.
-__device__ __forceinline__ constexpr int byte_channel(int b, int odd) { return (b == 0 ? 0 : b == 1 ? 4 : b == 2 ? 1 : 5) + 2 * odd; }
+// Codes -> fp32 without a conversion: a nibble in the low bits of an fp16 1024.0 is 1024 + c, one
+// in bits 4 .. 7 of an fp16 64.0 is 64 + c, and v_fma_mix_f32 takes either half of the register as
+// it stands: (1024 + c) s - (1024 + z) s, both terms and the result exact in fp32.  A word (w, and
+// w >> 8) gives its 8 codes in 5 instructions.
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 
-template <int B>
-__device__ __forceinline__ float byte_f32(uint32_t w) {
-  return static_cast<float>((w >> (8 * B)) & 0xFFu);  // v_cvt_f32_ubyteB
+// The masks in SGPRs and the biases in VGPRs, hidden from constant folding, so that each and-or is
+// one v_and_or_b32 (see NibbleConsts).
+struct FusedConsts {
+  uint32_t mask_low, mask_high, bias_low, bias_high;
+};
+
+__device__ __forceinline__ FusedConsts fused_consts() {
+  FusedConsts k{0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
+  asm volatile("" : "+s"(k.mask_low), "+s"(k.mask_high));
+  asm volatile("" : "+v"(k.bias_low), "+v"(k.bias_high));
+  return k;
+}
+
+struct RowScale {
+  float s, low, high;  // the scale; -(1024 + z) s and -(64 + z) s
+};
+
+__device__ __forceinline__ RowScale row_scale(float s, uint32_t meta) {
+  const float z = kv_meta_zero128(meta);
+  return RowScale{s, -s * (z + 896.0f), -s * (z - 64.0f)};
+}
+
+// Nibbles 0 and 4 (f[0], f[1]: channels 0, 1 of the word) and 1 and 5 (f[2], f[3]: channels 2, 3);
+// of w >> 8, channels 4 .. 7.
+__device__ __forceinline__ void four_values(float (&f)[4], uint32_t w, const RowScale& r, const FusedConsts& k) {
+  const f16x2_t a = __builtin_bit_cast(f16x2_t, (w & k.mask_low) | k.bias_low);
+  const f16x2_t b = __builtin_bit_cast(f16x2_t, (w & k.mask_high) | k.bias_high);
+  f[0] = __builtin_fmaf(static_cast<float>(a[0]), r.s, r.low);
+  f[1] = __builtin_fmaf(static_cast<float>(a[1]), r.s, r.low);
+  f[2] = __builtin_fmaf(static_cast<float>(b[0]), r.s, r.high);
+  f[3] = __builtin_fmaf(static_cast<float>(b[1]), r.s, r.high);
 }
 
 template <int D>
@@ -117,6 +148,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   KvRequest q = kv_request(a, r);
   bool left = false;
 
+  const FusedConsts fc = fused_consts();
   const int col = lane & 31, h = lane >> 5;
   const float scale = a.scale_log2e;
 
@@ -195,48 +227,53 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     auto convert = [&](int key_tile, int buf) {
       const int key = key_tile * kKeys + my_key;
       if (converts_v) {
-        float s[8], zs[8];
+        RowScale rs[8];
+        uint32_t top = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int k = key + (i < 4 ? i : i + 4);
-          const float scale_v = kv_meta_scale(meta[i]);
-          const bool use = held & (k < q.keys) & (fabsf(scale_v) < INFINITY);
-          s[i] = use ? scale_v : 0.0f;
-          zs[i] = use ? -scale_v * (kv_meta_zero128(meta[i]) - 128.0f) : 0.0f;
+          top = max(top, meta[i] & 0x7FFFFFFFu);
+          rs[i] = row_scale(kv_meta_scale(meta[i]), meta[i]);
         }
-        // bytes of the word: four nibbles (D = 128, a thread takes 4 channels) or two (D = 64)
-        const int odd = part & 1, shift = 4 * odd + (D == 64 ? 16 * (part >> 1) : 0);
+        if (__any(!held | (key + 12 > q.keys) | (top >= 0x7F800000u))) {
 #pragma unroll
-        for (int b = 0; b < D / 32; ++b) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t lo = (raw[2 * i] >> shift) & 0x0F0F0F0Fu, hi = (raw[2 * i + 1] >> shift) & 0x0F0F0F0Fu;
-            const float f0 = static_cast<float>((lo >> (8 * b)) & 0xFFu), f1 = static_cast<float>((hi >> (8 * b)) & 0xFFu);
-            w[i] = pack_bf16x2(__builtin_fmaf(f0, s[2 * i], zs[2 * i]), __builtin_fmaf(f1, s[2 * i + 1], zs[2 * i + 1]));
+          for (int i = 0; i < 8; ++i) {
+            const bool use = held & (key + (i < 4 ? i : i + 4) < q.keys) & (fabsf(rs[i].s) < INFINITY);
+            rs[i].s = use ? rs[i].s : 0.0f;
+            rs[i].low = use ? rs[i].low : 0.0f;
+            rs[i].high = use ? rs[i].high : 0.0f;
           }
-          const int ch = 8 * word + (D == 64 ? byte_channel(b, 0) + 2 * odd + (part >> 1) : byte_channel(b, 0) + 2 * odd);
-          *reinterpret_cast<uint4*>(&s_v[buf][ch][8 * vgroup]) = make_uint4(w[0], w[1], w[2], w[3]);
         }
+        // A thread's channels: 4 neighbours of a word (D = 128), or 2 (D = 64: nibbles 0 and 4, or 1 and 5).
+        const int shift = D == 128 ? 8 * part : 8 * (part >> 1) + 4 * (part & 1);
+        const int ch = 8 * word + (D == 128 ? 4 : 2) * part;
+        uint32_t w[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f[4], g[4];
+          four_values(f, raw[2 * i] >> shift, rs[2 * i], fc);
+          four_values(g, raw[2 * i + 1] >> shift, rs[2 * i + 1], fc);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) w[c][i] = pack_bf16x2(f[c], g[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c)
+          *reinterpret_cast<uint4*>(&s_v[buf][ch + c][8 * vgroup]) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
       } else {
         const bool use = held & (key < q.keys);
         const uint64_t all = __ballot(use);
         if (lane == 0) s_held[buf][wave] = all;
-        const float value_scale = kv_meta_scale(meta[1]);
-        const float s = use ? (fabsf(value_scale) < INFINITY ? kv_meta_scale(meta[0]) : __builtin_nanf("")) : 0.0f;
-        const float zs = use ? -s * (kv_meta_zero128(meta[0]) - 128.0f) : 0.0f;
+        const float nan = __builtin_nanf("");
+        RowScale rs = row_scale(fabsf(kv_meta_scale(meta[1])) < INFINITY ? kv_meta_scale(meta[0]) : nan, meta[0]);
+        rs.s = use ? rs.s : 0.0f;
+        rs.low = use ? rs.low : 0.0f;
+        rs.high = use ? rs.high : 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-          float f[8];
-#pragma unroll
-          for (int odd = 0; odd < 2; ++odd) {
-            const uint32_t w = (raw[i] >> (4 * odd)) & 0x0F0F0F0Fu;
-            f[byte_channel(0, odd)] = __builtin_fmaf(byte_f32<0>(w), s, zs);
-            f[byte_channel(1, odd)] = __builtin_fmaf(byte_f32<1>(w), s, zs);
-            f[byte_channel(2, odd)] = __builtin_fmaf(byte_f32<2>(w), s, zs);
-            f[byte_channel(3, odd)] = __builtin_fmaf(byte_f32<3>(w), s, zs);
-          }
-          *reinterpret_cast<uint4*>(&s_k[buf][t >> 2][(D / 4) * chunk + 8 * i]) = pack_bf16x8(f);
+          float f[4], g[4];
+          four_values(f, raw[i], rs, fc);
+          four_values(g, raw[i] >> 8, rs, fc);
+          *reinterpret_cast<uint4*>(&s_k[buf][t >> 2][(D / 4) * chunk + 8 * i]) =
+              make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]));
         }
       }
     };
@@ -274,6 +311,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
     float row_max = -INFINITY, row_sum = 0.0f;
+    const bf16x2_t ones = __builtin_bit_cast(bf16x2_t, 0x3F803F80u);
 
     if (t0 < t1) {
       convert(t0, 0);
@@ -286,43 +324,60 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 
     for (int kt = t0; kt < t1; ++kt) {
       const int buf = (kt - t0) & 1;
-      if (kt + 1 < t1) {
-        convert(kt + 1, buf ^ 1);
-        if (kt + 2 < t1) {
-          fetch(kt + 2);
-          fetch_id(min(kt + 3, t1 - 1));
+      // The two waves of a SIMD are a K and a V converter: one converts the next tile before its
+      // products, the other after, so that one's vector instructions run beside the other's
+      // matrix instructions.
+      auto next_tile = [&]() {
+        if (kt + 1 < t1) {
+          convert(kt + 1, buf ^ 1);
+          if (kt + 2 < t1) {
+            fetch(kt + 2);
+            fetch_id(min(kt + 3, t1 - 1));
+          }
         }
-      }
+      };
+      if (!converts_v) next_tile();
       const int key0 = kt * kKeys;
       if (key0 < any_sees) {
         f32x16_t sc[2];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
 #pragma unroll
-          for (int i = 0; i < kSteps; ++i) {
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
             const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(&s_k[buf][32 * n + col][16 * i + 8 * h]);
             sc[n] = mfma32(kf, qf[i], sc[n]);
           }
-        }
         const uint64_t held_keys[4] = {s_held[buf][0], s_held[buf][1], s_held[buf][2], s_held[buf][3]};
-        const bool whole = key0 + kKeys <= all_see &&
-                           (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
-        if (!whole) {
+        const bool all_held = (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
+        if (!(key0 + kKeys <= all_see && all_held)) {
+          if (all_held && !tree) {
+            const int lead = sees - key0 - 4 * h;
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int k = key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
-              const uint64_t on = held_keys[2 * n + (i >> 3)] >> (16 * h);
-              const unsigned fresh = static_cast<unsigned>(k - q.cached);
-              const uint32_t half = fresh & 32u ? static_cast<uint32_t>(bits >> 32) : static_cast<uint32_t>(bits);
-              const uint32_t named = fresh < 64u ? half >> (fresh & 31u) : 0u;
-              const bool visible = ((on >> (4 * (8 * ((i >> 2) & 1) + (i & 3)))) & 1) & ((k < sees) | ((named & 1u) != 0));
-              const float y = sc[n][i];
-              sc[n][i] = visible ? y : -INFINITY;
-            }
+              for (int i = 0; i < 16; ++i) {
+                const float y = sc[n][i];
+                sc[n][i] = 32 * n + 8 * (i >> 2) + (i & 3) < lead ? y : -INFINITY;
+              }
+          } else {
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const int k = key0 + 32 * n + 8 * (i >> 2) + 4 * h + (i & 3);
+                const uint64_t on = held_keys[2 * n + (i >> 3)] >> (16 * h);
+                const unsigned fresh = static_cast<unsigned>(k - q.cached);
+                const uint32_t half = fresh & 32u ? static_cast<uint32_t>(bits >> 32) : static_cast<uint32_t>(bits);
+                const uint32_t named = fresh < 64u ? half >> (fresh & 31u) : 0u;
+                const bool visible = ((on >> (4 * (8 * ((i >> 2) & 1) + (i & 3)))) & 1) & ((k < sees) | ((named & 1u) != 0));
+                const float y = sc[n][i];
+                sc[n][i] = visible ? y : -INFINITY;
+              }
+          }
         }
         float top = sc[0][0];
 #pragma unroll
@@ -355,8 +410,10 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
             for (int i = 0; i < 4; ++i) {
               const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i], scale, -ref));
               const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i + 1], scale, -ref));
-              row_sum += p0 + p1;
-              w[i] = pack_bf16x2(p0, p1);
+              const uint32_t pair = pack_bf16x2(p0, p1);
+              w[i] = pair;
+              // the sum takes the weights as the product does, rounded
+              row_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), ones, row_sum, false);
             }
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
 #pragma unroll
@@ -366,6 +423,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
             }
           }
       }
+      if (converts_v) next_tile();
       __syncthreads();
     }
 
