@@ -24,6 +24,7 @@ constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
 constexpr int kTileCost = 16;  // cost units of a tile of keys
 constexpr int kMinShare = 4 * kTileCost;
+constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
 __device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -88,8 +89,8 @@ struct RowScale {
   float s, low, high;  // the scale; -(1024 + z) s and -(64 + z) s
 };
 
-__device__ __forceinline__ RowScale row_scale(float s, uint32_t meta) {
-  const float z = kv_meta_zero128(meta);
+__device__ __forceinline__ RowScale row_scale(uint32_t meta) {
+  const float s = kv_meta_scale(meta), z = kv_meta_zero128(meta);
   return RowScale{s, -s * (z + 896.0f), -s * (z - 64.0f)};
 }
 
@@ -227,20 +228,14 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     auto convert = [&](int key_tile, int buf) {
       const int key = key_tile * kKeys + my_key;
       if (converts_v) {
-        RowScale rs[8];
         uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          top = max(top, meta[i] & 0x7FFFFFFFu);
-          rs[i] = row_scale(kv_meta_scale(meta[i]), meta[i]);
-        }
+        for (int i = 0; i < 8; ++i) top = max(top, meta[i] & 0x7FFFFFFFu);
         if (__any(!held | (key + 12 > q.keys) | (top >= 0x7F800000u))) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const bool use = held & (key + (i < 4 ? i : i + 4) < q.keys) & (fabsf(rs[i].s) < INFINITY);
-            rs[i].s = use ? rs[i].s : 0.0f;
-            rs[i].low = use ? rs[i].low : 0.0f;
-            rs[i].high = use ? rs[i].high : 0.0f;
+            const bool use = held & (key + (i < 4 ? i : i + 4) < q.keys) & (fabsf(kv_meta_scale(meta[i])) < INFINITY);
+            meta[i] = use ? meta[i] : kZeroMeta;
           }
         }
         // A thread's channels: 4 neighbours of a word (D = 128), or 2 (D = 64: nibbles 0 and 4, or 1 and 5).
@@ -250,8 +245,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float f[4], g[4];
-          four_values(f, raw[2 * i] >> shift, rs[2 * i], fc);
-          four_values(g, raw[2 * i + 1] >> shift, rs[2 * i + 1], fc);
+          four_values(f, raw[2 * i] >> shift, row_scale(meta[2 * i]), fc);
+          four_values(g, raw[2 * i + 1] >> shift, row_scale(meta[2 * i + 1]), fc);
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) w[c][i] = pack_bf16x2(f[c], g[c]);
         }
@@ -262,11 +257,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         const bool use = held & (key < q.keys);
         const uint64_t all = __ballot(use);
         if (lane == 0) s_held[buf][wave] = all;
-        const float nan = __builtin_nanf("");
-        RowScale rs = row_scale(fabsf(kv_meta_scale(meta[1])) < INFINITY ? kv_meta_scale(meta[0]) : nan, meta[0]);
-        rs.s = use ? rs.s : 0.0f;
-        rs.low = use ? rs.low : 0.0f;
-        rs.high = use ? rs.high : 0.0f;
+        uint32_t m = fabsf(kv_meta_scale(meta[1])) < INFINITY ? meta[0] : kNanMeta;
+        m = use ? m : kZeroMeta;
+        const RowScale rs = row_scale(m);
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           float f[4], g[4];
@@ -344,13 +337,29 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
+        // LDS reads run ahead of the matrix instructions by one group of four fragments (two steps
+        // of K, one of V); V's first group is read ahead of the softmax.  Left to itself the
+        // compiler reads each fragment just before its use.
+        bf16x8_t frag[2][4];
+        auto read_k = [&](int group_of, bf16x8_t (&f)[4]) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
+          for (int j = 0; j < 4; ++j)
+            f[j] = *reinterpret_cast<const bf16x8_t*>(&s_k[buf][32 * (j & 1) + col][16 * (2 * group_of + (j >> 1)) + 8 * h]);
+        };
+        auto read_v = [&](int step, bf16x8_t (&f)[4]) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(&s_k[buf][32 * n + col][16 * i + 8 * h]);
-            sc[n] = mfma32(kf, qf[i], sc[n]);
-          }
+          for (int c = 0; c < kTiles; ++c)
+            f[c] = *reinterpret_cast<const bf16x8_t*>(&s_v[buf][32 * c + col][8 * (2 * step + h)]);
+        };
+        read_k(0, frag[0]);
+#pragma unroll
+        for (int i = 0; i < kSteps / 2; ++i) {
+          if (i + 1 < kSteps / 2) read_k(i + 1, frag[(i + 1) & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sc[j & 1] = mfma32(frag[i & 1][j], qf[2 * i + (j >> 1)], sc[j & 1]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
         const uint64_t held_keys[4] = {s_held[buf][0], s_held[buf][1], s_held[buf][2], s_held[buf][3]};
         const bool all_held = (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
         if (!(key0 + kKeys <= all_see && all_held)) {
