@@ -344,6 +344,10 @@ int w4a16_kv_store(const uint16_t* k, int64_t k_stride_t, int64_t k_stride_h, co
 int w4a16_kv_load(const uint8_t* cache, const int32_t* slots, uint16_t* k, uint16_t* v, int T, int KV,
                   int D, int num_blocks, int block_size, void* stream);
 
+/* Ints that w4a16_kv_attention counts its workgroups' arrivals in: zero when a call starts, left
+ * zero by it.  Calls in flight at the same time must not share them. */
+#define W4A16_KV_COUNTERS 1024
+
 /* Bytes of workspace w4a16_kv_attention needs (its contents need no initialization and are not
  * kept; calls in flight at the same time must not share one). */
 size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int block_size, int width,
@@ -368,7 +372,7 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
                        const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale,
                        int T, int R, int H, int KV, int D, int num_blocks, int block_size, int width,
                        int max_query_len, int zero_tail, void* workspace, size_t workspace_bytes,
-                       void* stream);
+                       int32_t* counters, void* stream);
 
 #ifdef __cplusplus
 }

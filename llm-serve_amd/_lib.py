@@ -69,7 +69,7 @@ _SIGNATURES = {
     "w4a16_kv_attention_workspace": (_c_size, [_c_int] * 8),
     "w4a16_kv_attention": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                     ctypes.c_float, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
-                                    _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
+                                    _c_int, _c_int, _c_ptr, _c_size, _c_ptr, _c_ptr]),
 }
 ABI_VERSION = 5
 
@@ -324,14 +324,15 @@ class W4A16Library:
         return int(self.dll.w4a16_kv_attention_workspace(t, r, h, kv, head_dim, block_size, width, max_query_len))
 
     def kv_attention(self, q, cache, tables, seq_lens, cu_query_lens, tree_mask, out, scale: float, block_size: int,
-                     max_query_len: int, zero_tail: bool, workspace) -> None:
-        """out [T, H, D] = attention of the packed rows q over the cache's pages."""
+                     max_query_len: int, zero_tail: bool, workspace, counters) -> None:
+        """out [T, H, D] = attention of the packed rows q over the cache's pages; counters: 1024
+        zero int32 (left zero) that no other call in flight uses."""
         t, h, d = q.shape
         self._launch(self.dll.w4a16_kv_attention, "w4a16_kv_attention", cache, q.data_ptr(), q.stride(0), q.stride(1),
                      cache.data_ptr(), tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(),
                      cu_query_lens.data_ptr(), _ptr(tree_mask), out.data_ptr(), scale, t, seq_lens.shape[0], h,
                      cache.shape[1], d, cache.shape[0], block_size, tables.shape[1], max_query_len, int(zero_tail),
-                     workspace.data_ptr(), workspace.numel())
+                     workspace.data_ptr(), workspace.numel(), counters.data_ptr())
 
 
 _LOCK = threading.Lock()

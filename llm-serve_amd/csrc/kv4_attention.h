@@ -7,24 +7,25 @@
 
 namespace w4a16 {
 
-// What a combine needs to join one row tile's partial results.  A workgroup's share of the work is
-// contiguous, so it holds at most one tile that began before it (its result goes to slot 2 w) and
-// one that ends behind it (slot 2 w + 1); the workgroup where a tile begins describes it.
-struct KvSplit {
-  int request, head, tile;
-  int count;        // partial results (0: this entry joins nothing)
-  int first, next;  // slot of the first one, and of the second; the others lie 2 apart from there
-};
-
+// Partial results.  A workgroup's share of the work is contiguous, so it covers at most one tile
+// that began before it (its part goes to slot 2 w) and one that ends behind it (slot 2 w + 1).
+// The workgroups of a tile count their arrivals at the counter of the one where it begins; the
+// last to arrive joins the parts in the workgroups' order, so the result does not depend on which
+// one that is, and leaves the counter at zero.  Parts travel with the coherent policy of the
+// split-K exchange (w4a16_common.h).
 struct KvPartials {
-  float* out;      // [slots][rows][D], unnormalized
-  float* stats;    // [slots][rows][2]: maximum (raw score) and sum
-  KvSplit* split;  // one a worker
+  float* out;      // [slots][tile rows][D], unnormalized
+  float* stats;    // [slots][tile rows][2]: reference (a raw score) and sum
+  int* counters;   // [workers]
+  uint32_t out_bytes, stats_bytes;
 };
 
 // Prompt kernel: rows of a tile, and its grid (a workgroup a CU).
 constexpr int kKvPromptRows = 256;
 constexpr int kKvPromptWorkers = 256;
+// The split kernel's largest grid: three workgroups a CU.
+constexpr int kKvSplitWorkers = 768;
+static_assert(kKvSplitWorkers + kKvPromptWorkers == kKvAttentionCounters, "a counter a worker");
 // A call goes to the split kernel alone up to this many rows a request (longest query x heads of a
 // group); beyond, requests of at most kKvMixedMaxRows rows go to it, the others to the prompt kernel.
 constexpr int kKvSplitMaxRows = 64;
@@ -40,12 +41,16 @@ struct KvRequest {
   int keys;    // keys that its block table can hold of the sequence
 };
 
+// The lists that no kernel here writes, read through the scalar cache where the index is uniform.
+typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+__device__ __forceinline__ ConstInts const_ints(const int32_t* p) { return (ConstInts)p; }
+
 __device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r) {
   KvRequest q;
-  const int lo = a.cu_query_lens[r], hi = a.cu_query_lens[r + 1];
+  const int lo = const_ints(a.cu_query_lens)[r], hi = const_ints(a.cu_query_lens)[r + 1];
+  const int seq = max(const_ints(a.seq_lens)[r], 0);
   q.row = min(max(lo, 0), a.T);
   q.n = max(min(hi, a.T) - q.row, 0);
-  const int seq = max(a.seq_lens[r], 0);
   q.cached = seq - (hi - lo);
   const int64_t room = static_cast<int64_t>(a.width) << a.log2_block;
   q.keys = seq < room ? seq : static_cast<int>(room);
@@ -88,6 +93,103 @@ __device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int 
     *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(o[0] * inv, o[1] * inv);
   } else {
     *p = f32_to_bf16_bits(o[0] * inv);
+  }
+}
+
+// One part of a tile row's result: eight channels, or the row's statistics.
+__device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, uint32_t offset, const float (&o)[8]) {
+  store_fragment(r, offset, f32x4_t{o[0], o[1], o[2], o[3]});
+  store_fragment(r, offset + 16, f32x4_t{o[4], o[5], o[6], o[7]});
+}
+
+__device__ __forceinline__ void store_stats(__amdgpu_buffer_rsrc_t r, uint32_t offset, float top, float sum) {
+  const u32x2_t v = {__float_as_uint(top), __float_as_uint(sum)};
+  __builtin_amdgcn_raw_buffer_store_b64(v, r, offset, 0, kCoherentPolicy);
+}
+
+// Counts this workgroup's arrival, its part stored; whether it is the last of `count`.  All
+// threads call it; `flag` is LDS.
+__device__ __forceinline__ bool kv_arrive(int* counter, int count, int* flag) {
+  __builtin_amdgcn_s_waitcnt(0);  // this wave's part has reached memory
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const bool last = arrive(counter) == count - 1;
+    if (last) rearm(counter);
+    *flag = last;
+  }
+  __syncthreads();
+  return *flag != 0;
+}
+
+// Joins a tile's `count` parts, from worker `first` on, into the output: a thread takes eight
+// channels of a row; where a tile has fewer of them than the workgroup has threads, groups of
+// threads take every group-th part each and are joined through `scratch` (LDS, 10 floats a thread).
+template <int D, int THREADS>
+__device__ __forceinline__ void kv_join(const KvAttentionArgs& a, const KvPartials& part, int tile_rows, int first,
+                                        int count, const KvRequest& q, int head, int row0, int rows, float* scratch) {
+  constexpr int kChunks = D / 8, kBatch = 4;
+  const int group = a.H / a.KV, tid = threadIdx.x;
+  const int items = rows * kChunks, groups = items < THREADS ? THREADS / items : 1;
+  const __amdgpu_buffer_rsrc_t ro = make_buffer(part.out, part.out_bytes), rs = make_buffer(part.stats, part.stats_bytes);
+  for (int e0 = 0; e0 < items; e0 += THREADS) {
+    const int mine = groups > 1 ? tid / items : 0;
+    const int e = groups > 1 ? tid - mine * items : e0 + tid;
+    const bool live = e < items && mine < groups;
+    const int row = e / kChunks, ch = e % kChunks * 8;
+    float top = -INFINITY, sum = 0.0f, o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    for (int i0 = mine; i0 < count && live; i0 += kBatch * groups) {
+      f32x4_t lo[kBatch], hi[kBatch];
+      u32x2_t st[kBatch];
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int i = i0 + b * groups;
+        const uint32_t at = static_cast<uint32_t>(i == 0 ? 2 * first + 1 : 2 * (first + i)) * tile_rows + row;
+        const bool in = i < count;  // loads beyond the last part touch nothing and give zeros
+        st[b] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, in ? at * 8 : kOutOfRange, 0, kCoherentPolicy));
+        lo[b] = load_fragment(ro, in ? (at * D + ch) * 4 : kOutOfRange);
+        hi[b] = load_fragment(ro, in ? (at * D + ch) * 4 + 16 : kOutOfRange);
+      }
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const uint32_t mb = st[b][0], lb = st[b][1];
+        const float m = i0 + b * groups < count ? __uint_as_float(mb) : -INFINITY;
+        const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e);
+        const float g = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2e);
+        top = next;
+        sum = sum * f + __uint_as_float(lb) * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[j] = o[j] * f + lo[b][j] * g;
+          o[4 + j] = o[4 + j] * f + hi[b][j] * g;
+        }
+      }
+    }
+    if (groups > 1) {
+      if (live) {
+        float* s = scratch + tid * 10;
+        s[0] = top;
+        s[1] = sum;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[2 + j] = o[j];
+      }
+      __syncthreads();
+      if (mine > 0) return;
+      for (int k = 1; k < groups; ++k) {
+        const float* s = scratch + (tid + k * items) * 10;
+        const float next = fmaxf(top, s[0]), ref = next == -INFINITY ? 0.0f : next;
+        const float f = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e);
+        const float g = __builtin_amdgcn_exp2f((s[0] - ref) * a.scale_log2e);
+        top = next;
+        sum = sum * f + s[1] * g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = o[j] * f + s[2 + j] * g;
+      }
+    }
+    if (live) {
+      const int token = (row0 + row) / group;
+      kv_write(a, q.row + token, head * group + row0 + row - token * group, ch, sum, o);
+    }
   }
 }
 

@@ -94,17 +94,16 @@ __device__ __forceinline__ void load_values(KvSlice<D>& s, const KvPlace& p, con
 }
 
 // The page ids of the tiles at key and key + 16; keys behind the last one repeat its page.
-__device__ __forceinline__ void kv_ids(int (&id)[2], const int32_t* __restrict__ table, int key, int last, int log2_block) {
+__device__ __forceinline__ void kv_ids(int (&id)[2], ConstInts table, int key, int last, int log2_block) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
-    id[t] = __builtin_amdgcn_readfirstlane(table[min(key + 16 * t, last) >> log2_block]);
+    id[t] = table[min(key + 16 * t, last) >> log2_block];
 }
 
 // Split attention.  A row tile is up to 16 MT rows (tokens x heads of the group) of one request
 // and kv head; its keys are cut into units of 128.  All units of all tiles, in order, are dealt
 // to the grid's workgroups in equal contiguous shares, so that a batch of any lengths loads them
-// alike; a share that covers a tile's keys only in part leaves a partial result, joined in a
-// fixed order by kv_combine_kernel.  Inside a unit each of the 4 waves takes 32 keys and keeps
+// alike; a share that covers a tile's keys only in part leaves a partial result (KvPartials).  Inside a unit each of the 4 waves takes 32 keys and keeps
 // its own running maximum and sum; the waves are joined through LDS at the end of a tile.
 //
 // The next slice's keys are loaded into the registers that the scores have just consumed, and
@@ -117,48 +116,60 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
   constexpr int kRows = 16 * MT, kSteps = D / 32, kTiles = D / 16, kPitch = D + 4;
   __shared__ __align__(16) float s_out[kWaves][kRows][kPitch];
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
+  __shared__ int s_last;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int group = a.H / a.KV;
 
   // This workgroup's share.  Every wave sums the requests' units (64 requests at a time, a lane
   // each), then scans them to the request where the share begins.
-  int sum = 0;
-  for (int r = lane; r < a.R; r += 64) sum += kv_units<kRows>(a, kv_request(a, r), group);
-  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const bool few = a.R <= 64;
+  KvRequest mine{0, 0, 0, 0};
+  int my_units = 0, sum = 0;
+  for (int i = lane; i < a.R; i += 64) {
+    mine = kv_request(a, i);
+    my_units = kv_units<kRows>(a, mine, group);
+    sum += my_units;
+  }
+  int upto = wave_scan(sum);
+  const int total = __builtin_amdgcn_readlane(upto, 63);
   const int workers = min(total, static_cast<int>(gridDim.x));
   const int me = blockIdx.x;
-  KvSplit* split = out.split + me;
 
   if (a.zero_tail) {
-    const int end = min(max(a.cu_query_lens[a.R], 0), a.T);
+    const int end = min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
     const int chunks = a.H * D / 8;
     for (int row = end + me; row < a.T; row += gridDim.x)
       for (int c = tid; c < chunks; c += kThreads)
         reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
   }
-  if (me >= workers) {
-    if (tid == 0) split->count = 0;
-    return;
-  }
+  if (me >= workers) return;
   const KvShares shares{total / workers, total % workers};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
-  int r = 0, base = 0;  // the share's first request, and the units before it
-  for (;; r += 64) {
-    const int units = r + lane < a.R ? kv_units<kRows>(a, kv_request(a, r + lane), group) : 0;
-    const int upto = wave_scan(units);
-    const uint64_t past = __ballot(base + upto > begin);
-    if (past || r + 64 >= a.R) {
-      const int first = past ? __builtin_ctzll(past) : 0;
-      base += __builtin_amdgcn_readlane(upto - units, first);
-      r += first;
-      break;
+  int r = 0, base = 0, units;  // the share's first request, the units before it, and its own
+  KvRequest q;
+  if (few) {
+    r = __builtin_ctzll(__ballot(upto > begin));
+    base = __builtin_amdgcn_readlane(upto - my_units, r);
+    units = __builtin_amdgcn_readlane(my_units, r);
+    q = KvRequest{__builtin_amdgcn_readlane(mine.row, r), __builtin_amdgcn_readlane(mine.n, r),
+                  __builtin_amdgcn_readlane(mine.cached, r), __builtin_amdgcn_readlane(mine.keys, r)};
+  } else {
+    for (;; r += 64) {
+      my_units = r + lane < a.R ? kv_units<kRows>(a, kv_request(a, r + lane), group) : 0;
+      upto = wave_scan(my_units);
+      const uint64_t past = __ballot(base + upto > begin);
+      if (past || r + 64 >= a.R) {
+        const int first = past ? __builtin_ctzll(past) : 0;
+        base += __builtin_amdgcn_readlane(upto - my_units, first);
+        r += first;
+        break;
+      }
+      base += __builtin_amdgcn_readlane(upto, 63);
     }
-    base += __builtin_amdgcn_readlane(upto, 63);
+    q = kv_request(a, r);
+    units = kv_units<kRows>(a, q, group);
   }
-  KvRequest q = kv_request(a, r);
-  int units = kv_units<kRows>(a, q, group);
-  bool left = false;  // whether this workgroup left the first part of a tile
 
   const NibbleConsts nc = nibble_consts();
   const int col = lane & 15, g = lane >> 4;
@@ -169,7 +180,8 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
   for (int u = begin; u < end;) {
     while (u >= base + units) {
       base += units;
-      q = kv_request(a, ++r);
+      ++r;
+      q = kv_request(a, r);
       units = kv_units<kRows>(a, q, group);
     }
     const int tiles = (q.n * group + kRows - 1) / kRows, span = kv_span(q);
@@ -177,7 +189,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
     const int head = seg / tiles, tile = seg - head * tiles;
     const int n = min(span - k0, end - u);
     const int row0 = tile * kRows, rows = min(kRows, q.n * group - row0);
-    const int32_t* table = a.tables + static_cast<int64_t>(r) * a.table_stride;
+    const ConstInts table = const_ints(a.tables + static_cast<int64_t>(r) * a.table_stride);
 
     const int key_end = min((k0 + n) * kUnit, q.keys);
     int key = k0 * kUnit + 32 * wave;
@@ -399,8 +411,8 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
     }
     __syncthreads();
     const bool complete = k0 == 0 && n == span;
-    // A partial result's slot: 2 w for a tile begun before this share, 2 w + 1 for one begun in it.
-    const int slot = 2 * me + (k0 == 0);
+    const uint32_t slot = 2 * me + (k0 == 0);
+    const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
     constexpr int kChunks = D / 8;
     for (int e = tid; e < rows * kChunks; e += kThreads) {
       const int row = e / kChunks, ch = e % kChunks * 8;
@@ -420,67 +432,18 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
         const int token = (row0 + row) / group;
         kv_write(a, q.row + token, head * group + row0 + row - token * group, ch, all, o);
       } else {
-        float* p = out.out + (static_cast<size_t>(slot) * kRows + row) * D + ch;
-        *reinterpret_cast<f32x4_t*>(p) = f32x4_t{o[0], o[1], o[2], o[3]};
-        *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{o[4], o[5], o[6], o[7]};
-        if (ch == 0) {
-          float* st = out.stats + (static_cast<size_t>(slot) * kRows + row) * 2;
-          st[0] = high;
-          st[1] = all;
-        }
+        const uint32_t at = slot * kRows + row;
+        store_part(ro, (at * D + ch) * 4, o);
+        if (ch == 0) store_stats(rs, at * 8, high, all);
       }
     }
-    if (!complete && k0 == 0) {
-      left = true;
-      if (tid == 0)
-        *split = KvSplit{r, head, tile, shares.owner(u + span - 1) - me + 1, slot, 2 * (me + 1)};
+    if (!complete) {
+      const int first = shares.owner(u - k0), count = shares.owner(u - k0 + span - 1) - first + 1;
+      if (kv_arrive(out.counters + first, count, &s_last))
+        kv_join<D, kThreads>(a, out, kRows, first, count, q, head, row0, rows, &s_out[0][0][0]);
     }
     u += n;
     if (u < end) __syncthreads();
-  }
-  if (!left && tid == 0) split->count = 0;
-}
-
-// Joins the partial results of the tile that worker blockIdx.x begins and others end, in the
-// workers' order: a wave a row, its lanes over the channels (and, for the statistics, over the
-// parts).
-template <int D>
-__global__ __launch_bounds__(kThreads) void kv_combine_kernel(KvAttentionArgs a, KvPartials part, int tile_rows) {
-  constexpr int kPer = D / 64;
-  const KvSplit s = part.split[blockIdx.x];
-  if (s.count <= 0) return;
-  const int lane = threadIdx.x & 63;
-  const int group = a.H / a.KV;
-  const KvRequest q = kv_request(a, s.request);
-  const int row0 = s.tile * tile_rows, rows = min(tile_rows, q.n * group - row0);
-  for (int row = wave_id() + kWaves * blockIdx.y; row < rows; row += kWaves * gridDim.y) {
-    auto at = [&](int i) {
-      return static_cast<size_t>(i == 0 ? s.first : s.next + 2 * (i - 1)) * tile_rows + row;
-    };
-    float top = -INFINITY;
-    for (int i = lane; i < s.count; i += 64) top = fmaxf(top, part.stats[at(i) * 2]);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float ref = top == -INFINITY ? 0.0f : top;
-    float sum = 0.0f, o[kPer] = {};
-    for (int b = 0; b < s.count; b += 64) {
-      float f = 0.0f;
-      if (b + lane < s.count) {
-        const float* st = part.stats + at(b + lane) * 2;
-        f = __builtin_amdgcn_exp2f((st[0] - ref) * a.scale_log2e);
-        sum += f * st[1];
-      }
-      const int n = min(64, s.count - b);
-      for (int j = 0; j < n; ++j) {
-        const float fj = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f), j));
-        const float* p = part.out + at(b + j) * D + lane * kPer;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) o[i] += fj * p[i];
-      }
-    }
-    sum = wave_sum64(sum);
-    const int token = (row0 + row) / group;
-    kv_write(a, q.row + token, s.head * group + row0 + row - token * group, lane * kPer, sum, o);
   }
 }
 
@@ -505,7 +468,7 @@ KvPlan kv_plan(const KvAttentionArgs& a) {
   const int64_t tiles = (tile_rows + 16 * p.mt - 1) / (16 * p.mt);
   const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
   const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
-  const int64_t fill = p.mt == 1 ? 768 : 512;
+  const int64_t fill = p.mt == 1 ? kKvSplitWorkers : 512;
   p.split_workers = static_cast<int>(most < fill ? most : fill);
   p.prompt_workers = prompts ? kKvPromptWorkers : 0;
   return p;
@@ -516,39 +479,33 @@ size_t align256(size_t n) { return (n + 255) / 256 * 256; }
 // A kernel's part of the workspace: partial results of 2 tiles of `rows` rows a worker.
 size_t partials_bytes(int workers, int rows, int D) {
   const size_t n = static_cast<size_t>(2) * workers * rows;
-  return align256(n * D * sizeof(float)) + align256(n * 2 * sizeof(float)) + align256(workers * sizeof(KvSplit));
+  return align256(n * D * sizeof(float)) + align256(n * 2 * sizeof(float));
 }
 
-KvPartials partials_at(char* ws, int workers, int rows, int D) {
+KvPartials partials_at(char* ws, int* counters, int workers, int rows, int D) {
   const size_t n = static_cast<size_t>(2) * workers * rows;
   KvPartials part;
   part.out = reinterpret_cast<float*>(ws);
-  ws += align256(n * D * sizeof(float));
-  part.stats = reinterpret_cast<float*>(ws);
-  ws += align256(n * 2 * sizeof(float));
-  part.split = reinterpret_cast<KvSplit*>(ws);
+  part.stats = reinterpret_cast<float*>(ws + align256(n * D * sizeof(float)));
+  part.out_bytes = static_cast<uint32_t>(n * D * sizeof(float));
+  part.stats_bytes = static_cast<uint32_t>(n * 2 * sizeof(float));
+  part.counters = counters;
   return part;
 }
 
 template <int D>
-hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, hipStream_t stream) {
+hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, int* counters, hipStream_t stream) {
   const int rows = 16 * p.mt;
-  const KvPartials split = partials_at(ws, p.split_workers, rows, D);
+  const KvPartials split = partials_at(ws, counters, p.split_workers, rows, D);
   if (p.mt == 1)
     kv_attention_kernel<D, 1><<<p.split_workers, kThreads, 0, stream>>>(a, split);
   else
     kv_attention_kernel<D, 2><<<p.split_workers, kThreads, 0, stream>>>(a, split);
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const int64_t most = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
-  const int y = static_cast<int>(((most < rows ? most : rows) + kWaves - 1) / kWaves);
-  kv_combine_kernel<D><<<dim3(p.split_workers, y > 0 ? y : 1), kThreads, 0, stream>>>(a, split, rows);
-  if ((e = hipGetLastError()) != hipSuccess || p.prompt_workers == 0) return e;
-  const KvPartials prompt =
-      partials_at(ws + partials_bytes(p.split_workers, rows, D), p.prompt_workers, kKvPromptRows, D);
-  if ((e = launch_kv_prompt(a, prompt, p.prompt_workers, stream)) != hipSuccess) return e;
-  kv_combine_kernel<D><<<dim3(p.prompt_workers, kKvPromptRows / kWaves), kThreads, 0, stream>>>(a, prompt, kKvPromptRows);
-  return hipGetLastError();
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || p.prompt_workers == 0) return e;
+  const KvPartials prompt = partials_at(ws + partials_bytes(p.split_workers, rows, D), counters + kKvSplitWorkers,
+                                        p.prompt_workers, kKvPromptRows, D);
+  return launch_kv_prompt(a, prompt, p.prompt_workers, stream);
 }
 
 }  // namespace
@@ -559,12 +516,12 @@ size_t kv_attention_workspace(const KvAttentionArgs& a) {
          (p.prompt_workers ? partials_bytes(p.prompt_workers, kKvPromptRows, a.D) : 0);
 }
 
-hipError_t launch_kv_attention(const KvAttentionArgs& args, void* workspace, hipStream_t stream) {
+hipError_t launch_kv_attention(const KvAttentionArgs& args, void* workspace, int* counters, hipStream_t stream) {
   const KvPlan p = kv_plan(args);
   KvAttentionArgs a = args;
   a.split_rows = p.split_rows;
   char* ws = static_cast<char*>(workspace);
-  return a.D == 64 ? launch<64>(a, p, ws, stream) : launch<128>(a, p, ws, stream);
+  return a.D == 64 ? launch<64>(a, p, ws, counters, stream) : launch<128>(a, p, ws, counters, stream);
 }
 
 }  // namespace w4a16

@@ -56,6 +56,8 @@ struct KvAttentionArgs {
   bool zero_tail;
 };
 size_t kv_attention_workspace(const KvAttentionArgs& a);
-hipError_t launch_kv_attention(const KvAttentionArgs& a, void* workspace, hipStream_t stream);
+// counters: kKvAttentionCounters ints, zero before and after the call's kernels.
+constexpr int kKvAttentionCounters = 1024;
+hipError_t launch_kv_attention(const KvAttentionArgs& a, void* workspace, int* counters, hipStream_t stream);
 
 }  // namespace w4a16

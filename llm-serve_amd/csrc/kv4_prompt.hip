@@ -111,6 +111,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   constexpr int kSteps = D / 16, kTiles = D / 32;
   __shared__ __align__(16) uint16_t s_k[2][kKeys][kPitchK];
   __shared__ __align__(16) uint16_t s_v[2][D][kPitchV];
+  __shared__ int s_last;
   __shared__ uint64_t s_held[2][4];  // 4 bits a key: whether it is in the sequence and on a page
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
@@ -119,17 +120,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   // the same kv heads, whose pages then stay in that XCD's L2.
   const int per_xcd = gridDim.x / 8;
   const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
-  KvSplit* split = out.split + me;
 
   int64_t sum = 0;
   for (int r = lane; r < a.R; r += 64) sum += kv_request_cost(a, kv_request(a, r), group);
   const int64_t total = __shfl(wave_scan64(sum, lane), 63);
   const int64_t fit = (total + kMinShare - 1) / kMinShare;
   const int workers = fit < gridDim.x ? static_cast<int>(fit) : gridDim.x;
-  if (me >= workers) {
-    if (tid == 0) split->count = 0;
-    return;
-  }
+  if (me >= workers) return;
   const int64_t begin = share(total, workers, me), end = share(total, workers, me + 1);
   int r = 0;
   int64_t base = 0;
@@ -147,7 +144,6 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   }
   r = __builtin_amdgcn_readfirstlane(r);
   KvRequest q = kv_request(a, r);
-  bool left = false;
 
   const FusedConsts fc = fused_consts();
   const int col = lane & 31, h = lane >> 5;
@@ -157,7 +153,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     KvTileCosts costs = kv_costs(a, q, group);
     while (u >= base + costs.before(costs.tiles) * a.KV) {
       base += costs.before(costs.tiles) * a.KV;
-      q = kv_request(a, ++r);
+      ++r;
+      q = kv_request(a, r);
       costs = kv_costs(a, q, group);
     }
     const int64_t a_head = costs.before(costs.tiles);
@@ -176,7 +173,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     // The share's part of the tile's keys, in proportion to the cost.
     const int t0 = static_cast<int>(x0 * key_tiles / cost), t1 = static_cast<int>(x1 * key_tiles / cost);
     const bool complete = x0 == 0 && x1 == cost;
-    const int32_t* table = a.tables + static_cast<int64_t>(r) * a.table_stride;
+    const ConstInts table = const_ints(a.tables + static_cast<int64_t>(r) * a.table_stride);
 
     // This thread's part of a key tile.  K (waves 0 .. 3): D / 4 channels of one key.  V (waves 4
     // .. 7): D / 32 channels of the 8 keys of one lane half and contraction step, two quads.
@@ -439,9 +436,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     const u32x2_t both = __builtin_bit_cast(
         u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(row_sum), __float_as_uint(row_sum), false, false));
     row_sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-    const int slot = 2 * me + (x0 == 0);
+    const uint32_t at = (2 * me + (x0 == 0)) * kKvPromptRows + 32 * wave + col;
+    const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
     if (live) {
-      const size_t at = static_cast<size_t>(slot) * kKvPromptRows + 32 * wave + col;
 #pragma unroll
       for (int c = 0; c < kTiles; ++c)
 #pragma unroll
@@ -451,25 +448,22 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
           if (complete)
             kv_write(a, q.row + token, qh, ch, row_sum, o);
           else
-            *reinterpret_cast<f32x4_t*>(out.out + at * D + ch) = f32x4_t{o[0], o[1], o[2], o[3]};
+            store_fragment(ro, (at * D + ch) * 4, f32x4_t{o[0], o[1], o[2], o[3]});
         }
-      if (!complete && h == 0) {
-        out.stats[at * 2] = row_max;
-        out.stats[at * 2 + 1] = row_sum;
-      }
+      if (!complete && h == 0) store_stats(rs, at * 8, row_max, row_sum);
     }
-    if (!complete && x0 == 0) {
-      left = true;
-      if (tid == 0) {
-        // the worker whose share holds the tile's last unit
-        const int64_t last = u + cost - 1;
-        int owner = static_cast<int>(((last + 1) * workers - 1) / total);
-        *split = KvSplit{r, head, tile, owner - me + 1, slot, 2 * (me + 1)};
+    if (!complete) {
+      // the workers whose shares hold the tile's first and last unit
+      const int64_t unit = u - x0;
+      const int first = static_cast<int>(((unit + 1) * workers - 1) / total);
+      const int count = static_cast<int>(((unit + cost) * workers - 1) / total) - first + 1;
+      if (kv_arrive(out.counters + first, count, &s_last)) {
+        kv_join<D, kPromptThreads>(a, out, kKvPromptRows, first, count, q, head, row0, rows, reinterpret_cast<float*>(s_k));
+        __syncthreads();  // before the next tile's keys overwrite the scratch
       }
     }
     u += x1 - x0;
   }
-  if (!left && tid == 0) split->count = 0;
 }
 
 }  // namespace

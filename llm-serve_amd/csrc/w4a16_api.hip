@@ -1351,7 +1351,7 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
                        const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
                        const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale, int T,
                        int R, int H, int KV, int D, int num_blocks, int block_size, int width, int max_query_len,
-                       int zero_tail, void* workspace, size_t workspace_bytes, void* stream) {
+                       int zero_tail, void* workspace, size_t workspace_bytes, int32_t* counters, void* stream) {
   int log2_block = 0;
   int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block);
   if (e != W4A16_OK) return e;
@@ -1375,7 +1375,9 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
   if (!workspace || workspace_bytes < need)
     return fail(W4A16_ERR_WORKSPACE, "attention needs %zu bytes of workspace (got %zu)", need, workspace ? workspace_bytes : size_t(0));
   if (!aligned(workspace, 16)) return fail(W4A16_ERR_ALIGN, "the workspace must be 16-byte aligned");
-  return check_launch(w4a16::launch_kv_attention(a, workspace, static_cast<hipStream_t>(stream)), "kv attention");
+  if (!counters) return fail(W4A16_ERR_WORKSPACE, "attention needs %d zeroed counters", W4A16_KV_COUNTERS);
+  static_assert(W4A16_KV_COUNTERS == w4a16::kKvAttentionCounters, "the counters of the ABI and of the kernels");
+  return check_launch(w4a16::launch_kv_attention(a, workspace, counters, static_cast<hipStream_t>(stream)), "kv attention");
 }
 
 }  // extern "C"

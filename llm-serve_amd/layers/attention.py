@@ -16,13 +16,15 @@ one zero point z, as a group of an AWQ weight is; a channel stands for s * (c - 
 channels that is 68 bytes for a row of 256.
 
 Everything runs in the HIP library and raises without it or without a GPU; nothing synchronises
-the host, and every call may be captured in a HIP graph.  ``attention_int4`` takes its workspace
-from torch's allocator on each call (inside a capture: from the graph's own pool), so calls on
-several streams, and several graphs, share none.
+the host (but for the first ``attention_int4`` on a device, which sets up its counters), and every
+call may be captured in a HIP graph.  ``attention_int4`` takes its workspace from torch's allocator
+on each call (inside a capture: from the graph's own pool) and its counters from ``COUNTERS``, so
+calls on several streams, and several graphs, share neither.
 """
 from __future__ import annotations
 
 import functools
+import threading
 from dataclasses import dataclass
 
 import torch
@@ -181,6 +183,54 @@ def _workspace_bytes(*sizes: int) -> int:
     return lib().kv_attention_workspace(*sizes)
 
 
+class _CounterPool:
+    """Arrival counters of ``attention_int4``: 1024 int32 a call, zero before and after it.
+
+    Calls of one stream run in order and share one set.  A captured call gets a set of its own, for
+    good: its graph may be replayed beside anything else.  Sets come from one zeroed array a device
+    (16 MiB: 4096 sets), made by the device's first eager call, which waits for the zeros.  A call
+    without a set left, or captured before that array exists, takes a new zeroed tensor (inside a
+    capture its graph clears it on every replay)."""
+
+    SETS = 4096
+    SIZE = 1024
+
+    def __init__(self):
+        self._lock = threading.Lock()
+        self._free: dict[int, list[torch.Tensor]] = {}
+        self._streams: dict[tuple[int, int], torch.Tensor] = {}
+        self._captured: list[torch.Tensor] = []
+
+    def get(self, device: torch.device) -> torch.Tensor:
+        index = device.index
+        if torch._C._cuda_getDevice() != index:
+            with torch.cuda.device(index):
+                return self.get(device)
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        if torch._C._cuda_isCurrentStreamCapturing():
+            with self._lock:
+                free = self._free.get(index)
+                if free:
+                    self._captured.append(free.pop())
+                    return self._captured[-1]
+            return torch.zeros(self.SIZE, dtype=torch.int32, device=device)
+        counters = self._streams.get((index, stream))
+        if counters is not None:
+            return counters
+        with self._lock:
+            if index not in self._free:
+                array = torch.zeros(self.SETS, self.SIZE, dtype=torch.int32, device=device)
+                torch.cuda.current_stream(device).synchronize()
+                self._free[index] = list(array.unbind())
+            free = self._free[index]
+            if not free:
+                return torch.zeros(self.SIZE, dtype=torch.int32, device=device)
+            return self._streams.setdefault((index, stream), free.pop())
+
+
+COUNTERS = _CounterPool()
+
+
 def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                    cu_query_lens: torch.Tensor, *, block_size: int, scale: float | None = None,
                    max_query_len: int | None = None, tree_mask: torch.Tensor | None = None,
@@ -234,7 +284,7 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
         size = _workspace_bytes(rows, requests, heads, kv_heads, head_dim, block_size, width, max_query_len)
         workspace = torch.empty(size, dtype=torch.uint8, device=device)
         lib().kv_attention(q, cache, block_tables, seq_lens.contiguous(), cu_query_lens.contiguous(), tree_mask, out,
-                           scale, block_size, max_query_len, zero_tail, workspace)
+                           scale, block_size, max_query_len, zero_tail, workspace, COUNTERS.get(device))
     return out
 
 

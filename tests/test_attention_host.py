@@ -29,7 +29,7 @@ STORE = dict(k=P, kt=1024, kh=128, v=P, vt=1024, vh=128, cache=P, slots=P, T=3, 
 LOAD = dict(cache=P, slots=P, k=P, v=P, T=3, KV=8, D=128, blocks=4, block=16, stream=None)
 ATTENTION = dict(q=P, qt=4096, qh=128, cache=P, tables=P, stride=8, seq=P, cu=P, mask=None, out=P,
                  scale=ctypes.c_float(0.1), T=3, R=2, H=32, KV=8, D=128, blocks=4, block=16, width=8, longest=1, zero=1,
-                 ws=P, ws_bytes=1 << 40, stream=None)
+                 ws=P, ws_bytes=1 << 40, counters=P, stream=None)
 
 
 @pytest.mark.parametrize("change,status,message", [
@@ -66,7 +66,7 @@ def test_load_refusals(pkg, dll, change, status, message):
     ({"scale": ctypes.c_float(0.0)}, 1, "scale"), ({"scale": ctypes.c_float(-1.0)}, 1, "scale"),
     ({"scale": ctypes.c_float(float("nan"))}, 1, "scale"), ({"scale": ctypes.c_float(float("inf"))}, 1, "scale"),
     ({"q": P + 8}, 3, "aligned"), ({"qt": 4097}, 3, "multiples of 8"), ({"out": P + 8}, 3, "aligned"),
-    ({"ws": None}, 4, "workspace"), ({"ws_bytes": 64}, 4, "workspace"), ({"ws": P + 4}, 3, "aligned"),
+    ({"ws": None}, 4, "workspace"), ({"ws_bytes": 64}, 4, "workspace"), ({"ws": P + 4}, 3, "aligned"), ({"counters": None}, 4, "counters"),
     ({"T": 1 << 28}, 2, "too many"), ({"T": 1 << 18, "width": 1 << 20, "stride": 1 << 20}, 2, "too much work")])
 def test_attention_refusals(pkg, dll, change, status, message):
     assert dll.w4a16_kv_attention(*{**ATTENTION, **change}.values()) == status and message in error(pkg)

@@ -307,3 +307,64 @@ def test_extreme_prompt_queries(gpu_lib):
     b.qkv[5, 0, 0] = float("inf")
     out = b.run()
     assert bool(torch.isnan(out[5, 0].float()).all()) and bool(torch.isfinite(out[5, 1:].float()).all())
+
+
+def test_graphs_replayed_beside_each_other(gpu_lib):
+    """Two captured graphs of split work replayed on two streams while eager calls run on a third:
+    none shares a workspace or counters with another."""
+    b = Batch([1, 40], [3000, 900], 8, 2, 128, 16, seed=31)
+    args = b.args()
+    want = attn.attention_int4(*args, block_size=16, max_query_len=40)
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = [attn.attention_int4(*args, block_size=16, max_query_len=40) for _ in range(4)]
+        graphs.append((graph, outs, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for graph, outs, stream in graphs:
+            for o in outs:
+                o.fill_(3)
+        torch.cuda.synchronize()
+        for graph, outs, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        eager = [attn.attention_int4(*args, block_size=16, max_query_len=40) for _ in range(4)]
+        torch.cuda.synchronize()
+        for o in eager + graphs[0][1] + graphs[1][1]:
+            assert torch.equal(o, want)
+
+
+def test_capture_without_reserved_counters(gpu_lib, monkeypatch):
+    """A pool that has no set yet (or none left) gives a captured call a tensor that its graph clears."""
+    monkeypatch.setattr(attn, "COUNTERS", attn._CounterPool())
+    b = Batch([1, 3], [2500, 700], 8, 2, 128, 16, seed=32)
+    args = b.args()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = attn.attention_int4(*args, block_size=16)
+    want = attn.attention_int4(*args, block_size=16)
+    for _ in range(3):
+        out.fill_(5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+    pool = attn.COUNTERS
+    pool._free[0].clear()
+    pool._streams.clear()
+    assert torch.equal(attn.attention_int4(*args, block_size=16), want)
+
+
+def test_counters_are_left_zero(gpu_lib):
+    b = Batch([1, 300, 5], [3000, 900, 900], 8, 2, 128, 16, seed=33)
+    counters = torch.zeros(1024, dtype=torch.int32, device="cuda")
+    size = gpu_lib.kv_attention_workspace(306, 3, 8, 2, 128, 16, b.width, 300)
+    workspace = torch.full((size,), 255, dtype=torch.uint8, device="cuda")
+    q, cache, tables, seq, offsets = b.args()
+    out = torch.empty(306, 8, 128, dtype=torch.bfloat16, device="cuda")
+    gpu_lib.kv_attention(q, cache, tables, seq, offsets, None, out, 128 ** -0.5, 16, 300, True, workspace, counters)
+    torch.cuda.synchronize()
+    assert not bool(counters.any())
+    b.check(out)
