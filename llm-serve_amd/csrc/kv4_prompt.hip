@@ -23,6 +23,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
 constexpr int kTileCost = 16;  // cost units of a tile of keys
+constexpr int kSetupCost = 16;  // of a row tile besides its keys
 constexpr int kMinShare = 4 * kTileCost;
 constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
@@ -30,23 +31,14 @@ __device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-__device__ __forceinline__ int64_t wave_scan64(int64_t v, int lane) {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t u = __shfl_up(v, d);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-
 // Cost of a request's row tiles in sixteenths of a key tile: tile j of a head costs first +
-// step j, its keys growing with its last token (all keys under a tree mask), plus one key tile
-// for its own set-up.
+// step j, its keys growing with its last token (all keys under a tree mask), plus its set-up.  Host checks keep all sums below 2^31.
 struct KvTileCosts {
-  int tiles;
-  int64_t first, step;
-  __device__ __forceinline__ int64_t before(int j) const { return j * first + step * j * (j - 1) / 2; }
-  __device__ __forceinline__ int64_t of(int j) const { return first + step * j; }
+  int tiles, first, step;
+  __device__ __forceinline__ int before(int j) const {
+    return j * first + static_cast<int>(static_cast<unsigned>(step) * static_cast<unsigned>(j) * static_cast<unsigned>(j - 1) / 2u);
+  }
+  __device__ __forceinline__ int of(int j) const { return first + step * j; }
 };
 
 __device__ __forceinline__ KvTileCosts kv_costs(const KvAttentionArgs& a, const KvRequest& q, int group) {
@@ -54,17 +46,16 @@ __device__ __forceinline__ KvTileCosts kv_costs(const KvAttentionArgs& a, const 
   const int rows = q.n * group;
   c.tiles = rows > a.split_rows ? (rows + kKvPromptRows - 1) / kKvPromptRows : 0;
   c.step = a.tree_mask ? 0 : (kKvPromptRows / 4 + group - 1) / group;
-  c.first = (a.tree_mask ? q.keys : max(q.cached, 0)) / (kKeys / kTileCost) + c.step + kTileCost;
+  c.first = min(a.tree_mask ? q.keys : max(q.cached, 0), q.keys) / (kKeys / kTileCost) + c.step + kSetupCost;
   return c;
 }
 
-__device__ __forceinline__ int64_t kv_request_cost(const KvAttentionArgs& a, const KvRequest& q, int group) {
+__device__ __forceinline__ int kv_request_cost(const KvAttentionArgs& a, const KvRequest& q, int group) {
   const KvTileCosts c = kv_costs(a, q, group);
   return c.before(c.tiles) * a.KV;
 }
 
-// Share w of `total` cost units.
-__device__ __forceinline__ int64_t share(int64_t total, int workers, int w) { return total * w / workers; }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // Codes -> fp32 without a conversion: a nibble in the low bits of an fp16 1024.0 is 1024 + c, one
 // in bits 4 .. 7 of an fp16 64.0 is 64 + c, and v_fma_mix_f32 takes either half of the register as
@@ -121,57 +112,58 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const int per_xcd = gridDim.x / 8;
   const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
 
-  int64_t sum = 0;
+  int sum = 0;
   for (int r = lane; r < a.R; r += 64) sum += kv_request_cost(a, kv_request(a, r), group);
-  const int64_t total = __shfl(wave_scan64(sum, lane), 63);
-  const int64_t fit = (total + kMinShare - 1) / kMinShare;
-  const int workers = fit < gridDim.x ? static_cast<int>(fit) : gridDim.x;
+  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int workers = min(static_cast<int>(gridDim.x), (total + kMinShare - 1) / kMinShare);
   if (me >= workers) return;
-  const int64_t begin = share(total, workers, me), end = share(total, workers, me + 1);
-  int r = 0;
-  int64_t base = 0;
+  const KvShares shares{uniform(total / workers), uniform(total % workers)};
+  const int begin = shares.begin(me), end = shares.begin(me + 1);
+  int r = 0, base = 0;
   for (;; r += 64) {
-    const int64_t cost = r + lane < a.R ? kv_request_cost(a, kv_request(a, r + lane), group) : 0;
-    const int64_t upto = wave_scan64(cost, lane);
+    const int cost = r + lane < a.R ? kv_request_cost(a, kv_request(a, r + lane), group) : 0;
+    const int upto = wave_scan(cost);
     const uint64_t past = __ballot(base + upto > begin);
     if (past || r + 64 >= a.R) {
       const int first = past ? __builtin_ctzll(past) : 0;
-      base += __shfl(upto - cost, first);
+      base += __builtin_amdgcn_readlane(upto - cost, first);
       r += first;
       break;
     }
-    base += __shfl(upto, 63);
+    base += __builtin_amdgcn_readlane(upto, 63);
   }
-  r = __builtin_amdgcn_readfirstlane(r);
   KvRequest q = kv_request(a, r);
 
   const FusedConsts fc = fused_consts();
   const int col = lane & 31, h = lane >> 5;
   const float scale = a.scale_log2e;
 
-  for (int64_t u = begin; u < end;) {
+  for (int u = begin; u < end;) {
     KvTileCosts costs = kv_costs(a, q, group);
-    while (u >= base + costs.before(costs.tiles) * a.KV) {
-      base += costs.before(costs.tiles) * a.KV;
+    int a_head = costs.before(costs.tiles);
+    while (u >= base + a_head * a.KV) {
+      base += a_head * a.KV;
       ++r;
       q = kv_request(a, r);
       costs = kv_costs(a, q, group);
+      a_head = costs.before(costs.tiles);
     }
-    const int64_t a_head = costs.before(costs.tiles);
-    const int head = static_cast<int>((u - base) / a_head);
-    const int64_t x = u - base - head * a_head;
+    const int head = uniform((u - base) / a_head);
+    const int x = u - base - head * a_head;
     int tile = 0, over = costs.tiles;  // the last tile that begins at or before x
     while (over - tile > 1) {
       const int mid = (tile + over) >> 1;
       if (costs.before(mid) <= x) tile = mid; else over = mid;
     }
-    const int64_t cost = costs.of(tile), x0 = x - costs.before(tile);
-    const int64_t x1 = min(cost, x0 + end - u);
+    const int cost = costs.of(tile), x0 = x - costs.before(tile);
+    const int x1 = min(cost, x0 + end - u);
     const int row0 = tile * kKvPromptRows, rows = min(kKvPromptRows, q.n * group - row0);
-    const int key_end = a.tree_mask ? q.keys : max(min(q.cached + (row0 + rows - 1) / group + 1, q.keys), 0);
+    const int key_end = a.tree_mask ? q.keys : max(min(q.cached + uniform((row0 + rows - 1) / group) + 1, q.keys), 0);
     const int key_tiles = (key_end + kKeys - 1) / kKeys;
-    // The share's part of the tile's keys, in proportion to the cost.
-    const int t0 = static_cast<int>(x0 * key_tiles / cost), t1 = static_cast<int>(x1 * key_tiles / cost);
+    // The share's part of the tile's keys, in proportion to the cost; both sides of a border
+    // evaluate the same expression, exact at 0 and at the whole cost.
+    const double per_unit = static_cast<double>(key_tiles);
+    const int t0 = uniform(static_cast<int>(x0 * per_unit / cost)), t1 = uniform(static_cast<int>(x1 * per_unit / cost));
     const bool complete = x0 == 0 && x1 == cost;
     const ConstInts table = const_ints(a.tables + static_cast<int64_t>(r) * a.table_stride);
 
@@ -357,6 +349,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
           for (int j = 0; j < 4; ++j) sc[j & 1] = mfma32(frag[i & 1][j], qf[2 * i + (j >> 1)], sc[j & 1]);
           __builtin_amdgcn_sched_barrier(0);
         }
+        read_v(0, frag[0]);
+        __builtin_amdgcn_sched_barrier(0);
         const uint64_t held_keys[4] = {s_held[buf][0], s_held[buf][1], s_held[buf][2], s_held[buf][3]};
         const bool all_held = (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
         if (!(key0 + kKeys <= all_see && all_held)) {
@@ -411,6 +405,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
+            if (2 * n + s < 3) read_v(2 * n + s + 1, frag[(s + 1) & 1]);
             u32x4_t w;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -423,10 +418,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
             }
             const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
 #pragma unroll
-            for (int c = 0; c < kTiles; ++c) {
-              const bf16x8_t vf = *reinterpret_cast<const bf16x8_t*>(&s_v[buf][32 * c + col][8 * (4 * n + 2 * s + h)]);
-              acc[c] = mfma32(vf, pf, acc[c]);
-            }
+            for (int c = 0; c < kTiles; ++c) acc[c] = mfma32(frag[s & 1][c], pf, acc[c]);
           }
       }
       if (converts_v) next_tile();
@@ -453,10 +445,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
       if (!complete && h == 0) store_stats(rs, at * 8, row_max, row_sum);
     }
     if (!complete) {
-      // the workers whose shares hold the tile's first and last unit
-      const int64_t unit = u - x0;
-      const int first = static_cast<int>(((unit + 1) * workers - 1) / total);
-      const int count = static_cast<int>(((unit + cost) * workers - 1) / total) - first + 1;
+      const int first = shares.owner(u - x0), count = shares.owner(u - x0 + cost - 1) - first + 1;
       if (kv_arrive(out.counters + first, count, &s_last)) {
         kv_join<D, kPromptThreads>(a, out, kKvPromptRows, first, count, q, head, row0, rows, reinterpret_cast<float*>(s_k));
         __syncthreads();  // before the next tile's keys overwrite the scratch
