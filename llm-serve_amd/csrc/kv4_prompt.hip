@@ -24,7 +24,7 @@ constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
 constexpr int kTileCost = 16;  // cost units of a tile of keys
 constexpr int kSetupCost = 16;  // of a row tile besides its keys
-constexpr int kMinShare = 4 * kTileCost;
+constexpr int kMinShare = 8 * kTileCost;
 constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
 __device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
@@ -94,6 +94,58 @@ __device__ __forceinline__ void four_values(float (&f)[4], uint32_t w, const Row
   f[1] = __builtin_fmaf(static_cast<float>(a[1]), r.s, r.low);
   f[2] = __builtin_fmaf(static_cast<float>(b[0]), r.s, r.high);
   f[3] = __builtin_fmaf(static_cast<float>(b[1]), r.s, r.high);
+}
+
+// Byte offset of a lane's fragment f (four channels: 32 (f / 4) + 8 (f % 4) + 4 (lane / 32) ..) of
+// its wave's 32 rows in slot `slot`: whole waves of 16 bytes a lane, in the accumulators' layout.
+template <int D>
+__device__ __forceinline__ uint32_t part_offset(int slot, int wave, int f, int lane) {
+  return ((static_cast<uint32_t>(slot) * 8 + wave) * (D / 8) + f) * 1024u + lane * 16u;
+}
+
+// Joins a tile's `count` parts, from worker `first` on: every lane its own rows' fragments, two
+// parts' loads in flight.
+template <int D>
+__device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPartials& part, int first, int count, int wave,
+                                           int lane, bool live, int out_row, int out_head) {
+  constexpr int kFrags = D / 8, kBatch = 2;
+  const __amdgpu_buffer_rsrc_t ro = make_buffer(part.out, part.out_bytes), rs = make_buffer(part.stats, part.stats_bytes);
+  float top = -INFINITY, sum = 0.0f;
+  f32x4_t acc[kFrags];
+#pragma unroll
+  for (int f = 0; f < kFrags; ++f) acc[f] = f32x4_t{0, 0, 0, 0};
+  for (int i0 = 0; i0 < count; i0 += kBatch) {
+    f32x4_t v[kBatch][kFrags];
+    u32x2_t st[kBatch];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int i = i0 + b, slot = i == 0 ? 2 * first + 1 : 2 * (first + i);
+      const bool in = live && i < count;  // other loads touch nothing and give zeros
+      const uint32_t row = static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + (lane & 31);
+      st[b] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, in ? row * 8 : kOutOfRange, 0, kCoherentPolicy));
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f) v[b][f] = load_fragment(ro, in ? part_offset<D>(slot, wave, f, lane) : kOutOfRange);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const uint32_t mb = st[b][0], lb = st[b][1];
+      const float m = i0 + b < count ? __uint_as_float(mb) : -INFINITY;
+      const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
+      const float x = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e), y = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2e);
+      top = next;
+      sum = sum * x + __uint_as_float(lb) * y;
+#pragma unroll
+      for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[f][j] = acc[f][j] * x + v[b][f][j] * y;
+    }
+  }
+  if (!live) return;
+#pragma unroll
+  for (int f = 0; f < kFrags; ++f) {
+    const float o[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]};
+    kv_write(a, out_row, out_head, 32 * (f >> 2) + 8 * (f & 3) + 4 * (lane >> 5), sum, o);
+  }
 }
 
 template <int D>
@@ -428,28 +480,25 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     const u32x2_t both = __builtin_bit_cast(
         u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(row_sum), __float_as_uint(row_sum), false, false));
     row_sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-    const uint32_t at = (2 * me + (x0 == 0)) * kKvPromptRows + 32 * wave + col;
+    const int slot = 2 * me + (x0 == 0);
     const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
     if (live) {
 #pragma unroll
-      for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-          const float o[4] = {acc[c][4 * b], acc[c][4 * b + 1], acc[c][4 * b + 2], acc[c][4 * b + 3]};
-          const int ch = 32 * c + 8 * b + 4 * h;
-          if (complete)
-            kv_write(a, q.row + token, qh, ch, row_sum, o);
-          else
-            store_fragment(ro, (at * D + ch) * 4, f32x4_t{o[0], o[1], o[2], o[3]});
-        }
-      if (!complete && h == 0) store_stats(rs, at * 8, row_max, row_sum);
+      for (int f = 0; f < D / 8; ++f) {
+        const int c = f >> 2, b = f & 3;
+        const float o[4] = {acc[c][4 * b], acc[c][4 * b + 1], acc[c][4 * b + 2], acc[c][4 * b + 3]};
+        if (complete)
+          kv_write(a, q.row + token, qh, 32 * c + 8 * b + 4 * h, row_sum, o);
+        else
+          store_fragment(ro, part_offset<D>(slot, wave, f, lane), f32x4_t{o[0], o[1], o[2], o[3]});
+      }
+      if (!complete && h == 0)
+        store_stats(rs, (static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + col) * 8, row_max, row_sum);
     }
     if (!complete) {
       const int first = shares.owner(u - x0), count = shares.owner(u - x0 + cost - 1) - first + 1;
-      if (kv_arrive(out.counters + first, count, &s_last)) {
-        kv_join<D, kPromptThreads>(a, out, kKvPromptRows, first, count, q, head, row0, rows, reinterpret_cast<float*>(s_k));
-        __syncthreads();  // before the next tile's keys overwrite the scratch
-      }
+      if (kv_arrive(out.counters + first, count, &s_last))
+        join_parts<D>(a, out, first, count, wave, lane, live, q.row + token, qh);
     }
     u += x1 - x0;
   }
