@@ -18,6 +18,9 @@ REGIME_NONE = 0
 REGIME_DECODE = 1
 REGIME_TILE = 2
 
+_current_device = torch._C._cuda_getDevice
+_current_stream = torch._C._cuda_getCurrentRawStream
+
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t
 _c_ptr = ctypes.c_void_p
@@ -300,24 +303,48 @@ class W4A16Library:
                      regime, p0, p1, p2, split, ws_ptr, ws_len)
         return y
 
+    # The KV entry points are called once or twice a layer with few rows, where their host time
+    # counts: the common case (the tensors' GPU is current) goes straight to the C call.
     def kv_step(self, query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions, slots,
                 blocks_used, block_size: int) -> None:
-        self._launch(self.dll.w4a16_kv_step, "w4a16_kv_step", query_lens, query_lens.data_ptr(),
-                     context_lens.data_ptr(), tables.data_ptr(), tables.stride(0), free_blocks.data_ptr(),
-                     cu_query_lens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(),
-                     blocks_used.data_ptr(), query_lens.shape[0], tables.shape[1], free_blocks.shape[0], block_size,
-                     positions.shape[0])
+        index = query_lens.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.kv_step(query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions,
+                                    slots, blocks_used, block_size)
+        status = self.dll.w4a16_kv_step(
+            query_lens.data_ptr(), context_lens.data_ptr(), tables.data_ptr(), tables.stride(0), free_blocks.data_ptr(),
+            cu_query_lens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), blocks_used.data_ptr(),
+            query_lens.shape[0], tables.shape[1], free_blocks.shape[0], block_size, positions.shape[0],
+            _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_kv_step")
 
     def kv_store(self, k, v, cache, slots, head_dim: int, block_size: int) -> None:
         """Rows k, v [T, KV, D] quantized into the cache's slots."""
-        self._launch(self.dll.w4a16_kv_store, "w4a16_kv_store", cache, k.data_ptr(), k.stride(0), k.stride(1),
-                     v.data_ptr(), v.stride(0), v.stride(1), cache.data_ptr(), slots.data_ptr(), k.shape[0],
-                     cache.shape[1], head_dim, cache.shape[0], block_size)
+        index = cache.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.kv_store(k, v, cache, slots, head_dim, block_size)
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        blocks, kv_heads, _ = cache.shape
+        status = self.dll.w4a16_kv_store(k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, cache.data_ptr(), slots.data_ptr(),
+                                         k.shape[0], kv_heads, head_dim, blocks, block_size, _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_kv_store")
 
     def kv_load(self, cache, slots, k, v, head_dim: int, block_size: int) -> None:
         """The cache's rows at the slots into k, v [T, KV, D]."""
-        self._launch(self.dll.w4a16_kv_load, "w4a16_kv_load", cache, cache.data_ptr(), slots.data_ptr(), k.data_ptr(),
-                     v.data_ptr(), slots.shape[0], cache.shape[1], head_dim, cache.shape[0], block_size)
+        index = cache.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.kv_load(cache, slots, k, v, head_dim, block_size)
+        blocks, kv_heads, _ = cache.shape
+        status = self.dll.w4a16_kv_load(cache.data_ptr(), slots.data_ptr(), k.data_ptr(), v.data_ptr(), slots.shape[0],
+                                        kv_heads, head_dim, blocks, block_size, _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_kv_load")
 
     def kv_attention_workspace(self, t: int, r: int, h: int, kv: int, head_dim: int, block_size: int, width: int,
                                max_query_len: int) -> int:
@@ -327,12 +354,22 @@ class W4A16Library:
                      max_query_len: int, zero_tail: bool, workspace, counters) -> None:
         """out [T, H, D] = attention of the packed rows q over the cache's pages; counters: 1024
         zero int32 (left zero) that no other call in flight uses."""
+        index = cache.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.kv_attention(q, cache, tables, seq_lens, cu_query_lens, tree_mask, out, scale, block_size,
+                                         max_query_len, zero_tail, workspace, counters)
         t, h, d = q.shape
-        self._launch(self.dll.w4a16_kv_attention, "w4a16_kv_attention", cache, q.data_ptr(), q.stride(0), q.stride(1),
-                     cache.data_ptr(), tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(),
-                     cu_query_lens.data_ptr(), _ptr(tree_mask), out.data_ptr(), scale, t, seq_lens.shape[0], h,
-                     cache.shape[1], d, cache.shape[0], block_size, tables.shape[1], max_query_len, int(zero_tail),
-                     workspace.data_ptr(), workspace.numel(), counters.data_ptr())
+        q0, q1, _ = q.stride()
+        blocks, kv_heads, _ = cache.shape
+        requests, width = tables.shape
+        status = self.dll.w4a16_kv_attention(
+            q.data_ptr(), q0, q1, cache.data_ptr(), tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(),
+            cu_query_lens.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else None, out.data_ptr(), scale, t,
+            requests, h, kv_heads, d, blocks, block_size, width, max_query_len, zero_tail, workspace.data_ptr(),
+            workspace.numel(), counters.data_ptr(), _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_kv_attention")
 
 
 _LOCK = threading.Lock()

@@ -17,9 +17,9 @@ channels that is 68 bytes for a row of 256.
 
 Everything runs in the HIP library and raises without it or without a GPU; nothing synchronises
 the host (but for the first ``attention_int4`` on a device, which sets up its counters), and every
-call may be captured in a HIP graph.  ``attention_int4`` takes its workspace from torch's allocator
-on each call (inside a capture: from the graph's own pool) and its counters from ``COUNTERS``, so
-calls on several streams, and several graphs, share neither.
+call may be captured in a HIP graph.  ``attention_int4`` takes its workspace and counters from
+``SCRATCH``, one pair a stream and one a captured call, so calls on several streams, and several
+graphs, share neither.
 """
 from __future__ import annotations
 
@@ -30,9 +30,12 @@ from dataclasses import dataclass
 import torch
 from torch import nn
 
-from .._lib import lib
+from .._lib import _current_device, _current_stream, lib
 
 __all__ = ("Attention", "KVStep", "attention_int4", "kv_step", "load_kv_int4", "new_kv_cache_int4", "store_kv_int4")
+
+_capturing = torch._C._cuda_isCurrentStreamCapturing
+_BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 
 HEAD_DIMS = (64, 128)
 BLOCK_SIZES = (16, 32, 64, 128, 256)
@@ -65,30 +68,36 @@ def new_kv_cache_int4(num_blocks: int, block_size: int, num_kv_heads: int, head_
 
 
 def _cache_head_dim(cache: torch.Tensor, block_size: int) -> int:
+    shape = cache.shape
+    if (block_size in BLOCK_SIZES and cache.dtype is _U8 and len(shape) == 3 and cache.is_contiguous()
+            and cache.get_device() >= 0 and shape[0] > 0 and shape[1] > 0 and shape[0] * block_size < 1 << 31
+            and cache.data_ptr() % 16 == 0):
+        head_dim = shape[2] // block_size - 8
+        if head_dim in HEAD_DIMS and shape[2] == block_size * (head_dim + 8):
+            return head_dim
     _check_block_size(block_size)
     if cache.dtype != torch.uint8 or cache.ndim != 3 or not cache.is_contiguous():
         raise ValueError("a KV cache is a contiguous uint8 tensor [blocks, kv heads, page bytes]")
     if cache.device.type != "cuda":
         raise ValueError("a KV cache must be on a GPU (HIP) device")
-    head_dim = cache.shape[2] // block_size - 8
-    if head_dim not in HEAD_DIMS or cache.shape[2] != block_size * (head_dim + 8):
-        raise ValueError(f"KV page size must be block_size * (head_dim + 8) with head_dim in {HEAD_DIMS}")
     if cache.shape[0] < 1 or cache.shape[1] < 1:
         raise ValueError("a KV cache needs at least one block and one kv head")
     if cache.shape[0] * block_size >= 1 << 31:
         raise ValueError("a KV cache holds fewer than 2^31 tokens")
     if cache.data_ptr() % 16:
         raise ValueError("a KV cache must be 16-byte aligned")
-    return head_dim
+    raise ValueError(f"KV page size must be block_size * (head_dim + 8) with head_dim in {HEAD_DIMS}")
 
 
-def _rows(name: str, t: torch.Tensor, heads: int | None, head_dim: int, device: torch.device) -> torch.Tensor:
+def _rows(name: str, t: torch.Tensor, heads: int | None, head_dim: int, cache: torch.Tensor) -> torch.Tensor:
     """t as the kernels read it: [T, heads, head_dim], 16-byte aligned rows at any strides."""
-    if t.ndim != 3 or t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
+    shape = t.shape
+    if len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
         raise ValueError(f"KV {name} must be [tokens, {'heads' if heads is None else heads}, {head_dim}]")
-    if t.dtype != torch.bfloat16 or t.device != device:
+    if t.dtype is not _BF16 or t.get_device() != cache.get_device():
         raise ValueError(f"KV {name} must be a bfloat16 tensor on the cache's GPU")
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or (s0 | s1) % 8 or t.data_ptr() % 16:
         t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -117,6 +126,29 @@ def kv_step(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: 
     The host takes the first ``blocks_used`` entries off its free list (it can count them from the
     lengths without reading the tensor).  A token for which the list or the table's width is too
     short gets slot -1, and -1 as its table entry; ``blocks_used`` then exceeds the list."""
+    index, requests = query_lens.get_device(), query_lens.shape[0] if query_lens.ndim == 1 else 0
+    shape = block_tables.shape
+    if not (index >= 0 and 0 < requests <= MAX_STEP_REQUESTS and 0 <= num_tokens <= MAX_STEP_TOKENS
+            and block_size in BLOCK_SIZES
+            and query_lens.dtype is _I32 and query_lens.is_contiguous()
+            and context_lens.dtype is _I32 and context_lens.get_device() == index
+            and context_lens.is_contiguous() and context_lens.shape == (requests,)
+            and free_blocks.dtype is _I32 and free_blocks.get_device() == index
+            and free_blocks.is_contiguous() and free_blocks.ndim == 1
+            and block_tables.dtype is _I32 and block_tables.get_device() == index
+            and block_tables.is_contiguous() and len(shape) == 2 and shape[0] == requests and shape[1] > 0):
+        query_lens, context_lens, block_tables, free_blocks = _check_step(query_lens, context_lens, block_tables,
+                                                                          free_blocks, block_size, num_tokens)
+    # one allocation: offsets, lengths, blocks used, positions, slots
+    size = 2 * requests + 2 + 2 * num_tokens
+    out = torch.empty_strided((size,), (1,), dtype=_I32, device=index)
+    cu, seq, used, positions, slots = out.split_with_sizes((requests + 1, requests, 1, num_tokens, num_tokens))
+    lib().kv_step(query_lens, context_lens, block_tables, free_blocks, cu, seq, positions, slots, used, block_size)
+    return KVStep(cu, seq, positions, slots, block_tables, used)
+
+
+def _check_step(query_lens, context_lens, block_tables, free_blocks, block_size, num_tokens):
+    """The argument errors of ``kv_step``; its arguments as the kernel reads them."""
     _check_block_size(block_size)
     if query_lens.device.type != "cuda":
         raise ValueError("KV step lengths must be GPU (HIP) tensors")
@@ -136,12 +168,7 @@ def kv_step(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: 
         raise ValueError("KV block_tables rows must be contiguous and must not overlap")
     if requests == 1 and block_tables.stride(0) < block_tables.shape[1]:
         block_tables = block_tables.as_strided(block_tables.shape, (block_tables.shape[1], 1))
-    # one allocation: offsets, lengths, blocks used, positions, slots
-    out = torch.empty(2 * requests + 2 + 2 * num_tokens, dtype=torch.int32, device=device)
-    cu, seq, used, positions, slots = out.split([requests + 1, requests, 1, num_tokens, num_tokens])
-    lib().kv_step(query_lens.contiguous(), context_lens.contiguous(), block_tables, free_blocks.contiguous(), cu, seq,
-                  positions, slots, used, block_size)
-    return KVStep(cu, seq, positions, slots, block_tables, used)
+    return query_lens.contiguous(), context_lens.contiguous(), block_tables, free_blocks.contiguous()
 
 
 def store_kv_int4(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor, *,
@@ -153,9 +180,10 @@ def store_kv_int4(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: 
     Per row: s = bf16((max(x, 0) - min(x, 0)) / 15), z = round(-min(x, 0) / s),
     c = clamp(round(x / s) + z, 0, 15).  A row that holds a NaN or an infinity is stored as NaN."""
     head_dim = _cache_head_dim(cache, block_size)
-    k = _rows("keys", k, cache.shape[1], head_dim, cache.device)
-    v = _rows("values", v, cache.shape[1], head_dim, cache.device)
-    _require_int32(cache.device, slots=slots)
+    k = _rows("keys", k, cache.shape[1], head_dim, cache)
+    v = _rows("values", v, cache.shape[1], head_dim, cache)
+    if slots.dtype is not _I32 or slots.get_device() != cache.get_device():
+        _require_int32(cache.device, slots=slots)
     if k.shape != v.shape or slots.shape != k.shape[:1]:
         raise ValueError("KV keys, values and slots must have one entry a token")
     if k.shape[0] > 0:
@@ -166,12 +194,14 @@ def load_kv_int4(cache: torch.Tensor, slots: torch.Tensor, *, block_size: int) -
     """The rows at ``slots`` [tokens] (int32): (k, v) [tokens, kv heads, head_dim], the values
     s * (c - z) rounded to bf16; zeros for a slot outside the cache."""
     head_dim = _cache_head_dim(cache, block_size)
-    _require_int32(cache.device, slots=slots)
+    index, kv_heads = cache.get_device(), cache.shape[1]
+    if slots.dtype is not _I32 or slots.get_device() != index:
+        _require_int32(cache.device, slots=slots)
     if slots.ndim != 1:
         raise ValueError("KV slots must be one-dimensional")
-    shape = (slots.shape[0], cache.shape[1], head_dim)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    shape, stride = (slots.shape[0], kv_heads, head_dim), (kv_heads * head_dim, head_dim, 1)
+    k = torch.empty_strided(shape, stride, dtype=_BF16, device=index)
+    v = torch.empty_strided(shape, stride, dtype=_BF16, device=index)
     if slots.shape[0] > 0:
         lib().kv_load(cache, slots.contiguous(), k, v, head_dim, block_size)
     return k, v
@@ -183,14 +213,16 @@ def _workspace_bytes(*sizes: int) -> int:
     return lib().kv_attention_workspace(*sizes)
 
 
-class _CounterPool:
-    """Arrival counters of ``attention_int4``: 1024 int32 a call, zero before and after it.
+class _ScratchPool:
+    """Workspaces and arrival counters of ``attention_int4``; a call's counters (1024 int32) are zero
+    before and after it.
 
-    Calls of one stream run in order and share one set.  A captured call gets a set of its own, for
-    good: its graph may be replayed beside anything else.  Sets come from one zeroed array a device
-    (16 MiB: 4096 sets), made by the device's first eager call, which waits for the zeros.  A call
-    without a set left, or captured before that array exists, takes a new zeroed tensor (inside a
-    capture its graph clears it on every replay)."""
+    Eager calls of one stream run in order and share one pair.  A captured call takes its workspace
+    from the graph's pool and a set of counters of its own, for good: its graph may be replayed
+    beside anything else.  Counters come from one zeroed array a device (16 MiB: 4096 sets), made by
+    the device's first eager call, which waits for the zeros.  A call without a set left, or
+    captured before that array exists, takes a new zeroed tensor (inside a capture its graph clears
+    it on every replay)."""
 
     SETS = 4096
     SIZE = 1024
@@ -198,37 +230,41 @@ class _CounterPool:
     def __init__(self):
         self._lock = threading.Lock()
         self._free: dict[int, list[torch.Tensor]] = {}
-        self._streams: dict[tuple[int, int], torch.Tensor] = {}
+        self._streams: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
         self._captured: list[torch.Tensor] = []
 
-    def get(self, device: torch.device) -> torch.Tensor:
-        index = device.index
-        if torch._C._cuda_getDevice() != index:
+    def get(self, index: int, nbytes: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(workspace of at least nbytes, counters) for a call on GPU `index`'s current stream."""
+        if _current_device() != index:
             with torch.cuda.device(index):
-                return self.get(device)
-        stream = torch._C._cuda_getCurrentRawStream(index)
-        if torch._C._cuda_isCurrentStreamCapturing():
+                return self.get(index, nbytes)
+        if _capturing():
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=index)
             with self._lock:
                 free = self._free.get(index)
                 if free:
                     self._captured.append(free.pop())
-                    return self._captured[-1]
-            return torch.zeros(self.SIZE, dtype=torch.int32, device=device)
-        counters = self._streams.get((index, stream))
-        if counters is not None:
-            return counters
+                    return workspace, self._captured[-1]
+            return workspace, torch.zeros(self.SIZE, dtype=_I32, device=index)
+        key = (index, _current_stream(index))
+        pair = self._streams.get(key)
+        if pair is not None and pair[0].numel() >= nbytes:
+            return pair
         with self._lock:
             if index not in self._free:
-                array = torch.zeros(self.SETS, self.SIZE, dtype=torch.int32, device=device)
-                torch.cuda.current_stream(device).synchronize()
+                array = torch.zeros(self.SETS, self.SIZE, dtype=_I32, device=index)
+                torch.cuda.current_stream(index).synchronize()
                 self._free[index] = list(array.unbind())
             free = self._free[index]
-            if not free:
-                return torch.zeros(self.SIZE, dtype=torch.int32, device=device)
-            return self._streams.setdefault((index, stream), free.pop())
+            if pair is None and not free:
+                return (torch.empty(nbytes, dtype=torch.uint8, device=index),
+                        torch.zeros(self.SIZE, dtype=_I32, device=index))
+            counters = free.pop() if pair is None else pair[1]
+            pair = self._streams[key] = (torch.empty(nbytes, dtype=torch.uint8, device=index), counters)
+            return pair
 
 
-COUNTERS = _CounterPool()
+SCRATCH = _ScratchPool()
 
 
 def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -246,22 +282,27 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     cached tokens and those new ones j < 64 whose bit j is set.  A row that sees nothing is zero.
     Without ``out`` (contiguous, of q's shape), rows behind the last request are zero; in ``out``
     they are left as they were."""
-    head_dim = _cache_head_dim(cache, block_size)
-    device = cache.device
-    q = _rows("queries", q, None, head_dim, device)
-    rows, heads = q.shape[0], q.shape[1]
-    kv_heads = cache.shape[1]
-    if heads < 1 or heads % kv_heads:
-        raise ValueError(f"query heads ({heads}) must be a multiple of the cache's kv heads ({kv_heads})")
-    _require_int32(device, block_tables=block_tables, seq_lens=seq_lens, cu_query_lens=cu_query_lens)
-    requests = seq_lens.shape[0] if seq_lens.ndim == 1 else 0
-    if requests < 1 or cu_query_lens.shape != (requests + 1,):
-        raise ValueError("KV seq_lens must be [requests], at least one, and cu_query_lens [requests + 1]")
-    width = block_tables.shape[1] if block_tables.ndim == 2 else 0
-    if width < 1 or block_tables.shape[0] != requests:
-        raise ValueError("KV block_tables must be [requests, width]")
-    if block_tables.stride(1) != 1 or block_tables.stride(0) < width:
-        block_tables = block_tables.contiguous()
+    # One expression accepts what all the checks accept; only what it does not goes through them.
+    shape, tshape, index = q.shape, block_tables.shape, cache.get_device()
+    head_dim = shape[-1]
+    if not (index >= 0 and len(shape) == 3 and block_size in BLOCK_SIZES and head_dim in HEAD_DIMS
+            and cache.dtype is _U8 and cache.is_contiguous() and len(cache.shape) == 3
+            and cache.shape[2] == block_size * (head_dim + 8) and cache.shape[0] * block_size < 1 << 31
+            and shape[1] > 0 and cache.shape[1] > 0 and shape[1] % cache.shape[1] == 0
+            and q.dtype is _BF16 and q.get_device() == index
+            and q.stride(2) == 1 and q.stride(1) % 8 == 0 and q.stride(0) % 8 == 0
+            and (q.data_ptr() | cache.data_ptr()) % 16 == 0
+            and len(tshape) == 2 and tshape[0] > 0 and tshape[1] > 0
+            and block_tables.dtype is _I32 and block_tables.get_device() == index
+            and block_tables.is_contiguous()
+            and seq_lens.dtype is _I32 and seq_lens.get_device() == index and seq_lens.is_contiguous()
+            and seq_lens.shape == (tshape[0],)
+            and cu_query_lens.dtype is _I32 and cu_query_lens.get_device() == index
+            and cu_query_lens.is_contiguous() and cu_query_lens.shape == (tshape[0] + 1,)):
+        q, block_tables, seq_lens, cu_query_lens = _check_attention(q, cache, block_tables, seq_lens, cu_query_lens,
+                                                                    block_size)
+        shape, tshape, head_dim = q.shape, block_tables.shape, q.shape[2]
+    rows, heads = shape[0], shape[1]
     if scale is None:
         scale = head_dim ** -0.5
     elif not 0.0 < scale < 3e38:
@@ -271,21 +312,40 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     elif max_query_len < 1:
         raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.device != device or tree_mask.shape != (rows,):
+        if tree_mask.dtype != torch.int64 or tree_mask.get_device() != index or tree_mask.shape != (rows,):
             raise ValueError("tree_mask must be an int64 [rows] tensor on the cache's GPU")
         tree_mask = tree_mask.contiguous()
     zero_tail = out is None
     if out is None:
-        out = torch.empty((rows, heads, head_dim), dtype=torch.bfloat16, device=device)
-    elif (out.shape != q.shape or out.dtype != torch.bfloat16 or out.device != device or not out.is_contiguous()
+        out = torch.empty_strided(shape, (heads * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    elif (out.shape != shape or out.dtype != torch.bfloat16 or out.get_device() != index or not out.is_contiguous()
           or out.data_ptr() % 16):
         raise ValueError("attention out must be a contiguous, 16-byte aligned bfloat16 tensor of q's shape")
     if rows > 0:
-        size = _workspace_bytes(rows, requests, heads, kv_heads, head_dim, block_size, width, max_query_len)
-        workspace = torch.empty(size, dtype=torch.uint8, device=device)
-        lib().kv_attention(q, cache, block_tables, seq_lens.contiguous(), cu_query_lens.contiguous(), tree_mask, out,
-                           scale, block_size, max_query_len, zero_tail, workspace, COUNTERS.get(device))
+        size = _workspace_bytes(rows, tshape[0], heads, cache.shape[1], head_dim, block_size, tshape[1], max_query_len)
+        workspace, counters = SCRATCH.get(index, size)
+        lib().kv_attention(q, cache, block_tables, seq_lens, cu_query_lens, tree_mask, out, scale, block_size,
+                           max_query_len, zero_tail, workspace, counters)
     return out
+
+
+def _check_attention(q, cache, block_tables, seq_lens, cu_query_lens, block_size):
+    """The argument errors of ``attention_int4``; its arguments as the kernels read them."""
+    head_dim = _cache_head_dim(cache, block_size)
+    q = _rows("queries", q, None, head_dim, cache)
+    heads, kv_heads = q.shape[1], cache.shape[1]
+    if heads < 1 or heads % kv_heads:
+        raise ValueError(f"query heads ({heads}) must be a multiple of the cache's kv heads ({kv_heads})")
+    _require_int32(cache.device, block_tables=block_tables, seq_lens=seq_lens, cu_query_lens=cu_query_lens)
+    requests = seq_lens.shape[0] if seq_lens.ndim == 1 else 0
+    if requests < 1 or cu_query_lens.shape != (requests + 1,):
+        raise ValueError("KV seq_lens must be [requests], at least one, and cu_query_lens [requests + 1]")
+    width = block_tables.shape[1] if block_tables.ndim == 2 else 0
+    if width < 1 or block_tables.shape[0] != requests:
+        raise ValueError("KV block_tables must be [requests, width]")
+    if block_tables.stride(1) != 1 or block_tables.stride(0) < width:
+        block_tables = block_tables.contiguous()
+    return q, block_tables, seq_lens.contiguous(), cu_query_lens.contiguous()
 
 
 class Attention(nn.Module):

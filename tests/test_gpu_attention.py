@@ -339,7 +339,7 @@ def test_graphs_replayed_beside_each_other(gpu_lib):
 
 def test_capture_without_reserved_counters(gpu_lib, monkeypatch):
     """A pool that has no set yet (or none left) gives a captured call a tensor that its graph clears."""
-    monkeypatch.setattr(attn, "COUNTERS", attn._CounterPool())
+    monkeypatch.setattr(attn, "SCRATCH", attn._ScratchPool())
     b = Batch([1, 3], [2500, 700], 8, 2, 128, 16, seed=32)
     args = b.args()
     graph = torch.cuda.CUDAGraph()
@@ -351,7 +351,7 @@ def test_capture_without_reserved_counters(gpu_lib, monkeypatch):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
-    pool = attn.COUNTERS
+    pool = attn.SCRATCH
     pool._free[0].clear()
     pool._streams.clear()
     assert torch.equal(attn.attention_int4(*args, block_size=16), want)
