@@ -247,11 +247,18 @@ def prepare(case, seed):
 
 
 # ---------------------------------------------------------------------- run
+def framework():
+    """The framework's attention layer, imported once as a user's program imports it."""
+    if not hasattr(framework, "attention"):
+        framework.attention = importlib.import_module("llm-serve_amd.layers.attention")
+    return framework.attention
+
+
 def run(state):
     case = state["case"]
     block = case["block"]
     if own:
-        attention = importlib.import_module("llm-serve_amd.layers.attention")
+        attention = framework()
         if case["kind"] == "step":
             step = attention.kv_step(state["query_lens"], state["context_lens"], state["tables"], state["free"],
                                      block_size=block, num_tokens=state["tokens"])
