@@ -120,23 +120,30 @@ __device__ __forceinline__ float lanes_max(float v) {
   return v;
 }
 
+// x / s rounded to a multiple of 2^-11 (|x / s| < 16), by the reciprocal: enough to round it to a
+// code as the exact quotient would be.  x and s have at most 8 significant bits: where x / s lies
+// near a border k + 1/2 between two codes, |x| > s / 4 makes 2 x - (2 k + 1) s a multiple of s's
+// last place, so x / s is the border itself or at least 1 / 510 away.  The product is off by 2^-18
+// at most, and the sum with 1.5 * 2^12, whose last place is 2^-11, then returns a border as it is
+// and moves nothing across one.
+__device__ __forceinline__ float near_quotient(float x, float inverse) { return (x * inverse + 6144.0f) - 6144.0f; }
+
 // One row's eight channels in a lane -> its code word and the row's meta word.  The range takes
 // in zero, so z is in 0..15 and a row of one sign keeps its far end.  The scale is rounded to
 // bf16 (the cache's type) before the codes are formed, so codes are right for the scale that
-// readers multiply by.  x / s is the correctly rounded quotient of two values of at most 8
-// significant bits: it is exactly half way between two codes only if the real quotient is, and
-// its rounding to a code equals the real one's.  A row with a NaN or infinity becomes NaN as a
-// whole; a range beyond fp32 is formed a sixteenth at a time.
+// readers multiply by.  A row with a NaN or infinity becomes NaN as a whole; a range beyond fp32
+// is formed a sixteenth at a time; scales too small for the reciprocal take the division.
 template <int LANES>
 __device__ __forceinline__ uint32_t quantize_row(uint4 raw, int lane, uint32_t* meta) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
   float x[8];
   unpack_bf16x8(raw, x);
   const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  bool bad = false;
-  float hi = 0.0f, lo = 0.0f;
+  u16x2_t top = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    bad |= (w[i] & 0x7F800000u) == 0x7F800000u || (w[i] & 0x7F80u) == 0x7F80u;
+  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[i] & 0x7FFF7FFFu));
+  const bool bad = top[0] >= 0x7F80 || top[1] >= 0x7F80;
+  float hi = 0.0f, lo = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     hi = fmaxf(hi, x[i]);
@@ -156,15 +163,26 @@ __device__ __forceinline__ uint32_t quantize_row(uint4 raw, int lane, uint32_t* 
     *meta = 0x00004300u;
     return 0;
   }
-  const float z = fminf(rintf(-lo / s), 15.0f);
-  uint32_t word = 0;
+  float t[8], z;
+  if (s < 0x1p-100f || s > 0x1p100f) {
+    z = rintf(-lo / s);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float c = fminf(fmaxf(rintf(x[i] / s) + z, 0.0f), 15.0f);
-    word |= static_cast<uint32_t>(c) << awq_shift(i);
+    for (int i = 0; i < 8; ++i) t[i] = x[i] / s;
+  } else {
+    const float inverse = __builtin_amdgcn_rcpf(s);
+    z = rintf(near_quotient(-lo, inverse));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) t[i] = near_quotient(x[i], inverse);
   }
+  z = fminf(z, 15.0f);
+  uint32_t c[8];  // the code in the low bits of 2^23 + code
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(rintf(t[i]), -z, 15.0f - z) + (z + 8388608.0f));
   *meta = kv_meta(s, static_cast<int>(z));
-  return word;
+  const uint32_t p0 = __builtin_amdgcn_perm(c[1], c[0], 0x05040100u), p1 = __builtin_amdgcn_perm(c[3], c[2], 0x05040100u);
+  const uint32_t p2 = __builtin_amdgcn_perm(c[5], c[4], 0x05040100u), p3 = __builtin_amdgcn_perm(c[7], c[6], 0x05040100u);
+  return p0 | (p1 << 4) | (p2 << 8) | (p3 << 12);
 }
 
 // A wave takes 64 / (D / 8) consecutive tokens of one kv head, K and V: D / 8 lanes a row, 16
