@@ -26,10 +26,8 @@ constexpr int kKvPromptWorkers = 256;
 // The split kernel's largest grid: three workgroups a CU.
 constexpr int kKvSplitWorkers = 768;
 static_assert(kKvSplitWorkers + kKvPromptWorkers == kKvAttentionCounters, "a counter a worker");
-// A call goes to the split kernel alone up to this many rows a request (longest query x heads of a
-// group); beyond, requests of at most kKvMixedMaxRows rows go to it, the others to the prompt kernel.
+// Rows a request (tokens x heads of a group) up to which the split kernel takes it.
 constexpr int kKvSplitMaxRows = 64;
-constexpr int kKvMixedMaxRows = 32;
 
 hipError_t launch_kv_prompt(const KvAttentionArgs& a, const KvPartials& part, int workers, hipStream_t stream);
 

@@ -17,16 +17,16 @@ namespace {
 
 constexpr int kUnit = 128;      // keys of one work unit: 32 a wave
 constexpr int kWaves = 4;
+constexpr int kRows = 16;       // rows of a tile
 constexpr int kThreads = 64 * kWaves;
 
 // Units of one row tile (a tile whose rows see nothing still has its zeros to write).
 __device__ __forceinline__ int kv_span(const KvRequest& q) { return max((q.keys + kUnit - 1) / kUnit, 1); }
 
 // Units of a request (none if the prompt kernel takes it).
-template <int ROWS>
 __device__ __forceinline__ int kv_units(const KvAttentionArgs& a, const KvRequest& q, int group) {
   if (q.n * group > a.split_rows) return 0;
-  return (q.n * group + ROWS - 1) / ROWS * a.KV * kv_span(q);
+  return (q.n * group + kRows - 1) / kRows * a.KV * kv_span(q);
 }
 
 // One slice of 32 keys of a wave, in registers: two 16-key tiles, each inside one page.
@@ -102,20 +102,26 @@ __device__ __forceinline__ void kv_ids(int (&id)[2], ConstInts table, int key, i
     id[t] = table[min(key + 16 * t, last) >> log2_block];
 }
 
-// Split attention.  A row tile is up to 16 MT rows (tokens x heads of the group) of one request
+// Split attention.  A row tile is up to 16 rows (tokens x heads of the group) of one request
 // and kv head; its keys are cut into units of 128.  All units of all tiles, in order, are dealt
 // to the grid's workgroups in equal contiguous shares, so that a batch of any lengths loads them
-// alike; a share that covers a tile's keys only in part leaves a partial result (KvPartials).  Inside a unit each of the 4 waves takes 32 keys and keeps
-// its own running maximum and sum; the waves are joined through LDS at the end of a tile.
+// alike; a share that covers a tile's keys only in part leaves a partial result (KvPartials).
+// Inside a unit each of the 4 waves takes 32 keys and keeps its own running maximum and sum; the
+// waves are joined through LDS at the end of a tile.  More rows than 16 take several tiles, which
+// read the keys again, mostly from L2: 24 requests of 8 drafts (32 rows) take 24 us so, and took
+// 26 us with 32 rows a tile, whose registers leave room for two waves a SIMD.
 //
 // The next slice's keys are loaded into the registers that the scores have just consumed, and
 // its values into those that the second product has, so a wave has loads in flight throughout
-// without a second set of registers, and three waves fit a SIMD (MT = 1; two with MT = 2).  A
-// fourth would cost spills inside the loop: 128 sequences of up to 8192 keys took 255 us with
-// four, 149 us with three.
-template <int D, int MT>
-__global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {
-  constexpr int kRows = 16 * MT, kSteps = D / 32, kTiles = D / 16, kPitch = D + 4;
+// without a second set of registers, and three waves fit a SIMD.  A fourth would cost spills
+// inside the loop: 128 sequences of up to 8192 keys took 255 us with four, 149 us with three.
+//
+// 128 sequences of up to 8192 keys take 129 us, 4.7 TB/s of the cache's bytes (a large copy:
+// 5.2 TB/s); 2 of 131000 take 61 us.  Short calls are bound by latency: some 4 us to the first
+// keys, 2 us to join and write, and a tail of a few us between the first and the last workgroup.
+template <int D>
+__global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {
+  constexpr int kSteps = D / 32, kTiles = D / 16, kPitch = D + 4;
   __shared__ __align__(16) float s_out[kWaves][kRows][kPitch];
   __shared__ float s_max[kWaves][kRows], s_sum[kWaves][kRows];
   __shared__ int s_last;
@@ -130,7 +136,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
   int my_units = 0, sum = 0;
   for (int i = lane; i < a.R; i += 64) {
     mine = kv_request(a, i);
-    my_units = kv_units<kRows>(a, mine, group);
+    my_units = kv_units(a, mine, group);
     sum += my_units;
   }
   int upto = wave_scan(sum);
@@ -158,7 +164,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
                   __builtin_amdgcn_readlane(mine.cached, r), __builtin_amdgcn_readlane(mine.keys, r)};
   } else {
     for (;; r += 64) {
-      my_units = r + lane < a.R ? kv_units<kRows>(a, kv_request(a, r + lane), group) : 0;
+      my_units = r + lane < a.R ? kv_units(a, kv_request(a, r + lane), group) : 0;
       upto = wave_scan(my_units);
       const uint64_t past = __ballot(base + upto > begin);
       if (past || r + 64 >= a.R) {
@@ -170,7 +176,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
       base += __builtin_amdgcn_readlane(upto, 63);
     }
     q = kv_request(a, r);
-    units = kv_units<kRows>(a, q, group);
+    units = kv_units(a, q, group);
   }
 
   const NibbleConsts nc = nibble_consts();
@@ -184,7 +190,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
       base += units;
       ++r;
       q = kv_request(a, r);
-      units = kv_units<kRows>(a, q, group);
+      units = kv_units(a, q, group);
     }
     const int tiles = (q.n * group + kRows - 1) / kRows, span = kv_span(q);
     const int seg = (u - base) / span, k0 = u - base - seg * span;
@@ -207,45 +213,34 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
     }
 
     // The queries as the second operand: column = row of the tile, channels as K's words have them.
-    bf16x8_t qf[MT][kSteps];
-    float neg_sum[MT];
-    int sees[MT];       // leading keys that the lane's row sees
-    uint64_t bits[MT];  // and which of the request's new ones behind them
+    bf16x8_t qf[kSteps];
+    const int row = row0 + col;
+    const int token = row / group, h = head * group + row - token * group;
+    const bool live = col < rows;
+    float total_q = 0.0f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const int row = row0 + 16 * m + col;
-      const int token = row / group, h = head * group + row - token * group;
-      const bool live = 16 * m + col < rows;
-      float total_q = 0.0f;
+    for (int i = 0; i < kSteps; ++i) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (live)
+        w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + h * a.q_stride_h + (D / 4) * g +
+                                            8 * i);
+      float f[8];
+      unpack_bf16x8(w, f);
 #pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (live)
-          w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + h * a.q_stride_h + (D / 4) * g +
-                                              8 * i);
-        float f[8];
-        unpack_bf16x8(w, f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) total_q += f[j];
-        qf[m][i] = __builtin_bit_cast(bf16x8_t, w);
-      }
-      neg_sum[m] = -column_sum(total_q);
-      const bool tree = a.tree_mask != nullptr;
-      bits[m] = tree && live ? a.tree_mask[q.row + token] : 0;
-      sees[m] = live ? min(tree ? q.cached : q.cached + token + 1, q.keys) : 0;
+      for (int j = 0; j < 8; ++j) total_q += f[j];
+      qf[i] = __builtin_bit_cast(bf16x8_t, w);
     }
+    const float neg_sum = -column_sum(total_q);
+    const bool tree = a.tree_mask != nullptr;
+    // Leading keys that the lane's row sees, and which of the request's new ones behind them.
+    const uint64_t bits = tree && live ? a.tree_mask[q.row + token] : 0;
+    const int sees = live ? min(tree ? q.cached : q.cached + token + 1, q.keys) : 0;
     const int all_see = min(a.tree_mask ? q.cached : q.cached + row0 / group + 1, q.keys);
 
-    f32x4_t acc_o[MT][kTiles], acc_z[MT];
-    float row_max[MT], row_sum[MT];
+    f32x4_t acc_o[kTiles], acc_z = {0, 0, 0, 0};
+    float row_max = -INFINITY, row_sum = 0.0f;
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-#pragma unroll
-      for (int c = 0; c < kTiles; ++c) acc_o[m][c] = f32x4_t{0, 0, 0, 0};
-      acc_z[m] = f32x4_t{0, 0, 0, 0};
-      row_max[m] = -INFINITY;
-      row_sum[m] = 0.0f;
-    }
+    for (int c = 0; c < kTiles; ++c) acc_o[c] = f32x4_t{0, 0, 0, 0};
 
     // A SIMD issues its oldest wave first, so of equal shares the first workgroup's on a CU would end
     // a quarter sooner than the third's (96 against 126 us of 128 sequences up to 8192 keys).  The
@@ -264,23 +259,15 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
       const bool whole = key + 32 <= all_see && place.ok[0] && place.ok[1];
       const bool ok[2] = {place.ok[0], place.ok[1]};
 
-      f32x4_t sc[MT][2];
+      f32x4_t sc[2];
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int i = 0; i < 4; ++i) sc[t][i] = kv_meta_zero128(s.km[t][i]) * neg_sum;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) sc[m][t][i] = kv_meta_zero128(s.km[t][i]) * neg_sum[m];
+        for (int i = 0; i < kSteps; ++i) sc[t] = mfma16(unpack_codes(s.k[t][i], nc), qf[i], sc[t]);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          const bf16x8_t kf = unpack_codes(s.k[t][i], nc);
-#pragma unroll
-          for (int m = 0; m < MT; ++m) sc[m][t] = mfma16(kf, qf[m][i], sc[m][t]);
-        }
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[m][t][i] *= kv_meta_scale(s.km[t][i]);
+        for (int i = 0; i < 4; ++i) sc[t][i] *= kv_meta_scale(s.km[t][i]);
       }
       if (more) {
         place = kv_place<D>(a, id, head, key + kUnit);
@@ -288,13 +275,11 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
         if (key + 2 * kUnit < key_end) kv_ids(id, table, key + 2 * kUnit, key_end - 1, a.log2_block);
       }
 
-      float vs[MT][2][4];  // the values' scales as the rows see them
+      float vs[2][4];  // the values' scales as the rows see them
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) vs[m][t][i] = kv_meta_scale(s.vm[t][i]);
+        for (int i = 0; i < 4; ++i) vs[t][i] = kv_meta_scale(s.vm[t][i]);
       if (!whole) {
         // A lane's keys are 16 t + 4 g + i.  Keys outside the sequence, or on no page, hold
         // anything: their score becomes -inf, their scale 0 and their zero point 0.  Keys that
@@ -309,15 +294,12 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
             const bool held = ok[t] & (k < q.keys);
             const unsigned fresh = static_cast<unsigned>(k - q.cached);
             s.vm[t][i] = held ? s.vm[t][i] : 0x00004300u;
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              const uint32_t word = fresh & 32u ? static_cast<uint32_t>(bits[m] >> 32) : static_cast<uint32_t>(bits[m]);
-              const uint32_t named = fresh < 64u ? word >> (fresh & 31u) : 0u;
-              const bool visible = held & ((k < sees[m]) | ((named & 1u) != 0));
-              const float x = sc[m][t][i];
-              sc[m][t][i] = visible ? x : -INFINITY;
-              vs[m][t][i] = visible ? vs[m][t][i] : 0.0f;
-            }
+            const uint32_t word = fresh & 32u ? static_cast<uint32_t>(bits >> 32) : static_cast<uint32_t>(bits);
+            const uint32_t named = fresh < 64u ? word >> (fresh & 31u) : 0u;
+            const bool visible = held & ((k < sees) | ((named & 1u) != 0));
+            const float x = sc[t][i];
+            sc[t][i] = visible ? x : -INFINITY;
+            vs[t][i] = visible ? vs[t][i] : 0.0f;
           }
       }
       u32x4_t zf;  // the keys' 128 + z as the first operand of the offset tile
@@ -326,50 +308,37 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           zf[2 * t + i] = __builtin_amdgcn_perm(s.vm[t][2 * i + 1], s.vm[t][2 * i], 0x05040100u);
-      bool grew = false;
-      float top[MT];
+      const float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
+                             fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+      const float top = fmaxf(row_max, column_max(mx));
+      if (__any(top > row_max)) {
+        const float ref = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f((row_max - ref) * scale);
+        row_max = top;
+        row_sum *= f;
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const float mx = fmaxf(fmaxf(fmaxf(sc[m][0][0], sc[m][0][1]), fmaxf(sc[m][0][2], sc[m][0][3])),
-                               fmaxf(fmaxf(sc[m][1][0], sc[m][1][1]), fmaxf(sc[m][1][2], sc[m][1][3])));
-        top[m] = fmaxf(row_max[m], column_max(mx));
-        grew |= top[m] > row_max[m];
+        for (int c = 0; c < kTiles; ++c)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc_o[c][i] *= f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc_z[i] *= f;
       }
-      if (__any(grew)) {
+      const float ref = (row_max == -INFINITY ? 0.0f : row_max) * scale;
+      u32x4_t w;
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const float ref = top[m] == -INFINITY ? 0.0f : top[m];
-          const float f = __builtin_amdgcn_exp2f((row_max[m] - ref) * scale);
-          row_max[m] = top[m];
-          row_sum[m] *= f;
+      for (int t = 0; t < 2; ++t) {
+        float p[4];
 #pragma unroll
-          for (int c = 0; c < kTiles; ++c)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc_o[m][c][i] *= f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc_z[m][i] *= f;
+        for (int i = 0; i < 4; ++i) {
+          p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][i], scale, -ref));
+          row_sum += p[i];
+          p[i] *= vs[t][i];
         }
+        w[2 * t] = pack_bf16x2(p[0], p[1]);
+        w[2 * t + 1] = pack_bf16x2(p[2], p[3]);
       }
-      bf16x8_t pf[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        const float ref = (row_max[m] == -INFINITY ? 0.0f : row_max[m]) * scale;
-        u32x4_t w;
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          float p[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[m][t][i], scale, -ref));
-            row_sum[m] += p[i];
-            p[i] *= vs[m][t][i];
-          }
-          w[2 * t] = pack_bf16x2(p[0], p[1]);
-          w[2 * t + 1] = pack_bf16x2(p[2], p[3]);
-        }
-        pf[m] = __builtin_bit_cast(bf16x8_t, w);
-        acc_z[m] = mfma16(__builtin_bit_cast(bf16x8_t, zf), pf[m], acc_z[m]);
-      }
+      const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
+      acc_z = mfma16(__builtin_bit_cast(bf16x8_t, zf), pf, acc_z);
 
       // V: words of tokens paired into halves with 4 channels each (even ones, then odd ones);
       // nibble i of the halves is one channel of two tokens.  A 64-channel row has 8 words, and
@@ -389,9 +358,7 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
 #pragma unroll
           for (int i = 0; i < 4; ++i) f[i] = ((pair[i] >> (4 * c)) & nc.mask) | nc.bias;
           const int ch = D == 128 ? 2 * c + half : c;
-#pragma unroll
-          for (int m = 0; m < MT; ++m)
-            acc_o[m][ch] = mfma16(__builtin_bit_cast(bf16x8_t, f), pf[m], acc_o[m][ch]);
+          acc_o[ch] = mfma16(__builtin_bit_cast(bf16x8_t, f), pf, acc_o[ch]);
         }
       }
       if (more) load_values<D>(s, place, offset, a.log2_block);
@@ -399,28 +366,25 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
 
     // Join the waves.  Accumulator register i of a lane is operand row 4 g + i: the word (D =
     // 128) or word and half (D = 64) whose channels the tiles c count.
+    const float row_total = column_sum(row_sum);
+    if (g == 0) {
+      s_max[wave][col] = row_max;
+      s_sum[wave][col] = row_total;
+    }
 #pragma unroll
-    for (int m = 0; m < MT; ++m) {
-      const float row_total = column_sum(row_sum[m]);
-      if (g == 0) {
-        s_max[wave][16 * m + col] = row_max[m];
-        s_sum[wave][16 * m + col] = row_total;
-      }
+    for (int i = 0; i < 4; ++i) {
+      float* o = s_out[wave][col];
+      if constexpr (D == 128) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float* o = s_out[wave][16 * m + col];
-        if constexpr (D == 128) {
-#pragma unroll
-          for (int c = 0; c < 8; c += 4) {
-            const f32x4_t v = {acc_o[m][c][i] - acc_z[m][i], acc_o[m][c + 1][i] - acc_z[m][i],
-                               acc_o[m][c + 2][i] - acc_z[m][i], acc_o[m][c + 3][i] - acc_z[m][i]};
-            *reinterpret_cast<f32x4_t*>(o + 8 * (4 * g + i) + c) = v;
-          }
-        } else {
-          const int word = (4 * g + i) & 7, odd = g >> 1;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[8 * word + 2 * c + odd] = acc_o[m][c][i] - acc_z[m][i];
+        for (int c = 0; c < 8; c += 4) {
+          const f32x4_t v = {acc_o[c][i] - acc_z[i], acc_o[c + 1][i] - acc_z[i],
+                             acc_o[c + 2][i] - acc_z[i], acc_o[c + 3][i] - acc_z[i]};
+          *reinterpret_cast<f32x4_t*>(o + 8 * (4 * g + i) + c) = v;
         }
+      } else {
+        const int word = (4 * g + i) & 7, odd = g >> 1;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[8 * word + 2 * c + odd] = acc_o[c][i] - acc_z[i];
       }
     }
     __syncthreads();
@@ -466,24 +430,20 @@ __global__ __launch_bounds__(kThreads, MT == 1 ? 3 : 2) void kv_attention_kernel
 // split kernel, longer ones to the prompt kernel, which is launched only if the longest query
 // may be that long.
 struct KvPlan {
-  int mt;             // split kernel: 16-row tiles of a workgroup
-  int split_workers;  // its grid
+  int split_workers;   // the split kernel's grid
   int split_rows;
   int prompt_workers;  // the prompt kernel's grid (0: not launched)
 };
 
 KvPlan kv_plan(const KvAttentionArgs& a) {
   KvPlan p;
-  const int64_t rows = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
-  const bool prompts = rows > kKvSplitMaxRows;
-  p.mt = rows <= 16 || prompts ? 1 : 2;
-  p.split_rows = prompts ? kKvMixedMaxRows : 0x7FFFFFFF;
-  const int64_t tile_rows = prompts ? kKvMixedMaxRows : rows;
-  const int64_t tiles = (tile_rows + 16 * p.mt - 1) / (16 * p.mt);
+  const int64_t longest = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
+  const bool prompts = longest > kKvSplitMaxRows;
+  p.split_rows = prompts ? kKvSplitMaxRows : 0x7FFFFFFF;
+  const int64_t tiles = ((prompts ? kKvSplitMaxRows : longest) + kRows - 1) / kRows;
   const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
   const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
-  const int64_t fill = p.mt == 1 ? kKvSplitWorkers : 512;
-  p.split_workers = static_cast<int>(most < fill ? most : fill);
+  p.split_workers = static_cast<int>(most < kKvSplitWorkers ? most : kKvSplitWorkers);
   p.prompt_workers = prompts ? kKvPromptWorkers : 0;
   return p;
 }
@@ -509,15 +469,11 @@ KvPartials partials_at(char* ws, int* counters, int workers, int rows, int D) {
 
 template <int D>
 hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, int* counters, hipStream_t stream) {
-  const int rows = 16 * p.mt;
-  const KvPartials split = partials_at(ws, counters, p.split_workers, rows, D);
-  if (p.mt == 1)
-    kv_attention_kernel<D, 1><<<p.split_workers, kThreads, 0, stream>>>(a, split);
-  else
-    kv_attention_kernel<D, 2><<<p.split_workers, kThreads, 0, stream>>>(a, split);
+  const KvPartials split = partials_at(ws, counters, p.split_workers, kRows, D);
+  kv_attention_kernel<D><<<p.split_workers, kThreads, 0, stream>>>(a, split);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.prompt_workers == 0) return e;
-  const KvPartials prompt = partials_at(ws + partials_bytes(p.split_workers, rows, D), counters + kKvSplitWorkers,
+  const KvPartials prompt = partials_at(ws + partials_bytes(p.split_workers, kRows, D), counters + kKvSplitWorkers,
                                         p.prompt_workers, kKvPromptRows, D);
   return launch_kv_prompt(a, prompt, p.prompt_workers, stream);
 }
@@ -526,7 +482,7 @@ hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, int* coun
 
 size_t kv_attention_workspace(const KvAttentionArgs& a) {
   const KvPlan p = kv_plan(a);
-  return partials_bytes(p.split_workers, 16 * p.mt, a.D) +
+  return partials_bytes(p.split_workers, kRows, a.D) +
          (p.prompt_workers ? partials_bytes(p.prompt_workers, kKvPromptRows, a.D) : 0);
 }
 
