@@ -77,21 +77,22 @@ struct KvShares {
   }
 };
 
-// out[row, h, ch ..] = o / sum, rounded; a row that saw nothing (or only scores of -inf) is zero.
-template <int N>
-__device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int h, int ch, float sum, const float (&o)[N]) {
+// out[row, h, ch .. ch + 7] = o / sum, rounded; a row that saw nothing (or only scores of -inf) is zero.
+__device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int h, int ch, float sum, const float (&o)[8]) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-  uint16_t* p = a.out + (static_cast<size_t>(row) * a.H + h) * a.D + ch;
-  if constexpr (N == 8) {
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
-                                              pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
-  } else if constexpr (N == 4) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
-  } else if constexpr (N == 2) {
-    *reinterpret_cast<uint32_t*>(p) = pack_bf16x2(o[0] * inv, o[1] * inv);
-  } else {
-    *p = f32_to_bf16_bits(o[0] * inv);
-  }
+  float t[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) t[i] = o[i] * inv;
+  *reinterpret_cast<uint4*>(a.out + (static_cast<size_t>(row) * a.H + h) * a.D + ch) = pack_bf16x8(t);
+}
+
+// Zeros for the output rows behind the last request.
+__device__ __forceinline__ void kv_zero_tail(const KvAttentionArgs& a) {
+  const int end = min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
+  const int chunks = a.H * a.D / 8;
+  for (int row = end + blockIdx.x; row < a.T; row += gridDim.x)
+    for (int c = threadIdx.x; c < chunks; c += blockDim.x)
+      reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
 }
 
 // One part of a tile row's result: eight channels, or the row's statistics.
@@ -103,6 +104,15 @@ __device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t r, uint32_t of
 __device__ __forceinline__ void store_stats(__amdgpu_buffer_rsrc_t r, uint32_t offset, float top, float sum) {
   const u32x2_t v = {__float_as_uint(top), __float_as_uint(sum)};
   __builtin_amdgcn_raw_buffer_store_b64(v, r, offset, 0, kCoherentPolicy);
+}
+
+// Whether all other workgroups of a tile of `count` parts have arrived: then this one need not
+// store its own.  All threads call it; `flag` is LDS.
+__device__ __forceinline__ bool kv_is_last(int* counter, int count, int* flag) {
+  if (threadIdx.x == 0)
+    *flag = __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == count - 1;
+  __syncthreads();
+  return *flag != 0;
 }
 
 // Counts this workgroup's arrival, its part stored; whether it is the last of `count`.  All

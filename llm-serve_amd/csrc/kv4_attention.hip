@@ -144,13 +144,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionAr
   const int workers = min(total, static_cast<int>(gridDim.x));
   const int me = blockIdx.x;
 
-  if (a.zero_tail) {
-    const int end = min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
-    const int chunks = a.H * D / 8;
-    for (int row = end + me; row < a.T; row += gridDim.x)
-      for (int c = tid; c < chunks; c += kThreads)
-        reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
-  }
+  if (a.zero_tail) kv_zero_tail(a);
   if (me >= workers) return;
   const KvShares shares{total / workers, total % workers};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
@@ -430,7 +424,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionAr
 // split kernel, longer ones to the prompt kernel, which is launched only if the longest query
 // may be that long.
 struct KvPlan {
-  int split_workers;   // the split kernel's grid
+  int split_workers;   // the split kernel's grid (0: not launched)
   int split_rows;
   int prompt_workers;  // the prompt kernel's grid (0: not launched)
 };
@@ -439,11 +433,12 @@ KvPlan kv_plan(const KvAttentionArgs& a) {
   KvPlan p;
   const int64_t longest = static_cast<int64_t>(a.max_query_len) * (a.H / a.KV);
   const bool prompts = longest > kKvSplitMaxRows;
-  p.split_rows = prompts ? kKvSplitMaxRows : 0x7FFFFFFF;
+  const bool alone = prompts && a.R == 1;  // a prompt by itself: one launch
+  p.split_rows = alone ? 0 : prompts ? kKvSplitMaxRows : 0x7FFFFFFF;
   const int64_t tiles = ((prompts ? kKvSplitMaxRows : longest) + kRows - 1) / kRows;
   const int64_t units = ((static_cast<int64_t>(a.width) << a.log2_block) + kUnit - 1) / kUnit;
   const int64_t most = tiles * a.R * a.KV * (units > 0 ? units : 1);
-  p.split_workers = static_cast<int>(most < kKvSplitWorkers ? most : kKvSplitWorkers);
+  p.split_workers = alone ? 0 : static_cast<int>(most < kKvSplitWorkers ? most : kKvSplitWorkers);
   p.prompt_workers = prompts ? kKvPromptWorkers : 0;
   return p;
 }
@@ -470,9 +465,11 @@ KvPartials partials_at(char* ws, int* counters, int workers, int rows, int D) {
 template <int D>
 hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, int* counters, hipStream_t stream) {
   const KvPartials split = partials_at(ws, counters, p.split_workers, kRows, D);
-  kv_attention_kernel<D><<<p.split_workers, kThreads, 0, stream>>>(a, split);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.prompt_workers == 0) return e;
+  if (p.split_workers) {
+    kv_attention_kernel<D><<<p.split_workers, kThreads, 0, stream>>>(a, split);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || p.prompt_workers == 0) return e;
+  }
   const KvPartials prompt = partials_at(ws + partials_bytes(p.split_workers, kRows, D), counters + kKvSplitWorkers,
                                         p.prompt_workers, kKvPromptRows, D);
   return launch_kv_prompt(a, prompt, p.prompt_workers, stream);

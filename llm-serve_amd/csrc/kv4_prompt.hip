@@ -103,49 +103,66 @@ __device__ __forceinline__ uint32_t part_offset(int slot, int wave, int f, int l
   return ((static_cast<uint32_t>(slot) * 8 + wave) * (D / 8) + f) * 1024u + lane * 16u;
 }
 
-// Joins a tile's `count` parts, from worker `first` on: every lane its own rows' fragments, two
-// parts' loads in flight.
+// Two fragments of a lane -- channels 4 h .. of eights b and b + 1 -- to the output: the halves of
+// the wave exchange theirs, so that a lane writes one eight's 16 bytes.
 template <int D>
-__device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPartials& part, int first, int count, int wave,
-                                           int lane, bool live, int out_row, int out_head) {
-  constexpr int kFrags = D / 8, kBatch = 2;
+__device__ __forceinline__ void write_pair(const KvAttentionArgs& a, bool live, int row, int head, int f, int lane, float inv,
+                                           const f32x4_t& x, const f32x4_t& y) {
+  const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[0] * inv, x[1] * inv),
+                                                                                  pack_bf16x2(y[0] * inv, y[1] * inv), false, false));
+  const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[2] * inv, x[3] * inv),
+                                                                                  pack_bf16x2(y[2] * inv, y[3] * inv), false, false));
+  if (live)
+    *reinterpret_cast<uint4*>(a.out + (static_cast<size_t>(row) * a.H + head) * D + 8 * (f + (lane >> 5))) =
+        make_uint4(lo[0], hi[0], lo[1], hi[1]);
+}
+
+// Writes a wave's rows, o / sum (rows that saw nothing are zero).
+template <int D>
+__device__ __forceinline__ void write_rows(const KvAttentionArgs& a, bool live, int row, int head, int lane, float sum,
+                                           const f32x4_t (&o)[D / 8]) {
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+  for (int f = 0; f < D / 8; f += 2) write_pair<D>(a, live, row, head, f, lane, inv, o[f], o[f + 1]);
+}
+
+// Joins a tile's `count` parts, from worker `first` on, and writes the result; part `mine` is this
+// workgroup's own, in registers.  Parts are taken in order, the next one's loads in flight.
+template <int D>
+__device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPartials& part, int first, int count, int mine,
+                                           int wave, int lane, bool live, int out_row, int out_head, float own_top,
+                                           float own_sum, const f32x4_t (&own)[D / 8]) {
+  constexpr int kFrags = D / 8;
   const __amdgpu_buffer_rsrc_t ro = make_buffer(part.out, part.out_bytes), rs = make_buffer(part.stats, part.stats_bytes);
   float top = -INFINITY, sum = 0.0f;
-  f32x4_t acc[kFrags];
+  f32x4_t acc[kFrags], v[kFrags];
 #pragma unroll
   for (int f = 0; f < kFrags; ++f) acc[f] = f32x4_t{0, 0, 0, 0};
-  for (int i0 = 0; i0 < count; i0 += kBatch) {
-    f32x4_t v[kBatch][kFrags];
-    u32x2_t st[kBatch];
+  for (int i = 0; i < count; ++i) {
+    float m = own_top, l = own_sum;
+    if (i == mine) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int i = i0 + b, slot = i == 0 ? 2 * first + 1 : 2 * (first + i);
-      const bool in = live && i < count;  // other loads touch nothing and give zeros
+      for (int f = 0; f < kFrags; ++f) v[f] = own[f];
+    } else {
+      const int slot = i == 0 ? 2 * first + 1 : 2 * (first + i);
       const uint32_t row = static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + (lane & 31);
-      st[b] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, in ? row * 8 : kOutOfRange, 0, kCoherentPolicy));
+      const u32x2_t st = __builtin_bit_cast(
+          u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, live ? row * 8 : kOutOfRange, 0, kCoherentPolicy));
+      const uint32_t mb = st[0], lb = st[1];
+      m = __uint_as_float(mb), l = __uint_as_float(lb);
 #pragma unroll
-      for (int f = 0; f < kFrags; ++f) v[b][f] = load_fragment(ro, in ? part_offset<D>(slot, wave, f, lane) : kOutOfRange);
+      for (int f = 0; f < kFrags; ++f) v[f] = load_fragment(ro, live ? part_offset<D>(slot, wave, f, lane) : kOutOfRange);
     }
+    const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
+    const float x = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e), y = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2e);
+    top = next;
+    sum = sum * x + l * y;
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const uint32_t mb = st[b][0], lb = st[b][1];
-      const float m = i0 + b < count ? __uint_as_float(mb) : -INFINITY;
-      const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
-      const float x = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e), y = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2e);
-      top = next;
-      sum = sum * x + __uint_as_float(lb) * y;
+    for (int f = 0; f < kFrags; ++f)
 #pragma unroll
-      for (int f = 0; f < kFrags; ++f)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[f][j] = acc[f][j] * x + v[b][f][j] * y;
-    }
+      for (int j = 0; j < 4; ++j) acc[f][j] = acc[f][j] * x + v[f][j] * y;
   }
-  if (!live) return;
-#pragma unroll
-  for (int f = 0; f < kFrags; ++f) {
-    const float o[4] = {acc[f][0], acc[f][1], acc[f][2], acc[f][3]};
-    kv_write(a, out_row, out_head, 32 * (f >> 2) + 8 * (f & 3) + 4 * (lane >> 5), sum, o);
-  }
+  write_rows<D>(a, live, out_row, out_head, lane, sum, acc);
 }
 
 template <int D>
@@ -164,6 +181,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const int per_xcd = gridDim.x / 8;
   const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
 
+  if (a.split_rows == 0 && a.zero_tail) kv_zero_tail(a);  // no split kernel in this call
   int sum = 0;
   for (int r = lane; r < a.R; r += 64) sum += kv_request_cost(a, kv_request(a, r), group);
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
@@ -480,25 +498,31 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     const u32x2_t both = __builtin_bit_cast(
         u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(row_sum), __float_as_uint(row_sum), false, false));
     row_sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
-    const int slot = 2 * me + (x0 == 0);
-    const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
-    if (live) {
+    f32x4_t own[D / 8];
 #pragma unroll
-      for (int f = 0; f < D / 8; ++f) {
-        const int c = f >> 2, b = f & 3;
-        const float o[4] = {acc[c][4 * b], acc[c][4 * b + 1], acc[c][4 * b + 2], acc[c][4 * b + 3]};
-        if (complete)
-          kv_write(a, q.row + token, qh, 32 * c + 8 * b + 4 * h, row_sum, o);
-        else
-          store_fragment(ro, part_offset<D>(slot, wave, f, lane), f32x4_t{o[0], o[1], o[2], o[3]});
-      }
-      if (!complete && h == 0)
-        store_stats(rs, (static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + col) * 8, row_max, row_sum);
-    }
-    if (!complete) {
+    for (int f = 0; f < D / 8; ++f)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) own[f][j] = acc[f >> 2][4 * (f & 3) + j];
+    if (complete) {
+      write_rows<D>(a, live, q.row + token, qh, lane, row_sum, own);
+    } else {
       const int first = shares.owner(u - x0), count = shares.owner(u - x0 + cost - 1) - first + 1;
-      if (kv_arrive(out.counters + first, count, &s_last))
-        join_parts<D>(a, out, first, count, wave, lane, live, q.row + token, qh);
+      bool last = kv_is_last(out.counters + first, count, &s_last);
+      if (!last) {
+        const int slot = 2 * me + (x0 == 0);
+        const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
+        if (live) {
+#pragma unroll
+          for (int f = 0; f < D / 8; ++f) store_fragment(ro, part_offset<D>(slot, wave, f, lane), own[f]);
+          if (h == 0) store_stats(rs, (static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + col) * 8, row_max, row_sum);
+        }
+        last = kv_arrive(out.counters + first, count, &s_last);
+      } else if (tid == 0) {
+        rearm(out.counters + first);
+      }
+      if (last)
+        join_parts<D>(a, out, first, count, me - first, wave, lane, live, q.row + token, qh, row_max, row_sum, own);
+      __syncthreads();  // s_last is read by all before the next tile writes it
     }
     u += x1 - x0;
   }

@@ -368,3 +368,13 @@ def test_counters_are_left_zero(gpu_lib):
     torch.cuda.synchronize()
     assert not bool(counters.any())
     b.check(out)
+
+
+@pytest.mark.parametrize("n", [0, 1, 16, 100])
+def test_single_request_of_any_length(gpu_lib, n):
+    """A single request goes to the prompt kernel alone when the caller's longest query may be a
+    prompt: also where it is shorter than said, or empty, with rows behind it."""
+    b = Batch([n], [max(n, 1) + 150], 8, 2, 128, 16, seed=40 + n, pad=101 - n)
+    out = b.run(max_query_len=101)
+    b.check(out)
+    assert torch.equal(out[n:], torch.zeros_like(out[n:]))
