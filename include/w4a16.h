@@ -363,7 +363,7 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * earlier new ones, those new ones j < 64 whose bit j is set.  A row that sees no key gives
  * zeros; keys on a page id outside the cache are not seen; NaN and infinities in keys that a
  * row does not see have no effect on it.  Rows behind cu_query_lens[R] are set to zero if
- * zero_tail, else left as they are.  max_query_len (>= 1) is a hint that chooses kernels and
+ * zero_tail, else left as they are; offsets that decrease anywhere name no rows at all.  max_query_len (>= 1) is a hint that chooses kernels and
  * grid: the longest query of the batch; results are right for any.  scale > 0 and finite;
  * H % KV == 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache
  * (attention.py:118-132). */

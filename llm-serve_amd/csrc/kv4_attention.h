@@ -86,9 +86,15 @@ __device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int 
   *reinterpret_cast<uint4*>(a.out + (static_cast<size_t>(row) * a.H + h) * a.D + ch) = pack_bf16x8(t);
 }
 
-// Zeros for the output rows behind the last request.
-__device__ __forceinline__ void kv_zero_tail(const KvAttentionArgs& a) {
-  const int end = min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
+// Whether request r's offsets decrease.  Offsets that never do give requests of at most T rows in
+// all, which bounds every count of work; with others the kernels do none.
+__device__ __forceinline__ bool kv_decreases(const KvAttentionArgs& a, int r) {
+  return const_ints(a.cu_query_lens)[r + 1] < const_ints(a.cu_query_lens)[r];
+}
+
+// Zeros for the output rows behind the last request (all rows if there is no work).
+__device__ __forceinline__ void kv_zero_tail(const KvAttentionArgs& a, bool all) {
+  const int end = all ? 0 : min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
   const int chunks = a.H * a.D / 8;
   for (int row = end + blockIdx.x; row < a.T; row += gridDim.x)
     for (int c = threadIdx.x; c < chunks; c += blockDim.x)

@@ -134,7 +134,9 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionAr
   const bool few = a.R <= 64;
   KvRequest mine{0, 0, 0, 0};
   int my_units = 0, sum = 0;
+  bool bad = false;
   for (int i = lane; i < a.R; i += 64) {
+    bad |= kv_decreases(a, i);
     mine = kv_request(a, i);
     my_units = kv_units(a, mine, group);
     sum += my_units;
@@ -144,8 +146,9 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionAr
   const int workers = min(total, static_cast<int>(gridDim.x));
   const int me = blockIdx.x;
 
-  if (a.zero_tail) kv_zero_tail(a);
-  if (me >= workers) return;
+  bad = __any(bad);
+  if (a.zero_tail) kv_zero_tail(a, bad);
+  if (bad | (me >= workers)) return;
   const KvShares shares{total / workers, total % workers};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
   int r = 0, base = 0, units;  // the share's first request, the units before it, and its own

@@ -21,14 +21,7 @@
 
 namespace w4a16 {
 
-// Page geometry, sizes in bytes.  Blocks are a power of two of at least 16 tokens, so a
-// 16-token matrix tile never leaves its page.
-struct KvPages {
-  int log2_block;
-  int kv_heads;
-  int num_blocks;
-};
-
+// Blocks are a power of two of at least 16 tokens, so a 16-token matrix tile never leaves its page.
 template <int D>
 __device__ __forceinline__ size_t kv_page_bytes(int log2_block) {
   return static_cast<size_t>(D + 8) << log2_block;

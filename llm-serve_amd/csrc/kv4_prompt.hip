@@ -32,7 +32,8 @@ __device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
 }
 
 // Cost of a request's row tiles in sixteenths of a key tile: tile j of a head costs first +
-// step j, its keys growing with its last token (all keys under a tree mask), plus its set-up.  Host checks keep all sums below 2^31.
+// step j, its keys growing with its last token (all keys under a tree mask), plus its set-up.
+// Host checks keep all sums below 2^31.
 struct KvTileCosts {
   int tiles, first, step;
   __device__ __forceinline__ int before(int j) const {
@@ -181,12 +182,17 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const int per_xcd = gridDim.x / 8;
   const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
 
-  if (a.split_rows == 0 && a.zero_tail) kv_zero_tail(a);  // no split kernel in this call
   int sum = 0;
-  for (int r = lane; r < a.R; r += 64) sum += kv_request_cost(a, kv_request(a, r), group);
+  bool bad = false;
+  for (int r = lane; r < a.R; r += 64) {
+    bad |= kv_decreases(a, r);
+    sum += kv_request_cost(a, kv_request(a, r), group);
+  }
+  bad = __any(bad);
+  if (a.split_rows == 0 && a.zero_tail) kv_zero_tail(a, bad);  // no split kernel in this call
   const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int workers = min(static_cast<int>(gridDim.x), (total + kMinShare - 1) / kMinShare);
-  if (me >= workers) return;
+  if (bad | (me >= workers)) return;
   const KvShares shares{uniform(total / workers), uniform(total % workers)};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
   int r = 0, base = 0;

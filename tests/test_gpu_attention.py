@@ -378,3 +378,49 @@ def test_single_request_of_any_length(gpu_lib, n):
     out = b.run(max_query_len=101)
     b.check(out)
     assert torch.equal(out[n:], torch.zeros_like(out[n:]))
+
+
+@pytest.mark.parametrize("hint", [1, 40])
+def test_many_requests(gpu_lib, hint):
+    """More requests than a wave has lanes, twice over: empty ones, decode rows, drafts, chunks."""
+    rng = random.Random(7)
+    new = [rng.choice([0, 1, 1, 1, 2, 5, 16, 17, 40]) for _ in range(150)]
+    seq = [n + rng.choice([0, 0, 3, 60, 200, 390]) for n in new]
+    b = Batch(new, seq, 4, 1, 64, 16, seed=50, pad=3)
+    print("many", hint, sum(new), flush=True)
+    b.check(b.run(max_query_len=hint))
+
+
+@pytest.mark.parametrize("heads,kv_heads,new", [(8, 2, [16, 17]), (4, 4, [64, 65]), (32, 1, [2, 3, 20]), (128, 1, [1, 3]),
+                                                (7, 1, [9, 10, 37])])
+def test_around_the_kernels_border(gpu_lib, heads, kv_heads, new):
+    """Requests of up to 64 rows (tokens x heads of a group) and the next longer ones in one call."""
+    b = Batch(new, [n + 70 * i for i, n in enumerate(new)], heads, kv_heads, 64, 16, seed=heads)
+    b.check(b.run(max_query_len=max(new)))
+
+
+@pytest.mark.parametrize("hint", [1, 100])
+@pytest.mark.parametrize("requests", [1, 2])
+def test_fewer_keys_than_rows(gpu_lib, hint, requests):
+    """A sequence shorter than its new rows, or empty: the first rows see nothing and are zero."""
+    b = Batch([100] * requests, [37, 0][:requests], 8, 2, 128, 16, seed=51)
+    out = b.run(max_query_len=hint)
+    b.check(out)
+    assert torch.equal(out[:63], torch.zeros_like(out[:63])) and torch.equal(out[100:], torch.zeros_like(out[100:]))
+    none = Batch([100], [0], 8, 2, 128, 16, seed=52)
+    assert not bool(none.run(max_query_len=hint).any())
+
+
+@pytest.mark.parametrize("hint", [1, 100])
+def test_decreasing_offsets_name_no_rows(gpu_lib, hint):
+    """Offsets that decrease somewhere: a zero result, `out` left as it was, and the next call right."""
+    b = Batch([100, 90, 1], [150, 90, 300], 8, 2, 128, 16, seed=53)
+    q, cache, tables, seq, offsets = b.args()
+    for broken in ([0, 100, 50, 191], [0, 191, 0, 191], [5, 0, 0, 191], [0, 100, 190, -1]):
+        print("offsets", broken, flush=True)
+        args = q, cache, tables, seq, b.int32(broken)
+        assert not bool(attn.attention_int4(*args, block_size=16, max_query_len=hint).any())
+        mine = torch.full((191, 8, 128), 7.0, dtype=torch.bfloat16, device="cuda")
+        attn.attention_int4(*args, block_size=16, max_query_len=hint, out=mine)
+        assert bool((mine == 7.0).all())
+    b.check(b.run(max_query_len=hint))
