@@ -1265,12 +1265,12 @@ int validate_kv_heads(int T, int R, int H, int KV, int D, int log2_block, int wi
   if (T == 0 || R == 0) return W4A16_OK;
   if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
-  // The kernels count their work in 32 bits: units of 16 rows x 128 keys, and of 256 rows x 4 keys
-  // (with up to 80 more a tile) for requests of more than 64 rows.
+  // The kernels count their work in 32 bits: units of 16 rows x 128 keys, and for requests of more
+  // than 64 rows tiles of 256 rows that cost at most (keys + T) / 4 + rows / 256 + 160 each.
   const int64_t rows = static_cast<int64_t>(T) * (H / KV), keys = static_cast<int64_t>(width) << log2_block;
   const int64_t tiles = (rows + 15) / 16 + R, spans = (keys + 127) / 128;
   const int64_t longer = R < rows / 65 ? R : rows / 65, prompt_tiles = rows / 256 + longer;
-  if (spans > 0x7FFFFFFF / tiles / KV || (prompt_tiles > 0 && (keys + T) / 4 + 80 > 0x7FFFFFFF / prompt_tiles / KV))
+  if (spans > 0x7FFFFFFF / tiles / KV || (prompt_tiles > 0 && (keys + T) / 4 + rows / 256 + 160 > 0x7FFFFFFF / prompt_tiles / KV))
     return fail(W4A16_ERR_SHAPE, "%d rows over block tables of %d blocks are too much work for one call", T, width);
   return W4A16_OK;
 }

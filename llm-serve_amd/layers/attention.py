@@ -276,7 +276,7 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     request r's rows ``cu_query_lens[r]`` .. ``cu_query_lens[r + 1]`` are the last tokens of its
     ``seq_lens[r]``, on the pages ``block_tables[r]`` names.  Returns bf16 [rows, heads, head_dim].
 
-    ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest query of the batch if
+    Offsets that decrease name no rows at all.  ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest query of the batch if
     the caller knows it (1 for a decode step), picks kernels; results are right whatever it is.
     ``tree_mask`` (int64 [rows]) replaces causality among a request's new rows: row t sees the
     cached tokens and those new ones j < 64 whose bit j is set.  A row that sees nothing is zero.
@@ -284,8 +284,8 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     they are left as they were."""
     # One expression accepts what all the checks accept; only what it does not goes through them.
     shape, tshape, index = q.shape, block_tables.shape, cache.get_device()
-    head_dim = shape[-1]
-    if not (index >= 0 and len(shape) == 3 and block_size in BLOCK_SIZES and head_dim in HEAD_DIMS
+    head_dim = shape[2] if len(shape) == 3 else 0
+    if not (index >= 0 and block_size in BLOCK_SIZES and head_dim in HEAD_DIMS
             and cache.dtype is _U8 and cache.is_contiguous() and len(cache.shape) == 3
             and cache.shape[2] == block_size * (head_dim + 8) and cache.shape[0] * block_size < 1 << 31
             and shape[1] > 0 and cache.shape[1] > 0 and shape[1] % cache.shape[1] == 0

@@ -138,3 +138,24 @@ def test_oracle_attention_of_one_key_is_its_value():
     out, spread = ora.attention(x, cache, [[0]], [1], [0, 1], 16)
     assert torch.equal(out, ora.load(cache, [0], 16)[1])
     assert bool((spread >= 2 * 2.0 ** -8 * out.abs()).all())  # the weights' and the values' roundings
+
+
+def test_wrong_ranks_are_refused():
+    cache = torch.zeros(4, 2, 16 * 136, dtype=torch.uint8)
+    lists = torch.zeros(2, dtype=torch.int32)
+    for shape in ((), (128,), (3, 256), (1, 3, 2, 128)):
+        with pytest.raises(ValueError):
+            attn.attention_int4(torch.zeros(shape, dtype=torch.bfloat16), cache, lists[None], lists[:1], lists,
+                                block_size=16)
+
+
+def test_work_beyond_32_bits_is_refused(dll):
+    """Prompt work is counted as 8 heads x 513 tiles x (2^20 + 2^17) / 4 = 1.2e9 units for 2^17 rows over
+    2^20 keys, and as 8 x 1025 x (2^20 + 2^18) / 4 = 2.7e9 for 2^18 rows, beyond 2^31."""
+    assert dll.w4a16_kv_attention_workspace(1 << 17, 1, 8, 8, 128, 256, 1 << 12, 1 << 17) > 0
+    assert dll.w4a16_kv_attention_workspace(1 << 18, 1, 8, 8, 128, 256, 1 << 12, 1 << 18) == 0
+    for t, r, h, kv, width, longest in ((1 << 18, 1, 8, 8, 1 << 20, 1 << 18),     # a long prompt over 2^28 keys
+                                        (4096, 4096, 64, 64, 1 << 21, 1),         # decode rows over 2^29 keys
+                                        (1 << 20, 1, 1024, 1, 1 << 20, 1 << 20),  # many heads of one kv head
+                                        (1 << 24, 1, 128, 1, 16, 1)):             # rows x heads
+        assert dll.w4a16_kv_attention_workspace(t, r, h, kv, 128, 256, width, longest) == 0
