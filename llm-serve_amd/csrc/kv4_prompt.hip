@@ -13,6 +13,18 @@
 // slots 8 h + j of a lane half h are the keys 16 s + 4 h + j (j < 4) and 16 s + 8 + 4 h + j - 4,
 // and V's columns are written in that order.  The output is O^T = V^T P^T: every statistic of a
 // row sits in the two lanes that hold it.
+//
+// What bounds it: a tile of 64 keys costs a SIMD (two waves) some 2000 cycles of matrix
+// instructions, and 2600 of vector instructions: softmax, conversion.  They overlap between the two
+// waves in part only, as every tile ends in a barrier: about 2.2 us a tile, 930 TFLOP/s for 4096
+// rows behind 12288 cached tokens (1.03 ms; a large matrix product of the library reaches 1249).  A
+// row tile costs 4 to 5 us besides its keys (queries, the first keys, writing or joining), which is
+// what short prompts pay: 2039 tokens take 58 us, 590 TFLOP/s.  Workgroups take equal shares of
+// the cost of all row tiles, so a share may end inside a tile's keys; tiles as units would leave a
+// causal prompt's last rows to few workgroups.  Measured and not taken: a conversion interleaved with
+// the same wave's first product (4096 rows 3 % faster, 2039 rows 3 % slower: both converters' loops
+// are then apart, twice the code to fetch), and with it waves half a tile apart over three value
+// buffers (registers spill; 5 and 20 % slower).
 #include "kv4_attention.h"
 
 namespace w4a16 {
@@ -23,7 +35,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
 constexpr int kTileCost = 16;  // cost units of a tile of keys
-constexpr int kSetupCost = 16;  // of a row tile besides its keys
+constexpr int kSetupCost = 16;  // of a row tile besides its keys: 16, 40 and 80 give 2039 rows in 60, 62 and 63 us
 constexpr int kMinShare = 8 * kTileCost;
 constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
