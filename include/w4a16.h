@@ -358,7 +358,8 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * request r owns rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1, the last tokens of its
  * seq_lens[r] (at most width * block_size are reached) on the pages of tables[r]; query head h
  * reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v with
- * fp32 scores, statistics and sums; the weights enter the second product as bf16(p * s_v).
+ * fp32 scores, statistics and sums; the second product's operands are bf16(p * s_v) and exact
+ * codes, or (requests of more than 64 rows a kv head) fp16 weights, keys and values.
  * tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of the
  * earlier new ones, those new ones j < 64 whose bit j is set.  A row that sees no key gives
  * zeros; keys on a page id outside the cache are not seen; NaN and infinities in keys that a

@@ -4,9 +4,15 @@
 // 256 rows (tokens x heads of a kv head's group) of a request, 32 a wave, and walks their keys in
 // tiles of 64.  Eight waves would each have to unpack the same codes, and unpacking costs more
 // vector instructions than the softmax, so a tile is dequantized once for all of them: the first
-// four waves turn the K codes of the next tile into bf16 rows in LDS while the other four turn
-// the V codes into bf16 columns, into the buffer that is not being read.  Keys and values are
-// therefore bf16(s (c - z)) here, the values that kv_load_kernel returns.
+// four waves turn the K codes of the next tile into rows in LDS while the other four turn the V
+// codes into columns, into the buffer that is not being read.
+//
+// Operands are fp16, whose 11 bits hold s (c - z) to half a unit in 2^-11: an error an eighth of
+// bf16's, below the output's rounding.  (As bf16, keys and values moved outputs by 0.0036 of 64-bit
+// ones against 0.0017 for the rounding alone; codes as exact bf16 128 + c and scales applied to
+// scores and weights took 20 % longer, and lost as much in long sums of 128 P.)  fp16's range is
+// met by powers of two: one out of each 16 keys' scales and each row of queries.  Those of keys and
+// queries join the softmax's scale in the exponent's multiplier, those of values are its addend.
 //
 // Scores are formed transposed, S^T = K Q^T, so that a lane holds 16 keys' scores of one row in
 // the accumulator layout, and P^T is the second product's operand as it stands: its 16 contraction
@@ -16,21 +22,23 @@
 //
 // What bounds it: a tile of 64 keys costs a SIMD (two waves) some 2000 cycles of matrix
 // instructions, and 2600 of vector instructions: softmax, conversion.  They overlap between the two
-// waves in part only, as every tile ends in a barrier: about 2.2 us a tile, 930 TFLOP/s for 4096
-// rows behind 12288 cached tokens (1.03 ms; a large matrix product of the library reaches 1249).  A
+// waves in part only, as every tile ends in a barrier: about 2.2 us a tile, 890 TFLOP/s for 4096
+// rows behind 12288 cached tokens (1.08 ms; a large matrix product of the library reaches 1249).  A
 // row tile costs 4 to 5 us besides its keys (queries, the first keys, writing or joining), which is
-// what short prompts pay: 2039 tokens take 58 us, 590 TFLOP/s.  Workgroups take equal shares of
+// what short prompts pay: 2039 tokens take 62 us, 550 TFLOP/s.  Workgroups take equal shares of
 // the cost of all row tiles, so a share may end inside a tile's keys; tiles as units would leave a
-// causal prompt's last rows to few workgroups.  Measured and not taken: a conversion interleaved with
-// the same wave's first product (4096 rows 3 % faster, 2039 rows 3 % slower: both converters' loops
-// are then apart, twice the code to fetch), and with it waves half a tile apart over three value
-// buffers (registers spill; 5 and 20 % slower).
+// causal prompt's last rows to few workgroups.  Measured and not taken, with bf16 operands: a
+// conversion interleaved with the same wave's first product (4096 rows 3 % faster, 2039 rows 3 %
+// slower: both converters' loops are then apart, twice the code to fetch), and with it waves half a
+// tile apart over three value buffers (registers spill; 5 and 20 % slower).
 #include "kv4_attention.h"
 
 namespace w4a16 {
 namespace {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 
 constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
@@ -39,8 +47,15 @@ constexpr int kSetupCost = 16;  // of a row tile besides its keys: 16, 40 and 80
 constexpr int kMinShare = 8 * kTileCost;
 constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
-__device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+// Exponents.  fp16 has the codes' products with a scale to 11 bits, but not bf16's range, so a power
+// of two is taken out of each group of 16 keys' scales (the largest is brought to 2^10 .. 2^11) and of
+// each row of queries (2^14 .. 2^15), as fields of fp32 exponents.  What lies 2^-24 below its group's
+// largest loses bits: it is that much smaller in the sums.  Fields are held in range: groups whose
+// scales are all below 2^-63 keep that exponent and lose bits below 2^-87.
+constexpr int kGroupFactor = 264, kRowFactor = 268;
+
+__device__ __forceinline__ f32x16_t mfma32(f16x8_t a, f16x8_t b, f32x16_t c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
 
 // Cost of a request's row tiles in sixteenths of a key tile: tile j of a head costs first +
@@ -70,43 +85,44 @@ __device__ __forceinline__ int kv_request_cost(const KvAttentionArgs& a, const K
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-// Codes -> fp32 without a conversion: a nibble in the low bits of an fp16 1024.0 is 1024 + c, one
-// in bits 4 .. 7 of an fp16 64.0 is 64 + c, and v_fma_mix_f32 takes either half of the register as
-// it stands: (1024 + c) s - (1024 + z) s, both terms and the result exact in fp32.  A word (w, and
-// w >> 8) gives its 8 codes in 5 instructions.
-typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+// Sum / maximum of a value over a lane and the one of the wave's other half.
+__device__ __forceinline__ u32x2_t halves(float v) {
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+  const u32x2_t b = halves(v);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+__device__ __forceinline__ float halves_max(float v) {
+  const u32x2_t b = halves(v);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float x, float y) {
+  return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+}
+
+// 2^(field - 127).
+__device__ __forceinline__ float power(int field) { return __uint_as_float(static_cast<uint32_t>(field) << 23); }
+
+// Nibbles of a pair of keys or channels -> fp16 (c - z) s, rounded once: 1024 + c is exact with c in an
+// fp16's low bits, and so is the difference from 1024 + z.
+__device__ __forceinline__ uint32_t pair_value(uint32_t biased, uint32_t minus_zero, uint32_t scale) {
+  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2_t, biased) + __builtin_bit_cast(f16x2_t, minus_zero)) *
+                                          __builtin_bit_cast(f16x2_t, scale));
+}
 
 // The masks in SGPRs and the biases in VGPRs, hidden from constant folding, so that each and-or is
-// one v_and_or_b32 (see NibbleConsts).
-struct FusedConsts {
+// one v_and_or_b32 (see NibbleConsts).  In bits 4 .. 7 of an fp16 64.0 a nibble is 64 + c.
+struct HalfConsts {
   uint32_t mask_low, mask_high, bias_low, bias_high;
 };
 
-__device__ __forceinline__ FusedConsts fused_consts() {
-  FusedConsts k{0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
+__device__ __forceinline__ HalfConsts half_consts() {
+  HalfConsts k{0x000F000Fu, 0x00F000F0u, 0x64006400u, 0x54005400u};
   asm volatile("" : "+s"(k.mask_low), "+s"(k.mask_high));
   asm volatile("" : "+v"(k.bias_low), "+v"(k.bias_high));
   return k;
-}
-
-struct RowScale {
-  float s, low, high;  // the scale; -(1024 + z) s and -(64 + z) s
-};
-
-__device__ __forceinline__ RowScale row_scale(uint32_t meta) {
-  const float s = kv_meta_scale(meta), z = kv_meta_zero128(meta);
-  return RowScale{s, -s * (z + 896.0f), -s * (z - 64.0f)};
-}
-
-// Nibbles 0 and 4 (f[0], f[1]: channels 0, 1 of the word) and 1 and 5 (f[2], f[3]: channels 2, 3);
-// of w >> 8, channels 4 .. 7.
-__device__ __forceinline__ void four_values(float (&f)[4], uint32_t w, const RowScale& r, const FusedConsts& k) {
-  const f16x2_t a = __builtin_bit_cast(f16x2_t, (w & k.mask_low) | k.bias_low);
-  const f16x2_t b = __builtin_bit_cast(f16x2_t, (w & k.mask_high) | k.bias_high);
-  f[0] = __builtin_fmaf(static_cast<float>(a[0]), r.s, r.low);
-  f[1] = __builtin_fmaf(static_cast<float>(a[1]), r.s, r.low);
-  f[2] = __builtin_fmaf(static_cast<float>(b[0]), r.s, r.high);
-  f[3] = __builtin_fmaf(static_cast<float>(b[1]), r.s, r.high);
 }
 
 // Byte offset of a lane's fragment f (four channels: 32 (f / 4) + 8 (f % 4) + 4 (lane / 32) ..) of
@@ -115,6 +131,9 @@ template <int D>
 __device__ __forceinline__ uint32_t part_offset(int slot, int wave, int f, int lane) {
   return ((static_cast<uint32_t>(slot) * 8 + wave) * (D / 8) + f) * 1024u + lane * 16u;
 }
+
+// The exponent field of a group, from its largest scale.
+__device__ __forceinline__ int group_field(float top) { return min(max(static_cast<int>(__float_as_uint(top) >> 23), 64), 254); }
 
 // Two fragments of a lane -- channels 4 h .. of eights b and b + 1 -- to the output: the halves of
 // the wave exchange theirs, so that a lane writes one eight's 16 bytes.
@@ -167,7 +186,7 @@ __device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPar
       for (int f = 0; f < kFrags; ++f) v[f] = load_fragment(ro, live ? part_offset<D>(slot, wave, f, lane) : kOutOfRange);
     }
     const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
-    const float x = __builtin_amdgcn_exp2f((top - ref) * a.scale_log2e), y = __builtin_amdgcn_exp2f((m - ref) * a.scale_log2e);
+    const float x = __builtin_amdgcn_exp2f(top - ref), y = __builtin_amdgcn_exp2f(m - ref);
     top = next;
     sum = sum * x + l * y;
 #pragma unroll
@@ -184,6 +203,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   constexpr int kSteps = D / 16, kTiles = D / 32;
   __shared__ __align__(16) uint16_t s_k[2][kKeys][kPitchK];
   __shared__ __align__(16) uint16_t s_v[2][D][kPitchV];
+  // A group of 16 keys: what a raw score is multiplied by, and the values' power of two.
+  __shared__ __align__(16) float s_score[2][4], s_log[2][4], s_part[2][4];
   __shared__ int s_last;
   __shared__ uint64_t s_held[2][4];  // 4 bits a key: whether it is in the sequence and on a page
 
@@ -222,7 +243,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   }
   KvRequest q = kv_request(a, r);
 
-  const FusedConsts fc = fused_consts();
+  const HalfConsts hc = half_consts();
   const int col = lane & 31, h = lane >> 5;
   const float scale = a.scale_log2e;
 
@@ -298,10 +319,10 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         meta[1] = *reinterpret_cast<const uint32_t*>(m + (4 << a.log2_block));
       }
     };
-    // Fetched codes -> bf16(s (c - z)) in LDS.  Keys outside the sequence or on no page become
-    // zeros (they hold anything) and are masked by s_held.  A key whose value row is NaN would
-    // reach rows that do not see it (0 * NaN in the second product): its values become zeros and
-    // its scores NaN, which masks hide from those rows, and which make every row that sees it NaN.
+    // Fetched codes -> fp16 in LDS.  Keys outside the sequence or on no page become zeros (they hold
+    // anything) and are masked by s_held.  A key whose value row is NaN would reach rows that do not
+    // see it (0 * NaN in the second product): its values become zeros and its scores NaN, which masks
+    // hide from those rows, and which make every row that sees it NaN.
     auto convert = [&](int key_tile, int buf) {
       const int key = key_tile * kKeys + my_key;
       if (converts_v) {
@@ -309,41 +330,64 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
         for (int i = 0; i < 8; ++i) top = max(top, meta[i] & 0x7FFFFFFFu);
         if (__any(!held | (key + 12 > q.keys) | (top >= 0x7F800000u))) {
+          top = 0;
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const bool use = held & (key + (i < 4 ? i : i + 4) < q.keys) & (fabsf(kv_meta_scale(meta[i])) < INFINITY);
             meta[i] = use ? meta[i] : kZeroMeta;
+            top = max(top, meta[i] & 0x7FFFFFFFu);
           }
         }
-        // A thread's channels: 4 neighbours of a word (D = 128), or 2 (D = 64: nibbles 0 and 4, or 1 and 5).
-        const int shift = D == 128 ? 8 * part : 8 * (part >> 1) + 4 * (part & 1);
-        const int ch = 8 * word + (D == 128 ? 4 : 2) * part;
-        uint32_t w[4][4];
+        // the next lane has the other half of the 16 keys
+        const int field = group_field(fmaxf(__uint_as_float(top), dpp_f32<0xB1>(__uint_as_float(top))));
+        const float factor = power(kGroupFactor - field);
+        if (t < 8 && !(t & 1)) {
+          s_log[buf][vgroup >> 1] = static_cast<float>(field - (kGroupFactor - 127));
+          s_part[buf][vgroup >> 1] = factor;
+        }
+        // A half of a word is its even or its odd channels, nibble i being channel 2 i or 2 i + 1: the
+        // halves of two keys side by side, then a nibble of each.  A thread takes the 4 channels of a
+        // half (D = 128), or 2 of them (D = 64).
+        const int half = part & 1, nibble = D == 128 ? 0 : 2 * (part >> 1);
+        const uint32_t select = half ? 0x07060302u : 0x05040100u;
+        uint32_t w[D / 32][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          float f[4], g[4];
-          four_values(f, raw[2 * i] >> shift, row_scale(meta[2 * i]), fc);
-          four_values(g, raw[2 * i + 1] >> shift, row_scale(meta[2 * i + 1]), fc);
+          const uint32_t pair = __builtin_amdgcn_perm(raw[2 * i + 1], raw[2 * i], select) >> (4 * nibble);
+          const uint32_t zero = __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x05040100u);
+          const uint32_t scales = pack_f16x2(kv_meta_scale(meta[2 * i]) * factor, kv_meta_scale(meta[2 * i + 1]) * factor);
+          const uint32_t minus = ((zero & hc.mask_low) | hc.bias_low) ^ 0x80008000u;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) w[c][i] = pack_bf16x2(f[c], g[c]);
+          for (int c = 0; c < D / 32; ++c) w[c][i] = pair_value(((pair >> (4 * c)) & hc.mask_low) | hc.bias_low, minus, scales);
         }
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
-          *reinterpret_cast<uint4*>(&s_v[buf][ch + c][8 * vgroup]) = make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
+          *reinterpret_cast<uint4*>(&s_v[buf][8 * word + 2 * (nibble + c) + half][8 * vgroup]) =
+              make_uint4(w[c][0], w[c][1], w[c][2], w[c][3]);
       } else {
         const bool use = held & (key < q.keys);
         const uint64_t all = __ballot(use);
         if (lane == 0) s_held[buf][wave] = all;
         uint32_t m = fabsf(kv_meta_scale(meta[1])) < INFINITY ? meta[0] : kNanMeta;
         m = use ? m : kZeroMeta;
-        const RowScale rs = row_scale(m);
+        // a wave has the 16 keys of one group, a key in four lanes
+        const uint32_t bits = m & 0x7FFFFFFFu;
+        float top = bits < 0x7F800000u ? __uint_as_float(bits) : 0.0f;
+        top = fmaxf(top, dpp_f32<0x124>(top));
+        top = fmaxf(top, dpp_f32<0x128>(top));
+        const int field = group_field(column_max(top));
+        if (lane == 0) s_score[buf][wave] = power(field - (kGroupFactor - 254)) * scale;
+        const float s = kv_meta_scale(m) * power(kGroupFactor - field);
+        const uint32_t scales = pack_f16x2(s, s), z = m & 15u;
+        const uint32_t minus_low = (0xE400u | z) * 0x00010001u, minus_high = (0xD400u | (z << 4)) * 0x00010001u;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
-          float f[4], g[4];
-          four_values(f, raw[i], rs, fc);
-          four_values(g, raw[i] >> 8, rs, fc);
+          const uint32_t lo = raw[i], hi = raw[i] >> 8;
           *reinterpret_cast<uint4*>(&s_k[buf][t >> 2][(D / 4) * chunk + 8 * i]) =
-              make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(g[0], g[1]), pack_bf16x2(g[2], g[3]));
+              make_uint4(pair_value((lo & hc.mask_low) | hc.bias_low, minus_low, scales),
+                         pair_value((lo & hc.mask_high) | hc.bias_high, minus_high, scales),
+                         pair_value((hi & hc.mask_low) | hc.bias_low, minus_low, scales),
+                         pair_value((hi & hc.mask_high) | hc.bias_high, minus_high, scales));
         }
       }
     };
@@ -359,13 +403,35 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     const int row = first_row + col;
     const int token = row / group, qh = head * group + row - token * group;
     const bool live = 32 * wave + col < rows;
-    bf16x8_t qf[kSteps];
+    f16x8_t qf[kSteps];
+    float row_power;  // what a row's raw scores are multiplied by
+    {
+      typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+      uint4 raw_q[kSteps];
+      u16x2_t top = {0, 0};
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (live)
-        w = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + qh * a.q_stride_h + 16 * i + 8 * h);
-      qf[i] = __builtin_bit_cast(bf16x8_t, w);
+      for (int i = 0; i < kSteps; ++i) {
+        raw_q[i] = make_uint4(0, 0, 0, 0);
+        if (live)
+          raw_q[i] = *reinterpret_cast<const uint4*>(a.q + (q.row + token) * a.q_stride_t + qh * a.q_stride_h + 16 * i + 8 * h);
+        const uint32_t w[4] = {raw_q[i].x, raw_q[i].y, raw_q[i].z, raw_q[i].w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[j] & 0x7FFF7FFFu));
+      }
+      const uint16_t t0 = top[0], t1 = top[1];
+      const float most = halves_max(__uint_as_float(static_cast<uint32_t>(t0 > t1 ? t0 : t1) >> 7 << 23));
+      const int field = min(max(static_cast<int>(__float_as_uint(most) >> 23), 27), 254);
+      const float factor = power(kRowFactor - field);
+      row_power = power(field - (kRowFactor - 254));
+#pragma unroll
+      for (int i = 0; i < kSteps; ++i) {
+        float f[8];
+        unpack_bf16x8(raw_q[i], f);
+        u32x4_t w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pack_f16x2(f[2 * j] * factor, f[2 * j + 1] * factor);
+        qf[i] = __builtin_bit_cast(f16x8_t, w);
+      }
     }
     const bool tree = a.tree_mask != nullptr;
     const uint64_t bits = tree && live ? a.tree_mask[q.row + token] : 0;
@@ -381,7 +447,6 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[c][i] = 0.0f;
     float row_max = -INFINITY, row_sum = 0.0f;
-    const bf16x2_t ones = __builtin_bit_cast(bf16x2_t, 0x3F803F80u);
 
     if (t0 < t1) {
       convert(t0, 0);
@@ -417,16 +482,16 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         // LDS reads run ahead of the matrix instructions by one group of four fragments (two steps
         // of K, one of V); V's first group is read ahead of the softmax.  Left to itself the
         // compiler reads each fragment just before its use.
-        bf16x8_t frag[2][4];
-        auto read_k = [&](int group_of, bf16x8_t (&f)[4]) {
+        f16x8_t frag[2][4];
+        auto read_k = [&](int group_of, f16x8_t (&f)[4]) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            f[j] = *reinterpret_cast<const bf16x8_t*>(&s_k[buf][32 * (j & 1) + col][16 * (2 * group_of + (j >> 1)) + 8 * h]);
+            f[j] = *reinterpret_cast<const f16x8_t*>(&s_k[buf][32 * (j & 1) + col][16 * (2 * group_of + (j >> 1)) + 8 * h]);
         };
-        auto read_v = [&](int step, bf16x8_t (&f)[4]) {
+        auto read_v = [&](int step, f16x8_t (&f)[4]) {
 #pragma unroll
           for (int c = 0; c < kTiles; ++c)
-            f[c] = *reinterpret_cast<const bf16x8_t*>(&s_v[buf][32 * c + col][8 * (2 * step + h)]);
+            f[c] = *reinterpret_cast<const f16x8_t*>(&s_v[buf][32 * c + col][8 * (2 * step + h)]);
         };
         read_k(0, frag[0]);
 #pragma unroll
@@ -467,20 +532,29 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
               }
           }
         }
-        float top = sc[0][0];
+        // A weight is 2^(score + the values' power - reference): the powers of two of keys, values and
+        // queries are one multiplier and one addend a group.
+        const f32x4_t of_score = *reinterpret_cast<const f32x4_t*>(s_score[buf]), of_value = *reinterpret_cast<const f32x4_t*>(s_log[buf]);
+        const f32x4_t of_sum = *reinterpret_cast<const f32x4_t*>(s_part[buf]);
+        float by[4], top = -INFINITY;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[n][i]);
-        const u32x2_t other = __builtin_bit_cast(
-            u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false));
-        top = fmaxf(__uint_as_float(other[0]), __uint_as_float(other[1]));
-        // The reference follows the maximum only when that leads it by 2^8: weights up to 2^8 are as
-        // exact as weights up to 1, and sums are rescaled rarely.
-        const bool grew = top > row_max && (top - row_max) * scale > 8.0f;
+          for (int s = 0; s < 2; ++s) {
+            by[2 * n + s] = __builtin_amdgcn_fmed3f(of_score[2 * n + s] * row_power, 0x1p-126f, 0x1p127f);
+            float most = sc[n][8 * s];
+#pragma unroll
+            for (int i = 1; i < 8; ++i) most = fmaxf(most, sc[n][8 * s + i]);
+            top = fmaxf(top, __builtin_fmaf(most, by[2 * n + s], of_value[2 * n + s]));
+          }
+        top = halves_max(top);
+        // The reference is 7 below the maximum where it was set, and follows when that leads it by
+        // more than 15: weights stay below 2^15 as fp16, keep 11 bits down to 2^-21 of the row's
+        // largest at least, and sums are rescaled rarely.
+        const bool grew = top > row_max && top - row_max > 15.0f;
         if (__any(grew)) {
-          const float next = grew ? top : row_max;
-          const float f = __builtin_amdgcn_exp2f((row_max - (next == -INFINITY ? 0.0f : next)) * scale);
+          const float next = grew ? top - 7.0f : row_max;
+          const float f = __builtin_amdgcn_exp2f(row_max - (next == -INFINITY ? 0.0f : next));
           row_max = next;
           row_sum *= f;
 #pragma unroll
@@ -488,23 +562,25 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[c][i] *= f;
         }
-        const float ref = (row_max == -INFINITY ? 0.0f : row_max) * scale;
+        const float ref = row_max == -INFINITY ? 0.0f : row_max;
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             if (2 * n + s < 3) read_v(2 * n + s + 1, frag[(s + 1) & 1]);
             u32x4_t w;
+            const float from = of_value[2 * n + s] - ref;
+            float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i], scale, -ref));
-              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i + 1], scale, -ref));
-              const uint32_t pair = pack_bf16x2(p0, p1);
-              w[i] = pair;
-              // the sum takes the weights as the product does, rounded
-              row_sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, pair), ones, row_sum, false);
+              const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i], by[2 * n + s], from));
+              const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][8 * s + 2 * i + 1], by[2 * n + s], from));
+              sum += p0;
+              sum += p1;
+              w[i] = pack_f16x2(p0, p1);
             }
-            const bf16x8_t pf = __builtin_bit_cast(bf16x8_t, w);
+            row_sum = __builtin_fmaf(sum, of_sum[2 * n + s], row_sum);
+            const f16x8_t pf = __builtin_bit_cast(f16x8_t, w);
 #pragma unroll
             for (int c = 0; c < kTiles; ++c) acc[c] = mfma32(frag[s & 1][c], pf, acc[c]);
           }
@@ -513,9 +589,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
       __syncthreads();
     }
 
-    const u32x2_t both = __builtin_bit_cast(
-        u32x2_t, __builtin_amdgcn_permlane32_swap(__float_as_uint(row_sum), __float_as_uint(row_sum), false, false));
-    row_sum = __uint_as_float(both[0]) + __uint_as_float(both[1]);
+    row_sum = halves_sum(row_sum);
     f32x4_t own[D / 8];
 #pragma unroll
     for (int f = 0; f < D / 8; ++f)
