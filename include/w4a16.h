@@ -358,16 +358,17 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * request r owns rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1, the last tokens of its
  * seq_lens[r] (at most width * block_size are reached) on the pages of tables[r]; query head h
  * reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v with
- * fp32 scores, statistics and sums; the second product's operands are bf16(p * s_v) and exact
- * codes, or (requests of more than 64 rows a kv head) fp16 weights, keys and values.
- * tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of the
- * earlier new ones, those new ones j < 64 whose bit j is set.  A row that sees no key gives
- * zeros; keys on a page id outside the cache are not seen; NaN and infinities in keys that a
- * row does not see have no effect on it.  Rows behind cu_query_lens[R] are set to zero if
- * zero_tail, else left as they are; offsets that decrease anywhere name no rows at all.  max_query_len (>= 1) is a hint that chooses kernels and
- * grid: the longest query of the batch; results are right for any.  scale > 0 and finite;
- * H % KV == 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache
- * (attention.py:118-132). */
+ * fp32 scores, statistics and sums.  The second product's operands are bf16(p * s_v) and exact
+ * codes; for requests of more than 64 rows a kv head, all operands are fp16 with a power of two
+ * taken out of each query row and of every 16 keys: a key or value whose scale is 2^-24 of the
+ * largest among its 16 loses bits.  tree_mask (may be null) [T]: row t then sees its request's
+ * cached tokens and, instead of the earlier new ones, those new ones j < 64 whose bit j is set.
+ * A row that sees no key gives zeros; keys on a page id outside the cache are not seen; NaN and
+ * infinities in keys that a row does not see have no effect on it.  Rows behind cu_query_lens[R]
+ * are set to zero if zero_tail, else left as they are; offsets that decrease anywhere name no rows
+ * at all.  max_query_len (>= 1) is a hint that chooses kernels and grid: the longest query of the
+ * batch; results are right for any.  scale > 0 and finite; H % KV == 0.  Replaces
+ * flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:118-132). */
 int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
                        const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
                        const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale,

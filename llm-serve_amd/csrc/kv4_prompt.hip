@@ -107,8 +107,8 @@ __device__ __forceinline__ float power(int field) { return __uint_as_float(stati
 
 // Nibbles of a pair of keys or channels -> fp16 (c - z) s, rounded once: 1024 + c is exact with c in an
 // fp16's low bits, and so is the difference from 1024 + z.
-__device__ __forceinline__ uint32_t pair_value(uint32_t biased, uint32_t minus_zero, uint32_t scale) {
-  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2_t, biased) + __builtin_bit_cast(f16x2_t, minus_zero)) *
+__device__ __forceinline__ uint32_t pair_value(uint32_t biased, uint32_t zero, uint32_t scale) {
+  return __builtin_bit_cast(uint32_t, (__builtin_bit_cast(f16x2_t, biased) - __builtin_bit_cast(f16x2_t, zero)) *
                                           __builtin_bit_cast(f16x2_t, scale));
 }
 
@@ -199,7 +199,7 @@ __device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPar
 
 template <int D>
 __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentionArgs a, KvPartials out) {
-  constexpr int kPitchK = D + 8, kPitchV = kKeys + 8;  // bf16 elements; 16-byte reads of 16 lanes meet all banks
+  constexpr int kPitchK = D + 8, kPitchV = kKeys + 8;  // fp16 elements; 16-byte reads of 16 lanes meet all banks
   constexpr int kSteps = D / 16, kTiles = D / 32;
   __shared__ __align__(16) uint16_t s_k[2][kKeys][kPitchK];
   __shared__ __align__(16) uint16_t s_v[2][D][kPitchV];
@@ -354,11 +354,11 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const uint32_t pair = __builtin_amdgcn_perm(raw[2 * i + 1], raw[2 * i], select) >> (4 * nibble);
-          const uint32_t zero = __builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x05040100u);
+          const uint32_t zero =
+              (__builtin_amdgcn_perm(meta[2 * i + 1], meta[2 * i], 0x05040100u) & hc.mask_low) | hc.bias_low;
           const uint32_t scales = pack_f16x2(kv_meta_scale(meta[2 * i]) * factor, kv_meta_scale(meta[2 * i + 1]) * factor);
-          const uint32_t minus = ((zero & hc.mask_low) | hc.bias_low) ^ 0x80008000u;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) w[c][i] = pair_value(((pair >> (4 * c)) & hc.mask_low) | hc.bias_low, minus, scales);
+          for (int c = 0; c < D / 32; ++c) w[c][i] = pair_value(((pair >> (4 * c)) & hc.mask_low) | hc.bias_low, zero, scales);
         }
 #pragma unroll
         for (int c = 0; c < D / 32; ++c)
@@ -379,15 +379,15 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         if (lane == 0) s_score[buf][wave] = power(field - (kGroupFactor - 254)) * scale;
         const float s = kv_meta_scale(m) * power(kGroupFactor - field);
         const uint32_t scales = pack_f16x2(s, s), z = m & 15u;
-        const uint32_t minus_low = (0xE400u | z) * 0x00010001u, minus_high = (0xD400u | (z << 4)) * 0x00010001u;
+        const uint32_t zero_low = (0x6400u | z) * 0x00010001u, zero_high = (0x5400u | (z << 4)) * 0x00010001u;
 #pragma unroll
         for (int i = 0; i < D / 32; ++i) {
           const uint32_t lo = raw[i], hi = raw[i] >> 8;
           *reinterpret_cast<uint4*>(&s_k[buf][t >> 2][(D / 4) * chunk + 8 * i]) =
-              make_uint4(pair_value((lo & hc.mask_low) | hc.bias_low, minus_low, scales),
-                         pair_value((lo & hc.mask_high) | hc.bias_high, minus_high, scales),
-                         pair_value((hi & hc.mask_low) | hc.bias_low, minus_low, scales),
-                         pair_value((hi & hc.mask_high) | hc.bias_high, minus_high, scales));
+              make_uint4(pair_value((lo & hc.mask_low) | hc.bias_low, zero_low, scales),
+                         pair_value((lo & hc.mask_high) | hc.bias_high, zero_high, scales),
+                         pair_value((hi & hc.mask_low) | hc.bias_low, zero_low, scales),
+                         pair_value((hi & hc.mask_high) | hc.bias_high, zero_high, scales));
         }
       }
     };

@@ -424,3 +424,25 @@ def test_decreasing_offsets_name_no_rows(gpu_lib, hint):
         attn.attention_int4(*args, block_size=16, max_query_len=hint, out=mine)
         assert bool((mine == 7.0).all())
     b.check(b.run(max_query_len=hint))
+
+
+@pytest.mark.parametrize("hint", [1, 100])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("q_power,k_power,v_power,jumps", [(40, -40, 0, 0), (-40, 40, 0, 0), (0, 0, 100, 0), (0, 0, -50, 0),
+                                                           (-100, 0, 0, 0), (0, 0, 0, 30)])
+def test_powers_of_two(gpu_lib, hint, dim, q_power, k_power, v_power, jumps):
+    """Queries, keys and values far from 1, and values whose size differs by up to 2^16 between neighbours
+    and up to 2^60 between pages."""
+    b = Batch([90, 70], [200, 70], 8, 2, dim, 16, seed=60 + dim)
+    gen = torch.Generator().manual_seed(61)
+    meta = b.cache.view(torch.int32)[..., 16 * dim // 4:].view(b.cache.shape[0], 2, 2, 16)
+    power = torch.zeros(meta.shape, dtype=torch.int32)
+    power[:, :, 0], power[:, :, 1] = k_power, v_power
+    if jumps:
+        power[:, :, 1] += torch.randint(-8, 9, power[:, :, 1].shape, generator=gen, dtype=torch.int32)
+        power[:, :, 1] += torch.randint(-jumps, jumps + 1, (power.shape[0], 2, 1), generator=gen, dtype=torch.int32)
+    live = (meta >> 23 & 255) != 255
+    meta += torch.where(live, power << 23, 0)
+    b.qkv.mul_(2.0 ** q_power)
+    print("powers", hint, dim, q_power, k_power, v_power, jumps, flush=True)
+    b.check(b.run(max_query_len=hint))
