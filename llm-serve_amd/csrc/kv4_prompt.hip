@@ -43,8 +43,15 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 constexpr int kPromptThreads = 512;
 constexpr int kKeys = 64;      // keys of a tile
 constexpr int kTileCost = 16;  // cost units of a tile of keys
-constexpr int kSetupCost = 16;  // of a row tile besides its keys: 16, 40 and 80 give 2039 rows in 60, 62 and 63 us
-constexpr int kMinShare = 8 * kTileCost;
+constexpr int kSetupCost = 32;  // of a row tile besides its keys
+// Shares.  A part costs some 5 us besides its keys (set-up, its way through memory, its turn in the
+// join), so shares are no smaller than 3 key tiles and a row tile has at most some 12 parts: 40
+// tokens x 5 heads behind 2172 take 32 us (8 key tiles at least: 42), 20 x 4 behind 12000 46 us (as
+// many parts as workgroups: 56).  Where no row tile has more than 8 key tiles and there is a
+// workgroup for each, they are not split: 2 x 34 tokens x 8 heads 16 us (27 split), 400 x 4 23 (29).
+constexpr int kMinShare = 3 * kTileCost;
+constexpr int kMaxParts = 12;
+constexpr int kShortCost = kSetupCost + 8 * kTileCost;
 constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of zeros, of NaN
 
 // Exponents.  fp16 has the codes' products with a scale to 11 bits, but not bf16's range, so a power
@@ -69,18 +76,14 @@ struct KvTileCosts {
   __device__ __forceinline__ int of(int j) const { return first + step * j; }
 };
 
-__device__ __forceinline__ KvTileCosts kv_costs(const KvAttentionArgs& a, const KvRequest& q, int group) {
+__device__ __forceinline__ KvTileCosts kv_costs(const KvAttentionArgs& a, const KvRequest& q, int group, bool whole) {
   KvTileCosts c;
   const int rows = q.n * group;
   c.tiles = rows > a.split_rows ? (rows + kKvPromptRows - 1) / kKvPromptRows : 0;
   c.step = a.tree_mask ? 0 : (kKvPromptRows / 4 + group - 1) / group;
   c.first = min(a.tree_mask ? q.keys : max(q.cached, 0), q.keys) / (kKeys / kTileCost) + c.step + kSetupCost;
+  if (whole) c.first = 1, c.step = 0;
   return c;
-}
-
-__device__ __forceinline__ int kv_request_cost(const KvAttentionArgs& a, const KvRequest& q, int group) {
-  const KvTileCosts c = kv_costs(a, q, group);
-  return c.before(c.tiles) * a.KV;
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -210,27 +213,37 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int group = a.H / a.KV;
-  // Workers of one XCD (workgroups go to the 8 XCDs in turn) take neighbouring shares, mostly of
-  // the same kv heads, whose pages then stay in that XCD's L2.
-  const int per_xcd = gridDim.x / 8;
-  const int me = gridDim.x % 8 == 0 ? static_cast<int>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8 : blockIdx.x;
-
-  int sum = 0;
+  int sum = 0, tiles = 0;
+  int longest = 0;
   bool bad = false;
   for (int r = lane; r < a.R; r += 64) {
     bad |= kv_decreases(a, r);
-    sum += kv_request_cost(a, kv_request(a, r), group);
+    const KvTileCosts c = kv_costs(a, kv_request(a, r), group, false);
+    sum += c.before(c.tiles) * a.KV;
+    tiles += c.tiles * a.KV;
+    if (c.tiles > 0) longest = max(longest, c.of(c.tiles - 1));
   }
   bad = __any(bad);
   if (a.split_rows == 0 && a.zero_tail) kv_zero_tail(a, bad);  // no split kernel in this call
-  const int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
-  const int workers = min(static_cast<int>(gridDim.x), (total + kMinShare - 1) / kMinShare);
-  if (bad | (me >= workers)) return;
+  int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
+  const int all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
+  // Short tiles go to a workgroup each, if there are enough: parts of them would wait for each other.
+  longest = wave_max(longest);
+  const bool whole = (longest <= kShortCost) & (all_tiles <= static_cast<int>(gridDim.x));
+  if (whole) total = all_tiles;
+  const int least = whole ? 1 : max(kMinShare, longest / kMaxParts);
+  const int workers = min(static_cast<int>(gridDim.x), (total + least - 1) / least);
+  // Workers of one XCD (workgroups go to the 8 XCDs in turn) take neighbouring shares, mostly of
+  // the same kv heads, whose pages then stay in that XCD's L2.
+  const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);
+  const int me = static_cast<int>(blockIdx.x & 7) * per_xcd + turn;
+  if (bad | (turn >= per_xcd) | (me >= workers)) return;
   const KvShares shares{uniform(total / workers), uniform(total % workers)};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
   int r = 0, base = 0;
   for (;; r += 64) {
-    const int cost = r + lane < a.R ? kv_request_cost(a, kv_request(a, r + lane), group) : 0;
+    const KvTileCosts c = kv_costs(a, kv_request(a, min(r + lane, a.R - 1)), group, whole);
+    const int cost = r + lane < a.R ? c.before(c.tiles) * a.KV : 0;
     const int upto = wave_scan(cost);
     const uint64_t past = __ballot(base + upto > begin);
     if (past || r + 64 >= a.R) {
@@ -248,13 +261,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const float scale = a.scale_log2e;
 
   for (int u = begin; u < end;) {
-    KvTileCosts costs = kv_costs(a, q, group);
+    KvTileCosts costs = kv_costs(a, q, group, whole);
     int a_head = costs.before(costs.tiles);
     while (u >= base + a_head * a.KV) {
       base += a_head * a.KV;
       ++r;
       q = kv_request(a, r);
-      costs = kv_costs(a, q, group);
+      costs = kv_costs(a, q, group, whole);
       a_head = costs.before(costs.tiles);
     }
     const int head = uniform((u - base) / a_head);
