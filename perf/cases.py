@@ -4,7 +4,7 @@ Every case goes through the layer interface an engine calls.  Four kinds:
 
 * ``step``: two consecutive decoder layers' linear work (norm + QKV, q/k norm, O, norm +
   gate_up + SiLU * up, down) captured in a HIP graph as engines capture their decode and
-  verify steps, one replay per pass.  Attention itself is not part of the framework: its
+  verify steps, one replay per pass.  Attention is left out (operators.py has its cases): its
   output is an input here.  Two layers are 200 MB of weights, so replays over a few states
   stream them from HBM.
 * ``linear``: one projection called eagerly.
