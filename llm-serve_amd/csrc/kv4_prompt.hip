@@ -519,7 +519,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         __builtin_amdgcn_sched_barrier(0);
         const uint64_t held_keys[4] = {s_held[buf][0], s_held[buf][1], s_held[buf][2], s_held[buf][3]};
         const bool all_held = (held_keys[0] & held_keys[1] & held_keys[2] & held_keys[3]) == ~0ull;
-        if (!(key0 + kKeys <= all_see && all_held)) {
+        if (__builtin_expect(!(key0 + kKeys <= all_see && all_held), 0)) {
           if (all_held && !tree) {
             const int lead = sees - key0 - 4 * h;
 #pragma unroll
@@ -544,7 +544,13 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
                 sc[n][i] = visible ? y : -INFINITY;
               }
           }
+#pragma unroll
+          for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(sc[n]));
         }
+        // The scores as whole accumulators on both sides of the branch's end: taken apart, they would be
+        // copied on the path that masks nothing (32 instructions a tile, 4 % of a long chunk's time).
+#pragma unroll
+        for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(sc[n]));
         // A weight is 2^(score + the values' power - reference): the powers of two of keys, values and
         // queries are one multiplier and one addend a group.
         const f32x4_t of_score = *reinterpret_cast<const f32x4_t*>(s_score[buf]), of_value = *reinterpret_cast<const f32x4_t*>(s_log[buf]);
