@@ -135,8 +135,18 @@ __device__ __forceinline__ uint32_t part_offset(int slot, int wave, int f, int l
   return ((static_cast<uint32_t>(slot) * 8 + wave) * (D / 8) + f) * 1024u + lane * 16u;
 }
 
-// The exponent field of a group, from its largest scale.
-__device__ __forceinline__ int group_field(float top) { return min(max(static_cast<int>(__float_as_uint(top) >> 23), 64), 254); }
+// The largest of a wave's values where four neighbouring lanes have the same.
+__device__ __forceinline__ uint32_t group_max(uint32_t v) {
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x124, 0xF, 0xF, true)));
+  v = max(v, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x128, 0xF, 0xF, true)));
+  const u32x2_t a = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(v, v, false, false));
+  v = max(a[0], a[1]);
+  const u32x2_t b = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(v, v, false, false));
+  return max(b[0], b[1]);
+}
+
+// The exponent field of a group, from the bits of its largest scale.
+__device__ __forceinline__ int group_field(uint32_t top) { return min(max(static_cast<int>(top >> 23), 64), 254); }
 
 // Two fragments of a lane -- channels 4 h .. of eights b and b + 1 -- to the output: the halves of
 // the wave exchange theirs, so that a lane writes one eight's 16 bytes.
@@ -305,13 +315,14 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     auto fetch = [&](int key_tile) {
       const int key = key_tile * kKeys + my_key;
       const bool page_ok = static_cast<unsigned>(id) < static_cast<unsigned>(a.num_blocks);
+      const uint32_t index = static_cast<uint32_t>(page_ok ? id : 0) * static_cast<uint32_t>(a.KV) + head;
       const char* page = reinterpret_cast<const char*>(a.cache) +
-                         (static_cast<size_t>(page_ok ? id : 0) * a.KV + head) * kv_page_bytes<D>(a.log2_block);
-      const int token = key & ((1 << a.log2_block) - 1);
+                         static_cast<uint64_t>(index) * static_cast<uint32_t>(kv_page_bytes<D>(a.log2_block));
+      const uint32_t token = key & ((1 << a.log2_block) - 1);
       held = page_ok;
       if (converts_v) {
-        const char* v = page + ((D / 2) << a.log2_block) + token * (D / 2) + word * 16;
-        const char* m = page + ((D + 4) << a.log2_block) + token * 4;
+        const char* v = page + (((D / 2u) << a.log2_block) + token * (D / 2) + word * 16);
+        const char* m = page + (((D + 4u) << a.log2_block) + token * 4);
         const uint4 v0 = *reinterpret_cast<const uint4*>(v), v1 = *reinterpret_cast<const uint4*>(v + 4 * D);
         const uint4 m0 = *reinterpret_cast<const uint4*>(m), m1 = *reinterpret_cast<const uint4*>(m + 32);
         raw[0] = v0.x, raw[1] = v0.y, raw[2] = v0.z, raw[3] = v0.w;
@@ -319,7 +330,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         meta[0] = m0.x, meta[1] = m0.y, meta[2] = m0.z, meta[3] = m0.w;
         meta[4] = m1.x, meta[5] = m1.y, meta[6] = m1.z, meta[7] = m1.w;
       } else {
-        const char* k = page + token * (D / 2) + chunk * (D / 8);
+        const char* k = page + (token * (D / 2) + chunk * (D / 8));
         if constexpr (D == 128) {
           const uint4 w = *reinterpret_cast<const uint4*>(k);
           raw[0] = w.x, raw[1] = w.y, raw[2] = w.z, raw[3] = w.w;
@@ -327,9 +338,9 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
           const uint2 w = *reinterpret_cast<const uint2*>(k);
           raw[0] = w.x, raw[1] = w.y;
         }
-        const char* m = page + (D << a.log2_block) + token * 4;
+        const char* m = page + ((static_cast<uint32_t>(D) << a.log2_block) + token * 4);
         meta[0] = *reinterpret_cast<const uint32_t*>(m);
-        meta[1] = *reinterpret_cast<const uint32_t*>(m + (4 << a.log2_block));
+        meta[1] = *reinterpret_cast<const uint32_t*>(m + (4u << a.log2_block));
       }
     };
     // Fetched codes -> fp16 in LDS.  Keys outside the sequence or on no page become zeros (they hold
@@ -352,7 +363,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
           }
         }
         // the next lane has the other half of the 16 keys
-        const int field = group_field(fmaxf(__uint_as_float(top), dpp_f32<0xB1>(__uint_as_float(top))));
+        const int field = group_field(max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xF, 0xF, true))));
         const float factor = power(kGroupFactor - field);
         if (t < 8 && !(t & 1)) {
           s_log[buf][vgroup >> 1] = static_cast<float>(field - (kGroupFactor - 127));
@@ -385,10 +396,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         m = use ? m : kZeroMeta;
         // a wave has the 16 keys of one group, a key in four lanes
         const uint32_t bits = m & 0x7FFFFFFFu;
-        float top = bits < 0x7F800000u ? __uint_as_float(bits) : 0.0f;
-        top = fmaxf(top, dpp_f32<0x124>(top));
-        top = fmaxf(top, dpp_f32<0x128>(top));
-        const int field = group_field(column_max(top));
+        const int field = group_field(group_max(bits < 0x7F800000u ? bits : 0u));
         if (lane == 0) s_score[buf][wave] = power(field - (kGroupFactor - 254)) * scale;
         const float s = kv_meta_scale(m) * power(kGroupFactor - field);
         const uint32_t scales = pack_f16x2(s, s), z = m & 15u;
