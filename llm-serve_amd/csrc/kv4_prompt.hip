@@ -21,16 +21,17 @@
 // row sits in the two lanes that hold it.
 //
 // What bounds it: a tile of 64 keys costs a SIMD (two waves) some 2000 cycles of matrix
-// instructions, and 2600 of vector instructions: softmax, conversion.  They overlap between the two
-// waves in part only, as every tile ends in a barrier: about 2.2 us a tile, 890 TFLOP/s for 4096
-// rows behind 12288 cached tokens (1.08 ms; a large matrix product of the library reaches 1249).  A
-// row tile costs 4 to 5 us besides its keys (queries, the first keys, writing or joining), which is
-// what short prompts pay: 2039 tokens take 62 us, 550 TFLOP/s.  Workgroups take equal shares of
-// the cost of all row tiles, so a share may end inside a tile's keys; tiles as units would leave a
-// causal prompt's last rows to few workgroups.  Measured and not taken, with bf16 operands: a
-// conversion interleaved with the same wave's first product (4096 rows 3 % faster, 2039 rows 3 %
-// slower: both converters' loops are then apart, twice the code to fetch), and with it waves half a
-// tile apart over three value buffers (registers spill; 5 and 20 % slower).
+// instructions and 3000 of vector instructions (softmax, conversion).  The two waves are in the same
+// phase, every tile ends in a barrier, and little of it overlaps: for 4096 rows behind 12288 cached
+// tokens (1.02 ms, 940 TFLOP/s; a large matrix product of the library reaches 1249) matrix
+// instructions fill 40 % of the cycles and vector instructions 62 %.  A row tile costs 4 to 5 us
+// besides its keys (queries, the first keys, writing or joining), which is what short prompts pay:
+// 2039 tokens take 58 us, 590 TFLOP/s.  Workgroups take equal shares of the cost of all row tiles,
+// so a share may end inside a tile's keys; tiles as units would leave a causal prompt's last rows to
+// few workgroups.  Measured and not taken, with bf16 operands: a conversion interleaved with the same
+// wave's first product (4096 rows 3 % faster, 2039 rows 3 % slower: both converters' loops are then
+// apart, twice the code to fetch), and with it waves half a tile apart over three value buffers
+// (registers spill; 5 and 20 % slower).
 #include "kv4_attention.h"
 
 namespace w4a16 {
