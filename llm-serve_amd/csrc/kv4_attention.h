@@ -15,7 +15,7 @@ namespace w4a16 {
 // split-K exchange (w4a16_common.h).
 struct KvPartials {
   float* out;      // [slots][tile rows][D], unnormalized
-  float* stats;    // [slots][tile rows][2]: reference (a raw score) and sum
+  float* stats;    // [slots][tile rows][2]: reference (a raw score; the prompt kernel: its base-2 exponent) and sum
   int* counters;   // [workers]
   uint32_t out_bytes, stats_bytes;
 };

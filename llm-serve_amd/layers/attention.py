@@ -281,7 +281,7 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     ``tree_mask`` (int64 [rows]) replaces causality among a request's new rows: row t sees the
     cached tokens and those new ones j < 64 whose bit j is set.  A row that sees nothing is zero.
     Without ``out`` (contiguous, of q's shape), rows behind the last request are zero; in ``out``
-    they are left as they were."""
+    they are left as they were.  ``out`` may be q itself, and overlaps no other operand."""
     # One expression accepts what all the checks accept; only what it does not goes through them.
     shape, tshape, index = q.shape, block_tables.shape, cache.get_device()
     head_dim = shape[2] if len(shape) == 3 else 0

@@ -446,3 +446,27 @@ def test_powers_of_two(gpu_lib, hint, dim, q_power, k_power, v_power, jumps):
     b.qkv.mul_(2.0 ** q_power)
     print("powers", hint, dim, q_power, k_power, v_power, jumps, flush=True)
     b.check(b.run(max_query_len=hint))
+
+
+@pytest.mark.parametrize("hint", [1, 300])
+def test_in_place(gpu_lib, hint):
+    """out = q: tiles whose keys several workgroups share read their rows before any is written."""
+    b = Batch([1, 300, 5], [3000, 900, 900], 8, 2, 128, 16, seed=70, pad=2)
+    q, cache, tables, seq, offsets = b.args()
+    want = attn.attention_int4(q, cache, tables, seq, offsets, block_size=16, max_query_len=hint)
+    for _ in range(5):
+        mine = q.clone(memory_format=torch.contiguous_format)
+        got = attn.attention_int4(mine, cache, tables, seq, offsets, block_size=16, max_query_len=hint, out=mine)
+        assert got is mine and torch.equal(mine[:306], want[:306]) and torch.equal(mine[306:], q[306:])
+
+
+def test_largest_and_smallest_batches(gpu_lib):
+    """One row and one key in all; 4096 requests of a row or two."""
+    one = Batch([1], [1], 1, 1, 64, 16, seed=71)
+    one.check(one.run())
+    rng = random.Random(72)
+    new = [rng.choice([0, 1, 1, 2]) for _ in range(4096)]
+    b = Batch(new, [n + rng.choice([0, 1, 14]) for n in new], 1, 1, 64, 16, seed=72)
+    print("4096 requests", flush=True)
+    for hint in (2, 65):
+        b.check(b.run(max_query_len=hint))
