@@ -18,8 +18,10 @@ REGIME_NONE = 0
 REGIME_DECODE = 1
 REGIME_TILE = 2
 
-_current_device = torch._C._cuda_getDevice
-_current_stream = torch._C._cuda_getCurrentRawStream
+# None in a torch built without GPU support, which imports the package all the same; only calls
+# that have a GPU tensor in hand reach them.
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 _c_int = ctypes.c_int
 _c_size = ctypes.c_size_t

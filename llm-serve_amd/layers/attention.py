@@ -34,7 +34,7 @@ from .._lib import _current_device, _current_stream, lib
 
 __all__ = ("Attention", "KVStep", "attention_int4", "kv_step", "load_kv_int4", "new_kv_cache_int4", "store_kv_int4")
 
-_capturing = torch._C._cuda_isCurrentStreamCapturing
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)  # None without GPU support
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
 
 HEAD_DIMS = (64, 128)
