@@ -364,11 +364,11 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * largest among its 16 loses bits.  tree_mask (may be null) [T]: row t then sees its request's
  * cached tokens and, instead of the earlier new ones, those new ones j < 64 whose bit j is set.
  * A row that sees no key gives zeros; keys on a page id outside the cache are not seen; NaN and
- * infinities in keys that a row does not see have no effect on it.  Rows behind cu_query_lens[R]
- * are set to zero if zero_tail, else left as they are; offsets that decrease anywhere name no rows
- * at all.  max_query_len (>= 1) is a hint that chooses kernels and grid: the longest query of the
- * batch; results are right for any.  out may be q where that is contiguous, and overlaps no other
- * operand.  scale > 0 and finite; H % KV == 0.  Replaces
+ * infinities in keys that a row does not see have no effect on it.  Rows of no request (before
+ * cu_query_lens[0], behind cu_query_lens[R]) are set to zero if zero_tail, else left as they are;
+ * offsets that decrease anywhere name no rows at all.  max_query_len (>= 1) is a hint that chooses
+ * kernels and grid: the longest query of the batch; results are right for any.  out may be q where
+ * that is contiguous, and overlaps no other operand.  scale > 0 and finite; H % KV == 0.  Replaces
  * flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:118-132). */
 int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
                        const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,

@@ -103,13 +103,17 @@ __device__ __forceinline__ bool kv_decreases(const KvAttentionArgs& a, int r) {
   return const_ints(a.cu_query_lens)[r + 1] < const_ints(a.cu_query_lens)[r];
 }
 
-// Zeros for the output rows behind the last request (all rows if there is no work).
-__device__ __forceinline__ void kv_zero_tail(const KvAttentionArgs& a, bool all) {
+// Zeros for the output rows of no request: those before the first one's and behind the last one's
+// (all rows if there is no work).
+__device__ __forceinline__ void kv_zero_unowned(const KvAttentionArgs& a, bool all) {
+  const int first = all ? 0 : min(max(const_ints(a.cu_query_lens)[0], 0), a.T);
   const int end = all ? 0 : min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
-  const int chunks = a.H * a.D / 8;
-  for (int row = end + blockIdx.x; row < a.T; row += gridDim.x)
+  const int unowned = first + a.T - end, chunks = a.H * a.D / 8;
+  for (int i = blockIdx.x; i < unowned; i += gridDim.x) {
+    const int row = i < first ? i : end + i - first;
     for (int c = threadIdx.x; c < chunks; c += blockDim.x)
       reinterpret_cast<uint4*>(a.out)[static_cast<size_t>(row) * chunks + c] = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // One part of a tile row's result: eight channels, or the row's statistics.

@@ -147,7 +147,7 @@ __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionAr
   const int me = blockIdx.x;
 
   bad = __any(bad);
-  if (a.zero_tail) kv_zero_tail(a, bad);
+  if (a.zero_tail) kv_zero_unowned(a, bad);
   if (bad | (me >= workers)) return;
   const KvShares shares{total / workers, total % workers};
   const int begin = shares.begin(me), end = shares.begin(me + 1);

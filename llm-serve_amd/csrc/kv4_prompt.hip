@@ -235,7 +235,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
     if (c.tiles > 0) longest = max(longest, c.of(c.tiles - 1));
   }
   bad = __any(bad);
-  if (a.split_rows == 0 && a.zero_tail) kv_zero_tail(a, bad);  // no split kernel in this call
+  if (a.split_rows == 0 && a.zero_tail) kv_zero_unowned(a, bad);  // no split kernel in this call
   int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   // Short tiles go to a workgroup each, if there are enough: parts of them would wait for each other.

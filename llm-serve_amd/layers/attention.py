@@ -276,12 +276,13 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     request r's rows ``cu_query_lens[r]`` .. ``cu_query_lens[r + 1]`` are the last tokens of its
     ``seq_lens[r]``, on the pages ``block_tables[r]`` names.  Returns bf16 [rows, heads, head_dim].
 
-    Offsets that decrease name no rows at all.  ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest query of the batch if
-    the caller knows it (1 for a decode step), picks kernels; results are right whatever it is.
+    Offsets that decrease name no rows at all.  ``scale`` defaults to 1 / sqrt(head_dim).
+    ``max_query_len``, the longest query of the batch if the caller knows it (1 for a decode step),
+    picks kernels; results are right whatever it is.
     ``tree_mask`` (int64 [rows]) replaces causality among a request's new rows: row t sees the
     cached tokens and those new ones j < 64 whose bit j is set.  A row that sees nothing is zero.
-    Without ``out`` (contiguous, of q's shape), rows behind the last request are zero; in ``out``
-    they are left as they were.  ``out`` may be q itself, and overlaps no other operand."""
+    Without ``out`` (contiguous, of q's shape), rows of no request (before the first one's, behind the
+    last one's) are zero; in ``out`` they are left as they were.  ``out`` may be q itself, and overlaps no other operand."""
     # One expression accepts what all the checks accept; only what it does not goes through them.
     shape, tshape, index = q.shape, block_tables.shape, cache.get_device()
     head_dim = shape[2] if len(shape) == 3 else 0
