@@ -321,9 +321,10 @@ size_t w4a16_workspace_bytes_config(int M, int N, int regime, int p0, int split)
  * [num_free], in order of request and position, and entered in tables (row stride table_stride
  * elements); blocks_used [1] receives how many are needed.  A token whose block the free list or
  * the table's width lacks gets slot -1 (and -1 in the table).  The lists are not consumed: the
- * same call again gives the same result.  R <= 4096, T <= 2^18; T < sum(query_lens) drops the
- * last rows.  Replaces the host loops of prepare_prefill / prepare_decode (model_runner.py:
- * 279-333). */
+ * same call again gives the same result.  R <= 4096, T <= 2^18, and a query counts as at most 2^18
+ * rows.  T < sum(query_lens) drops the last rows: they have no position and no slot, but offsets,
+ * lengths, blocks_used and tables count them.  Replaces the host loops of prepare_prefill /
+ * prepare_decode (model_runner.py:279-333). */
 int w4a16_kv_step(const int32_t* query_lens, const int32_t* context_lens, int32_t* tables,
                   int64_t table_stride, const int32_t* free_blocks, int32_t* cu_query_lens,
                   int32_t* seq_lens, int32_t* positions, int32_t* slots, int32_t* blocks_used, int R,

@@ -33,7 +33,9 @@ __device__ __forceinline__ int block_scan(int v, int* part, int* total) {
 // of the row offsets.  The block of a row's position is the table's where the request had it
 // before this step, and else the free list's at the request's offset -- so nothing that another
 // workgroup writes is read.  A row that opens a block enters it in the table; rows cover all
-// positions of a request, so each new block is entered exactly once.  Latency bounds it: two
+// positions of a request, so each new block is entered exactly once.  Where the lengths count more
+// rows than there are, the blocks that rows behind the last one would open are entered by request,
+// so that every block counted in blocks_used is in its table.  Latency bounds it: two
 // dependent loads, a scan, and the search.  2.5 us for 8 decode requests, 4.3 us for 512 rows of
 // requests with chunks among them.
 __global__ __launch_bounds__(kStepThreads) void kv_step_kernel(KvStepArgs a) {
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(kStepThreads) void kv_step_kernel(KvStepArgs a) {
   const int max_context = static_cast<int>(room < (1 << 30) ? room : (1 << 30));
   int rows = 0, blocks = 0;
   for (int r = r0; r < r1; ++r) {
-    const int n = min(max(a.query_lens[r], 0), a.T + 1);
+    const int n = min(max(a.query_lens[r], 0), kKvStepMaxTokens);
     const int c = min(max(a.context_lens[r], 0), max_context);
     s_context[r] = c;
     s_first_row[r] = n;
@@ -81,6 +83,17 @@ __global__ __launch_bounds__(kStepThreads) void kv_step_kernel(KvStepArgs a) {
   }
   __syncthreads();
   const int t = blockIdx.x * kStepThreads + tid;
+  if (total_rows > a.T) {
+    for (int r = t; r < a.R; r += gridDim.x * kStepThreads) {
+      const int c = s_context[r], n = s_first_row[r + 1] - s_first_row[r];
+      const int have = (c + block - 1) >> a.log2_block, need = min((c + n + block - 1) >> a.log2_block, a.width);
+      const int there = min(max(a.T - s_first_row[r], 0), n);  // the request's rows that exist
+      for (int i = max((c + there + block - 1) >> a.log2_block, have); i < need; ++i) {
+        const int f = s_first_block[r] + i - have;
+        a.tables[static_cast<int64_t>(r) * a.table_stride + i] = f < a.num_free ? a.free_blocks[f] : -1;
+      }
+    }
+  }
   if (t >= a.T) return;
   int position = 0, slot = -1;
   if (t < total_rows) {

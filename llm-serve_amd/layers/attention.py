@@ -121,7 +121,8 @@ def kv_step(query_lens: torch.Tensor, context_lens: torch.Tensor, block_tables: 
     and gets, in place, the blocks that the new tokens open: those of ``free_blocks``, in order of
     request and position.  ``num_tokens`` is the number of packed rows, at least the sum of
     ``query_lens``; rows behind the last request get position 0 and slot -1, which
-    ``store_kv_int4`` skips.
+    ``store_kv_int4`` skips.  (With fewer, the last tokens have no row to be stored from; offsets,
+    lengths and block tables count them all the same.)
 
     The host takes the first ``blocks_used`` entries off its free list (it can count them from the
     lengths without reading the tensor).  A token for which the list or the table's width is too

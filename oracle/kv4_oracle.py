@@ -117,18 +117,16 @@ def step(query_lens, context_lens, tables, free, block, tokens):
     for r, (n, c) in enumerate(zip(query_lens, context_lens)):
         n, c = max(n, 0), max(c, 0)
         have, need = -(-c // block), -(-(c + n) // block)
+        for index in range(have, min(need, width)):
+            at = used + index - have
+            tables[r][index] = free[at] if at < len(free) else -1
         for t in range(n):
             row, position = offsets[-1] + t, c + t
             if row >= tokens:
                 break
             positions[row] = position
             index = position // block
-            if index >= width:
-                continue
-            if index >= have and position % block == 0:
-                at = used + index - have
-                tables[r][index] = free[at] if at < len(free) else -1
-            if tables[r][index] >= 0:
+            if index < width and tables[r][index] >= 0:
                 slots[row] = tables[r][index] * block + position % block
         used += need - have
         offsets.append(offsets[-1] + n)
