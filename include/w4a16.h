@@ -309,7 +309,8 @@ size_t w4a16_workspace_bytes_config(int M, int N, int regime, int p0, int split)
  * token for the keys and one for the values: bf16(s) in the high half, bf16(128 + z) in the low.
  * A slot is block * block_size + token; slots outside the cache name no row.  Tables, slots and
  * lengths are int32 on the device and are never trusted: an id or length that points outside
- * the cache, the tables or the packed rows reads and writes nothing there.
+ * the cache, the tables or the packed rows reads and writes nothing there.  A table's row reaches at
+ * most 2^31 - 2^19 - 1 tokens (width * block_size).
  * ------------------------------------------------------------------------- */
 
 /* One step's bookkeeping from the request lengths.  Request r has context_lens[r] tokens in the

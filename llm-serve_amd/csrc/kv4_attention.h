@@ -50,8 +50,7 @@ __device__ __forceinline__ KvRequest kv_request(const KvAttentionArgs& a, int r)
   q.row = min(max(lo, 0), a.T);
   q.n = max(min(hi, a.T) - q.row, 0);
   q.cached = seq - (hi - lo);
-  const int64_t room = static_cast<int64_t>(a.width) << a.log2_block;
-  q.keys = seq < room ? seq : static_cast<int>(room);
+  q.keys = min(seq, a.width << a.log2_block);
   return q;
 }
 

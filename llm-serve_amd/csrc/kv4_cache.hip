@@ -47,9 +47,7 @@ __global__ __launch_bounds__(kStepThreads) void kv_step_kernel(KvStepArgs a) {
   const int per = (a.R + kStepThreads - 1) / kStepThreads;
   const int r0 = tid * per, r1 = min(a.R, r0 + per);
   const int block = 1 << a.log2_block;
-  // no position lies behind the table; sums stay in range
-  const int64_t room = static_cast<int64_t>(a.width) << a.log2_block;
-  const int max_context = static_cast<int>(room < (1 << 30) ? room : (1 << 30));
+  const int max_context = a.width << a.log2_block;  // no cached token lies behind the table; sums stay in range
   int rows = 0, blocks = 0;
   for (int r = r0; r < r1; ++r) {
     const int n = min(max(a.query_lens[r], 0), kKvStepMaxTokens);

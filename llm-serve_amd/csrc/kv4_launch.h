@@ -13,6 +13,10 @@ constexpr int kKvStepMaxRequests = 4096;
 // Packed rows of one step; with kKvStepMaxRequests lengths clamped to it, sums stay below 2^31.
 constexpr int kKvStepMaxTokens = 1 << 18;
 
+// Tokens that a block table's row may reach.  A sequence's keys rounded up to the kernels' tiles, and
+// a step's tokens behind it, then stay below 2^31.
+constexpr int64_t kKvMaxReach = 0x7FFFFFFF - (1 << 19);
+
 struct KvStepArgs {
   const int32_t* query_lens;    // [R]
   const int32_t* context_lens;  // [R]

@@ -243,7 +243,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const bool whole = (longest <= kShortCost) & (all_tiles <= static_cast<int>(gridDim.x));
   if (whole) total = all_tiles;
   const int least = whole ? 1 : max(kMinShare, longest / kMaxParts);
-  const int workers = min(static_cast<int>(gridDim.x), (total + least - 1) / least);
+  const int workers = total > 0 ? min(static_cast<int>(gridDim.x), (total - 1) / least + 1) : 0;
   // Workers of one XCD (workgroups go to the 8 XCDs in turn) take neighbouring shares, mostly of
   // the same kv heads, whose pages then stay in that XCD's L2.
   const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);

@@ -1229,6 +1229,13 @@ int kv_log2_block(int block_size) {
   return -1;
 }
 
+int validate_kv_reach(int width, int log2_block) {
+  if (static_cast<int64_t>(width) << log2_block > w4a16::kKvMaxReach)
+    return fail(W4A16_ERR_SHAPE, "block tables of %d blocks of %d reach more than %lld tokens", width, 1 << log2_block,
+                static_cast<long long>(w4a16::kKvMaxReach));
+  return W4A16_OK;
+}
+
 int validate_kv_cache(const void* cache, int KV, int D, int num_blocks, int block_size, int* log2_block) {
   if (!cache) return fail(W4A16_ERR_ARG, "the KV cache pointer is null");
   if (KV <= 0 || num_blocks <= 0) return fail(W4A16_ERR_ARG, "kv heads (%d) and num_blocks (%d) must be positive", KV, num_blocks);
@@ -1262,6 +1269,8 @@ int validate_kv_heads(int T, int R, int H, int KV, int D, int log2_block, int wi
   if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
   if (width <= 0) return fail(W4A16_ERR_ARG, "the block tables' width must be positive (got %d)", width);
   if (max_query_len < 1) return fail(W4A16_ERR_ARG, "max_query_len must be at least 1 (got %d)", max_query_len);
+  const int e = validate_kv_reach(width, log2_block);
+  if (e != W4A16_OK) return e;
   if (T == 0 || R == 0) return W4A16_OK;
   if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
@@ -1295,6 +1304,10 @@ int w4a16_kv_step(const int32_t* query_lens, const int32_t* context_lens, int32_
   const int log2_block = kv_log2_block(block_size);
   if (log2_block < 0)
     return fail(W4A16_ERR_SHAPE, "block_size must be a power of two in 16 .. 256 (got %d)", block_size);
+  if (R) {
+    const int e = validate_kv_reach(width, log2_block);
+    if (e != W4A16_OK) return e;
+  }
   const w4a16::KvStepArgs a{query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions, slots,
                             blocks_used, table_stride, R, width, num_free, log2_block, T};
   return check_launch(w4a16::launch_kv_step(a, static_cast<hipStream_t>(stream)), "kv step");
