@@ -314,10 +314,12 @@ class W4A16Library:
             with torch.cuda.device(index):
                 return self.kv_step(query_lens, context_lens, tables, free_blocks, cu_query_lens, seq_lens, positions,
                                     slots, blocks_used, block_size)
+        requests, width = tables.shape
         status = self.dll.w4a16_kv_step(
-            query_lens.data_ptr(), context_lens.data_ptr(), tables.data_ptr(), tables.stride(0), free_blocks.data_ptr(),
-            cu_query_lens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(), slots.data_ptr(), blocks_used.data_ptr(),
-            query_lens.shape[0], tables.shape[1], free_blocks.shape[0], block_size, positions.shape[0],
+            query_lens.data_ptr(), context_lens.data_ptr(), tables.data_ptr(),
+            tables.stride(0) if requests > 1 else width,  # a single row's stride may be anything
+            free_blocks.data_ptr(), cu_query_lens.data_ptr(), seq_lens.data_ptr(), positions.data_ptr(),
+            slots.data_ptr(), blocks_used.data_ptr(), requests, width, free_blocks.shape[0], block_size, positions.shape[0],
             _current_stream(index))
         if status != 0:
             self.check(status, "w4a16_kv_step")
@@ -366,7 +368,8 @@ class W4A16Library:
         blocks, kv_heads, _ = cache.shape
         requests, width = tables.shape
         status = self.dll.w4a16_kv_attention(
-            q.data_ptr(), q0, q1, cache.data_ptr(), tables.data_ptr(), tables.stride(0), seq_lens.data_ptr(),
+            q.data_ptr(), q0, q1, cache.data_ptr(), tables.data_ptr(),
+            tables.stride(0) if requests > 1 else width, seq_lens.data_ptr(),
             cu_query_lens.data_ptr(), tree_mask.data_ptr() if tree_mask is not None else None, out.data_ptr(), scale, t,
             requests, h, kv_heads, d, blocks, block_size, width, max_query_len, zero_tail, workspace.data_ptr(),
             workspace.numel(), counters.data_ptr(), _current_stream(index))

@@ -165,10 +165,9 @@ def _check_step(query_lens, context_lens, block_tables, free_blocks, block_size,
         raise ValueError(f"a KV step takes 1 to {MAX_STEP_REQUESTS} requests (got {requests})")
     if num_tokens < 0 or num_tokens > MAX_STEP_TOKENS:
         raise ValueError(f"a KV step takes 0 to {MAX_STEP_TOKENS} rows (got {num_tokens})")
-    if block_tables.stride(1) != 1 or (requests > 1 and block_tables.stride(0) < block_tables.shape[1]):
+    width = block_tables.shape[1]  # a dimension of one entry may have any stride
+    if (width > 1 and block_tables.stride(1) != 1) or (requests > 1 and block_tables.stride(0) < width):
         raise ValueError("KV block_tables rows must be contiguous and must not overlap")
-    if requests == 1 and block_tables.stride(0) < block_tables.shape[1]:
-        block_tables = block_tables.as_strided(block_tables.shape, (block_tables.shape[1], 1))
     return query_lens.contiguous(), context_lens.contiguous(), block_tables, free_blocks.contiguous()
 
 
@@ -345,7 +344,7 @@ def _check_attention(q, cache, block_tables, seq_lens, cu_query_lens, block_size
     width = block_tables.shape[1] if block_tables.ndim == 2 else 0
     if width < 1 or block_tables.shape[0] != requests:
         raise ValueError("KV block_tables must be [requests, width]")
-    if block_tables.stride(1) != 1 or block_tables.stride(0) < width:
+    if (width > 1 and block_tables.stride(1) != 1) or (requests > 1 and block_tables.stride(0) < width):
         block_tables = block_tables.contiguous()
     return q, block_tables, seq_lens.contiguous(), cu_query_lens.contiguous()
 
