@@ -370,8 +370,8 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * cu_query_lens[0], behind cu_query_lens[R]) are set to zero if zero_tail, else left as they are;
  * offsets that decrease anywhere name no rows at all.  max_query_len (>= 1) is a hint that chooses
  * kernels and grid: the longest query of the batch; results are right for any.  out may be q where
- * that is contiguous, and overlaps no other operand.  scale > 0 and finite; H % KV == 0.  Replaces
- * flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:118-132). */
+ * that is contiguous, and overlaps no other operand.  scale > 0 and scale * log2(e) finite; H % KV ==
+ * 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:118-132). */
 int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
                        const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
                        const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale,

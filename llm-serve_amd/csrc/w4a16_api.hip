@@ -1371,7 +1371,9 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
   int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &log2_block);
   if (e != W4A16_OK) return e;
   if ((e = validate_kv_heads(T, R, H, KV, D, log2_block, width, max_query_len)) != W4A16_OK) return e;
-  if (!(scale > 0.0f) || scale > 3.0e38f) return fail(W4A16_ERR_ARG, "scale must be positive and finite (got %g)", static_cast<double>(scale));
+  const float scale_log2e = scale * 1.44269504088896341f;
+  if (!(scale > 0.0f) || !(scale_log2e <= 3.402823466e38f))
+    return fail(W4A16_ERR_ARG, "scale must be positive and finite, times log2(e) too (got %g)", static_cast<double>(scale));
   if (T == 0) return ok();
   if (R == 0) return fail(W4A16_ERR_ARG, "%d rows of no request", T);
   if (!tables || !seq_lens || !cu_query_lens || !out) return fail(W4A16_ERR_ARG, "an attention pointer is null");
@@ -1382,7 +1384,7 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
   a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
   a.cache = cache, a.tables = tables, a.table_stride = table_stride;
   a.seq_lens = seq_lens, a.cu_query_lens = cu_query_lens, a.tree_mask = tree_mask, a.out = out;
-  a.scale_log2e = scale * 1.44269504088896341f;
+  a.scale_log2e = scale_log2e;
   a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.num_blocks = num_blocks, a.log2_block = log2_block, a.width = width;
   a.max_query_len = max_query_len < T ? max_query_len : T;
   a.zero_tail = zero_tail != 0;

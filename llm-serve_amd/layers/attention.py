@@ -41,6 +41,7 @@ HEAD_DIMS = (64, 128)
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 MAX_STEP_REQUESTS = 4096
 MAX_STEP_TOKENS = 1 << 18
+MAX_SCALE = 2.3e38  # times log2(e), the kernels' multiplier, it is finite in 32 bits
 
 
 def _require_int32(device: torch.device, **tensors: torch.Tensor) -> None:
@@ -306,8 +307,8 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     rows, heads = shape[0], shape[1]
     if scale is None:
         scale = head_dim ** -0.5
-    elif not 0.0 < scale < 3e38:
-        raise ValueError(f"attention scale must be positive and finite (got {scale})")
+    elif not 0.0 < scale < MAX_SCALE:
+        raise ValueError(f"attention scale must be positive and below {MAX_SCALE} (got {scale})")
     if max_query_len is None:
         max_query_len = max(rows, 1)
     elif max_query_len < 1:
