@@ -16,8 +16,8 @@ one zero point z, as a group of an AWQ weight is; a channel stands for s * (c - 
 channels that is 68 bytes for a row of 256.
 
 Everything runs in the HIP library and raises without it or without a GPU; nothing synchronises
-the host (but for the first ``attention_int4`` on a device, which sets up its counters), and every
-call may be captured in a HIP graph.  ``attention_int4`` takes its workspace and counters from
+the host (but for the first ``attention_int4`` on a device, which sets up its counters, and one in
+4096 captured calls), and every call may be captured in a HIP graph.  ``attention_int4`` takes its workspace and counters from
 ``SCRATCH``, one pair a stream and one a captured call, so calls on several streams, and several
 graphs, share neither.
 """
@@ -218,12 +218,14 @@ class _ScratchPool:
     """Workspaces and arrival counters of ``attention_int4``; a call's counters (1024 int32) are zero
     before and after it.
 
-    Eager calls of one stream run in order and share one pair.  A captured call takes its workspace
-    from the graph's pool and a set of counters of its own, for good: its graph may be replayed
-    beside anything else.  Counters come from one zeroed array a device (16 MiB: 4096 sets), made by
-    the device's first eager call, which waits for the zeros.  A call without a set left, or
-    captured before that array exists, takes a new zeroed tensor (inside a capture its graph clears
-    it on every replay)."""
+    Eager calls of one stream run in order and share one pair, whose workspace is as large as their
+    largest (up to some 80 MB where prompts are among them) and stays with the stream.  A captured
+    call takes its workspace from the graph's pool and a set of counters (4 KiB) of its own, for
+    good: its graph may be replayed beside anything else, and nothing tells when it is destroyed.
+    Counters come from a zeroed array a device (16 MiB: 4096 sets), made by the device's first eager
+    call, which waits for the zeros, and again by the next eager call once captured ones have used
+    it up.  A call captured while there is none takes a new zeroed tensor, which its graph clears on
+    every replay."""
 
     SETS = 4096
     SIZE = 1024
@@ -249,19 +251,17 @@ class _ScratchPool:
             return workspace, torch.zeros(self.SIZE, dtype=_I32, device=index)
         key = (index, _current_stream(index))
         pair = self._streams.get(key)
-        if pair is not None and pair[0].numel() >= nbytes:
+        if pair is not None and pair[0].numel() >= nbytes and self._free.get(index):
             return pair
         with self._lock:
-            if index not in self._free:
+            if not self._free.get(index):
                 array = torch.zeros(self.SETS, self.SIZE, dtype=_I32, device=index)
                 torch.cuda.current_stream(index).synchronize()
                 self._free[index] = list(array.unbind())
-            free = self._free[index]
-            if pair is None and not free:
-                return (torch.empty(nbytes, dtype=torch.uint8, device=index),
-                        torch.zeros(self.SIZE, dtype=_I32, device=index))
-            counters = free.pop() if pair is None else pair[1]
-            pair = self._streams[key] = (torch.empty(nbytes, dtype=torch.uint8, device=index), counters)
+            pair = self._streams.get(key)  # another thread may have made or grown it since
+            if pair is None or pair[0].numel() < nbytes:
+                counters = self._free[index].pop() if pair is None else pair[1]
+                pair = self._streams[key] = (torch.empty(nbytes, dtype=torch.uint8, device=index), counters)
             return pair
 
 
