@@ -135,8 +135,9 @@ def step(query_lens, context_lens, tables, free, block, tokens):
 
 
 def attention(q, cache, tables, seq_lens, offsets, block, scale=None, tree_mask=None):
-    """(out, spread) float64 [rows, heads, dim] and a bound [rows, heads, dim] on how far a kernel
-    with bf16 weights may be off before its output is rounded (see ``tolerance``)."""
+    """(out, spread) float64 [rows, heads, dim] and a bound [rows, heads, dim] on how far any kernel
+    with bf16 operands may be off before its output is rounded (see ``tolerance``).  What the present
+    kernels round is less: ``attention_errors`` has a bound for each."""
     rows, heads, dim = q.shape
     kv_heads = cache.shape[1]
     group = heads // kv_heads
@@ -179,7 +180,7 @@ def attention(q, cache, tables, seq_lens, offsets, block, scale=None, tree_mask=
 def _spread(p, s, values, k, k_scale, v_scale, q, scale):
     """Error bound of one row before the output's rounding, u = 2^-8 being bf16's half step:
     * each weight p s_v rounded to bf16: u sum p |v|;
-    * keys and values as bf16(s (c - z)), as a kernel for long queries takes them: another
+    * keys and values as bf16(s (c - z)), as a kernel might take them (none does now): another
       u sum p |v|, and scores off by u scale sum_x |q_x k_x|, which changes p by that much
       relatively, on both sides of the quotient -- as independent roundings, 4 standard deviations
       of a uniform error in [-u, u]: 4 u / sqrt(3) scale sqrt(sum_x (q_x k_x)^2);
@@ -198,3 +199,104 @@ def _spread(p, s, values, k, k_scale, v_scale, q, scale):
 def tolerance(out, spread):
     """How far a bf16 output may be from `out`: the bound above, and its own rounding."""
     return spread + 2.0 ** -8 * (out.abs() + spread) + 1e-30
+
+
+def attention_errors(q, cache, tables, seq_lens, offsets, block, kernel, scale=None, values=None):
+    """(out, sigma, worst) float64 [rows, heads, dim] of causal attention: the output, and the error
+    of one of the two kernels before its output is rounded, as a standard deviation of independent
+    roundings and as what all of them together cannot pass.  ``values`` (a function of a request, its
+    keys' values and its slots) may replace values, for errors planted by a test.
+
+    With P = p / sum p, u the half step of a rounding and r = u / sqrt(3) the standard deviation of one
+    that is uniform in [-u, u]:
+
+    * "split" (requests of up to 64 rows a kv head, all where the caller's longest query is that
+      short): codes and zero points are exact and a weight times its value's scale becomes bf16
+      (u = 2^-8): sigma^2 = r^2 sum P^2 v^2, worst u sum P |v|.  A score's sum has products of up
+      to (128 + 15) |q|, rounded at most D / 16 + 2 times by 2^-23; sums of weights times
+      (128 + 15) s_v are rounded once for each 32 keys of a wave and a few times in joining.
+    * "prompt" (longer requests): keys, values and weights are fp16 (u = 2^-11; queries fit it).  Values
+      and weights: sigma^2 = 2 r^2 sum P^2 v^2, worst 2 u sum P |v|.  A score is off by
+      r scale sqrt(sum_x (q_x k_x)^2), at worst u scale sum_x |q_x k_x|, which changes P by as much
+      relatively, on both sides of the quotient: sigma^2 += sum P^2 (score's)^2 (v - out)^2.  A score is rounded
+      once for each 16 channels, sums of weights once for each 16 keys, by 2^-23 of their absolute sums;
+      weights 2^-21 below the row's largest lose bits, 2^-32 of it each.
+    * Both: the exponent's argument and the exponential, 2^-20 of a weight."""
+    rows, heads, dim = q.shape
+    kv_heads = cache.shape[1]
+    group = heads // kv_heads
+    scale = dim ** -0.5 if scale is None else scale
+    u = 2.0 ** -8 if kernel == "split" else 2.0 ** -11
+    r2 = u * u / 3
+    out, sigma, worst = (torch.zeros(rows, heads, dim, dtype=torch.float64) for _ in range(3))
+    q, cache = q.cpu().double(), cache.cpu()
+    for r, seq in enumerate(seq_lens):
+        first, n = offsets[r], offsets[r + 1] - offsets[r]
+        slots = [tables[r][p // block] * block + p % block for p in range(seq)]
+        k, v, ks, vs = load(cache, slots, block)
+        if values is not None:
+            v = values(r, v, slots)
+        sees = torch.arange(seq)[None] < (seq - n + torch.arange(n) + 1)[:, None]
+        sees = sees.repeat_interleave(group, 0)
+        for g in range(kv_heads):
+            own = q[first:first + n, g * group:(g + 1) * group].reshape(n * group, dim)
+            s = (scale * own @ k[:, g].t()).masked_fill(~sees, -torch.inf)
+            p = torch.softmax(s, 1)
+            x, magnitude = v[:, g], p @ v[:, g].abs()
+            o = p @ x
+            if kernel == "split":
+                variance, most = r2 * (p * p) @ (x * x), u * magnitude
+                score = scale * ks[:, g].abs() * 143 * own.abs().sum(1, True) * (dim / 16 + 2) * 2.0 ** -23
+                sums = (seq / 128 + 24) * 2.0 ** -23 * 143 * (p @ vs[:, g].abs())[:, None]
+            else:
+                of_score = r2 * scale * scale * (own * own) @ (k[:, g] * k[:, g]).t()
+                w = p * p * of_score
+                variance = 2 * r2 * (p * p) @ (x * x)
+                variance = variance + w @ (x * x) - 2 * o * (w @ x) + o * o * w.sum(1, True)
+                score = scale * own.abs() @ k[:, g].abs().t()
+                most = 2 * u * magnitude + 2 * u * torch.where(sees, score, 0).amax(1, True) * magnitude
+                score = score * (dim / 16 + 4) * 2.0 ** -23
+                sums = (seq / 16 + 24) * 2.0 ** -23 * magnitude
+                sums = sums + seq * 2.0 ** -32 * 15 * (p.amax(1) * vs[:, g].abs().max())[:, None]
+            exact = 2 * (torch.where(sees, score, 0).amax(1, True) + 2.0 ** -20) * magnitude + sums
+
+            def put(to, what):
+                to[first:first + n, g * group:(g + 1) * group] = what.reshape(n, group, dim)
+
+            put(out, o)
+            put(sigma, variance.clamp(min=0).sqrt())
+            put(worst, exact)
+            worst[first:first + n, g * group:(g + 1) * group] += torch.minimum(
+                most, 7 * variance.clamp(min=0).sqrt()).reshape(n, group, dim)
+    return out, sigma, worst
+
+
+def check_errors(got, out, sigma, worst):
+    """What is wrong with a bf16 output, as a text, or None.
+
+    * Every element lies within its bound: ``worst`` (of which roundings count 7 standard deviations, or
+      all of them at once where that is less) and its own rounding, 2^-8.
+    * The squared error of all elements together is what a kernel's must be.  Rounding the exact output
+      once gives E0 = sum (bf16(out) - out)^2, and a kernel's own error moves values across rounding
+      borders without changing that sum but by chance: N elements' squares, each in [0, 1] of a
+      half step's with a variance of 4/45 around 1/3, vary by sqrt(4/45) / (1/3) = 0.9 of 1 / sqrt(N), and unequal
+      elements by some more; 8 / sqrt(N) is allowed.  The kernel's own error adds sum sigma^2, of
+      which one (row, head) pair's part may be a single rounding's, so that M pairs' sum of squares varies by
+      sqrt(2 / M): 1 + 8 / sqrt(M) times it is allowed."""
+    got = got.cpu().double()
+    off = (got - out).abs()
+    limit = worst + 2.0 ** -8 * (out.abs() + worst) + 1e-30
+    bad = ~(off <= limit)
+    if bool(bad.any()):
+        return f"{int(bad.sum())} elements, up to {float((off / limit).nan_to_num(9e9).max()):.2f} of their bound"
+    live = out.abs().amax((1, 2)) > 0
+    n, m = int(live.sum()) * out.shape[1] * out.shape[2], int(live.sum()) * out.shape[1]
+    if n == 0:
+        return None
+    # heads of one size: an error in a row of small values counts as much as in one of large ones
+    size = out[live].square().mean((2,), True).sqrt()
+    whole = float((off[live] / size).square().sum())
+    once = float(((bf16_rne(out[live]) - out[live]) / size).square().sum())
+    own = float((sigma[live] / size).square().sum())
+    allowed = once * (1 + 8 / n ** 0.5) + own * (1 + 8 / m ** 0.5) + n * 2.0 ** -40
+    return None if whole <= allowed else f"squared error {whole:.4g}, allowed {allowed:.4g} (rounding once: {once:.4g})"
