@@ -363,7 +363,8 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * fp32 scores, statistics and sums.  The second product's operands are bf16(p * s_v) and exact
  * codes; for requests of more than 64 rows a kv head, all operands are fp16 with a power of two
  * taken out of each query row and of every 16 keys: a key or value whose scale is 2^-24 of the
- * largest among its 16 loses bits.  tree_mask (may be null) [T]: row t then sees its request's
+ * largest among its 16 loses bits.  Sums of weights times values, up to 143 scales each, are fp32: a
+ * row with values of 2^120 and more may be infinite or NaN.  tree_mask (may be null) [T]: row t then sees its request's
  * cached tokens and, instead of the earlier new ones, those new ones j < 64 whose bit j is set.
  * A row that sees no key gives zeros; keys on a page id outside the cache are not seen; NaN and
  * infinities in keys that a row does not see have no effect on it.  Rows of no request (before

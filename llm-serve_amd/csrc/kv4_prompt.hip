@@ -62,6 +62,14 @@ constexpr uint32_t kZeroMeta = 0x00004300u, kNanMeta = 0x7FC04300u;  // rows of 
 // scales are all below 2^-63 keep that exponent and lose bits below 2^-87.
 constexpr int kGroupFactor = 264, kRowFactor = 268;
 
+// A weight carries its values' power of two, 2^(field - 137), and the sum of weights takes it out
+// again.  Beside values of a very large power, the weights of keys with small ones, or with zeros, would
+// leave fp32's range below although they are large by themselves.  So once a workgroup has met a field
+// above this border (scales of 2^15 and more, which are rare), it forms sums of weights without that
+// power, an exponential more a score.  Below the border fields lie between 64 and 142, and a weight that
+// is lost, 133 powers under the reference's maximum, is 2^-55 of the row's largest at most.
+constexpr int kLargeField = 142;
+
 __device__ __forceinline__ f32x16_t mfma32(f16x8_t a, f16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
@@ -104,6 +112,12 @@ __device__ __forceinline__ float halves_max(float v) {
 
 __device__ __forceinline__ uint32_t pack_f16x2(float x, float y) {
   return __builtin_bit_cast(uint32_t, f16x2_t{static_cast<_Float16>(x), static_cast<_Float16>(y)});
+}
+
+// l 2^d, also where 2^d alone lies below fp32's range.
+__device__ __forceinline__ float scaled(float l, float d) {
+  const float h = __builtin_amdgcn_exp2f(0.5f * d);
+  return l * h * h;
 }
 
 // 2^(field - 127).
@@ -201,8 +215,8 @@ __device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPar
     }
     const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
     const float x = __builtin_amdgcn_exp2f(top - ref), y = __builtin_amdgcn_exp2f(m - ref);
+    sum = scaled(sum, top - ref) + scaled(l, m - ref);
     top = next;
-    sum = sum * x + l * y;
 #pragma unroll
     for (int f = 0; f < kFrags; ++f)
 #pragma unroll
@@ -217,7 +231,8 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   constexpr int kSteps = D / 16, kTiles = D / 32;
   __shared__ __align__(16) uint16_t s_k[2][kKeys][kPitchK];
   __shared__ __align__(16) uint16_t s_v[2][D][kPitchV];
-  // A group of 16 keys: what a raw score is multiplied by, and the values' power of two.
+  // A group of 16 keys: what a raw score is multiplied by, the values' power of two, and what takes it out
+  // of a sum of weights (0: these sums are formed without it).
   __shared__ __align__(16) float s_score[2][4], s_log[2][4], s_part[2][4];
   __shared__ int s_last;
   __shared__ uint64_t s_held[2][4];  // 4 bits a key: whether it is in the sequence and on a page
@@ -270,6 +285,7 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
   const HalfConsts hc = half_consts();
   const int col = lane & 31, h = lane >> 5;
   const float scale = a.scale_log2e;
+  bool large = false;  // a converter of values has met a field above the border
 
   for (int u = begin; u < end;) {
     KvTileCosts costs = kv_costs(a, q, group, whole);
@@ -366,9 +382,10 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         // the next lane has the other half of the 16 keys
         const int field = group_field(max(top, static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(top), 0xB1, 0xF, 0xF, true))));
         const float factor = power(kGroupFactor - field);
+        large |= __any(field > kLargeField) != 0;
         if (t < 8 && !(t & 1)) {
           s_log[buf][vgroup >> 1] = static_cast<float>(field - (kGroupFactor - 127));
-          s_part[buf][vgroup >> 1] = factor;
+          s_part[buf][vgroup >> 1] = large ? 0.0f : factor;
         }
         // A half of a word is its even or its odd channels, nibble i being channel 2 i or 2 i + 1: the
         // halves of two keys side by side, then a nibble of each.  A thread takes the 4 channels of a
@@ -579,16 +596,24 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         // The reference is 7 below the maximum where it was set, and follows when that leads it by
         // more than 15: weights stay below 2^15 as fp16, keep 11 bits down to 2^-21 of the row's
         // largest at least, and sums are rescaled rarely.
-        const bool grew = top > row_max && top - row_max > 15.0f;
-        if (__any(grew)) {
-          const float next = grew ? top - 7.0f : row_max;
-          const float f = __builtin_amdgcn_exp2f(row_max - (next == -INFINITY ? 0.0f : next));
+        const bool grew = top > row_max && top - row_max > 15.0f, large_values = of_sum[0] == 0.0f;
+        if (__any(grew | large_values)) {
+          const float next = grew ? top - 7.0f : row_max, change = row_max - (next == -INFINITY ? 0.0f : next);
+          const float f = __builtin_amdgcn_exp2f(change);
           row_max = next;
-          row_sum *= f;
+          row_sum = scaled(row_sum, change);
 #pragma unroll
           for (int c = 0; c < kTiles; ++c)
 #pragma unroll
             for (int i = 0; i < 16; ++i) acc[c][i] *= f;
+          if (large_values) {
+            const float from = next == -INFINITY ? 0.0f : -next;
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                row_sum += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], by[2 * n + (i >> 3)], from));
+          }
         }
         const float ref = row_max == -INFINITY ? 0.0f : row_max;
 #pragma unroll

@@ -257,7 +257,8 @@ def attention_errors(q, cache, tables, seq_lens, offsets, block, kernel, scale=N
                 most = 2 * u * magnitude + 2 * u * torch.where(sees, score, 0).amax(1, True) * magnitude
                 score = score * (dim / 16 + 4) * 2.0 ** -23
                 sums = (seq / 16 + 24) * 2.0 ** -23 * magnitude
-                sums = sums + seq * 2.0 ** -32 * 15 * (p.amax(1) * vs[:, g].abs().max())[:, None]
+                seen = torch.where(sees, vs[:, g].abs(), 0).amax(1)
+                sums = sums + seq * 2.0 ** -32 * 15 * (p.amax(1) * seen)[:, None]
             exact = 2 * (torch.where(sees, score, 0).amax(1, True) + 2.0 ** -20) * magnitude + sums
 
             def put(to, what):
