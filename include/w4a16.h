@@ -360,7 +360,7 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * request r owns rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1, the last tokens of its
  * seq_lens[r] (at most width * block_size are reached) on the pages of tables[r]; query head h
  * reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v with
- * fp32 scores, statistics and sums.  The second product's operands are bf16(p * s_v) and exact
+ * fp32 scores, statistics and sums.  The second product's operands are p * s_v in 16 bits and exact
  * codes; for requests of more than 64 rows a kv head, all operands are fp16 with a power of two
  * taken out of each query row and of every 16 keys: a key or value whose scale is 2^-24 of the
  * largest among its 16 loses bits.  Sums of weights times values, up to 143 scales each, are fp32: a

@@ -211,8 +211,9 @@ def attention_errors(q, cache, tables, seq_lens, offsets, block, kernel, scale=N
     that is uniform in [-u, u]:
 
     * "split" (requests of up to 64 rows a kv head, all where the caller's longest query is that
-      short): codes and zero points are exact and a weight times its value's scale becomes bf16
-      (u = 2^-8): sigma^2 = r^2 sum P^2 v^2, worst u sum P |v|.  A score's sum has products of up
+      short): codes and zero points are exact and a weight times its value's scale becomes two bf16
+      values, the second one the first one's error (u = 2^-16): sigma^2 = r^2 sum P^2 v^2, worst
+      u sum P |v|.  A score's sum has products of up
       to (128 + 15) |q|, rounded at most D / 16 + 2 times by 2^-23; sums of weights times
       (128 + 15) s_v are rounded once for each 32 keys of a wave and a few times in joining.
     * "prompt" (longer requests): keys, values and weights are fp16 (u = 2^-11; queries fit it).  Values
@@ -226,7 +227,7 @@ def attention_errors(q, cache, tables, seq_lens, offsets, block, kernel, scale=N
     kv_heads = cache.shape[1]
     group = heads // kv_heads
     scale = dim ** -0.5 if scale is None else scale
-    u = 2.0 ** -8 if kernel == "split" else 2.0 ** -11
+    u = 2.0 ** -16 if kernel == "split" else 2.0 ** -11
     r2 = u * u / 3
     out, sigma, worst = (torch.zeros(rows, heads, dim, dtype=torch.float64) for _ in range(3))
     q, cache = q.cpu().double(), cache.cpu()

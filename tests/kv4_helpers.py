@@ -31,12 +31,13 @@ def marked_channel(key, dim, keys=16):
 
 def emulate(q, cache, tables, seq_lens, offsets, block, kernel):
     """The output of a kernel that rounds what the split ("split") or the prompt kernel ("prompt") rounds,
-    or keys, values and weights to bf16 ("bf16"), and nothing else, as bf16."""
+    or keys, values and weights to bf16 ("bf16"), or weights times scales alone to bf16 ("weights"), and nothing
+    else, as bf16."""
     rows, heads, dim = q.shape
     kv_heads = cache.shape[1]
     group = heads // kv_heads
     out = torch.zeros(rows, heads, dim, dtype=torch.float64)
-    to = {"split": lambda x: x, "prompt": lambda x: x.half().double(), "bf16": lambda x: x.bfloat16().double()}[kernel]
+    to = {"split": lambda x: x, "weights": lambda x: x, "prompt": lambda x: x.half().double(), "bf16": lambda x: x.bfloat16().double()}[kernel]
     for r, seq in enumerate(seq_lens):
         first, n = offsets[r], offsets[r + 1] - offsets[r]
         slots = [tables[r][p // block] * block + p % block for p in range(seq)]
@@ -48,6 +49,10 @@ def emulate(q, cache, tables, seq_lens, offsets, block, kernel):
                 s = dim ** -0.5 * to(k[:sees, g]) @ q[first + t, h].double()
                 p = torch.exp(s - s.max())
                 if kernel == "split":
+                    x = p * vs[:sees, g]
+                    high = x.bfloat16().double()
+                    w = (high + (x - high).bfloat16().double()) / vs[:sees, g]
+                elif kernel == "weights":
                     w = (p * vs[:sees, g]).bfloat16().double() / vs[:sees, g]
                 else:
                     w = to(p)

@@ -53,6 +53,14 @@ def test_bf16_operands_fail_for_prompts(dim):
     assert "squared" in ora.check_errors(got, out, sigma, 100 * worst)
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+def test_bf16_weights_fail_for_decode_rows(dim):
+    """Weights of 8 bits where the kernel's have 16, in the squared error of all elements."""
+    b = HostBatch([1] * 4, [90, 300, 200, 128], 4, 2, dim, 16, 6)
+    got, (out, sigma, worst) = emulate(*b.args(), "weights"), ora.attention_errors(*b.args(), "split")
+    assert "squared" in ora.check_errors(got, out, sigma, worst)
+
+
 @pytest.mark.parametrize("kernel", ["split", "prompt"])
 @pytest.mark.parametrize("factor", [0, 2])
 def test_any_lost_or_doubled_keys_fail(kernel, factor):
