@@ -363,16 +363,18 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * fp32 scores, statistics and sums.  The second product's operands are p * s_v in 16 bits and exact
  * codes; for requests of more than 64 rows a kv head, all operands are fp16 with a power of two
  * taken out of each query row and of every 16 keys: a key or value whose scale is 2^-24 of the
- * largest among its 16 loses bits.  Sums of weights times values, up to 143 scales each, are fp32: a
- * row with values of 2^120 and more may be infinite or NaN.  tree_mask (may be null) [T]: row t then sees its request's
- * cached tokens and, instead of the earlier new ones, those new ones j < 64 whose bit j is set.
+ * largest among its 16, seen by the row or not, loses bits.  Sums are fp32 and have terms of up to
+ * 143 |q| and 143 scales of values: a row with queries or values of 2^110 and more may be infinite
+ * or NaN.  tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of
+ * the earlier new ones, those new ones j < 64 whose bit j is set.
  * A row that sees no key gives zeros; keys on a page id outside the cache are not seen; NaN and
  * infinities in keys that a row does not see have no effect on it.  Rows of no request (before
  * cu_query_lens[0], behind cu_query_lens[R]) are set to zero if zero_tail, else left as they are;
  * offsets that decrease anywhere name no rows at all.  max_query_len (>= 1) is a hint that chooses
- * kernels and grid: the longest query of the batch; results are right for any.  out may be q where
- * that is contiguous, and overlaps no other operand.  scale > 0 and scale * log2(e) finite; H % KV ==
- * 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:118-132). */
+ * kernels and grid: the longest query of the batch; results are right for any, if not the same bits.
+ * out may be q where that is contiguous, and overlaps no other operand.  scale > 0 and scale * log2(e)
+ * finite; H % KV == 0.  Replaces flash_attn_varlen_func / flash_attn_with_kvcache (attention.py:
+ * 118-132). */
 int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint8_t* cache,
                        const int32_t* tables, int64_t table_stride, const int32_t* seq_lens,
                        const int32_t* cu_query_lens, const uint64_t* tree_mask, uint16_t* out, float scale,

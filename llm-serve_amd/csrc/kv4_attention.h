@@ -26,7 +26,12 @@ constexpr int kKvPromptWorkers = 256;
 // The split kernel's largest grid: three workgroups a CU.
 constexpr int kKvSplitWorkers = 768;
 static_assert(kKvSplitWorkers + kKvPromptWorkers == kKvAttentionCounters, "a counter a worker");
-// Rows a request (tokens x heads of a group) up to which the split kernel takes it.
+// Rows a request (tokens x heads of a group) up to which the split kernel takes it.  Below the border it
+// is the faster one.  Above it, given longer requests (a caller's hint of 1), it still is for a while: 20
+// tokens x 4 heads behind 500, 12000 and 131000 take 14, 27 and 131 us where the prompt kernel takes 26,
+// 46 and 263; 64 x 4 take 30, 48 and 355 (31, 62 and 371).  The prompt kernel is the faster one from some
+// 400 rows on: 128 x 4 behind 2000 and 12000 take 41 and 71 us there (47 and 80), 256 x 4 42 and 87 (91
+// and 137).
 constexpr int kKvSplitMaxRows = 64;
 
 hipError_t launch_kv_prompt(const KvAttentionArgs& a, const KvPartials& part, int workers, hipStream_t stream);

@@ -111,16 +111,17 @@ __device__ __forceinline__ void kv_ids(int (&id)[2], ConstInts table, int key, i
 // alike; a share that covers a tile's keys only in part leaves a partial result (KvPartials).
 // Inside a unit each of the 4 waves takes 32 keys and keeps its own running maximum and sum; the
 // waves are joined through LDS at the end of a tile.  More rows than 16 take several tiles, which
-// read the keys again, mostly from L2: 24 requests of 8 drafts (32 rows) take 24 us so, and took
-// 26 us with 32 rows a tile, whose registers leave room for two waves a SIMD.
+// read the keys again, mostly from L2: 24 requests of 8 drafts (32 rows) took 24 us so when weights
+// were one operand (24.6 with two), and 26 us with 32 rows a tile, whose registers leave room for two
+// waves a SIMD.
 //
 // The next slice's keys are loaded into the registers that the scores have just consumed, and
 // its values into those that the second product has, so a wave has loads in flight throughout
 // without a second set of registers, and three waves fit a SIMD.  A fourth would cost spills
 // inside the loop: 128 sequences of up to 8192 keys took 255 us with four, 149 us with three.
 //
-// 128 sequences of up to 8192 keys take 129 us, 4.7 TB/s of the cache's bytes (a large copy:
-// 5.2 TB/s); 2 of 131000 take 61 us.  Short calls are bound by latency: some 4 us to the first
+// 128 sequences of up to 8192 keys take 133 us, 4.6 TB/s of the cache's bytes (a large copy:
+// 5.1 to 5.2 TB/s); 2 of 131000 take 62 us.  Short calls are bound by latency: some 4 us to the first
 // keys, 2 us to join and write, and a tail of a few us between the first and the last workgroup.
 template <int D>
 __global__ __launch_bounds__(kThreads, 3) void kv_attention_kernel(KvAttentionArgs a, KvPartials out) {

@@ -12,7 +12,8 @@
 // ones against 0.0017 for the rounding alone; codes as exact bf16 128 + c and scales applied to
 // scores and weights took 20 % longer, and lost as much in long sums of 128 P.)  fp16's range is
 // met by powers of two: one out of each 16 keys' scales and each row of queries.  Those of keys and
-// queries join the softmax's scale in the exponent's multiplier, those of values are its addend.
+// queries join the softmax's scale in the exponent's multiplier, those of values are its addend.  The 16
+// keys share it whether a row sees them or not.
 //
 // Scores are formed transposed, S^T = K Q^T, so that a lane holds 16 keys' scores of one row in
 // the accumulator layout, and P^T is the second product's operand as it stands: its 16 contraction
@@ -23,10 +24,10 @@
 // What bounds it: a tile of 64 keys costs a SIMD (two waves) some 2000 cycles of matrix
 // instructions and 3000 of vector instructions (softmax, conversion).  The two waves are in the same
 // phase, every tile ends in a barrier, and little of it overlaps: for 4096 rows behind 12288 cached
-// tokens (1.02 ms, 940 TFLOP/s; a large matrix product of the library reaches 1249) matrix
-// instructions fill 40 % of the cycles and vector instructions 62 %.  A row tile costs 4 to 5 us
-// besides its keys (queries, the first keys, writing or joining), which is what short prompts pay:
-// 2039 tokens take 58 us, 590 TFLOP/s.  Workgroups take equal shares of the cost of all row tiles,
+// tokens (1.00 to 1.03 ms, 935 to 960 TFLOP/s; a large matrix product of the library reaches 1250 to
+// 1266) matrix instructions fill 41 % of the cycles and vector instructions 61 %.  A row tile costs 4 to
+// 5 us besides its keys (queries, the first keys, writing or joining), which is what short prompts pay:
+// 2039 tokens take 59 to 62 us, 550 to 580 TFLOP/s.  Workgroups take equal shares of the cost of all row tiles,
 // so a share may end inside a tile's keys; tiles as units would leave a causal prompt's last rows to
 // few workgroups.  Measured and not taken, with bf16 operands: a conversion interleaved with the same
 // wave's first product (4096 rows 3 % faster, 2039 rows 3 % slower: both converters' loops are then
@@ -50,6 +51,9 @@ constexpr int kSetupCost = 32;  // of a row tile besides its keys
 // tokens x 5 heads behind 2172 take 32 us (8 key tiles at least: 42), 20 x 4 behind 12000 46 us (as
 // many parts as workgroups: 56).  Where no row tile has more than 8 key tiles and there is a
 // workgroup for each, they are not split: 2 x 34 tokens x 8 heads 16 us (27 split), 400 x 4 23 (29).
+// The bound on parts was measured at those two contexts and costs more behind longer ones, where the
+// join is small beside a part's keys: 20 x 4 take 85 us behind 32000 and 262 behind 131000 (the split
+// kernel 44 and 131, see kKvSplitMaxRows).
 constexpr int kMinShare = 3 * kTileCost;
 constexpr int kMaxParts = 12;
 constexpr int kShortCost = kSetupCost + 8 * kTileCost;
@@ -187,7 +191,8 @@ __device__ __forceinline__ void write_rows(const KvAttentionArgs& a, bool live, 
 }
 
 // Joins a tile's `count` parts, from worker `first` on, and writes the result; part `mine` is this
-// workgroup's own, in registers.  Parts are taken in order, the next one's loads in flight.
+// workgroup's own, in registers.  Parts are taken in order, one at a time: there are registers for one
+// part's fragments beside the sums, so each part's loads are waited for before the next one's are sent.
 template <int D>
 __device__ __forceinline__ void join_parts(const KvAttentionArgs& a, const KvPartials& part, int first, int count, int mine,
                                            int wave, int lane, bool live, int out_row, int out_head, float own_top,

@@ -279,7 +279,7 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
 
     Offsets that decrease name no rows at all.  ``scale`` defaults to 1 / sqrt(head_dim).
     ``max_query_len``, the longest query of the batch if the caller knows it (1 for a decode step),
-    picks kernels; results are right whatever it is.
+    picks kernels; results are right whatever it is, if not the same bits.
     ``tree_mask`` (int64 [rows]) replaces causality among a request's new rows: row t sees the
     cached tokens and those new ones j < 64 whose bit j is set.  A row that sees nothing is zero.
     Without ``out`` (contiguous, of q's shape), rows of no request (before the first one's, behind the
