@@ -382,6 +382,56 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
                        int max_query_len, int zero_tail, void* workspace, size_t workspace_bytes,
                        int32_t* counters, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * From the QKV projection to attention: per-head norms and position rotation, the same on the way
+ * into the 4-bit cache, and attention of whole prompts over their own keys and values.
+ * ------------------------------------------------------------------------- */
+
+/* Per-head RMSNorm and position rotation of q [T, H, D] and k [T, KV, D] (bf16, strides as in
+ * w4a16_kv_store, D in {64, 128}) into q_out and k_out (contiguous, overlapping no input).  A row x
+ * becomes y = x * r * w with r = 1 / sqrt(mean(x^2) + eps) and the weight w [D] (q_weight, k_weight;
+ * null: y = x), and channels i and i + rotary / 2 of y turn by the angle of the row's position:
+ *   z[i] = y[i] cos - y[i + rotary / 2] sin,  z[i + rotary / 2] = y[i + rotary / 2] cos + y[i] sin;
+ * channels from rotary on are y.  table [table_rows, rotary] (fp32) holds a position's rotary / 2
+ * cosines, then its sines; rotary is a multiple of 16 up to D.  A row whose position [T] lies outside
+ * the table becomes NaN.  The sum of squares is fp64, r the nearest fp32, every other step one fp32
+ * operation in the order written, and z is rounded to bf16 once.  Replaces q_norm, k_norm and
+ * rotary_emb of the reference's attention (qwen3.py:87-94, rotary_embedding.py:37-48), which round
+ * after each of their steps. */
+int w4a16_qk_norm_rope(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
+                       int64_t k_stride_t, int64_t k_stride_h, const int32_t* positions,
+                       const float* table, int table_rows, int rotary, const uint16_t* q_weight,
+                       const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out, int T,
+                       int H, int KV, int D, void* stream);
+
+/* w4a16_qk_norm_rope, and w4a16_kv_store of the keys it gives (the bf16 ones) and of v, in one
+ * launch: the same bits.  k_out may be null.  Rows of a slot outside the cache are not stored (q_out
+ * and k_out get them). */
+int w4a16_kv_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
+                    int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
+                    int64_t v_stride_h, uint8_t* cache, const int32_t* slots, const int32_t* positions,
+                    const float* table, int table_rows, int rotary, const uint16_t* q_weight,
+                    const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out, int T, int H,
+                    int KV, int D, int num_blocks, int block_size, void* stream);
+
+/* Bytes of workspace w4a16_prompt_attention needs (as w4a16_kv_attention_workspace). */
+size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D);
+
+/* Causal attention of whole prompts over their own keys and values: q [T, H, D], k and v [T, KV, D]
+ * (bf16, strides as in w4a16_kv_store; rows of k and v at most 2^24 elements apart), sequence r being
+ * rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1 of all three.  Its row t sees its rows 0 .. t;
+ * query head h reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v
+ * with fp32 scores, statistics and sums; the weights are rounded to bf16 for the second product.  NaN
+ * and infinities in keys and values that a row does not see have no effect on it.  Rows of no sequence,
+ * offsets that decrease, zero_tail, workspace and counters are as in w4a16_kv_attention.  out may be q
+ * where that is contiguous, and overlaps no other operand.  Replaces flash_attn_varlen_func where
+ * nothing is cached (attention.py:118-125). */
+int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
+                           int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
+                           int64_t v_stride_h, const int32_t* cu_query_lens, uint16_t* out, float scale,
+                           int T, int R, int H, int KV, int D, int zero_tail, void* workspace,
+                           size_t workspace_bytes, int32_t* counters, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

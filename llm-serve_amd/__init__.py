@@ -9,7 +9,9 @@ from ._lib import REGIME_DECODE, REGIME_NONE, REGIME_TILE, W4A16Error, W4A16Libr
 from .layers.attention import (
     Attention,
     KVStep,
+    append_kv_int4,
     attention_int4,
+    attention_prompt,
     kv_step,
     load_kv_int4,
     new_kv_cache_int4,
@@ -32,6 +34,7 @@ from .layers.quantization.awq import (
     repack_awq_qweight,
     unpack_awq_int4,
 )
+from .layers.rotary_embedding import RotaryEmbedding, qk_norm_rope, rotary_table
 
 __all__ = (
     "AWQLinearMethod",
@@ -43,10 +46,13 @@ __all__ = (
     "REGIME_DECODE",
     "REGIME_NONE",
     "REGIME_TILE",
+    "RotaryEmbedding",
     "W4A16Error",
     "W4A16Library",
     "add_rms_norm",
+    "append_kv_int4",
     "attention_int4",
+    "attention_prompt",
     "awq_linear",
     "awq_linear_residual",
     "awq_linear_residual_stats",
@@ -59,7 +65,9 @@ __all__ = (
     "lib",
     "load_kv_int4",
     "new_kv_cache_int4",
+    "qk_norm_rope",
     "repack_awq_qweight",
+    "rotary_table",
     "store_kv_int4",
     "unpack_awq_int4",
 )

@@ -75,6 +75,13 @@ _SIGNATURES = {
     "w4a16_kv_attention": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_ptr, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                     ctypes.c_float, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
                                     _c_int, _c_int, _c_ptr, _c_size, _c_ptr, _c_ptr]),
+    "w4a16_qk_norm_rope": (_c_int, [_c_ptr, _c_i64, _c_i64] * 2 + [_c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr,
+                                                                   ctypes.c_float, _c_ptr, _c_ptr] + [_c_int] * 4 + [_c_ptr]),
+    "w4a16_kv_append": (_c_int, [_c_ptr, _c_i64, _c_i64] * 3 + [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr,
+                                                                ctypes.c_float, _c_ptr, _c_ptr] + [_c_int] * 6 + [_c_ptr]),
+    "w4a16_prompt_attention_workspace": (_c_size, [_c_int] * 5),
+    "w4a16_prompt_attention": (_c_int, [_c_ptr, _c_i64, _c_i64] * 3 + [_c_ptr, _c_ptr, ctypes.c_float] + [_c_int] * 6
+                               + [_c_ptr, _c_size, _c_ptr, _c_ptr]),
 }
 ABI_VERSION = 5
 
@@ -375,6 +382,64 @@ class W4A16Library:
             workspace.numel(), counters.data_ptr(), _current_stream(index))
         if status != 0:
             self.check(status, "w4a16_kv_attention")
+
+    def qk_norm_rope(self, q, k, positions, table, q_weight, k_weight, eps: float, q_out, k_out) -> None:
+        """q [T, H, D] and k [T, KV, D] normed (with a weight) and rotated into q_out, k_out."""
+        index = q.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, q_out, k_out)
+        t, h, d = q.shape
+        q0, q1, _ = q.stride()
+        k0, k1, _ = k.stride()
+        table_rows, rotary = table.shape
+        status = self.dll.w4a16_qk_norm_rope(
+            q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, positions.data_ptr(), table.data_ptr(), table_rows, rotary,
+            _ptr(q_weight), _ptr(k_weight), eps, q_out.data_ptr(), k_out.data_ptr(), t, h, k.shape[1], d,
+            _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_qk_norm_rope")
+
+    def kv_append(self, q, k, v, cache, slots, positions, table, q_weight, k_weight, eps: float, q_out, k_out,
+                  block_size: int) -> None:
+        """``qk_norm_rope``, with the keys and v quantized into the cache's slots; k_out may be None."""
+        index = q.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.kv_append(q, k, v, cache, slots, positions, table, q_weight, k_weight, eps, q_out, k_out,
+                                      block_size)
+        t, h, d = q.shape
+        q0, q1, _ = q.stride()
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        table_rows, rotary = table.shape
+        blocks, kv_heads, _ = cache.shape
+        status = self.dll.w4a16_kv_append(
+            q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, cache.data_ptr(), slots.data_ptr(),
+            positions.data_ptr(), table.data_ptr(), table_rows, rotary, _ptr(q_weight), _ptr(k_weight), eps,
+            q_out.data_ptr(), _ptr(k_out), t, h, kv_heads, d, blocks, block_size, _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_kv_append")
+
+    def prompt_attention_workspace(self, t: int, r: int, h: int, kv: int, head_dim: int) -> int:
+        return int(self.dll.w4a16_prompt_attention_workspace(t, r, h, kv, head_dim))
+
+    def prompt_attention(self, q, k, v, cu_query_lens, out, scale: float, zero_tail: bool, workspace, counters) -> None:
+        """out [T, H, D] = causal attention of the packed sequences' rows; counters as in ``kv_attention``."""
+        index = q.get_device()
+        if _current_device() != index:
+            with torch.cuda.device(index):
+                return self.prompt_attention(q, k, v, cu_query_lens, out, scale, zero_tail, workspace, counters)
+        t, h, d = q.shape
+        q0, q1, _ = q.stride()
+        k0, k1, _ = k.stride()
+        v0, v1, _ = v.stride()
+        status = self.dll.w4a16_prompt_attention(
+            q.data_ptr(), q0, q1, k.data_ptr(), k0, k1, v.data_ptr(), v0, v1, cu_query_lens.data_ptr(), out.data_ptr(),
+            scale, t, cu_query_lens.shape[0] - 1, h, k.shape[1], d, zero_tail, workspace.data_ptr(), workspace.numel(),
+            counters.data_ptr(), _current_stream(index))
+        if status != 0:
+            self.check(status, "w4a16_prompt_attention")
 
 
 _LOCK = threading.Lock()

@@ -20,6 +20,25 @@ struct KvPartials {
   uint32_t out_bytes, stats_bytes;
 };
 
+inline size_t align256(size_t n) { return (n + 255) / 256 * 256; }
+
+// A kernel's part of the workspace: partial results of 2 tiles of `rows` rows a worker.
+inline size_t partials_bytes(int workers, int rows, int D) {
+  const size_t n = static_cast<size_t>(2) * workers * rows;
+  return align256(n * D * sizeof(float)) + align256(n * 2 * sizeof(float));
+}
+
+inline KvPartials partials_at(char* ws, int* counters, int workers, int rows, int D) {
+  const size_t n = static_cast<size_t>(2) * workers * rows;
+  KvPartials part;
+  part.out = reinterpret_cast<float*>(ws);
+  part.stats = reinterpret_cast<float*>(ws + align256(n * D * sizeof(float)));
+  part.out_bytes = static_cast<uint32_t>(n * D * sizeof(float));
+  part.stats_bytes = static_cast<uint32_t>(n * 2 * sizeof(float));
+  part.counters = counters;
+  return part;
+}
+
 // Prompt kernel: rows of a tile, and its grid (a workgroup a CU).
 constexpr int kKvPromptRows = 256;
 constexpr int kKvPromptWorkers = 256;
@@ -103,13 +122,15 @@ __device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int 
 
 // Whether request r's offsets decrease.  Offsets that never do give requests of at most T rows in
 // all, which bounds every count of work; with others the kernels do none.
-__device__ __forceinline__ bool kv_decreases(const KvAttentionArgs& a, int r) {
+template <class Args>
+__device__ __forceinline__ bool kv_decreases(const Args& a, int r) {
   return const_ints(a.cu_query_lens)[r + 1] < const_ints(a.cu_query_lens)[r];
 }
 
 // Zeros for the output rows of no request: those before the first one's and behind the last one's
 // (all rows if there is no work).
-__device__ __forceinline__ void kv_zero_unowned(const KvAttentionArgs& a, bool all) {
+template <class Args>
+__device__ __forceinline__ void kv_zero_unowned(const Args& a, bool all) {
   const int first = all ? 0 : min(max(const_ints(a.cu_query_lens)[0], 0), a.T);
   const int end = all ? 0 : min(max(const_ints(a.cu_query_lens)[a.R], 0), a.T);
   const int unowned = first + a.T - end, chunks = a.H * a.D / 8;

@@ -457,25 +457,6 @@ KvPlan kv_plan(const KvAttentionArgs& a) {
   return p;
 }
 
-size_t align256(size_t n) { return (n + 255) / 256 * 256; }
-
-// A kernel's part of the workspace: partial results of 2 tiles of `rows` rows a worker.
-size_t partials_bytes(int workers, int rows, int D) {
-  const size_t n = static_cast<size_t>(2) * workers * rows;
-  return align256(n * D * sizeof(float)) + align256(n * 2 * sizeof(float));
-}
-
-KvPartials partials_at(char* ws, int* counters, int workers, int rows, int D) {
-  const size_t n = static_cast<size_t>(2) * workers * rows;
-  KvPartials part;
-  part.out = reinterpret_cast<float*>(ws);
-  part.stats = reinterpret_cast<float*>(ws + align256(n * D * sizeof(float)));
-  part.out_bytes = static_cast<uint32_t>(n * D * sizeof(float));
-  part.stats_bytes = static_cast<uint32_t>(n * 2 * sizeof(float));
-  part.counters = counters;
-  return part;
-}
-
 template <int D>
 hipError_t launch(const KvAttentionArgs& a, const KvPlan& p, char* ws, int* counters, hipStream_t stream) {
   const KvPartials split = partials_at(ws, counters, p.split_workers, kRows, D);

@@ -1,7 +1,7 @@
 // The 4-bit key/value cache's bookkeeping and rows: the step's slots and block tables from the
 // request lengths, quantizing rows into the cache, and reading rows back.
-#include "kv4_common.h"
 #include "kv4_launch.h"
+#include "kv4_quantize.h"
 
 namespace w4a16 {
 namespace {
@@ -122,81 +122,6 @@ __global__ __launch_bounds__(kStepThreads) void kv_step_kernel(KvStepArgs a) {
   a.slots[t] = slot;
 }
 
-// Maximum over the LANES neighbouring lanes (8 or 16) of a row, every lane getting it.
-template <int LANES>
-__device__ __forceinline__ float lanes_max(float v) {
-  v = fmaxf(v, dpp_f32<0xB1>(v));
-  v = fmaxf(v, dpp_f32<0x4E>(v));
-  v = fmaxf(v, dpp_f32<0x141>(v));
-  if (LANES == 16) v = fmaxf(v, dpp_f32<0x140>(v));
-  return v;
-}
-
-// x / s rounded to a multiple of 2^-11 (|x / s| < 16), by the reciprocal: enough to round it to a
-// code as the exact quotient would be.  x and s have at most 8 significant bits: where x / s lies
-// near a border k + 1/2 between two codes, |x| > s / 4 makes 2 x - (2 k + 1) s a multiple of s's
-// last place, so x / s is the border itself or at least 1 / 510 away.  The product is off by 2^-18
-// at most, and the sum with 1.5 * 2^12, whose last place is 2^-11, then returns a border as it is
-// and moves nothing across one.
-__device__ __forceinline__ float near_quotient(float x, float inverse) { return (x * inverse + 6144.0f) - 6144.0f; }
-
-// One row's eight channels in a lane -> its code word and the row's meta word.  The range takes
-// in zero, so z is in 0..15 and a row of one sign keeps its far end.  The scale is rounded to
-// bf16 (the cache's type) before the codes are formed, so codes are right for the scale that
-// readers multiply by.  A row with a NaN or infinity becomes NaN as a whole; a range beyond fp32
-// is formed a sixteenth at a time; scales too small for the reciprocal take the division.
-template <int LANES>
-__device__ __forceinline__ uint32_t quantize_row(uint4 raw, int lane, uint32_t* meta) {
-  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-  float x[8];
-  unpack_bf16x8(raw, x);
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  u16x2_t top = {0, 0};
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[i] & 0x7FFF7FFFu));
-  const bool bad = top[0] >= 0x7F80 || top[1] >= 0x7F80;
-  float hi = 0.0f, lo = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    hi = fmaxf(hi, x[i]);
-    lo = fminf(lo, x[i]);
-  }
-  hi = lanes_max<LANES>(hi);
-  lo = -lanes_max<LANES>(-lo);
-  constexpr uint64_t kRow = LANES == 16 ? 0xFFFFull : 0xFFull;
-  if (__ballot(bad) >> (lane & ~(LANES - 1)) & kRow) {
-    *meta = 0x7FC04300u;
-    return 0;
-  }
-  const float range = hi - lo;
-  const float exact = __builtin_isinf(range) ? (hi * 0.0625f - lo * 0.0625f) / 15.0f * 16.0f : range / 15.0f;
-  const float s = bf16_bits_to_f32(pack_bf16x2(exact, 0.0f) & 0xFFFFu);
-  if (!(s > 0.0f)) {  // all zeros, or below the smallest scale
-    *meta = 0x00004300u;
-    return 0;
-  }
-  float t[8], z;
-  if (s < 0x1p-100f || s > 0x1p100f) {
-    z = rintf(-lo / s);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = x[i] / s;
-  } else {
-    const float inverse = __builtin_amdgcn_rcpf(s);
-    z = rintf(near_quotient(-lo, inverse));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) t[i] = near_quotient(x[i], inverse);
-  }
-  z = fminf(z, 15.0f);
-  uint32_t c[8];  // the code in the low bits of 2^23 + code
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    c[i] = __float_as_uint(__builtin_amdgcn_fmed3f(rintf(t[i]), -z, 15.0f - z) + (z + 8388608.0f));
-  *meta = kv_meta(s, static_cast<int>(z));
-  const uint32_t p0 = __builtin_amdgcn_perm(c[1], c[0], 0x05040100u), p1 = __builtin_amdgcn_perm(c[3], c[2], 0x05040100u);
-  const uint32_t p2 = __builtin_amdgcn_perm(c[5], c[4], 0x05040100u), p3 = __builtin_amdgcn_perm(c[7], c[6], 0x05040100u);
-  return p0 | (p1 << 4) | (p2 << 8) | (p3 << 12);
-}
-
 // A wave takes 64 / (D / 8) consecutive tokens of one kv head, K and V: D / 8 lanes a row, 16
 // bytes a lane.  Consecutive tokens usually follow each other in a page, where the wave's words
 // are then whole lines.  Reads and writes bound it: 16384 tokens of 8 heads (85 MB) take 20.8 us,
@@ -216,17 +141,16 @@ __global__ __launch_bounds__(256) void kv_store_kernel(KvRowsArgs a) {
     k = *reinterpret_cast<const uint4*>(a.k + t * a.k_stride_t + head * a.k_stride_h + w * 8);
     v = *reinterpret_cast<const uint4*>(a.v + t * a.v_stride_t + head * a.v_stride_h + w * 8);
   }
-  uint32_t k_meta, v_meta;
-  const uint32_t kw = quantize_row<kLanes>(k, lane, &k_meta);
-  const uint32_t vw = quantize_row<kLanes>(v, lane, &v_meta);
+  uint32_t kw[1], vw[1];
+  const uint32_t k_meta = quantize_row<kLanes>({k}, lane, kw), v_meta = quantize_row<kLanes>({v}, lane, vw);
   const int id = slot >> a.log2_block;
   if (slot < 0 || id >= a.num_blocks) return;
   const int token = slot & ((1 << a.log2_block) - 1);
   uint32_t* page = reinterpret_cast<uint32_t*>(
       a.cache + (static_cast<size_t>(id) * a.KV + head) * kv_page_bytes<D>(a.log2_block));
   const int part = kLanes << a.log2_block;  // words of the K or V codes
-  page[token * kLanes + w] = kw;
-  page[part + kv_v_word<D>(token, w)] = vw;
+  page[token * kLanes + w] = kw[0];
+  page[part + kv_v_word<D>(token, w)] = vw[0];
   if (w == 0) {
     page[2 * part + token] = k_meta;
     page[2 * part + (1 << a.log2_block) + token] = v_meta;

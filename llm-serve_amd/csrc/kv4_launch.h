@@ -1,4 +1,5 @@
-// Host-side launchers of the 4-bit key/value cache kernels (kv4_cache.hip, kv4_attention.hip).
+// Host-side launchers of the 4-bit key/value cache kernels (kv4_cache.hip, kv4_attention.hip), of the
+// norm and rotation in front of them (qk_rope.hip) and of prompt attention in bf16 (prompt_attention.hip).
 // Arguments are checked by the callers (w4a16_api.hip).
 #pragma once
 
@@ -43,6 +44,24 @@ struct KvRowsArgs {
 hipError_t launch_kv_store(const KvRowsArgs& a, hipStream_t stream);
 hipError_t launch_kv_load(const KvRowsArgs& a, hipStream_t stream);
 
+// Up to this many tokens a wave of the norm-and-rotation kernel takes one group of heads.
+constexpr int kQkRopeFewTokens = 512;
+
+struct QkRopeArgs {
+  const uint16_t *q, *k, *v;  // [T, H or KV, D] at strides (elements); v only with a cache
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int32_t* positions;  // [T]
+  const float* table;        // [table_rows, rotary]: cosines, then sines
+  const uint16_t *q_weight, *k_weight;  // [D], or null: no norm
+  uint16_t* q_out;           // [T, H, D]
+  uint16_t* k_out;           // [T, KV, D], or null with a cache
+  uint8_t* cache;            // or null: keys and values are not stored
+  const int32_t* slots;      // [T]
+  float eps;
+  int T, H, KV, D, table_rows, rotary, num_blocks, log2_block;
+};
+hipError_t launch_qk_rope(const QkRopeArgs& a, hipStream_t stream);
+
 struct KvAttentionArgs {
   const uint16_t* q;  // [T, H, D] at strides (elements)
   int64_t q_stride_t, q_stride_h;
@@ -63,5 +82,18 @@ size_t kv_attention_workspace(const KvAttentionArgs& a);
 // counters: kKvAttentionCounters ints, zero before and after the call's kernels.
 constexpr int kKvAttentionCounters = 1024;
 hipError_t launch_kv_attention(const KvAttentionArgs& a, void* workspace, int* counters, hipStream_t stream);
+
+struct PromptArgs {
+  const uint16_t *q, *k, *v;  // [T, H or KV, D] at strides (elements)
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int32_t* cu_query_lens;
+  uint16_t* out;  // [T, H, D] contiguous
+  float scale_log2e;
+  int T, R, H, KV, D;
+  bool zero_tail;
+};
+size_t prompt_attention_workspace(const PromptArgs& a);
+// counters: kKvAttentionCounters ints, zero before and after the call's kernel.
+hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream);
 
 }  // namespace w4a16

@@ -1397,4 +1397,121 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
   return check_launch(w4a16::launch_kv_attention(a, workspace, counters, static_cast<hipStream_t>(stream)), "kv attention");
 }
 
+// What the rotating entry points share; a's sizes and pointers but for v, cache, slots and k_out.
+static int validate_rope(const w4a16::QkRopeArgs& a) {
+  if (a.T < 0) return fail(W4A16_ERR_ARG, "T must not be negative (got %d)", a.T);
+  if (a.H <= 0 || a.KV <= 0) return fail(W4A16_ERR_ARG, "query heads (%d) and kv heads (%d) must be positive", a.H, a.KV);
+  if (a.H > 0xFFFF || a.KV > 0xFFFF) return fail(W4A16_ERR_SHAPE, "%d query heads and %d kv heads are too many", a.H, a.KV);
+  if (a.D != 64 && a.D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", a.D);
+  if (a.rotary <= 0 || a.rotary % 16 || a.rotary > a.D)
+    return fail(W4A16_ERR_SHAPE, "the rotated channels must be a multiple of 16 up to the head size (got %d of %d)", a.rotary, a.D);
+  if (a.table_rows <= 0) return fail(W4A16_ERR_ARG, "the rotation's table needs a row (got %d)", a.table_rows);
+  if (!(a.eps >= 0.0f) || !(a.eps <= 3.402823466e38f)) return fail(W4A16_ERR_ARG, "eps must be finite and not negative (got %g)", static_cast<double>(a.eps));
+  if (a.T == 0) return W4A16_OK;
+  if (!a.positions || !a.table || !a.q_out) return fail(W4A16_ERR_ARG, "a pointer of the norm and rotation is null");
+  int e = validate_kv_rows("q", a.q, a.q_stride_t, a.q_stride_h);
+  if (e == W4A16_OK) e = validate_kv_rows("k", a.k, a.k_stride_t, a.k_stride_h);
+  if (e != W4A16_OK) return e;
+  if (!aligned(a.table, 16) || !aligned(a.q_weight, 16) || !aligned(a.k_weight, 16) || !aligned(a.q_out, 16) || !aligned(a.k_out, 16))
+    return fail(W4A16_ERR_ALIGN, "the rotation's table, the weights and the outputs must be 16-byte aligned");
+  return W4A16_OK;
+}
+
+int w4a16_qk_norm_rope(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k, int64_t k_stride_t,
+                       int64_t k_stride_h, const int32_t* positions, const float* table, int table_rows, int rotary,
+                       const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out,
+                       int T, int H, int KV, int D, void* stream) {
+  w4a16::QkRopeArgs a{};
+  a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
+  a.k = k, a.k_stride_t = k_stride_t, a.k_stride_h = k_stride_h;
+  a.positions = positions, a.table = table, a.table_rows = table_rows, a.rotary = rotary;
+  a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps, a.q_out = q_out, a.k_out = k_out;
+  a.T = T, a.H = H, a.KV = KV, a.D = D;
+  const int e = validate_rope(a);
+  if (e != W4A16_OK) return e;
+  if (T == 0) return ok();
+  if (!k_out) return fail(W4A16_ERR_ARG, "k_out is null");
+  return check_launch(w4a16::launch_qk_rope(a, static_cast<hipStream_t>(stream)), "qk norm and rotation");
+}
+
+int w4a16_kv_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k, int64_t k_stride_t,
+                    int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t, int64_t v_stride_h, uint8_t* cache,
+                    const int32_t* slots, const int32_t* positions, const float* table, int table_rows, int rotary,
+                    const uint16_t* q_weight, const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out,
+                    int T, int H, int KV, int D, int num_blocks, int block_size, void* stream) {
+  w4a16::QkRopeArgs a{};
+  int e = validate_kv_cache(cache, KV, D, num_blocks, block_size, &a.log2_block);
+  if (e != W4A16_OK) return e;
+  a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
+  a.k = k, a.k_stride_t = k_stride_t, a.k_stride_h = k_stride_h;
+  a.v = v, a.v_stride_t = v_stride_t, a.v_stride_h = v_stride_h;
+  a.positions = positions, a.table = table, a.table_rows = table_rows, a.rotary = rotary;
+  a.q_weight = q_weight, a.k_weight = k_weight, a.eps = eps, a.q_out = q_out, a.k_out = k_out;
+  a.cache = cache, a.slots = slots;
+  a.T = T, a.H = H, a.KV = KV, a.D = D, a.num_blocks = num_blocks;
+  if ((e = validate_rope(a)) != W4A16_OK) return e;
+  if (T == 0) return ok();
+  if (!slots) return fail(W4A16_ERR_ARG, "slots is null");
+  if ((e = validate_kv_rows("v", v, v_stride_t, v_stride_h)) != W4A16_OK) return e;
+  return check_launch(w4a16::launch_qk_rope(a, static_cast<hipStream_t>(stream)), "kv append");
+}
+
+static int validate_prompts(int T, int R, int H, int KV, int D) {
+  if (T < 0 || R < 0) return fail(W4A16_ERR_ARG, "T (%d) and R (%d) must not be negative", T, R);
+  if (H <= 0 || KV <= 0 || H % KV) return fail(W4A16_ERR_SHAPE, "query heads (%d) must be a multiple of kv heads (%d)", H, KV);
+  if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
+  if (T == 0 || R == 0) return W4A16_OK;
+  if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
+    return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
+  // The kernel counts its work in 32 bits.  Tile j of a sequence's m costs ceil(64 / group) (j + 1) + 32, and
+  // m <= rows / 256 + 1: the last costs at most T / 4 + rows / 256 + 98, the mean of all half of that and 50.
+  const int64_t rows = static_cast<int64_t>(T) * (H / KV), tiles = rows / 256 + (R < rows ? R : rows);
+  if (static_cast<int64_t>(T) / 8 + rows / 512 + 100 > 0x7FFFFFFF / tiles / KV)
+    return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too much work for one call", T, H);
+  return W4A16_OK;
+}
+
+size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D) {
+  if (validate_prompts(T, R, H, KV, D) != W4A16_OK || T == 0 || R == 0) return 0;
+  w4a16::PromptArgs a{};
+  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D;
+  return w4a16::prompt_attention_workspace(a);
+}
+
+int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
+                           int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
+                           int64_t v_stride_h, const int32_t* cu_query_lens, uint16_t* out, float scale, int T, int R,
+                           int H, int KV, int D, int zero_tail, void* workspace, size_t workspace_bytes,
+                           int32_t* counters, void* stream) {
+  int e = validate_prompts(T, R, H, KV, D);
+  if (e != W4A16_OK) return e;
+  const float scale_log2e = scale * 1.44269504088896341f;
+  if (!(scale > 0.0f) || !(scale_log2e <= 3.402823466e38f))
+    return fail(W4A16_ERR_ARG, "scale must be positive and finite, times log2(e) too (got %g)", static_cast<double>(scale));
+  if (T == 0) return ok();
+  if (R == 0) return fail(W4A16_ERR_ARG, "%d rows of no request", T);
+  if (!cu_query_lens || !out) return fail(W4A16_ERR_ARG, "an attention pointer is null");
+  if ((e = validate_kv_rows("q", q, q_stride_t, q_stride_h)) != W4A16_OK) return e;
+  if ((e = validate_kv_rows("k", k, k_stride_t, k_stride_h)) != W4A16_OK) return e;
+  if ((e = validate_kv_rows("v", v, v_stride_t, v_stride_h)) != W4A16_OK) return e;
+  // The 64 keys of a tile are addressed by 32-bit byte offsets.
+  constexpr int64_t kMostStride = 1 << 24;
+  if (k_stride_t < 0 || v_stride_t < 0 || k_stride_t > kMostStride || v_stride_t > kMostStride)
+    return fail(W4A16_ERR_SHAPE, "rows of k and v must be 0 to 2^24 elements apart (got %lld and %lld)",
+                static_cast<long long>(k_stride_t), static_cast<long long>(v_stride_t));
+  if (!aligned(out, 16)) return fail(W4A16_ERR_ALIGN, "out must be 16-byte aligned");
+  w4a16::PromptArgs a{};
+  a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
+  a.k = k, a.k_stride_t = k_stride_t, a.k_stride_h = k_stride_h;
+  a.v = v, a.v_stride_t = v_stride_t, a.v_stride_h = v_stride_h;
+  a.cu_query_lens = cu_query_lens, a.out = out, a.scale_log2e = scale_log2e;
+  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.zero_tail = zero_tail != 0;
+  const size_t need = w4a16::prompt_attention_workspace(a);
+  if (!workspace || workspace_bytes < need)
+    return fail(W4A16_ERR_WORKSPACE, "attention needs %zu bytes of workspace (got %zu)", need, workspace ? workspace_bytes : size_t(0));
+  if (!aligned(workspace, 16)) return fail(W4A16_ERR_ALIGN, "the workspace must be 16-byte aligned");
+  if (!counters) return fail(W4A16_ERR_WORKSPACE, "attention needs %d zeroed counters", W4A16_KV_COUNTERS);
+  return check_launch(w4a16::launch_prompt_attention(a, workspace, counters, static_cast<hipStream_t>(stream)), "prompt attention");
+}
+
 }  // extern "C"

@@ -7,19 +7,22 @@ flash-attn calls (llmserve/layers/attention.py:21-133).
                          ``prepare_prefill`` / ``prepare_decode``, model_runner.py:279-333)
 * ``store_kv_int4``      new rows quantized into the cache (``store_kvcache``, attention.py:21-57)
 * ``load_kv_int4``       rows read back as the values they stand for
+* ``append_kv_int4``     per-head norms and rotation of new rows on their way into the cache, in one launch
 * ``attention_int4``     causal attention of packed rows over their sequences' pages: decode,
                          draft verification, chunks and prompts in one call (attention.py:118-132)
-* ``Attention``          the layer between QKV and O: ``store_kv_int4``, then ``attention_int4``
+* ``attention_prompt``   causal attention of whole prompts over their own keys and values in bf16
+* ``Attention``          the layer between QKV and O: ``store_kv_int4``, then ``attention_int4``; from the
+                         QKV projection's output, ``append_kv_int4``, then either attention
 
 A row of the cache (one token of one kv head) is a code c in 0..15 a channel, one bf16 scale s and
 one zero point z, as a group of an AWQ weight is; a channel stands for s * (c - z).  With 128
 channels that is 68 bytes for a row of 256.
 
 Everything runs in the HIP library and raises without it or without a GPU; nothing synchronises
-the host (but for the first ``attention_int4`` on a device, which sets up its counters, and one in
-4096 captured calls), and every call may be captured in a HIP graph.  ``attention_int4`` takes its workspace and counters from
-``SCRATCH``, one pair a stream and one a captured call, so calls on several streams, and several
-graphs, share neither.
+the host (but for the first attention call on a device, which sets up its counters, and one in
+4096 captured calls), and every call may be captured in a HIP graph.  ``attention_int4`` and
+``attention_prompt`` take their workspace and counters from ``SCRATCH``, one pair a stream and one a
+captured call, so calls on several streams, and several graphs, share neither.
 """
 from __future__ import annotations
 
@@ -31,8 +34,10 @@ import torch
 from torch import nn
 
 from .._lib import _current_device, _current_stream, lib
+from .rotary_embedding import _head_rows, norm_weight, rope_operands
 
-__all__ = ("Attention", "KVStep", "attention_int4", "kv_step", "load_kv_int4", "new_kv_cache_int4", "store_kv_int4")
+__all__ = ("Attention", "KVStep", "append_kv_int4", "attention_int4", "attention_prompt", "kv_step", "load_kv_int4",
+           "new_kv_cache_int4", "store_kv_int4")
 
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)  # None without GPU support
 _BF16, _I32, _U8 = torch.bfloat16, torch.int32, torch.uint8
@@ -208,6 +213,44 @@ def load_kv_int4(cache: torch.Tensor, slots: torch.Tensor, *, block_size: int) -
     return k, v
 
 
+def append_kv_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,
+                   positions: torch.Tensor, table: torch.Tensor, *, block_size: int,
+                   q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                   return_keys: bool = False) -> torch.Tensor | tuple[torch.Tensor, torch.Tensor]:
+    """A step's rows from the QKV projection's output to where attention reads them, in one launch: q
+    [tokens, heads, head_dim] and k [tokens, kv heads, head_dim] (bf16; views of the split output are read
+    in place) normed and rotated as by ``qk_norm_rope``, those keys and v quantized into the cache's
+    ``slots`` (int32 [tokens]) as by ``store_kv_int4``: the same bits as the two calls.
+
+    Returns the queries, and with ``return_keys`` the bf16 keys too, which ``attention_prompt`` reads.
+    Slots outside the cache (-1) are skipped, the others must differ from each other.  A row whose
+    position the table does not have becomes NaN, in the cache too."""
+    head_dim = _cache_head_dim(cache, block_size)
+    kv_heads, index = cache.shape[1], cache.get_device()
+    if q.get_device() != index:
+        raise ValueError("KV queries must be a bfloat16 tensor on the cache's GPU")
+    q, k, positions, table = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
+    q_weight, k_weight = norm_weight(q_weight), norm_weight(k_weight)
+    if q.shape[2] != head_dim or k.shape[1] != kv_heads:
+        raise ValueError(f"KV keys must be [tokens, {kv_heads}, {head_dim}] and queries [tokens, heads, {head_dim}]")
+    v = _rows("values", v, kv_heads, head_dim, cache)
+    if slots.dtype is not _I32 or slots.get_device() != index:
+        _require_int32(cache.device, slots=slots)
+    if v.shape != k.shape or slots.shape != k.shape[:1]:
+        raise ValueError("KV keys, values and slots must have one entry a token")
+    q_out = torch.empty(q.shape, dtype=_BF16, device=cache.device)
+    k_out = torch.empty(k.shape, dtype=_BF16, device=cache.device) if return_keys else None
+    if q.shape[0] > 0:
+        lib().kv_append(q, k, v, cache, slots.contiguous(), positions, table, q_weight, k_weight, eps, q_out, k_out,
+                        block_size)
+    return (q_out, k_out) if return_keys else q_out
+
+
+@functools.lru_cache(maxsize=4096)
+def _prompt_workspace_bytes(*sizes: int) -> int:
+    return lib().prompt_attention_workspace(*sizes)
+
+
 @functools.lru_cache(maxsize=4096)
 def _workspace_bytes(*sizes: int) -> int:
     """The library's answer for these sizes, which depends on nothing else."""
@@ -215,7 +258,7 @@ def _workspace_bytes(*sizes: int) -> int:
 
 
 class _ScratchPool:
-    """Workspaces and arrival counters of ``attention_int4``; a call's counters (1024 int32) are zero
+    """Workspaces and arrival counters of the attention calls; a call's counters (1024 int32) are zero
     before and after it.
 
     Eager calls of one stream run in order and share one pair, whose workspace is as large as their
@@ -350,6 +393,56 @@ def _check_attention(q, cache, block_tables, seq_lens, cu_query_lens, block_size
     return q, block_tables, seq_lens.contiguous(), cu_query_lens.contiguous()
 
 
+def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query_lens: torch.Tensor, *,
+                     scale: float | None = None, max_query_len: int | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of whole prompts over their own keys and values in bf16, nothing being cached before
+    them: q [rows, heads, head_dim], k and v [rows, kv heads, head_dim] (views of the split QKV output are
+    read in place), request r being rows ``cu_query_lens[r]`` .. ``cu_query_lens[r + 1]`` (int32
+    [requests + 1]) of all three, its row t attending to its rows 0 .. t.  Returns bf16
+    [rows, heads, head_dim].
+
+    A prompt's rows give what ``attention_int4`` gives over their cached copies, but for the 4 bits.
+    ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest prompt if the caller knows it,
+    is checked and otherwise free.  Offsets that decrease name no rows at all.  Without ``out``
+    (contiguous, of q's shape), rows of no request are zero; in ``out`` they are left as they were.
+    ``out`` may be q itself, and overlaps no other operand."""
+    index, head_dim = q.get_device(), q.shape[2] if q.ndim == 3 else 0
+    if index < 0:
+        raise ValueError("attention_prompt's queries must be on a GPU (HIP) device")
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"attention_prompt's queries must be [rows, heads, head_dim] with head_dim in {HEAD_DIMS}")
+    q = _head_rows("queries", q, None, head_dim, index)
+    k = _head_rows("keys", k, None, head_dim, index)
+    rows, heads, _ = q.shape
+    kv_heads = k.shape[1]
+    v = _head_rows("values", v, kv_heads, head_dim, index)
+    if k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError("queries, keys and values must have one entry a row")
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"query heads ({heads}) must be a multiple of kv heads ({kv_heads})")
+    if (cu_query_lens.dtype is not _I32 or cu_query_lens.get_device() != index or cu_query_lens.ndim != 1
+            or cu_query_lens.shape[0] < 2):
+        raise ValueError("cu_query_lens must be an int32 [requests + 1] tensor, of at least one request, on the queries' GPU")
+    if scale is None:
+        scale = head_dim ** -0.5
+    elif not 0.0 < scale < MAX_SCALE:
+        raise ValueError(f"attention scale must be positive and below {MAX_SCALE} (got {scale})")
+    if max_query_len is not None and max_query_len < 1:
+        raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
+    zero_tail = out is None
+    if out is None:
+        out = torch.empty((rows, heads, head_dim), dtype=_BF16, device=q.device)
+    elif (out.shape != q.shape or out.dtype is not _BF16 or out.get_device() != index or not out.is_contiguous()
+          or out.data_ptr() % 16):
+        raise ValueError("attention out must be a contiguous, 16-byte aligned bfloat16 tensor of q's shape")
+    if rows > 0:
+        size = _prompt_workspace_bytes(rows, cu_query_lens.shape[0] - 1, heads, kv_heads, head_dim)
+        workspace, counters = SCRATCH.get(index, size)
+        lib().prompt_attention(q, k, v, cu_query_lens.contiguous(), out, scale, zero_tail, workspace, counters)
+    return out
+
+
 class Attention(nn.Module):
     """The reference's ``Attention`` (attention.py:21-133) over a 4-bit cache: ``forward(q, k, v,
     step)`` stores the step's keys and values and attends.  ``kv_cache`` is the layer's cache
@@ -385,3 +478,32 @@ class Attention(nn.Module):
                              block_size=self.block_size, scale=self.scale, max_query_len=max_query_len,
                              tree_mask=tree_mask)
         return out.view(rows, self.num_heads * self.head_dim)
+
+    def forward_qkv(self, qkv: torch.Tensor, step: KVStep, table: torch.Tensor, *,
+                    q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6,
+                    whole_prompts: bool = False, max_query_len: int | None = None,
+                    tree_mask: torch.Tensor | None = None) -> torch.Tensor:
+        """From the QKV projection's output [rows, (heads + 2 kv heads) * head_dim] to O's input [rows,
+        heads * head_dim]: per-head norms (with weights), rotation by ``step.positions`` and the store in one
+        launch, then attention (the reference's Qwen3Attention.forward between its projections,
+        qwen3.py:87-94).  ``table`` is ``rotary_table``'s.
+
+        ``whole_prompts`` says that every request of the step is a prompt with nothing cached before it:
+        its rows then attend to their own keys and values as they are, in bf16, and not to their 4-bit
+        copies in the cache."""
+        if self.kv_cache is None:
+            raise RuntimeError("Attention.kv_cache must be set before the first step")
+        if whole_prompts and tree_mask is not None:
+            raise ValueError("whole prompts are causal: they take no tree_mask")
+        heads, kv_heads, rows = self.num_heads, self.num_kv_heads, qkv.shape[0]
+        q, k, v = qkv.view(rows, heads + 2 * kv_heads, self.head_dim).split((heads, kv_heads, kv_heads), 1)
+        q = append_kv_int4(q, k, v, self.kv_cache, step.slots, step.positions, table, block_size=self.block_size,
+                           q_weight=q_weight, k_weight=k_weight, eps=eps, return_keys=whole_prompts)
+        if whole_prompts:
+            q, k = q
+            out = attention_prompt(q, k, v, step.cu_query_lens, scale=self.scale, max_query_len=max_query_len, out=None)
+        else:
+            out = attention_int4(q, self.kv_cache, step.block_tables, step.seq_lens, step.cu_query_lens,
+                                 block_size=self.block_size, scale=self.scale, max_query_len=max_query_len,
+                                 tree_mask=tree_mask)
+        return out.view(rows, heads * self.head_dim)
