@@ -1,8 +1,6 @@
-// What the kernels of long queries share: 256 rows a workgroup, 32 a wave, whose output O^T lies in
+// What the kernels of long queries share: workgroups of WAVES waves with 32 rows each, whose output O^T lies in
 // accumulators of 32 x 32 -- a lane has one row, lane % 32, and of each 32 channels those of its half of
 // the wave, lane / 32 -- and goes to the output, or to a part of it that is joined with others.
-//
-// Args are a kernel's arguments: out [T, H, D] and H.
 #pragma once
 
 #include "kv4_attention.h"
@@ -46,41 +44,39 @@ __device__ __forceinline__ float scaled(float l, float d) {
 
 // Byte offset of a lane's fragment f (four channels: 32 (f / 4) + 8 (f % 4) + 4 (lane / 32) ..) of
 // its wave's 32 rows in slot `slot`: whole waves of 16 bytes a lane, in the accumulators' layout.
-template <int D>
+template <int D, int WAVES>
 __device__ __forceinline__ uint32_t part_offset(int slot, int wave, int f, int lane) {
-  return ((static_cast<uint32_t>(slot) * 8 + wave) * (D / 8) + f) * 1024u + lane * 16u;
+  return ((static_cast<uint32_t>(slot) * WAVES + wave) * (D / 8) + f) * 1024u + lane * 16u;
 }
 
-// Two fragments of a lane -- channels 4 h .. of eights b and b + 1 -- to the output: the halves of
-// the wave exchange theirs, so that a lane writes one eight's 16 bytes.
-template <int D, class Args>
-__device__ __forceinline__ void write_pair(const Args& a, bool live, int row, int head, int f, int lane, float inv,
-                                           const f32x4_t& x, const f32x4_t& y) {
+// Two fragments of a lane -- channels 4 h .. of eights b and b + 1 -- times inv, rounded: the halves of the
+// wave exchange theirs, so that a lane has one eight's 16 bytes, b + lane / 32.
+__device__ __forceinline__ u32x4_t row_pair(float inv, const f32x4_t& x, const f32x4_t& y) {
   const u32x2_t lo = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[0] * inv, x[1] * inv),
                                                                                   pack_bf16x2(y[0] * inv, y[1] * inv), false, false));
   const u32x2_t hi = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane32_swap(pack_bf16x2(x[2] * inv, x[3] * inv),
                                                                                   pack_bf16x2(y[2] * inv, y[3] * inv), false, false));
-  if (live)
-    *reinterpret_cast<uint4*>(a.out + (static_cast<size_t>(row) * a.H + head) * D + 8 * (f + (lane >> 5))) =
-        make_uint4(lo[0], hi[0], lo[1], hi[1]);
+  return u32x4_t{lo[0], hi[0], lo[1], hi[1]};
 }
 
-// Writes a wave's rows, o / sum (rows that saw nothing are zero).
+// Writes a wave's rows, o / sum (rows that saw nothing are zero), to out [T, H, D] of the kernel's arguments.
 template <int D, class Args>
 __device__ __forceinline__ void write_rows(const Args& a, bool live, int row, int head, int lane, float sum,
                                            const f32x4_t (&o)[D / 8]) {
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-  for (int f = 0; f < D / 8; f += 2) write_pair<D>(a, live, row, head, f, lane, inv, o[f], o[f + 1]);
+  for (int f = 0; f < D / 8; f += 2) {
+    const u32x4_t w = row_pair(inv, o[f], o[f + 1]);
+    if (live) *reinterpret_cast<u32x4_t*>(a.out + (static_cast<size_t>(row) * a.H + head) * D + 8 * (f + (lane >> 5))) = w;
+  }
 }
 
-// Joins a tile's `count` parts, from worker `first` on, and writes the result; part `mine` is this
-// workgroup's own, in registers.  Parts are taken in order, one at a time: there are registers for one
-// part's fragments beside the sums, so each part's loads are waited for before the next one's are sent.
-template <int D, class Args>
-__device__ __forceinline__ void join_parts(const Args& a, const KvPartials& part, int first, int count, int mine,
-                                           int wave, int lane, bool live, int out_row, int out_head, float own_top,
-                                           float own_sum, const f32x4_t (&own)[D / 8]) {
+// Joins a tile's `count` parts, from worker `first` on, into `own` (channels) and `own_sum`; part `mine` is
+// this workgroup's own, in these registers.  Parts are taken in order, one at a time: there are registers for
+// one part's fragments beside the sums, so each part's loads are waited for before the next one's are sent.
+template <int D, int WAVES>
+__device__ __forceinline__ void join_parts(const KvPartials& part, int first, int count, int mine, int wave, int lane,
+                                           bool live, float own_top, float& own_sum, f32x4_t (&own)[D / 8]) {
   constexpr int kFrags = D / 8;
   const __amdgpu_buffer_rsrc_t ro = make_buffer(part.out, part.out_bytes), rs = make_buffer(part.stats, part.stats_bytes);
   float top = -INFINITY, sum = 0.0f;
@@ -94,13 +90,13 @@ __device__ __forceinline__ void join_parts(const Args& a, const KvPartials& part
       for (int f = 0; f < kFrags; ++f) v[f] = own[f];
     } else {
       const int slot = i == 0 ? 2 * first + 1 : 2 * (first + i);
-      const uint32_t row = static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + (lane & 31);
+      const uint32_t row = static_cast<uint32_t>(slot) * (32 * WAVES) + 32 * wave + (lane & 31);
       const u32x2_t st = __builtin_bit_cast(
           u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(rs, live ? row * 8 : kOutOfRange, 0, kCoherentPolicy));
       const uint32_t mb = st[0], lb = st[1];
       m = __uint_as_float(mb), l = __uint_as_float(lb);
 #pragma unroll
-      for (int f = 0; f < kFrags; ++f) v[f] = load_fragment(ro, live ? part_offset<D>(slot, wave, f, lane) : kOutOfRange);
+      for (int f = 0; f < kFrags; ++f) v[f] = load_fragment(ro, live ? part_offset<D, WAVES>(slot, wave, f, lane) : kOutOfRange);
     }
     const float next = fmaxf(top, m), ref = next == -INFINITY ? 0.0f : next;
     const float x = __builtin_amdgcn_exp2f(top - ref), y = __builtin_amdgcn_exp2f(m - ref);
@@ -111,7 +107,9 @@ __device__ __forceinline__ void join_parts(const Args& a, const KvPartials& part
 #pragma unroll
       for (int j = 0; j < 4; ++j) acc[f][j] = acc[f][j] * x + v[f][j] * y;
   }
-  write_rows<D>(a, live, out_row, out_head, lane, sum, acc);
+  own_sum = sum;
+#pragma unroll
+  for (int f = 0; f < kFrags; ++f) own[f] = acc[f];
 }
 
 }  // namespace w4a16

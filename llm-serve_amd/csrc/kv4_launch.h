@@ -90,6 +90,9 @@ struct PromptArgs {
   uint16_t* out;  // [T, H, D] contiguous
   float scale_log2e;
   int T, R, H, KV, D;
+  int group;              // H / KV, and x / group = x * group_inverse >> group_shift for 0 <= x < 2^31
+  uint32_t group_inverse;
+  int group_shift;
   bool zero_tail;
 };
 size_t prompt_attention_workspace(const PromptArgs& a);

@@ -560,15 +560,17 @@ __global__ __launch_bounds__(kPromptThreads, 2) void kv_prompt_kernel(KvAttentio
         const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
         if (live) {
 #pragma unroll
-          for (int f = 0; f < D / 8; ++f) store_fragment(ro, part_offset<D>(slot, wave, f, lane), own[f]);
+          for (int f = 0; f < D / 8; ++f) store_fragment(ro, part_offset<D, kPromptThreads / 64>(slot, wave, f, lane), own[f]);
           if (h == 0) store_stats(rs, (static_cast<uint32_t>(slot) * kKvPromptRows + 32 * wave + col) * 8, row_max, row_sum);
         }
         last = kv_arrive(out.counters + first, count, &s_last);
       } else if (tid == 0) {
         rearm(out.counters + first);
       }
-      if (last)
-        join_parts<D>(a, out, first, count, me - first, wave, lane, live, q.row + token, qh, row_max, row_sum, own);
+      if (last) {
+        join_parts<D, kPromptThreads / 64>(out, first, count, me - first, wave, lane, live, row_max, row_sum, own);
+        write_rows<D>(a, live, q.row + token, qh, lane, row_sum, own);
+      }
       __syncthreads();  // s_last is read by all before the next tile writes it
     }
     u += x1 - x0;

@@ -1506,6 +1506,12 @@ int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stri
   a.v = v, a.v_stride_t = v_stride_t, a.v_stride_h = v_stride_h;
   a.cu_query_lens = cu_query_lens, a.out = out, a.scale_log2e = scale_log2e;
   a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.zero_tail = zero_tail != 0;
+  // x / group as a product: with 2^l >= group the inverse's error, below 1, times x < 2^31 stays below 2^(31 + l).
+  a.group = H / KV;
+  int l = 0;
+  while (1 << l < a.group) ++l;
+  a.group_shift = 31 + l;
+  a.group_inverse = static_cast<uint32_t>(((uint64_t(1) << a.group_shift) + a.group - 1) / a.group);
   const size_t need = w4a16::prompt_attention_workspace(a);
   if (!workspace || workspace_bytes < need)
     return fail(W4A16_ERR_WORKSPACE, "attention needs %zu bytes of workspace (got %zu)", need, workspace ? workspace_bytes : size_t(0));
