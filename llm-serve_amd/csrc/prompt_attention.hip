@@ -32,6 +32,7 @@ __device__ __forceinline__ int by_group(const PromptArgs& a, int x) {
 // One sequence, safe whatever the offsets hold.
 struct Sequence {
   int row, n;  // first packed row, length
+  bool decreases;
 };
 
 __device__ __forceinline__ Sequence sequence(const PromptArgs& a, int r) {
@@ -39,6 +40,7 @@ __device__ __forceinline__ Sequence sequence(const PromptArgs& a, int r) {
   Sequence s;
   s.row = min(max(lo, 0), a.T);
   s.n = max(min(hi, a.T) - s.row, 0);
+  s.decreases = hi < lo;
   return s;
 }
 
@@ -74,47 +76,45 @@ __device__ __forceinline__ int swizzle(int row) {
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
 }
-// The same from an address of each lane's own.
-__device__ __forceinline__ void load_row(const void* from, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(to) : "memory");
-}
 template <int LATER>
 __device__ __forceinline__ void wait_loads() {  // but for the last LATER ones; loads to LDS complete in order
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
 }
 
-// A value that is no number would reach rows that do not see its key (0 * NaN in the second product).  Each
-// thread makes such values of its 16 bytes of each KiB zeros; whether there were any.  The kernel adds them
-// to the rows that see them.  All threads call it; `flags` is a word a wave.
+// A value that is no number would reach rows that do not see its key (0 * NaN in the second product).  Where a
+// tile is masked, each wave looks through its loads' part of the values (`found` in its flag) ...
 template <int BYTES, int WAVES>
-__device__ __forceinline__ bool clean_values(uint8_t (&tile)[BYTES], int (&flags)[WAVES], int wave, int lane) {
-  constexpr int kEach = BYTES / WAVES / 1024;
-  bool found = false;
+__device__ __forceinline__ void look_through(const uint8_t* tile, int (&flags)[WAVES], int wave, int lane) {
+  typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
+  u16x2_t top = {0, 0};
 #pragma unroll
-  for (int j = 0; j < kEach; ++j) {
-    uint4* p = reinterpret_cast<uint4*>(&tile[(wave * kEach + j) * 1024 + lane * 16]);
-    const uint4 v = *p;
-    uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    bool here = false;
+  for (int j = 0; j < BYTES / WAVES / 1024; ++j) {
+    const uint4 v = *reinterpret_cast<const uint4*>(&tile[(wave * (BYTES / WAVES / 1024) + j) * 1024 + lane * 16]);
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) here |= ((w[i] & 0x7F80u) == 0x7F80u) | ((w[i] & 0x7F800000u) == 0x7F800000u);
-    if (here) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if ((w[i] & 0x7F80u) == 0x7F80u) w[i] &= 0xFFFF0000u;
-        if ((w[i] & 0x7F800000u) == 0x7F800000u) w[i] &= 0xFFFFu;
-      }
-      *p = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    found |= here;
+    for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, w[i] & 0x7FFF7FFFu));
   }
-  found = __any(found);
+  const bool found = __any((top[0] >= 0x7F80) | (top[1] >= 0x7F80));
   if (lane == 0) flags[wave] = found;
-  __syncthreads();
+}
+
+// ... and if any wave found one, they become zeros, and the kernel adds them to the rows that see them.  All
+// threads call it, behind a barrier that follows look_through.
+template <int BYTES, int WAVES>
+__device__ __forceinline__ bool clean_values(uint8_t* tile, const int (&flags)[WAVES], int wave, int lane) {
   int any = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) any |= flags[w];
-  return uniform(any) != 0;
+  if (__builtin_expect(uniform(any) == 0, 1)) return false;
+  for (int j = 0; j < BYTES / WAVES / 1024; ++j) {
+    uint32_t* p = reinterpret_cast<uint32_t*>(&tile[(wave * (BYTES / WAVES / 1024) + j) * 1024 + lane * 16]);
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = p[i];
+      p[i] = ((w & 0x7F80u) == 0x7F80u ? 0 : w & 0xFFFFu) | ((w & 0x7F800000u) == 0x7F800000u ? 0 : w & 0xFFFF0000u);
+    }
+  }
+  __syncthreads();
+  return true;
 }
 
 // The lane's number, formed anew: what depends on it is then formed where it is used, and takes no registers
@@ -143,18 +143,18 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
   // Each lane has a sequence of the first 64; more are gone through in turn.
   const Sequence mine = sequence(a, min(lane, a.R - 1));
   KvTileCosts my_costs = tile_costs<kRows>(a, mine, false);
-  bool bad = kv_decreases(a, min(lane, a.R - 1));
+  bool bad = mine.decreases;
   int sum = lane < a.R ? my_costs.before(my_costs.tiles) * a.KV : 0, tiles = lane < a.R ? my_costs.tiles * a.KV : 0;
   int longest = my_costs.tiles > 0 ? my_costs.of(my_costs.tiles - 1) : 0;
   for (int r = 64 + lane; r < a.R; r += 64) {
-    bad |= kv_decreases(a, r);
-    const KvTileCosts c = tile_costs<kRows>(a, sequence(a, r), false);
+    const Sequence s = sequence(a, r);
+    bad |= s.decreases;
+    const KvTileCosts c = tile_costs<kRows>(a, s, false);
     sum += c.before(c.tiles) * a.KV;
     tiles += c.tiles * a.KV;
     if (c.tiles > 0) longest = max(longest, c.of(c.tiles - 1));
   }
   bad = __any(bad);
-  if (a.zero_tail) kv_zero_unowned(a, bad);
   int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   longest = wave_max(longest);
@@ -163,12 +163,16 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     total = all_tiles;
     my_costs.first = 1, my_costs.step = 0;
   }
-  const int least = whole ? 1 : max(kMinShare, longest / kMaxParts);
-  const int workers = total > 0 ? min(static_cast<int>(gridDim.x), (total - 1) / least + 1) : 0;
+  int workers = total;
+  if (!whole) workers = total > 0 ? min(static_cast<int>(gridDim.x), (total - 1) / max(kMinShare, longest / kMaxParts) + 1) : 0;
   const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);
   const int me = static_cast<int>(blockIdx.x & 7) * per_xcd + turn;
-  if (bad | (turn >= per_xcd) | (me >= workers)) return;
-  const KvShares shares{uniform(total / workers), uniform(total % workers)};
+  if (bad | (turn >= per_xcd) | (me >= workers)) {
+    if (a.zero_tail) kv_zero_unowned(a, bad);
+    return;
+  }
+  KvShares shares{1, 0};
+  if (!whole) shares = KvShares{uniform(total / workers), uniform(total % workers)};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
   // The sequence that the share begins in, and the units before it.
   int r = 0, base = 0;
@@ -264,14 +268,38 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     issue_v(t0);
     // The wave's 32 rows: queries as the second operand, and what they see.
     const int first_row = row0 + 32 * wave;
-#pragma unroll
-    for (int j = 0; j < 32 * kPitch / 1024; ++j) {
+    // The wave's rows as whole memory rows: a lane's 16 bytes of row j kEach + lane / (chunks of a row), and where
+    // that row lies, a token and a head of the group, from the tile's first token and head on.
+    constexpr int kEach = 1024 / kPitch, kChunks = kPitch / 16;
+    const int token0 = uniform(by_group(a, row0)), last_row = row0 + rows - 1;
+    const int skip = uniform(by_group(a, kEach)), skip_heads = kEach - skip * group;
+    struct Place {
+      int row, token, head;
+    };
+    auto first_place = [&](int lane) {
+      const int row = first_row + lane / kChunks, token = by_group(a, row);
+      return Place{row, token - token0, row - token * group};
+    };
+    auto next_place = [&](Place& p) {
+      p.row += kEach;
+      p.token += skip;
+      p.head += skip_heads;
+      if (p.head >= group) p.head -= group, ++p.token;
+    };
+    {
+      const uint32_t by_token = 2 * a.q_stride_t, by_head = 2 * a.q_stride_h;
+      const uint16_t* from = a.q + (q.row + token0) * a.q_stride_t + head * group * a.q_stride_h;
+      const int last_token = by_group(a, last_row);
+      const uint32_t last = (last_token - token0) * by_token + (last_row - last_token * group) * by_head;
       const int lane = lane_again();
-      const int r0 = j * (1024 / kPitch) + lane / (kPitch / 16), from_row = min(first_row + r0, row0 + rows - 1);
-      const int t = by_group(a, from_row);
-      const uint32_t chunk = (lane % (kPitch / 16)) ^ (r0 & (kPitch / 16 - 1));
-      load_row(a.q + (q.row + t) * a.q_stride_t + (head * group + from_row - t * group) * a.q_stride_h + chunk * 8,
-               rows_at(t0 + 1) + j * 1024);
+      Place p = first_place(lane);
+#pragma unroll
+      for (int j = 0; j < 32 / kEach; ++j) {
+        const uint32_t chunk = (lane % kChunks) ^ ((lane / kChunks + j * kEach) & (kChunks - 1));
+        const uint32_t at = p.row <= last_row ? p.token * by_token + p.head * by_head : last;
+        load_to_lds(from, at + chunk * 16, rows_at(t0 + 1) + j * 1024);
+        next_place(p);
+      }
     }
     // keys that this lane's row sees (none where there is no row)
     auto sees = [&]() {
@@ -321,8 +349,15 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       barrier();
       issue_k(kt + 1);
       issue_v(kt + 1);
-      const bool broken = key0 + kKeys > tile_sees && clean_values(s_tiles[kt & 1][1], s_bad, wave, lane);
-      if (key0 >= any_sees) continue;
+      const bool masked = key0 + kKeys > tile_sees;
+      if (masked) look_through<kTileBytes, WAVES>(s_tiles[kt & 1][1], s_bad, wave, lane);
+      if (key0 >= any_sees) {
+        if (masked) {
+          __syncthreads();
+          clean_values<kTileBytes, WAVES>(s_tiles[kt & 1][1], s_bad, wave, lane);
+        }
+        continue;
+      }
       const uint32_t k_at = k_read + (kt & 1) * 2 * kTileBytes, v_at = v_read + (kt & 1) * 2 * kTileBytes;
       bf16x8_t ring[kRing];
       f32x16_t sc[2];
@@ -337,6 +372,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
         if (i + kRing - 1 < 2 * kSteps) ring[(i + kRing - 1) % kRing] = read_k(k_at, i + kRing - 1);
         __builtin_amdgcn_sched_barrier(0);
         sc[i / kSteps] = mfma32(ring[i % kRing], qf[i % kSteps], sc[i / kSteps]);
+      }
+      bool broken = false;
+      if (masked) {
+        __syncthreads();
+        broken = clean_values<kTileBytes, WAVES>(s_tiles[kt & 1][1], s_bad, wave, lane);
       }
       // the values' first fragments are read beside the softmax
 #pragma unroll
@@ -451,21 +491,21 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       const uint32_t rows_lds = rows_at(t1), at = rows_lds + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
 #pragma unroll
       for (int f = 0; f < D / 8; f += 2) *(lds_u32x4_t*)static_cast<uintptr_t>(at ^ (16 * f)) = row_pair(inv, own[f], own[f + 1]);
-      const int r0 = lane / (kPitch / 16);
+      char* to = reinterpret_cast<char*>(a.out + (static_cast<int64_t>(q.row + token0) * a.H + head * group) * D);
+      Place p = first_place(lane);
 #pragma unroll
-      for (int j = 0; j < 32 * kPitch / 1024; ++j) {
+      for (int j = 0; j < 32 / kEach; ++j) {
         const u32x4_t w = *(const lds_u32x4_t*)static_cast<uintptr_t>(rows_lds + j * 1024 + lane * 16);
-        const int r = r0 + j * (1024 / kPitch), to_row = first_row + r;
-        const int t = by_group(a, to_row);
-        const int chunk = (lane % (kPitch / 16)) ^ (r & (kPitch / 16 - 1));
-        if (32 * wave + r < rows)
-          *reinterpret_cast<u32x4_t*>(a.out + (static_cast<int64_t>(q.row + t) * a.H + head * group + to_row - t * group) * D + chunk * 8) = w;
+        const uint32_t chunk = (lane % kChunks) ^ ((lane / kChunks + j * kEach) & (kChunks - 1));
+        if (p.row <= last_row) *reinterpret_cast<u32x4_t*>(to + (static_cast<uint32_t>(p.token * a.H + p.head) * kPitch + chunk * 16)) = w;
+        next_place(p);
       }
     }
     __syncthreads();  // all are done with this tile's LDS
     u += x1 - x0;
   }
   wait_loads<0>();  // none may land when the workgroup's LDS is another's
+  if (a.zero_tail) kv_zero_unowned(a, false);
 }
 
 template <int D, int WAVES>

@@ -1461,7 +1461,7 @@ static int validate_prompts(int T, int R, int H, int KV, int D) {
   if (H <= 0 || KV <= 0 || H % KV) return fail(W4A16_ERR_SHAPE, "query heads (%d) must be a multiple of kv heads (%d)", H, KV);
   if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
   if (T == 0 || R == 0) return W4A16_OK;
-  if (static_cast<int64_t>(T) * H > 0x3FFFFFFF)
+  if (H > 1 << 14 || static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
   // The kernel counts its work in 32 bits.  Tile j of a sequence's m costs ceil(64 / group) (j + 1) + 32, and
   // m <= rows / 256 + 1: the last costs at most T / 4 + rows / 256 + 98, the mean of all half of that and 50.
@@ -1494,11 +1494,12 @@ int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stri
   if ((e = validate_kv_rows("q", q, q_stride_t, q_stride_h)) != W4A16_OK) return e;
   if ((e = validate_kv_rows("k", k, k_stride_t, k_stride_h)) != W4A16_OK) return e;
   if ((e = validate_kv_rows("v", v, v_stride_t, v_stride_h)) != W4A16_OK) return e;
-  // The 64 keys of a tile are addressed by 32-bit byte offsets.
-  constexpr int64_t kMostStride = 1 << 24;
-  if (k_stride_t < 0 || v_stride_t < 0 || k_stride_t > kMostStride || v_stride_t > kMostStride)
-    return fail(W4A16_ERR_SHAPE, "rows of k and v must be 0 to 2^24 elements apart (got %lld and %lld)",
-                static_cast<long long>(k_stride_t), static_cast<long long>(v_stride_t));
+  // A tile's 64 keys and the 257 tokens that 256 rows may span are addressed by 32-bit byte offsets.
+  constexpr int64_t kMostStride = 1 << 22;
+  if (q_stride_t < 0 || k_stride_t < 0 || v_stride_t < 0 || q_stride_t > kMostStride || k_stride_t > kMostStride ||
+      v_stride_t > kMostStride || q_stride_h < 0 || q_stride_h > kMostStride * 64 / (H / KV))
+    return fail(W4A16_ERR_SHAPE, "rows of q, k and v must be 0 to 2^22 elements apart (got %lld, %lld and %lld), a group of q's heads within 2^28",
+                static_cast<long long>(q_stride_t), static_cast<long long>(k_stride_t), static_cast<long long>(v_stride_t));
   if (!aligned(out, 16)) return fail(W4A16_ERR_ALIGN, "out must be 16-byte aligned");
   w4a16::PromptArgs a{};
   a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;

@@ -34,7 +34,7 @@ import torch
 from torch import nn
 
 from .._lib import _current_device, _current_stream, lib
-from .rotary_embedding import _head_rows, norm_weight, rope_operands
+from .rotary_embedding import _head_rows, rope_operands, rope_ready
 
 __all__ = ("Attention", "KVStep", "append_kv_int4", "attention_int4", "attention_prompt", "kv_step", "load_kv_int4",
            "new_kv_cache_int4", "store_kv_int4")
@@ -46,6 +46,7 @@ HEAD_DIMS = (64, 128)
 BLOCK_SIZES = (16, 32, 64, 128, 256)
 MAX_STEP_REQUESTS = 4096
 MAX_STEP_TOKENS = 1 << 18
+MAX_PROMPT_STRIDE = 1 << 22  # elements between rows, whose offsets the prompt kernel forms in 32 bits
 MAX_SCALE = 2.3e38  # times log2(e), the kernels' multiplier, it is finite in 32 bits
 
 
@@ -229,18 +230,21 @@ def append_kv_int4(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: tor
     kv_heads, index = cache.shape[1], cache.get_device()
     if q.get_device() != index:
         raise ValueError("KV queries must be a bfloat16 tensor on the cache's GPU")
-    q, k, positions, table = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
-    q_weight, k_weight = norm_weight(q_weight), norm_weight(k_weight)
-    if q.shape[2] != head_dim or k.shape[1] != kv_heads:
+    if not rope_ready(q, k, positions, table, q_weight, k_weight, eps):
+        q, k, positions, table, q_weight, k_weight = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
+    shape, kshape = q.shape, k.shape
+    if shape[2] != head_dim or kshape[1] != kv_heads:
         raise ValueError(f"KV keys must be [tokens, {kv_heads}, {head_dim}] and queries [tokens, heads, {head_dim}]")
     v = _rows("values", v, kv_heads, head_dim, cache)
     if slots.dtype is not _I32 or slots.get_device() != index:
         _require_int32(cache.device, slots=slots)
-    if v.shape != k.shape or slots.shape != k.shape[:1]:
+    if v.shape != kshape or slots.shape != kshape[:1]:
         raise ValueError("KV keys, values and slots must have one entry a token")
-    q_out = torch.empty(q.shape, dtype=_BF16, device=cache.device)
-    k_out = torch.empty(k.shape, dtype=_BF16, device=cache.device) if return_keys else None
-    if q.shape[0] > 0:
+    q_out = torch.empty_strided(shape, (shape[1] * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    k_out = None
+    if return_keys:
+        k_out = torch.empty_strided(kshape, (kv_heads * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    if shape[0] > 0:
         lib().kv_append(q, k, v, cache, slots.contiguous(), positions, table, q_weight, k_weight, eps, q_out, k_out,
                         block_size)
     return (q_out, k_out) if return_keys else q_out
@@ -407,23 +411,21 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query
     is checked and otherwise free.  Offsets that decrease name no rows at all.  Without ``out``
     (contiguous, of q's shape), rows of no request are zero; in ``out`` they are left as they were.
     ``out`` may be q itself, and overlaps no other operand."""
-    index, head_dim = q.get_device(), q.shape[2] if q.ndim == 3 else 0
-    if index < 0:
-        raise ValueError("attention_prompt's queries must be on a GPU (HIP) device")
-    if head_dim not in HEAD_DIMS:
-        raise ValueError(f"attention_prompt's queries must be [rows, heads, head_dim] with head_dim in {HEAD_DIMS}")
-    q = _head_rows("queries", q, None, head_dim, index)
-    k = _head_rows("keys", k, None, head_dim, index)
-    rows, heads, _ = q.shape
-    kv_heads = k.shape[1]
-    v = _head_rows("values", v, kv_heads, head_dim, index)
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError("queries, keys and values must have one entry a row")
-    if heads < 1 or kv_heads < 1 or heads % kv_heads:
-        raise ValueError(f"query heads ({heads}) must be a multiple of kv heads ({kv_heads})")
-    if (cu_query_lens.dtype is not _I32 or cu_query_lens.get_device() != index or cu_query_lens.ndim != 1
-            or cu_query_lens.shape[0] < 2):
-        raise ValueError("cu_query_lens must be an int32 [requests + 1] tensor, of at least one request, on the queries' GPU")
+    # One expression accepts what all the checks accept; only what it does not goes through them.
+    shape, kshape, index = q.shape, k.shape, q.get_device()
+    if not (index >= 0 and len(shape) == 3 and len(kshape) == 3 and v.shape == kshape and shape[2] in HEAD_DIMS
+            and kshape[2] == shape[2] and kshape[0] == shape[0] and kshape[1] > 0 and shape[1] > 0
+            and shape[1] % kshape[1] == 0
+            and q.dtype is _BF16 and k.dtype is _BF16 and v.dtype is _BF16
+            and k.get_device() == index and v.get_device() == index
+            and _in_place(q.stride()) and _in_place(k.stride()) and _in_place(v.stride())
+            and q.stride(1) * shape[1] <= 64 * MAX_PROMPT_STRIDE
+            and (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16 == 0
+            and cu_query_lens.dtype is _I32 and cu_query_lens.get_device() == index
+            and len(cu_query_lens.shape) == 1 and cu_query_lens.shape[0] > 1 and cu_query_lens.is_contiguous()):
+        q, k, v, cu_query_lens = _check_prompt(q, k, v, cu_query_lens)
+        shape, kshape = q.shape, k.shape
+    rows, heads, head_dim = shape
     if scale is None:
         scale = head_dim ** -0.5
     elif not 0.0 < scale < MAX_SCALE:
@@ -432,15 +434,44 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query
         raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
     zero_tail = out is None
     if out is None:
-        out = torch.empty((rows, heads, head_dim), dtype=_BF16, device=q.device)
-    elif (out.shape != q.shape or out.dtype is not _BF16 or out.get_device() != index or not out.is_contiguous()
+        out = torch.empty_strided(shape, (heads * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    elif (out.shape != shape or out.dtype is not _BF16 or out.get_device() != index or not out.is_contiguous()
           or out.data_ptr() % 16):
         raise ValueError("attention out must be a contiguous, 16-byte aligned bfloat16 tensor of q's shape")
     if rows > 0:
-        size = _prompt_workspace_bytes(rows, cu_query_lens.shape[0] - 1, heads, kv_heads, head_dim)
+        size = _prompt_workspace_bytes(rows, cu_query_lens.shape[0] - 1, heads, kshape[1], head_dim)
         workspace, counters = SCRATCH.get(index, size)
-        lib().prompt_attention(q, k, v, cu_query_lens.contiguous(), out, scale, zero_tail, workspace, counters)
+        lib().prompt_attention(q, k, v, cu_query_lens, out, scale, zero_tail, workspace, counters)
     return out
+
+
+def _in_place(strides: tuple[int, int, int]) -> bool:
+    """Whether the prompt kernel reads rows of these strides where they are."""
+    s0, s1, s2 = strides
+    return s2 == 1 and (s0 | s1) % 8 == 0 and s0 <= MAX_PROMPT_STRIDE
+
+
+def _check_prompt(q, k, v, cu_query_lens):
+    """The argument errors of ``attention_prompt``; its arguments as the kernel reads them."""
+    index, head_dim = q.get_device(), q.shape[2] if q.ndim == 3 else 0
+    if index < 0:
+        raise ValueError("attention_prompt's queries must be on a GPU (HIP) device")
+    if head_dim not in HEAD_DIMS:
+        raise ValueError(f"attention_prompt's queries must be [rows, heads, head_dim] with head_dim in {HEAD_DIMS}")
+    q = _head_rows("queries", q, None, head_dim, index)
+    k = _head_rows("keys", k, None, head_dim, index)
+    v = _head_rows("values", v, k.shape[1], head_dim, index)
+    if k.shape[0] != q.shape[0] or v.shape[0] != q.shape[0]:
+        raise ValueError("queries, keys and values must have one entry a row")
+    heads, kv_heads = q.shape[1], k.shape[1]
+    if heads < 1 or kv_heads < 1 or heads % kv_heads:
+        raise ValueError(f"query heads ({heads}) must be a multiple of kv heads ({kv_heads})")
+    if (cu_query_lens.dtype is not _I32 or cu_query_lens.get_device() != index or cu_query_lens.ndim != 1
+            or cu_query_lens.shape[0] < 2):
+        raise ValueError("cu_query_lens must be an int32 [requests + 1] tensor, of at least one request, on the queries' GPU")
+    q, k, v = (t if t.stride(0) <= MAX_PROMPT_STRIDE and t.stride(1) * t.shape[1] <= 64 * MAX_PROMPT_STRIDE
+               else t.clone(memory_format=torch.contiguous_format) for t in (q, k, v))
+    return q, k, v, cu_query_lens.contiguous()
 
 
 class Attention(nn.Module):

@@ -19,7 +19,7 @@ from .._lib import lib
 
 __all__ = ("RotaryEmbedding", "qk_norm_rope", "rotary_table")
 
-_BF16 = torch.bfloat16
+_BF16, _I32, _F32 = torch.bfloat16, torch.int32, torch.float32
 HEAD_DIMS = (64, 128)
 MAX_HEADS = 0xFFFF
 
@@ -54,8 +54,36 @@ def _head_rows(name: str, t: torch.Tensor, heads: int | None, head_dim: int, ind
     return t
 
 
+def rope_ready(q, k, positions, table, q_weight, k_weight, eps) -> bool:
+    """Whether the kernel can read all operands as they are: one expression accepts what ``rope_operands``
+    accepts, but for what it has to copy; a call with few rows is over in less time than its checks."""
+    shape, kshape, tshape, index = q.shape, k.shape, table.shape, q.get_device()
+    if not (index >= 0 and len(shape) == 3 and len(kshape) == 3 and len(tshape) == 2):
+        return False
+    tokens, heads, head_dim = shape
+    count, rotary = tshape
+    q0, q1, q2 = q.stride()
+    k0, k1, k2 = k.stride()
+    return (head_dim in HEAD_DIMS and kshape[2] == head_dim and kshape[0] == tokens
+            and 0 < heads <= MAX_HEADS and 0 < kshape[1] <= MAX_HEADS
+            and q.dtype is _BF16 and k.dtype is _BF16 and k.get_device() == index
+            and q2 == 1 and k2 == 1 and (q0 | q1 | k0 | k1) % 8 == 0
+            and (q.data_ptr() | k.data_ptr() | table.data_ptr()) % 16 == 0
+            and positions.dtype is _I32 and positions.get_device() == index and positions.shape == (tokens,)
+            and positions.is_contiguous()
+            and table.dtype is _F32 and table.get_device() == index and table.is_contiguous()
+            and 0 < count < 1 << 31 and 0 < rotary <= head_dim and rotary % 16 == 0
+            and (q_weight is None or (q_weight.dtype is _BF16 and q_weight.get_device() == index
+                                      and q_weight.shape == (head_dim,) and q_weight.is_contiguous()
+                                      and q_weight.data_ptr() % 16 == 0))
+            and (k_weight is None or (k_weight.dtype is _BF16 and k_weight.get_device() == index
+                                      and k_weight.shape == (head_dim,) and k_weight.is_contiguous()
+                                      and k_weight.data_ptr() % 16 == 0))
+            and 0.0 <= eps <= 3.4e38)
+
+
 def rope_operands(q, k, positions, table, q_weight, k_weight, eps):
-    """The checks that the rotating calls share; (q, k, positions, table) as the kernel reads them."""
+    """The argument errors of the rotating calls; their operands as the kernel reads them."""
     index = q.get_device()
     if index < 0:
         raise ValueError("queries must be on a GPU (HIP) device")
@@ -69,9 +97,9 @@ def rope_operands(q, k, positions, table, q_weight, k_weight, eps):
         raise ValueError("queries and keys must have one row a token")
     if not (0 < q.shape[1] <= MAX_HEADS and 0 < k.shape[1] <= MAX_HEADS):
         raise ValueError(f"queries and keys must have 1 to {MAX_HEADS} heads")
-    if positions.dtype is not torch.int32 or positions.get_device() != index or positions.shape != (tokens,):
+    if positions.dtype is not _I32 or positions.get_device() != index or positions.shape != (tokens,):
         raise ValueError("positions must be an int32 [tokens] tensor on the queries' GPU")
-    if (table.dtype is not torch.float32 or table.get_device() != index or table.ndim != 2 or table.shape[0] < 1
+    if (table.dtype is not _F32 or table.get_device() != index or table.ndim != 2 or table.shape[0] < 1
             or table.shape[1] < 16 or table.shape[1] % 16 or table.shape[1] > head_dim):
         raise ValueError("the rotary table must be a float32 [positions, rotary_dim] tensor on the queries' GPU, rotary_dim "
                          "a multiple of 16 up to head_dim")
@@ -84,13 +112,12 @@ def rope_operands(q, k, positions, table, q_weight, k_weight, eps):
             raise ValueError("norm weights must be bfloat16 [head_dim] tensors on the queries' GPU")
     if not 0.0 <= eps <= 3.4e38:
         raise ValueError(f"eps must be finite and not negative (got {eps})")
-    return q, k, positions.contiguous(), table
+    return q, k, positions.contiguous(), table, _weight(q_weight), _weight(k_weight)
 
 
-def norm_weight(w: torch.Tensor | None) -> torch.Tensor | None:
-    """The weight as the kernel reads it: contiguous and 16-byte aligned."""
-    if w is not None and (w.stride(0) != 1 or w.data_ptr() % 16):
-        w = w.detach().clone(memory_format=torch.contiguous_format)
+def _weight(w: torch.Tensor | None) -> torch.Tensor | None:
+    if w is not None and (not w.is_contiguous() or w.data_ptr() % 16):
+        w = w.clone(memory_format=torch.contiguous_format)
     return w
 
 
@@ -105,11 +132,13 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     i + rotary_dim / 2, and channels from rotary_dim on keep their place.  A row whose position the table
     does not have becomes NaN.  All steps are fp32, each rounded by itself (the sum of squares is fp64),
     and the result is rounded to bf16 once, where the reference rounds after each norm's step too."""
-    q, k, positions, table = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
-    q_weight, k_weight = norm_weight(q_weight), norm_weight(k_weight)
-    q_out = torch.empty(q.shape, dtype=_BF16, device=q.device)
-    k_out = torch.empty(k.shape, dtype=_BF16, device=q.device)
-    if q.shape[0] > 0:
+    if not rope_ready(q, k, positions, table, q_weight, k_weight, eps):
+        q, k, positions, table, q_weight, k_weight = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
+    shape, kshape, index = q.shape, k.shape, q.get_device()
+    head_dim = shape[2]
+    q_out = torch.empty_strided(shape, (shape[1] * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    k_out = torch.empty_strided(kshape, (kshape[1] * head_dim, head_dim, 1), dtype=_BF16, device=index)
+    if shape[0] > 0:
         lib().qk_norm_rope(q, k, positions, table, q_weight, k_weight, eps, q_out, k_out)
     return q_out, k_out
 

@@ -62,7 +62,7 @@ def test_append_refusals(pkg, dll, change, status, message):
     ({"KV": 0}, 2, "multiple"), ({"D": 256}, 2, "head size"), ({"scale": ctypes.c_float(0.0)}, 1, "scale"),
     ({"scale": ctypes.c_float(float("nan"))}, 1, "scale"), ({"scale": ctypes.c_float(3e38)}, 1, "scale"),
     ({"q": P + 8}, 3, "aligned"), ({"kt": 4}, 3, "multiples of 8"), ({"vh": 12}, 3, "multiples of 8"), ({"out": P + 8}, 3, "aligned"),
-    ({"kt": (1 << 24) + 8}, 2, "2^24"), ({"vt": -8}, 2, "2^24"), ({"ws": None}, 4, "workspace"), ({"ws_bytes": 64}, 4, "workspace"),
+    ({"kt": (1 << 22) + 8}, 2, "2^22"), ({"vt": -8}, 2, "2^22"), ({"qt": 1 << 23}, 2, "2^22"), ({"qh": 1 << 27}, 2, "2^28"), ({"H": 32768, "KV": 1}, 2, "too many"), ({"ws": None}, 4, "workspace"), ({"ws_bytes": 64}, 4, "workspace"),
     ({"ws": P + 4}, 3, "aligned"), ({"counters": None}, 4, "counters"), ({"T": 1 << 28}, 2, "too many"),
     ({"T": 1 << 20}, 2, "too much work")])
 def test_prompt_refusals(pkg, dll, change, status, message):
