@@ -44,8 +44,8 @@ struct KvRowsArgs {
 hipError_t launch_kv_store(const KvRowsArgs& a, hipStream_t stream);
 hipError_t launch_kv_load(const KvRowsArgs& a, hipStream_t stream);
 
-// Up to this many tokens a wave of the norm-and-rotation kernel takes one group of heads.
-constexpr int kQkRopeFewTokens = 512;
+// Up to this many tokens a wave of the norm-and-rotation kernel takes one group of heads (qk_rope.hip).
+constexpr int kQkRopeFewTokens = 2048;
 
 struct QkRopeArgs {
   const uint16_t *q, *k, *v;  // [T, H or KV, D] at strides (elements); v only with a cache

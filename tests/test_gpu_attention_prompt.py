@@ -289,3 +289,61 @@ def test_keys_beyond_4_gib_of_a_prompt(gpu_lib):
         off = (out[row, 0].double() - want).abs()
         reach = (k[seen, 0].double().abs() @ q[row, 0].double().abs()).amax().expand(1) * 64 ** -0.5
         assert bool((off <= ora.prompt_tolerance(want[None], spread[None], reach, row)[0]).all())
+
+
+@pytest.mark.parametrize("rows,heads", [(300, 2), (600, 86)])
+def test_rows_at_the_widest_steps(gpu_lib, rows, heads):
+    """Rows of q, k and v 2^22 elements apart, which the kernel steps through, and further, which are copied;
+    a tile of one token a row then spans 2 GiB."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(rows, 3 * heads, 64, generator=gen, device="cuda").to(torch.bfloat16)
+    o = int32([0, rows - 40, rows])
+    want = attn.attention_prompt(*x.split(heads, 1), o)
+    for stride in (1 << 22, (1 << 22) + 8):
+        store = torch.empty(rows, stride, dtype=torch.bfloat16, device="cuda")
+        wide = store[:, :3 * heads * 64].view(rows, 3 * heads, 64)
+        wide.copy_(x)
+        assert torch.equal(attn.attention_prompt(*wide.split(heads, 1), o), want)
+        del wide, store
+    q, k, v = x.split(heads, 1)
+    check(want, q, k, v, [0, rows - 40, rows])
+
+
+def test_heads_far_apart(gpu_lib):
+    """Heads of q up to 2^28 elements apart in a group, and beyond (copied)."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    x = torch.randn(70, 6, 64, generator=gen, device="cuda").to(torch.bfloat16)
+    q, k, v = x.split((4, 1, 1), 1)
+    want = attn.attention_prompt(q, k, v, int32([0, 70]))
+    for apart in (1 << 26, (1 << 26) + 8):
+        store = torch.empty(4 * apart, dtype=torch.bfloat16, device="cuda")
+        far = store.as_strided((70, 4, 64), (64, apart, 1))
+        far.copy_(q)
+        assert torch.equal(attn.attention_prompt(far, k, v, int32([0, 70])), want)
+        del far, store
+
+
+def test_refusals(gpu_lib):
+    """Arguments that the kernel cannot take raise in front of any launch."""
+    q, k, v, offsets = batch([20, 5], 4, 2, 128, seed=51)
+    o = int32(offsets)
+    out = torch.empty(25, 4, 128, dtype=torch.bfloat16, device="cuda")
+    for change in ({"q": q.float()}, {"q": q.cpu()}, {"q": q[..., :96]}, {"q": q[:, :3]}, {"q": q[:24]}, {"q": q[0]},
+                   {"k": k[..., :64]}, {"k": k[:, :0], "v": v[:, :0]}, {"k": k.half()}, {"k": k[:24]}, {"v": v[:, :1]}, {"v": v[:24]},
+                   {"v": v.cpu()}, {"cu_query_lens": o.long()}, {"cu_query_lens": o[:1]}, {"cu_query_lens": o.cpu()},
+                   {"cu_query_lens": o[None]}, {"scale": 0.0}, {"scale": -1.0}, {"scale": float("nan")},
+                   {"scale": float("inf")}, {"max_query_len": 0}, {"out": out[:24]}, {"out": out.float()},
+                   {"out": out.transpose(0, 1).contiguous().transpose(0, 1)}, {"out": out.cpu()}):
+        with pytest.raises(ValueError):
+            attn.attention_prompt(**{**dict(q=q, k=k, v=v, cu_query_lens=o), **change})
+
+
+def test_more_requests_than_lanes(gpu_lib):
+    """Empty places and prompts of one to some tokens, more than a wave looks at in one turn, and a long one
+    behind them."""
+    lengths = ([0, 1, 2, 0, 5] * 60) + [400] + [0] * 70 + [3]
+    for heads, kv_heads, dim in ((8, 2, 128), (3, 3, 64)):
+        q, k, v, offsets = batch(lengths, heads, kv_heads, dim, seed=52, before=3, behind=9)
+        out = attn.attention_prompt(q, k, v, int32(offsets))
+        check(out, q, k, v, offsets)
+        assert not bool(out[:3].any()) and not bool(out[-9:].any())

@@ -173,6 +173,27 @@ def test_append_is_the_two_calls(gpu_lib, heads, kv_heads, dim, tokens, block):
         assert torch.equal(cache, other)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", LAYOUTS)
+@pytest.mark.parametrize("tokens,block", [(2047, 64), (2049, 256), (2501, 16)])
+def test_larger_steps(gpu_lib, heads, kv_heads, dim, tokens, block):
+    """Where a wave takes more of a token's rows, and in front of that."""
+    gen = generator(tokens + heads)
+    q, k, v = rows(gen, tokens, heads, kv_heads, dim)
+    positions = torch.randint(0, 3000, (tokens,), generator=gen, device="cuda", dtype=torch.int32)
+    wq, wk = weight(gen, dim), weight(gen, dim)
+    table = rope.rotary_table(dim, 3000)
+    a, b = rope.qk_norm_rope(q, k, positions, table, q_weight=wq, k_weight=wk)
+    check(a, q, positions, table, dim, wq)
+    check(b, k, positions, table, dim, wk)
+    blocks = tokens // block + 2
+    slots = torch.randperm(blocks * block, generator=gen, device="cuda")[:tokens].to(torch.int32)
+    cache, other = (attn.new_kv_cache_int4(blocks, block, kv_heads, dim) for _ in range(2))
+    attn.store_kv_int4(b, v, cache, slots, block_size=block)
+    c, d = attn.append_kv_int4(q, k, v, other, slots, positions, table, block_size=block, q_weight=wq, k_weight=wk,
+                               return_keys=True)
+    assert torch.equal(a, c) and torch.equal(b, d) and torch.equal(cache, other)
+
+
 def test_no_tokens(gpu_lib):
     q = torch.zeros(0, 4, 128, dtype=torch.bfloat16, device="cuda")
     none = torch.zeros(0, dtype=torch.int32, device="cuda")
@@ -219,3 +240,31 @@ def test_captured_and_on_another_stream(gpu_lib):
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(got, want, again)), i
         assert torch.equal(cache, other) and torch.equal(cache, third), i
+
+
+def test_refusals(gpu_lib):
+    """Arguments that the kernels cannot take raise in front of any launch."""
+    gen = generator(9)
+    q, k, v = rows(gen, 6, 4, 2, 128)
+    positions = torch.arange(6, device="cuda", dtype=torch.int32)
+    table, w = rope.rotary_table(128, 64), weight(gen, 128)
+    cache = attn.new_kv_cache_int4(2, 16, 2, 128)
+    for change in ({"q": q.float()}, {"q": q[..., :96]}, {"q": q[0]}, {"k": k[:5]}, {"k": k[..., :64]}, {"k": k.cpu()},
+                   {"k": k[:, :0]}, {"positions": positions.long()}, {"positions": positions[:5]},
+                   {"positions": positions.cpu()}, {"table": table.half()}, {"table": table[:0]}, {"table": table[:, :8]},
+                   {"table": table[:, :24]}, {"table": torch.cat((table, table), -1)}, {"table": table.cpu()},
+                   {"q_weight": w.float()}, {"k_weight": w[:64]}, {"q_weight": w.cpu()}, {"eps": -1e-6},
+                   {"eps": float("nan")}, {"eps": float("inf")}):
+        args = {**dict(q=q, k=k, positions=positions, table=table), **change}
+        with pytest.raises(ValueError):
+            rope.qk_norm_rope(**args)
+        with pytest.raises(ValueError):
+            attn.append_kv_int4(**{**dict(v=v, cache=cache, slots=positions, block_size=16), **args})
+    for change in ({"v": v[:5]}, {"v": v.float()}, {"v": v[:, :1]}, {"v": v.cpu()}, {"slots": positions[:5]},
+                   {"slots": positions.long()}, {"slots": positions.cpu()}, {"cache": cache[..., :64]}, {"cache": cache.cpu()},
+                   {"cache": attn.new_kv_cache_int4(2, 16, 2, 64)}, {"cache": attn.new_kv_cache_int4(2, 16, 4, 128)},
+                   {"block_size": 32}):
+        with pytest.raises(ValueError):
+            attn.append_kv_int4(**{**dict(q=q, k=k, v=v, cache=cache, slots=positions, positions=positions, table=table,
+                                          block_size=16), **change})
+    assert not bool(cache.any())
