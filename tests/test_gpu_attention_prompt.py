@@ -347,3 +347,30 @@ def test_more_requests_than_lanes(gpu_lib):
         out = attn.attention_prompt(q, k, v, int32(offsets))
         check(out, q, k, v, offsets)
         assert not bool(out[:3].any()) and not bool(out[-9:].any())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(32, 8, 128, [2039]), (86, 86, 64, [300, 333]), (32, 8, 128, [40] * 30)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_values_that_are_no_numbers_in_larger_batches(gpu_lib, heads, kv_heads, dim, lengths, value):
+    """One channel of some values is no number: every row in front of them, every other channel and every
+    other sequence keeps its bits; rows that see one get it."""
+    q, k, v, offsets = batch(lengths, heads, kv_heads, dim, seed=53)
+    v = v.clone()
+    rows, o = q.shape[0], int32(offsets)
+    want = attn.attention_prompt(q, k, v, o)
+    clean = v.clone()
+    spots = [(0, 0, 3), (rows // 3, 1, dim - 1), (rows - 1, kv_heads - 1, 17), (offsets[1] - 1, 0, 40), (rows // 2, 2, 0)]
+    hit = torch.zeros(rows, heads, dim, dtype=torch.bool, device="cuda")
+    group = heads // kv_heads
+    for row, head, channel in spots:
+        v[row, head, channel] = value
+        clean[row, head, channel] = 0
+        end = next(e for e in offsets if e > row)
+        hit[row:end, head * group:(head + 1) * group, channel] = True
+    got = attn.attention_prompt(q, k, v, o)
+    base = attn.attention_prompt(q, k, clean, o)
+    touched = torch.zeros_like(hit)
+    for row, head, channel in spots:
+        touched[:, head * group:(head + 1) * group, channel] = True
+    assert torch.equal(got[~hit], base[~hit]) and torch.equal(got[~touched], want[~touched])
+    assert torch.equal(got[hit].float().nan_to_num(7.0, 8.0, 9.0), torch.full_like(got[hit].float(), value).nan_to_num(7.0, 8.0, 9.0))
