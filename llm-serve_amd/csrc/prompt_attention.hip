@@ -2,23 +2,54 @@
 // lengths, query heads sharing key heads in groups.
 //
 // For row t of a sequence, o = sum_j p_j v_j / sum_j p_j over j <= t with p_j = 2^(c s_j - m), s_j = q k_j
-// and c = scale log2(e), in one pass over the keys with a running reference m.
+// and c = scale log2(e), in one pass over the keys with a running reference m, which follows the largest
+// c s_j where that leads it by more than 8.  All heads of a kv head share its tiles: a row tile holds the
+// (token, head of the group) pairs of one kv head.
+//
+// Scores are formed turned over, S^T = K Q^T, in tiles of 64 keys and 32 rows a wave (v_mfma_f32_32x32x16):
+// a lane then holds 32 keys' scores of one row, its maximum and sum need one exchange with the other half of
+// the wave, and the weights, rounded to bf16, are in place as the second operand of O^T = V^T P^T.  V is read
+// by rows and turned over by ds_read_b64_tr_b16.  Weights are rounded to bf16 because the matrix cores multiply
+// bf16; their sum is of the fp32 values, so that the rounding errors average out in the quotient
+// (error against 64 bits 1.2 times that of a computation in fp32 with one rounding at the end).
+//
+// Keys and values go to LDS by loads that pass no register, a tile ahead (two stages); queries and outputs
+// go through LDS too, so that memory is read and written in whole rows.  A row's channels lie in LDS in an order
+// of their own (swizzle), which spreads neighbouring rows over the banks.
+//
+// One prompt of 16384 rows, 32 + 8 heads of 128 channels (2.2 TFLOP): 2.1 to 2.2 ms, 1000 to 1050 TFLOP/s, 85 %
+// of what large library products of the same data reach (1230 to 1250).  What bounds it there is power: the
+// core clock is 1.9 to 2.0 GHz in the loop, and 2.4 with zeros in place of the data (1150 TFLOP/s).  A wave
+// needs 1024 cycles of matrix instructions for a tile and takes 2000 of a SIMD; loops that overlap one tile's
+// products with another's softmax within a wave need a sixth fewer cycles, at a lower clock: 3 % less time, which
+// they lose again at both ends of a row tile in prompts of a few thousand rows.  Nor is anything gained by waves half a tile apart, by
+// wave priorities, or by a next row tile's first loads beside the present one's last tile (0 to 4 % slower).
+// Short prompts are bound by a chain of latencies: 1 us to find the part, 2 for queries and first tile, 0.7 to
+// 1.2 a tile, 1.2 to write.
 #include "attention_rows.h"
 
 namespace w4a16 {
 namespace {
 
-constexpr int kKeys = 64;        // keys of a tile
-constexpr int kSetupCost = 64;   // of a row tile besides its keys
-constexpr int kRing = 6;         // operand fragments in flight
+constexpr int kKeys = 64;  // keys of a tile
+// Of a row tile besides its keys: finding it, queries, output take as long as four tiles of keys (with half of
+// that in the shares, nine prompts of up to 2500 rows take 313 us instead of 305).
+constexpr int kSetupCost = 4 * kKeyTileCost;
+// Operand fragments in flight between LDS and matrix instructions; 5 or 8 make no difference that shows.
+constexpr int kRing = 6;
+// A worker's least share, and the parts of the longest row tile at most: joining them costs some 3 us, and more
+// with each.
 constexpr int kMinShare = 3 * kKeyTileCost;
 constexpr int kMaxParts = 12;
+// Row tiles of up to this cost are taken whole where each finds a workgroup of its own: 700 rows of 32 + 8 heads
+// take 21 us in whole tiles and 28 in shares.
 constexpr int kShortCost = kSetupCost + 12 * kKeyTileCost;
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4_t;
 typedef __attribute__((address_space(3))) bf16x8_t lds_bf16x8_t;
 typedef __attribute__((address_space(3))) u32x4_t lds_u32x4_t;
+typedef __attribute__((address_space(3))) f32x4_t lds_f32x4_t;
 
 __device__ __forceinline__ f32x16_t mfma32(bf16x8_t a, bf16x8_t b, f32x16_t c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
@@ -54,9 +85,6 @@ __device__ __forceinline__ KvTileCosts tile_costs(const PromptArgs& a, const Seq
   return c;
 }
 
-// Which 16-byte chunk of a row lies where: chunk c of row r is stored at c ^ swizzle(r).  Sixteen
-// neighbouring rows' same chunk (the first product's operand) and four rows' same 64 bytes (the
-// second's) then lie in different banks.
 // A barrier and nothing else: no wait for loads on their way.
 __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
@@ -64,6 +92,9 @@ __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Which 16-byte chunk of a row lies where: chunk c of row r is stored at c ^ swizzle(r).  Sixteen
+// neighbouring rows' same chunk (the first product's operand) and four rows' same 64 bytes (the
+// second's) then lie in different banks.
 template <int D>
 __device__ __forceinline__ int swizzle(int row) {
   return D == 128 ? ((row & 3) << 2) | ((row >> 2) & 3) : ((row & 2) << 1) | ((row >> 2) & 3);
@@ -125,20 +156,28 @@ __device__ __forceinline__ int lane_again() {
   return lane;
 }
 
-template <int D, int WAVES>
+// WAVES waves of 32 rows each, or, with SPLIT 2, half as many rows, each with two waves that take half of every
+// tile's keys and are joined in LDS.
+//
+// Work is dealt out by cost, not by row tile: workers (as many workgroups as the chip holds at once) take equal
+// shares of all row tiles' costs, in order, those of one XCD neighbouring ones; a row tile that a border cuts is
+// joined by the last of its workers to arrive, in the workers' order, so that results do not depend on it.
+template <int D, int WAVES, int SPLIT>
 __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptArgs a, KvPartials out) {
   constexpr int kPitch = 2 * D, kTileBytes = kKeys * kPitch;  // bytes
-  constexpr int kRows = 32 * WAVES, kSteps = D / 16, kTiles = D / 32, kLoads = kTileBytes / WAVES / 1024;
+  constexpr int kRowWaves = WAVES / SPLIT, kRows = 32 * kRowWaves, kMine = kKeys / SPLIT, kSteps = D / 16, kTiles = D / 32, kLoads = kTileBytes / WAVES / 1024;
   // Two stages of a tile of keys and one of values.
   __shared__ __align__(1024) uint8_t s_tiles[2][2][kTileBytes];
   // Queries on their way in and the output on its way out: whole rows in memory, a lane each in the products.
   // Eight waves have a part of LDS for them, four take the stage that is idle at that time.
-  constexpr bool kOwnRows = kRows * kPitch > 2 * kTileBytes;
-  __shared__ __align__(1024) uint8_t s_rows[kOwnRows ? kRows * kPitch : 16];
+  constexpr bool kOwnRows = WAVES * 32 * kPitch > 2 * kTileBytes;
+  __shared__ __align__(1024) uint8_t s_rows[kOwnRows ? WAVES * 32 * kPitch : 16];
+  __shared__ float2 s_join[SPLIT > 1 ? 32 * kRowWaves : 1];
   __shared__ __align__(16) int s_bad[WAVES];
   __shared__ int s_last;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
+  const int row_wave = wave % kRowWaves, key_part = wave / kRowWaves;
   const int group = a.group;
   // Each lane has a sequence of the first 64; more are gone through in turn.
   const Sequence mine = sequence(a, min(lane, a.R - 1));
@@ -211,8 +250,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
   // step of 16 channels; of the values, its four rows' 8 bytes, the others by exclusive or with 64 a step of
   // 32 channels and with 32 for the second four rows, which are 8 rows further.
   const int v_row = 4 * h + ((lane >> 2) & 3);
-  const uint32_t k_read = tiles_lds + col * kPitch + (h ^ swizzle<D>(col)) * 16;
-  const uint32_t v_read = tiles_lds + kTileBytes + v_row * kPitch + ((((lane >> 3) & 2) | ((lane >> 1) & 1)) ^ swizzle<D>(v_row)) * 16 + (lane & 1) * 8;
+  const uint32_t k_read = tiles_lds + (key_part * kMine + col) * kPitch + (h ^ swizzle<D>(col)) * 16;
+  const uint32_t v_read = tiles_lds + kTileBytes + (key_part * kMine + v_row) * kPitch + ((((lane >> 3) & 2) | ((lane >> 1) & 1)) ^ swizzle<D>(v_row)) * 16 + (lane & 1) * 8;
   const float scale = a.scale_log2e;
 
   for (int u = begin; u < end;) {
@@ -267,7 +306,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     issue_k(t0);
     issue_v(t0);
     // The wave's 32 rows: queries as the second operand, and what they see.
-    const int first_row = row0 + 32 * wave;
+    const int first_row = row0 + 32 * row_wave;
     // The wave's rows as whole memory rows: a lane's 16 bytes of row j kEach + lane / (chunks of a row), and where
     // that row lies, a token and a head of the group, from the tile's first token and head on.
     constexpr int kEach = 1024 / kPitch, kChunks = kPitch / 16;
@@ -304,11 +343,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     // keys that this lane's row sees (none where there is no row)
     auto sees = [&]() {
       const int c = lane_again() & 31;
-      return 32 * wave + c < rows ? by_group(a, first_row + c) + 1 : 0;
+      return 32 * row_wave + c < rows ? by_group(a, first_row + c) + 1 : 0;
     };
     // keys that all rows of the wave see, and that some row may; keys that all rows of the tile see
     const int all_see = uniform(by_group(a, first_row)) + 1;
-    const int any_sees = 32 * wave >= rows ? 0 : uniform(by_group(a, row0 + min(32 * wave + 32, rows) - 1)) + 1;
+    const int any_sees = 32 * row_wave >= rows ? 0 : uniform(by_group(a, row0 + min(32 * row_wave + 32, rows) - 1)) + 1;
     const int tile_sees = uniform(by_group(a, row0)) + 1;
 
 
@@ -351,7 +390,8 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       issue_v(kt + 1);
       const bool masked = key0 + kKeys > tile_sees;
       if (masked) look_through<kTileBytes, WAVES>(s_tiles[kt & 1][1], s_bad, wave, lane);
-      if (key0 >= any_sees) {
+      const int my_key0 = key0 + key_part * kMine;
+      if (my_key0 >= any_sees) {
         if (masked) {
           __syncthreads();
           clean_values<kTileBytes, WAVES>(s_tiles[kt & 1][1], s_bad, wave, lane);
@@ -360,16 +400,17 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       }
       const uint32_t k_at = k_read + (kt & 1) * 2 * kTileBytes, v_at = v_read + (kt & 1) * 2 * kTileBytes;
       bf16x8_t ring[kRing];
-      f32x16_t sc[2];
+      constexpr int kHalves = kMine / 32;
+      f32x16_t sc[kHalves];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kHalves; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) sc[n][i] = 0.0f;
 #pragma unroll
       for (int i = 0; i < kRing - 1; ++i) ring[i] = read_k(k_at, i);
 #pragma unroll
-      for (int i = 0; i < 2 * kSteps; ++i) {
-        if (i + kRing - 1 < 2 * kSteps) ring[(i + kRing - 1) % kRing] = read_k(k_at, i + kRing - 1);
+      for (int i = 0; i < kHalves * kSteps; ++i) {
+        if (i + kRing - 1 < kHalves * kSteps) ring[(i + kRing - 1) % kRing] = read_k(k_at, i + kRing - 1);
         __builtin_amdgcn_sched_barrier(0);
         sc[i / kSteps] = mfma32(ring[i % kRing], qf[i % kSteps], sc[i / kSteps]);
       }
@@ -382,25 +423,25 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
 #pragma unroll
       for (int i = 0; i < kRing - 1; ++i) ring[i] = read_v(v_at, i);
       __builtin_amdgcn_sched_barrier(0);
-      if (__builtin_expect(key0 + kKeys > all_see, 0)) {
-        const int lead = sees() - key0 - 4 * (lane_again() >> 5);
+      if (__builtin_expect(my_key0 + kMine > all_see, 0)) {
+        const int lead = sees() - my_key0 - 4 * (lane_again() >> 5);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < kHalves; ++n)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const float y = sc[n][i];
             sc[n][i] = 32 * n + 8 * (i >> 2) + (i & 3) < lead ? y : -INFINITY;
           }
 #pragma unroll
-        for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(sc[n]));
+        for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
       }
       // The scores as whole accumulators on both sides of the branch's end: taken apart, they would be
       // copied on the path that masks nothing.
 #pragma unroll
-      for (int n = 0; n < 2; ++n) asm volatile("" : "+v"(sc[n]));
+      for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
       float top = sc[0][0];
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kHalves; ++n)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, sc[n][i]);
       top = halves_max(top) * scale;
@@ -417,7 +458,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       }
       const float from = row_max == -INFINITY ? 0.0f : -row_max;
       // Weights of 16 keys at a time, beside the products of the 16 before them.
-      constexpr int kPv = 4 * kTiles, kPairs = 4 / kTiles;  // matrix instructions; pairs of weights beside one
+      constexpr int kPv = 2 * kHalves * kTiles, kPairs = 4 / kTiles;  // matrix instructions; pairs of weights beside one
       u32x4_t now, next;
       auto pair = [&](int i, u32x4_t& w) {  // weights 2 i and 2 i + 1 of a lane's 32
         float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], scale, from));
@@ -435,7 +476,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
         __builtin_amdgcn_sched_barrier(0);
         acc[c] = mfma32(ring[i % kRing], __builtin_bit_cast(bf16x8_t, now), acc[c]);
         __builtin_amdgcn_sched_barrier(0);
-        if (s < 3) {
+        if (s < 2 * kHalves - 1) {
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) pair(4 * (s + 1) + c * kPairs + j, next);
         }
@@ -443,7 +484,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
       }
       if (__builtin_expect(broken, 0)) {
         const int see = sees();
-        for (int key = key0; key < min(key0 + kKeys, any_sees); ++key) {
+        for (int key = my_key0; key < min(my_key0 + kMine, any_sees); ++key) {
           const uint16_t* v = v_base + key * a.v_stride_t + 4 * h;
           if (key < see) {
 #pragma unroll
@@ -464,10 +505,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     for (int f = 0; f < D / 8; ++f)
 #pragma unroll
       for (int j = 0; j < 4; ++j) own[f][j] = acc[f >> 2][4 * (f & 3) + j];
+    if (SPLIT > 1) {  // the waves of the tiles' second half hand over what they have, through the idle stage
+      const uint32_t at = tiles_lds + (t1 & 1) * 2 * kTileBytes + row_wave * 64 * kPitch + lane_again() * 16;
+      const int of_row = 32 * row_wave + (lane_again() & 31);
+      if (key_part) {
+#pragma unroll
+        for (int f = 0; f < D / 8; ++f) *(lds_f32x4_t*)static_cast<uintptr_t>(at + f * 1024) = own[f];
+        s_join[of_row] = make_float2(row_max, row_sum);
+      }
+      __syncthreads();
+      if (!key_part) {
+        const float2 with = s_join[of_row];
+        const float top = fmaxf(row_max, with.x), ref = top == -INFINITY ? 0.0f : top;
+        const float x = __builtin_amdgcn_exp2f(row_max - ref), y = __builtin_amdgcn_exp2f(with.x - ref);
+        row_sum = scaled(row_sum, row_max - ref) + scaled(with.y, with.x - ref);
+        row_max = top;
+#pragma unroll
+        for (int f = 0; f < D / 8; ++f) own[f] = own[f] * x + *(const lds_f32x4_t*)static_cast<uintptr_t>(at + f * 1024) * y;
+      }
+    }
     bool last = true;
     if (!complete) {
       const int lane = lane_again();
-      const bool live = 32 * wave + (lane & 31) < rows;
+      const bool live = key_part == 0 && 32 * row_wave + (lane & 31) < rows;
       const int first = shares.owner(u - x0), count = shares.owner(u - x0 + cost - 1) - first + 1;
       // A tile's other parts stand at the beginning of their workgroups' shares and are rarely the last to be done.
       last = x0 == 0 && kv_is_last(out.counters + first, count, &s_last);
@@ -476,19 +536,19 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
         const __amdgpu_buffer_rsrc_t ro = make_buffer(out.out, out.out_bytes), rs = make_buffer(out.stats, out.stats_bytes);
         if (live) {
 #pragma unroll
-          for (int f = 0; f < D / 8; ++f) store_fragment(ro, part_offset<D, WAVES>(slot, wave, f, lane), own[f]);
-          if (lane < 32) store_stats(rs, (static_cast<uint32_t>(slot) * kRows + 32 * wave + lane) * 8, row_max, row_sum);
+          for (int f = 0; f < D / 8; ++f) store_fragment(ro, part_offset<D, kRowWaves>(slot, row_wave, f, lane), own[f]);
+          if (lane < 32) store_stats(rs, (static_cast<uint32_t>(slot) * kRows + 32 * row_wave + lane) * 8, row_max, row_sum);
         }
         last = kv_arrive(out.counters + first, count, &s_last);
       } else if (tid == 0) {
         rearm(out.counters + first);
       }
-      if (last) join_parts<D, WAVES>(out, first, count, me - first, wave, lane, live, row_max, row_sum, own);
+      if (last) join_parts<D, kRowWaves>(out, first, count, me - first, row_wave, lane, live, row_max, row_sum, own);
     }
-    if (last) {
+    if (last && key_part == 0) {
       const float inv = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
       const int lane = lane_again(), c = lane & 31;
-      const uint32_t rows_lds = rows_at(t1), at = rows_lds + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
+      const uint32_t rows_lds = rows_at(t1) + wave * (SPLIT - 1) * 32 * kPitch, at = rows_lds + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
 #pragma unroll
       for (int f = 0; f < D / 8; f += 2) *(lds_u32x4_t*)static_cast<uintptr_t>(at ^ (16 * f)) = row_pair(inv, own[f], own[f + 1]);
       char* to = reinterpret_cast<char*>(a.out + (static_cast<int64_t>(q.row + token0) * a.H + head * group) * D);
@@ -508,12 +568,29 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
   if (a.zero_tail) kv_zero_unowned(a, false);
 }
 
-template <int D, int WAVES>
+template <int D, int WAVES, int SPLIT>
 hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
   constexpr int kWorkers = kKvPromptWorkers * 8 / WAVES;
-  const KvPartials part = partials_at(static_cast<char*>(workspace), counters, kWorkers, 32 * WAVES, D);
-  prompt_attention_kernel<D, WAVES><<<kWorkers, 64 * WAVES, 0, stream>>>(a, part);
+  const KvPartials part = partials_at(static_cast<char*>(workspace), counters, kWorkers, 32 * WAVES / SPLIT, D);
+  prompt_attention_kernel<D, WAVES, SPLIT><<<kWorkers, 64 * WAVES, 0, stream>>>(a, part);
   return hipGetLastError();
+}
+
+template <int D>
+hipError_t launch_for(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
+  const int64_t rows = static_cast<int64_t>(a.T) * a.H;
+  // While row tiles of 64 find a CU each, the longest of them is what takes time: with its keys split between
+  // two waves, one prompt of 511 rows (32 + 8 heads of 128) takes 14.4 us instead of 16.5, one of 700 rows of 16
+  // heads of 64 12.6 instead of 14.9.  With more tiles than CUs it loses (four prompts of up to 250 rows 12.8
+  // instead of 11.7), and with many requests (128 of 4 rows 20 instead of 18).
+  //
+  // Of the others, long prompts take eight waves: a tile of keys and values is loaded for twice the rows (16384
+  // rows 2118 us instead of 2348, 2039 rows 49 instead of 52).  Four waves, two workgroups a CU, waste less on
+  // short row tiles and have more of them (24 prompts of up to 120 rows 13 us instead of 23, 128 of up to 100 43
+  // instead of 48, 32 of up to 200 in 16 heads of 64 19 instead of 22); about 500 rows a request are the border.
+  if (rows <= 256 * 64 && static_cast<int64_t>(a.R) * a.KV <= 256) return launch<D, 4, 2>(a, workspace, counters, stream);
+  if (rows >= 200 * 256 && a.T / 512 >= a.R) return launch<D, 8, 1>(a, workspace, counters, stream);
+  return launch<D, 4, 1>(a, workspace, counters, stream);
 }
 
 }  // namespace
@@ -521,9 +598,7 @@ hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream
 size_t prompt_attention_workspace(const PromptArgs& a) { return partials_bytes(kKvPromptWorkers, kKvPromptRows, a.D); }
 
 hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
-  const bool many = static_cast<int64_t>(a.T) * a.H >= 200 * 256 && a.T / 512 >= a.R;
-  if (a.D == 64) return many ? launch<64, 8>(a, workspace, counters, stream) : launch<64, 4>(a, workspace, counters, stream);
-  return many ? launch<128, 8>(a, workspace, counters, stream) : launch<128, 4>(a, workspace, counters, stream);
+  return a.D == 64 ? launch_for<64>(a, workspace, counters, stream) : launch_for<128>(a, workspace, counters, stream);
 }
 
 }  // namespace w4a16

@@ -374,3 +374,47 @@ def test_values_that_are_no_numbers_in_larger_batches(gpu_lib, heads, kv_heads, 
         touched[:, head * group:(head + 1) * group, channel] = True
     assert torch.equal(got[~hit], base[~hit]) and torch.equal(got[~touched], want[~touched])
     assert torch.equal(got[hit].float().nan_to_num(7.0, 8.0, 9.0), torch.full_like(got[hit].float(), value).nan_to_num(7.0, 8.0, 9.0))
+
+
+def larger(lengths, heads, rows):
+    """The lengths and a prompt behind them that makes it that many rows of all heads together."""
+    return lengths + [max(1, -(-rows // heads) - sum(lengths))]
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (16, 2, 64), (40, 8, 128), (12, 12, 64)])
+@pytest.mark.parametrize("rows", [16000, 17000, 52000])
+def test_packed_lengths_in_batches_of_each_size(gpu_lib, heads, kv_heads, dim, rows):
+    """The same lengths where keys are split among waves, and in workgroups of four waves and of eight."""
+    lengths = larger([0, 129, 1, 33], heads, rows)
+    q, k, v, offsets = batch(lengths, heads, kv_heads, dim, seed=54)
+    check(attn.attention_prompt(q, k, v, int32(offsets)), q, k, v, offsets)
+
+
+@pytest.mark.parametrize("rows", [16000, 17000, 52000])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_keys_that_are_no_numbers_in_batches_of_each_size(gpu_lib, dim, rows):
+    """A key that is no number reaches the rows that see it, and no others; rows whose every score is
+    minus infinity stay zero; scores that lead all before them by far take over."""
+    lengths = larger([200, 70], 16, rows)
+    q, k, v, offsets = batch(lengths, 16, 4, dim, seed=55)
+    o = int32(offsets)
+    want = attn.attention_prompt(q, k, v, o)
+    k = k.clone()
+    k[150, 0, 5] = float("nan")
+    k[230, 3, 5] = float("inf")
+    out = attn.attention_prompt(q, k, v, o)
+    spoilt = torch.zeros(q.shape[:2], dtype=torch.bool, device="cuda")
+    spoilt[150:200, :4] = True
+    spoilt[230:270, 12:] = True
+    assert torch.equal(out[~spoilt], want[~spoilt])
+    assert bool(out[150:200, :4].isnan().all())
+    q, k = q.clone(), k.nan_to_num(0.0, 0.0, 0.0)
+    q[200:270, 2] = 1.0
+    k[200:270, 0] = -float("inf")
+    out = attn.attention_prompt(q, k, v, o)
+    assert not bool(out[200:270, 2].any())
+    q, k, v, offsets = batch(lengths, 16, 4, dim, seed=56)
+    k = k.clone()
+    k[190] *= 20  # leads by far in about half of the rows
+    k[offsets[-1] - 40:] *= 12
+    check(attn.attention_prompt(q, k, v, int32(offsets)), q, k, v, offsets)
