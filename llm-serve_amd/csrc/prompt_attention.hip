@@ -41,8 +41,12 @@ constexpr int kRing = 6;
 // with each.
 constexpr int kMinShare = 3 * kKeyTileCost;
 constexpr int kMaxParts = 12;
-// Row tiles of up to this cost are taken whole where each finds a workgroup of its own: 700 rows of 32 + 8 heads
-// take 21 us in whole tiles and 28 in shares.
+// Row tiles of up to four tiles of keys are dealt out whole, as many to each worker: no share of them saves what
+// its join costs (64 prompts of up to 60 rows, 32 + 8 heads, 16.2 us instead of 23.5, 128 of up to 100 32 instead
+// of 41, 32 of up to 250 29.0 instead of 33.0; with up to eight, 32 of up to 500 take 70 instead of 61).
+constexpr int kWholeCost = kSetupCost + 4 * kKeyTileCost;
+// Where each finds a workgroup of its own, row tiles of up to this cost are taken whole too: 700 rows of 32 + 8
+// heads take 21 us in whole tiles and 28 in shares.
 constexpr int kShortCost = kSetupCost + 12 * kKeyTileCost;
 
 typedef __attribute__((address_space(3))) uint8_t lds_u8_t;
@@ -197,12 +201,12 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
   int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   longest = wave_max(longest);
-  const bool whole = (longest <= kShortCost) & (all_tiles <= static_cast<int>(gridDim.x));
+  const bool whole = (longest <= kWholeCost) | ((longest <= kShortCost) & (all_tiles <= static_cast<int>(gridDim.x)));
   if (whole) {
     total = all_tiles;
     my_costs.first = 1, my_costs.step = 0;
   }
-  int workers = total;
+  int workers = min(total, static_cast<int>(gridDim.x));
   if (!whole) workers = total > 0 ? min(static_cast<int>(gridDim.x), (total - 1) / max(kMinShare, longest / kMaxParts) + 1) : 0;
   const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);
   const int me = static_cast<int>(blockIdx.x & 7) * per_xcd + turn;
@@ -210,8 +214,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     if (a.zero_tail) kv_zero_unowned(a, bad);
     return;
   }
-  KvShares shares{1, 0};
-  if (!whole) shares = KvShares{uniform(total / workers), uniform(total % workers)};
+  const KvShares shares{uniform(total / workers), uniform(total % workers)};
   const int begin = shares.begin(me), end = shares.begin(me + 1);
   // The sequence that the share begins in, and the units before it.
   int r = 0, base = 0;
