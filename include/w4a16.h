@@ -418,12 +418,13 @@ int w4a16_kv_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, c
 size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D);
 
 /* Causal attention of whole prompts over their own keys and values: q [T, H, D], k and v [T, KV, D]
- * (bf16, strides as in w4a16_kv_store; rows at most 2^22 elements apart, q's heads of a kv head within
- * 2^28; H <= 2^14), sequence r being
- * rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1 of all three.  Its row t sees its rows 0 .. t;
- * query head h reads kv head h / (H / KV).  out [T, H, D] (bf16, contiguous) = softmax(scale * q k^T) v
- * with fp32 scores, statistics and sums; the weights are rounded to bf16 for the second product.  NaN
- * and infinities in keys and values that a row does not see have no effect on it.  Rows of no sequence,
+ * (bf16, strides as in w4a16_kv_store; rows 0 to 2^22 elements apart, q's heads of a kv head within
+ * 2^28; H <= 2^14), sequence r being rows cu_query_lens[r] .. cu_query_lens[r + 1] - 1 of all three.
+ * Its row t sees its rows 0 .. t; query head h reads kv head h / (H / KV).  out [T, H, D] (bf16,
+ * contiguous) = softmax(scale * q k^T) v with fp32 scores, statistics and sums; the weights, up to 2^8
+ * of the row's largest, are rounded to bf16 for the second product (so that values beyond 2^119
+ * divided by the row's number of keys may overflow in the sum).  NaN and infinities in keys and
+ * values that a row does not see have no effect on it.  Rows of no sequence,
  * offsets that decrease, zero_tail, workspace and counters are as in w4a16_kv_attention.  out may be q
  * where that is contiguous, and overlaps no other operand.  Replaces flash_attn_varlen_func where
  * nothing is cached (attention.py:118-125). */

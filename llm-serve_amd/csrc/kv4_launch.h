@@ -95,6 +95,8 @@ struct PromptArgs {
   int group_shift;
   bool zero_tail;
 };
+// Rows (tokens x heads of a group) of the row tiles of a call of these sizes (T, R, H, KV).
+int prompt_attention_tile_rows(const PromptArgs& a);
 size_t prompt_attention_workspace(const PromptArgs& a);
 // counters: kKvAttentionCounters ints, zero before and after the call's kernel.
 hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream);

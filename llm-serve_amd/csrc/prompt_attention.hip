@@ -581,22 +581,29 @@ hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream
 
 template <int D>
 hipError_t launch_for(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
-  const int64_t rows = static_cast<int64_t>(a.T) * a.H;
-  // While row tiles of 64 find a CU each, the longest of them is what takes time: with its keys split between
-  // two waves, one prompt of 511 rows (32 + 8 heads of 128) takes 14.4 us instead of 16.5, one of 700 rows of 16
-  // heads of 64 12.6 instead of 14.9.  With more tiles than CUs it loses (four prompts of up to 250 rows 12.8
-  // instead of 11.7), and with many requests (128 of 4 rows 20 instead of 18).
-  //
-  // Of the others, long prompts take eight waves: a tile of keys and values is loaded for twice the rows (16384
-  // rows 2118 us instead of 2348, 2039 rows 49 instead of 52).  Four waves, two workgroups a CU, waste less on
-  // short row tiles and have more of them (24 prompts of up to 120 rows 13 us instead of 23, 128 of up to 100 43
-  // instead of 48, 32 of up to 200 in 16 heads of 64 19 instead of 22); about 500 rows a request are the border.
-  if (rows <= 256 * 64 && static_cast<int64_t>(a.R) * a.KV <= 256) return launch<D, 4, 2>(a, workspace, counters, stream);
-  if (rows >= 200 * 256 && a.T / 512 >= a.R) return launch<D, 8, 1>(a, workspace, counters, stream);
-  return launch<D, 4, 1>(a, workspace, counters, stream);
+  switch (prompt_attention_tile_rows(a)) {
+    case 64: return launch<D, 4, 2>(a, workspace, counters, stream);
+    case 128: return launch<D, 4, 1>(a, workspace, counters, stream);
+    default: return launch<D, 8, 1>(a, workspace, counters, stream);
+  }
 }
 
 }  // namespace
+
+// While row tiles of 64 find a CU each, the longest of them is what takes time: with its keys split between
+// two waves, one prompt of 511 rows (32 + 8 heads of 128) takes 14.4 us instead of 16.5, one of 700 rows of 16
+// heads of 64 12.6 instead of 14.9.  With more tiles than CUs it loses (four prompts of up to 250 rows 12.8
+// instead of 11.7), and with many requests (128 of 4 rows 20 instead of 18).
+//
+// Of the others, long prompts take eight waves: a tile of keys and values is loaded for twice the rows (16384
+// rows 2118 us instead of 2348, 2039 rows 49 instead of 52).  Four waves, two workgroups a CU, waste less on
+// short row tiles and have more of them (24 prompts of up to 120 rows 13 us instead of 23, 128 of up to 100 43
+// instead of 48, 32 of up to 200 in 16 heads of 64 19 instead of 22); about 500 rows a request are the border.
+int prompt_attention_tile_rows(const PromptArgs& a) {
+  const int64_t rows = static_cast<int64_t>(a.T) * a.H;
+  if (rows <= 256 * 64 && static_cast<int64_t>(a.R) * a.KV <= 256) return 64;
+  return rows >= 200 * 256 && a.T / 512 >= a.R ? 256 : 128;
+}
 
 size_t prompt_attention_workspace(const PromptArgs& a) { return partials_bytes(kKvPromptWorkers, kKvPromptRows, a.D); }
 

@@ -1401,6 +1401,7 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
 static int validate_rope(const w4a16::QkRopeArgs& a) {
   if (a.T < 0) return fail(W4A16_ERR_ARG, "T must not be negative (got %d)", a.T);
   if (a.H <= 0 || a.KV <= 0) return fail(W4A16_ERR_ARG, "query heads (%d) and kv heads (%d) must be positive", a.H, a.KV);
+  if (a.T > 1 << 30) return fail(W4A16_ERR_SHAPE, "%d tokens are too many for one call", a.T);
   if (a.H > 0xFFFF || a.KV > 0xFFFF) return fail(W4A16_ERR_SHAPE, "%d query heads and %d kv heads are too many", a.H, a.KV);
   if (a.D != 64 && a.D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", a.D);
   if (a.rotary <= 0 || a.rotary % 16 || a.rotary > a.D)
@@ -1463,10 +1464,14 @@ static int validate_prompts(int T, int R, int H, int KV, int D) {
   if (T == 0 || R == 0) return W4A16_OK;
   if (H > 1 << 14 || static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
-  // The kernel counts its work in 32 bits.  Tile j of a sequence's m costs ceil(64 / group) (j + 1) + 32, and
-  // m <= rows / 256 + 1: the last costs at most T / 4 + rows / 256 + 98, the mean of all half of that and 50.
-  const int64_t rows = static_cast<int64_t>(T) * (H / KV), tiles = rows / 256 + (R < rows ? R : rows);
-  if (static_cast<int64_t>(T) / 8 + rows / 512 + 100 > 0x7FFFFFFF / tiles / KV)
+  // The kernel counts its work in 32 bits.  With n rows a tile, tile j of a sequence's m costs 64 + s (j + 1) with
+  // s = ceil(n / 4 / group), and m <= rows / n + 1: their mean, 64 + s (m + 1) / 2, is at most
+  // T / 8 + rows / (2 n) + n / 4 + 65.
+  w4a16::PromptArgs a{};
+  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D;
+  const int64_t n = w4a16::prompt_attention_tile_rows(a);
+  const int64_t rows = static_cast<int64_t>(T) * (H / KV), tiles = rows / n + (R < rows ? R : rows);
+  if (static_cast<int64_t>(T) / 8 + rows / (2 * n) + n / 4 + 65 > 0x7FFFFFFF / tiles / KV)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too much work for one call", T, H);
   return W4A16_OK;
 }

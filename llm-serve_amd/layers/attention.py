@@ -407,9 +407,11 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query
     [rows, heads, head_dim].
 
     A prompt's rows give what ``attention_int4`` gives over their cached copies, but for the 4 bits.
-    ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest prompt if the caller knows it,
-    is checked and otherwise free.  Offsets that decrease name no rows at all.  Without ``out``
-    (contiguous, of q's shape), rows of no request are zero; in ``out`` they are left as they were.
+    ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest prompt if the caller knows it
+    (as ``attention_int4`` takes it), must be positive and changes nothing here.  Sums are fp32 with weights
+    of up to 2^8: values beyond 2^119 divided by a row's number of keys may overflow in them.  Offsets that
+    decrease name no rows at all.  Without ``out`` (contiguous, of q's shape), rows of no request are zero; in
+    ``out`` they are left as they were.
     ``out`` may be q itself, and overlaps no other operand."""
     # One expression accepts what all the checks accept; only what it does not goes through them.
     shape, kshape, index = q.shape, k.shape, q.get_device()

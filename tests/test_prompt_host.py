@@ -43,7 +43,7 @@ SHARED = [
     ({"k_out": P + 2}, 3, "aligned")]
 
 
-@pytest.mark.parametrize("change,status,message", SHARED + [({"k_out": None}, 1, "null")])
+@pytest.mark.parametrize("change,status,message", SHARED + [({"k_out": None}, 1, "null"), ({"T": (1 << 30) + 1}, 2, "too many")])
 def test_rope_refusals(pkg, dll, change, status, message):
     assert dll.w4a16_qk_norm_rope(*{**ROPE, **change}.values()) == status and message in error(pkg)
 
@@ -83,13 +83,21 @@ def test_workspace_is_bounded(dll):
 
 
 def test_work_beyond_32_bits_is_refused(dll):
-    """A prompt of 2^19 rows of 8 heads counts 8 x (2^11 + 1) x (2^16 + 2^10 + 100) = 1.1e9 units at most,
-    one of 2^20 rows 8 x (2^12 + 1) x (2^17 + 2^11 + 100) = 4.4e9, beyond 2^31.  Where a kv head has 1024
+    """A prompt of 2^19 rows of 8 heads counts 8 x (2^11 + 1) x (2^16 + 2^10 + 129) = 1.1e9 units at most,
+    one of 2^20 rows 8 x (2^12 + 1) x (2^17 + 2^11 + 129) = 4.4e9, beyond 2^31.  Where a kv head has 1024
     heads, a tile is a quarter of a token but costs a unit at least."""
     assert dll.w4a16_prompt_attention_workspace(1 << 19, 1, 8, 8, 128) > 0
     assert dll.w4a16_prompt_attention_workspace(1 << 20, 1, 8, 8, 128) == 0
     assert dll.w4a16_prompt_attention_workspace(1 << 13, 1, 1024, 1, 128) > 0
     assert dll.w4a16_prompt_attention_workspace(1 << 15, 1, 1024, 1, 128) == 0
+
+
+def test_work_of_smaller_row_tiles_beyond_32_bits_is_refused(dll):
+    """With more than a request a 512 rows, row tiles have 128 rows and there are twice as many: one prompt of
+    2^19 rows among 1100 requests counts 8 x 2^12 x (64 + 32 (2^12 + 1) / 2) = 2.15e9 units, beyond 2^31."""
+    assert 8 * 2 ** 12 * (64 + 16 * (2 ** 12 + 1)) > 2 ** 31
+    assert dll.w4a16_prompt_attention_workspace(1 << 19, 1100, 8, 8, 128) == 0
+    assert dll.w4a16_prompt_attention_workspace(1 << 18, 1100, 8, 8, 128) > 0
 
 
 def test_python_refusals():
