@@ -418,3 +418,26 @@ def test_keys_that_are_no_numbers_in_batches_of_each_size(gpu_lib, dim, rows):
     k[190] *= 20  # leads by far in about half of the rows
     k[offsets[-1] - 40:] *= 12
     check(attn.attention_prompt(q, k, v, int32(offsets)), q, k, v, offsets)
+
+
+@pytest.mark.parametrize("heads,lengths", [(8, [700, 900]), (16, [1100, 60, 900]), (32, [2039]), (32, [1500, 0, 1100, 1])])
+def test_each_form_captured_repeated_and_in_place(gpu_lib, heads, lengths):
+    """The same bits from eager calls, from a captured one on every replay with eager calls between them, and
+    with the output in the queries' place."""
+    q, k, v, offsets = batch(lengths, heads, 4, 128, seed=57)
+    q, o = q.contiguous(), int32(offsets)
+    want = attn.attention_prompt(q, k, v, o)
+    check(want, q, k, v, offsets)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = attn.attention_prompt(q, k, v, o)
+    for _ in range(4):
+        got.fill_(5)
+        graph.replay()
+        assert torch.equal(attn.attention_prompt(q, k, v, o), want)
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+    for _ in range(4):
+        mine = q.clone()
+        assert attn.attention_prompt(mine, k, v, o, out=mine) is mine
+        assert torch.equal(mine, want)
