@@ -35,11 +35,12 @@ constexpr int kKeys = 64;  // keys of a tile
 // Of a row tile besides its keys: finding it, queries, output take as long as four tiles of keys (with half of
 // that in the shares, nine prompts of up to 2500 rows take 313 us instead of 305).
 constexpr int kSetupCost = 4 * kKeyTileCost;
-// Operand fragments in flight between LDS and matrix instructions; 5 or 8 make no difference that shows.
-constexpr int kRing = 6;
 // A worker's least share, and the parts of the longest row tile at most: joining them costs some 3 us, and more
 // with each.
 constexpr int kMinShare = 3 * kKeyTileCost;
+// Workgroups beyond two waves a SIMD work from this share on: below it more joins cost what they gain (3 prompts of up
+// to 1500, 16 + 16 heads of 64, 33 us instead of 30), and a number in between leaves CUs unevenly filled (43).
+constexpr int kFullShare = 12 * kKeyTileCost;
 constexpr int kMaxParts = 12;
 // Row tiles of up to four tiles of keys are dealt out whole, as many to each worker: no share of them saves what
 // its join costs (64 prompts of up to 60 rows, 32 + 8 heads, 16.2 us instead of 23.5, 128 of up to 100 32 instead
@@ -95,6 +96,12 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+
+// Waves that a SIMD holds: heads of 64 channels need 128 registers a wave, of 128 channels 222.  Four waves overlap
+// their products with each other's softmax, which is the longer part there: one prompt of 8000 rows of 16 + 16 heads of 64
+// 163 us instead of 176 with two, 6 of up to 2500 71 instead of 80, 64 of up to 100 10.9 instead of 14.1.
+template <int D>
+constexpr int kWavesPerSimd = D == 64 ? 4 : 2;
 
 // Which 16-byte chunk of a row lies where: chunk c of row r is stored at c ^ swizzle(r).  Sixteen
 // neighbouring rows' same chunk (the first product's operand) and four rows' same 64 bytes (the
@@ -163,12 +170,15 @@ __device__ __forceinline__ int lane_again() {
 // WAVES waves of 32 rows each, or, with SPLIT 2, half as many rows, each with two waves that take half of every
 // tile's keys and are joined in LDS.
 //
-// Work is dealt out by cost, not by row tile: workers (as many workgroups as the chip holds at once) take equal
+// Work is dealt out by cost, not by row tile: workers (workgroups, as many as the chip holds at once) take equal
 // shares of all row tiles' costs, in order, those of one XCD neighbouring ones; a row tile that a border cuts is
 // joined by the last of its workers to arrive, in the workers' order, so that results do not depend on it.
 template <int D, int WAVES, int SPLIT>
-__global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptArgs a, KvPartials out) {
+__global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention_kernel(PromptArgs a, KvPartials out) {
   constexpr int kPitch = 2 * D, kTileBytes = kKeys * kPitch;  // bytes
+  // Operand fragments in flight between LDS and matrix instructions; 5 or 8 make no difference that shows with 128
+  // channels, 5 spill registers with 64.
+  constexpr int kRing = D == 64 ? 4 : 6;
   constexpr int kRowWaves = WAVES / SPLIT, kRows = 32 * kRowWaves, kMine = kKeys / SPLIT, kSteps = D / 16, kTiles = D / 32, kLoads = kTileBytes / WAVES / 1024;
   // Two stages of a tile of keys and one of values.
   __shared__ __align__(1024) uint8_t s_tiles[2][2][kTileBytes];
@@ -207,7 +217,10 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
     my_costs.first = 1, my_costs.step = 0;
   }
   int workers = min(total, static_cast<int>(gridDim.x));
-  if (!whole) workers = total > 0 ? min(static_cast<int>(gridDim.x), (total - 1) / max(kMinShare, longest / kMaxParts) + 1) : 0;
+  if (!whole) {
+    workers = total > 0 ? min(workers, (total - 1) / max(kMinShare, longest / kMaxParts) + 1) : 0;
+    if (D == 64 && total / kFullShare < static_cast<int>(gridDim.x)) workers = min(workers, static_cast<int>(gridDim.x / 2));
+  }
   const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);
   const int me = static_cast<int>(blockIdx.x & 7) * per_xcd + turn;
   if (bad | (turn >= per_xcd) | (me >= workers)) {
@@ -573,7 +586,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void prompt_attention_kernel(PromptA
 
 template <int D, int WAVES, int SPLIT>
 hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
-  constexpr int kWorkers = kKvPromptWorkers * 8 / WAVES;
+  constexpr int kWorkers = 256 * 4 * kWavesPerSimd<D> / WAVES;
   const KvPartials part = partials_at(static_cast<char*>(workspace), counters, kWorkers, 32 * WAVES / SPLIT, D);
   prompt_attention_kernel<D, WAVES, SPLIT><<<kWorkers, 64 * WAVES, 0, stream>>>(a, part);
   return hipGetLastError();
@@ -605,7 +618,9 @@ int prompt_attention_tile_rows(const PromptArgs& a) {
   return rows >= 200 * 256 && a.T / 512 >= a.R ? 256 : 128;
 }
 
-size_t prompt_attention_workspace(const PromptArgs& a) { return partials_bytes(kKvPromptWorkers, kKvPromptRows, a.D); }
+size_t prompt_attention_workspace(const PromptArgs& a) {
+  return partials_bytes(kKvPromptWorkers * (a.D == 64 ? kWavesPerSimd<64> : kWavesPerSimd<128>) / 2, kKvPromptRows, a.D);
+}
 
 hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
   return a.D == 64 ? launch_for<64>(a, workspace, counters, stream) : launch_for<128>(a, workspace, counters, stream);

@@ -441,3 +441,13 @@ def test_each_form_captured_repeated_and_in_place(gpu_lib, heads, lengths):
         mine = q.clone()
         assert attn.attention_prompt(mine, k, v, o, out=mine) is mine
         assert torch.equal(mine, want)
+
+
+@pytest.mark.parametrize("heads,kv_heads,lengths", [(16, 16, [290] * 50), (16, 4, [64] * 120 + [3]), (16, 16, [4100])])
+def test_grids_of_small_heads(gpu_lib, heads, kv_heads, lengths):
+    """Heads of 64 channels in batches that fill four waves a SIMD, cut row tiles and whole ones."""
+    q, k, v, offsets = batch(lengths, heads, kv_heads, 64, seed=58)
+    o = int32(offsets)
+    out = attn.attention_prompt(q, k, v, o)
+    check(out, q, k, v, offsets)
+    assert all(torch.equal(attn.attention_prompt(q, k, v, o), out) for _ in range(5))
