@@ -426,8 +426,8 @@ size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D);
  * divided by the row's number of keys may overflow in the sum).  NaN and infinities in keys and
  * values that a row does not see have no effect on it.  Rows of no sequence,
  * offsets that decrease, zero_tail, workspace and counters are as in w4a16_kv_attention.  out may be q
- * where that is contiguous, and overlaps no other operand.  Replaces flash_attn_varlen_func where
- * nothing is cached (attention.py:118-125). */
+ * where that is contiguous, and overlaps no other operand.  Replaces the reference's attention of
+ * prompts where nothing is cached (attention.py:118-125). */
 int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
                            int64_t k_stride_t, int64_t k_stride_h, const uint16_t* v, int64_t v_stride_t,
                            int64_t v_stride_h, const int32_t* cu_query_lens, uint16_t* out, float scale,
