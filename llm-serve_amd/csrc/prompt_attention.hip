@@ -116,7 +116,7 @@ __device__ __forceinline__ int swizzle(int row) {
 // every LDS read.  Its caller waits (wait_loads) before the barrier that hands the bytes over.  The wait states
 // are those of a scalar register that a vector instruction wrote, and of m0.
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "memory");
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "m0", "memory");
 }
 template <int LATER>
 __device__ __forceinline__ void wait_loads() {  // but for the last LATER ones; loads to LDS complete in order
