@@ -451,3 +451,11 @@ def test_grids_of_small_heads(gpu_lib, heads, kv_heads, lengths):
     out = attn.attention_prompt(q, k, v, o)
     check(out, q, k, v, offsets)
     assert all(torch.equal(attn.attention_prompt(q, k, v, o), out) for _ in range(5))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(130, 1, 64, [1, 40, 3]), (300, 2, 128, [150, 1, 60]), (100, 1, 64, [600]),
+                                                        (96, 1, 128, [1030]), (77, 1, 128, [333, 9])])
+def test_large_groups(gpu_lib, heads, kv_heads, dim, lengths):
+    """Groups of more heads than a wave, or a row tile, has rows: a tile is part of a token, or ends inside one."""
+    q, k, v, offsets = batch(lengths, heads, kv_heads, dim, seed=59, before=1, behind=2)
+    check(attn.attention_prompt(q, k, v, int32(offsets)), q, k, v, offsets)
