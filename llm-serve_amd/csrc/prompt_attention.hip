@@ -260,7 +260,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
   const uint32_t k_lds = tiles_lds + wave * kLoads * 1024, v_lds = k_lds + kTileBytes;
   auto rows_at = [&](int kt) {  // of this wave, where tile kt's stage is idle
     const uint32_t rows_lds = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_u8_t*)&s_rows[0]));
-    return (kOwnRows ? rows_lds : tiles_lds + (kt & 1) * 2 * kTileBytes) + wave * 32 * kPitch;
+    return (kOwnRows ? rows_lds : tiles_lds + (kt & 1) * 2 * kTileBytes) + row_wave * 32 * kPitch;
   };
   // This lane's operands in a tile: of the keys, row col and chunk h, the others by exclusive or with 32 a
   // step of 16 channels; of the values, its four rows' 8 bytes, the others by exclusive or with 64 a step of
@@ -347,12 +347,13 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
       const int last_token = by_group(a, last_row);
       const uint32_t last = (last_token - token0) * by_token + (last_row - last_token * group) * by_head;
       const int lane = lane_again();
-      Place p = first_place(lane);
+      constexpr int kMyRows = 32 / SPLIT;  // two waves of the same rows load half of them each
+      Place p = first_place(lane + key_part * (kMyRows * kChunks));
 #pragma unroll
-      for (int j = 0; j < 32 / kEach; ++j) {
-        const uint32_t chunk = (lane % kChunks) ^ ((lane / kChunks + j * kEach) & (kChunks - 1));
+      for (int j = 0; j < kMyRows / kEach; ++j) {
+        const uint32_t chunk = (lane % kChunks) ^ ((key_part * kMyRows + lane / kChunks + j * kEach) & (kChunks - 1));
         const uint32_t at = p.row <= last_row ? p.token * by_token + p.head * by_head : last;
-        load_to_lds(from, at + chunk * 16, rows_at(t0 + 1) + j * 1024);
+        load_to_lds(from, at + chunk * 16, rows_at(t0 + 1) + (key_part * (kMyRows / kEach) + j) * 1024);
         next_place(p);
       }
     }
@@ -390,6 +391,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
 
     bf16x8_t qf[kSteps];
     wait_loads<0>();
+    if (SPLIT > 1) barrier();
     {
       const int lane = lane_again(), c = lane & 31;
       const uint32_t at = rows_at(t0 + 1) + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
@@ -564,7 +566,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
     if (last && key_part == 0) {
       const float inv = row_sum == 0.0f ? 0.0f : 1.0f / row_sum;
       const int lane = lane_again(), c = lane & 31;
-      const uint32_t rows_lds = rows_at(t1) + wave * (SPLIT - 1) * 32 * kPitch, at = rows_lds + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
+      const uint32_t rows_lds = rows_at(t1) + row_wave * (SPLIT - 1) * 32 * kPitch, at = rows_lds + c * kPitch + ((lane >> 5) ^ (c & (kPitch / 16 - 1))) * 16;
 #pragma unroll
       for (int f = 0; f < D / 8; f += 2) *(lds_u32x4_t*)static_cast<uintptr_t>(at ^ (16 * f)) = row_pair(inv, own[f], own[f + 1]);
       char* to = reinterpret_cast<char*>(a.out + (static_cast<int64_t>(q.row + token0) * a.H + head * group) * D);
