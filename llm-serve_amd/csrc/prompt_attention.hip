@@ -478,11 +478,14 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
       // Weights of 16 keys at a time, beside the products of the 16 before them.
       constexpr int kPv = 2 * kHalves * kTiles, kPairs = 4 / kTiles;  // matrix instructions; pairs of weights beside one
       u32x4_t now, next;
+      // Summed for the tile first: single weights added to the sum of all tiles would all be rounded at its last
+      // place, equal ones the same way (350000 rows of weights of 0.7 were off by 0.0026).
+      float tile_sum = 0.0f;
       auto pair = [&](int i, u32x4_t& w) {  // weights 2 i and 2 i + 1 of a lane's 32
         float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], scale, from));
         float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], scale, from));
-        row_sum += p0;
-        row_sum += p1;
+        tile_sum += p0;
+        tile_sum += p1;
         w[i & 3] = pack_bf16x2(p0, p1);
       };
 #pragma unroll
@@ -500,6 +503,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
         }
         if (c == kTiles - 1) now = next;
       }
+      row_sum += tile_sum;
       if (__builtin_expect(broken, 0)) {
         const int see = sees();
         for (int key = my_key0; key < min(my_key0 + kMine, any_sees); ++key) {
