@@ -32,6 +32,10 @@ namespace w4a16 {
 namespace {
 
 constexpr int kKeys = 64;  // keys of a tile
+// The weights' exponents c s - m are formed without rounding c s, and m is a rounded c s: weights are larger by
+// half of m's last place at most, 2^(2^-5) below this border.  Beyond it, in rows of their own, c s is rounded as m is:
+// for scores of 2^31 and more that place is 2^7 and takes the largest weight of a row out of fp32.
+constexpr float kFarReference = 0x1p20f;
 // Of a row tile besides its keys: finding it, queries, output take as long as four tiles of keys (with half of
 // that in the shares, nine prompts of up to 2500 rows take 313 us instead of 305).
 constexpr int kSetupCost = 4 * kKeyTileCost;
@@ -474,7 +478,32 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[c][i] *= f;
       }
-      const float from = row_max == -INFINITY ? 0.0f : -row_max;
+      const bool my_far = (fabsf(row_max) > kFarReference) & (row_max != -INFINITY), far = __any(my_far);
+      if (__builtin_expect(far, 0)) {  // the exponents themselves, of each row as its own reference asks
+        if (my_far) {
+#pragma unroll
+          for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[n][i] *= scale;
+#pragma unroll
+          for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
+#pragma unroll
+          for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[n][i] -= row_max;
+        } else {
+          const float from = row_max == -INFINITY ? 0.0f : -row_max;
+#pragma unroll
+          for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[n][i] = __builtin_fmaf(sc[n][i], scale, from);
+        }
+#pragma unroll
+        for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
+      }
+#pragma unroll
+      for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
+      const float factor = far ? 1.0f : scale, from = (far | (row_max == -INFINITY)) ? 0.0f : -row_max;
       // Weights of 16 keys at a time, beside the products of the 16 before them.
       constexpr int kPv = 2 * kHalves * kTiles, kPairs = 4 / kTiles;  // matrix instructions; pairs of weights beside one
       u32x4_t now, next;
@@ -482,8 +511,8 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
       // place, equal ones the same way (350000 rows of weights of 0.7 were off by 0.0026).
       float tile_sum = 0.0f;
       auto pair = [&](int i, u32x4_t& w) {  // weights 2 i and 2 i + 1 of a lane's 32
-        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], scale, from));
-        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], scale, from));
+        float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7)], factor, from));
+        float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i >> 3][2 * (i & 7) + 1], factor, from));
         tile_sum += p0;
         tile_sum += p1;
         w[i & 3] = pack_bf16x2(p0, p1);

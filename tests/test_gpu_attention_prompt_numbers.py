@@ -1,4 +1,4 @@
-"""Prompt attention where its arithmetic is at its limits: sums over very long prompts."""
+"""Prompt attention where its arithmetic is at its limits: sums over very long prompts, scores of any size."""
 import importlib
 import math
 
@@ -40,3 +40,52 @@ def test_sums_of_equal_weights_over_a_long_prompt(gpu_lib):
     error = 2.0 ** -18 + 2.0 ** -22 + (5469 + 40 + 10) * 2.0 ** -24
     bad = off > error * want
     assert not bool(bad.any()), (int(bad.sum()), int(bad.any(1).nonzero()[0]), float((off / want.clamp(min=1e-9)).max()))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(4, 2, 128, [300]), (4, 4, 64, [100, 270]), (16, 4, 64, [1500]), (32, 8, 128, [700, 600]),
+                                                        (32, 8, 128, [2039])])
+@pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 17, 2.0 ** 20, 2.0 ** 45])
+def test_rows_of_very_large_scores(gpu_lib, heads, kv_heads, dim, lengths, size):
+    """Scores of 2^23 to 2^95, where a last place of fp32 is worth far more than 1: a row is the value of its
+    largest score.  (The scale is no power of two, so that scores are rounded on their way into the exponent.)
+
+    Key j of a sequence is size (1 + j // dim) in channel j % dim; query t is size in one channel and -size in all
+    others.  Of the keys in its channel that it sees the last one wins, by at least size^2 / 16; where it sees none
+    in it, all that it sees (fewer than dim) have the same score, and it is their mean.  All weights are 1 or 0, so
+    what is left is the sums' and the quotient's roundings, below 2 dim 2^-24 of values below 8, and the output's."""
+    rows, group = sum(lengths), heads // kv_heads
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    v = torch.randn(rows, kv_heads, dim, generator=gen, device="cuda").to(torch.bfloat16)
+    q = torch.full((rows, heads, dim), -size, device="cuda")
+    k, want = torch.zeros(rows, kv_heads, dim, device="cuda"), torch.zeros(rows, heads, dim, dtype=torch.float64, device="cuda")
+    offsets = [0]
+    for n in lengths:
+        first, t = offsets[-1], torch.arange(n, device="cuda")
+        k[first + t, :, t % dim] = (size * (1 + t // dim))[:, None]
+        for h in range(heads):
+            channel = (7 * t + h) % dim
+            q[first + t, h, channel] = size
+            last = t - (t - channel) % dim
+            seen = v[first:first + n, h // group].double()
+            mean = seen.cumsum(0) / (1 + t)[:, None]
+            want[first:first + n, h] = torch.where((last >= 0)[:, None], seen[last.clamp(min=0)], mean)
+        offsets.append(first + n)
+    assert float(v.abs().max()) < 8
+    out = attn.attention_prompt(q.to(torch.bfloat16), k.to(torch.bfloat16), v, int32(offsets), scale=0.11)
+    off = (out.double() - want).abs()
+    bad = ~(off <= 2.0 ** -8 * want.abs() + 8 * 2 * dim * 2.0 ** -24)
+    assert not bool(bad.any()), (int(bad.any(-1).sum()), bad.any(-1).nonzero()[0].tolist())
+
+
+@pytest.mark.parametrize("heads,lengths", [(4, [300]), (16, [700, 400]), (32, [2039])])
+def test_rows_of_very_large_scores_are_alone(gpu_lib, heads, lengths):
+    """A row beside one of very large scores keeps its bits."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q, k, v = (torch.randn(sum(lengths), h, 128, generator=gen, device="cuda").to(torch.bfloat16) for h in (heads, 4, 4))
+    offsets = int32([0] + [sum(lengths[:i + 1]) for i in range(len(lengths))])
+    want = attn.attention_prompt(q, k, v, offsets)
+    large = torch.rand(sum(lengths), heads, generator=gen, device="cuda") < 0.05
+    q = torch.where(large[..., None], q * 2.0 ** 40, q)
+    out = attn.attention_prompt(q, k, v, offsets)
+    assert torch.equal(out[~large], want[~large]) and bool(torch.isfinite(out).all())
+    assert not torch.equal(out[large], want[large])
