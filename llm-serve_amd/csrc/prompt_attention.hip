@@ -88,8 +88,8 @@ template <int ROWS>
 __device__ __forceinline__ KvTileCosts tile_costs(const PromptArgs& a, const Sequence& s, bool whole) {
   KvTileCosts c;
   c.tiles = (s.n * a.group + ROWS - 1) / ROWS;
-  c.step = by_group(a, ROWS / (kKeys / kKeyTileCost) + a.group - 1);
-  c.first = c.step + kSetupCost;
+  c.step = by_group(a, (ROWS / (kKeys / kKeyTileCost) >> a.cost_shift) + a.group - 1);
+  c.first = c.step + (kSetupCost >> a.cost_shift);
   if (whole) c.first = 1, c.step = 0;
   return c;
 }
@@ -215,15 +215,16 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
   int total = __builtin_amdgcn_readlane(wave_scan(sum), 63);
   const int all_tiles = __builtin_amdgcn_readlane(wave_scan(tiles), 63);
   longest = wave_max(longest);
-  const bool whole = (longest <= kWholeCost) | ((longest <= kShortCost) & (all_tiles <= static_cast<int>(gridDim.x)));
+  const bool whole = (longest <= kWholeCost >> a.cost_shift) |
+                     ((longest <= kShortCost >> a.cost_shift) & (all_tiles <= static_cast<int>(gridDim.x)));
   if (whole) {
     total = all_tiles;
     my_costs.first = 1, my_costs.step = 0;
   }
   int workers = min(total, static_cast<int>(gridDim.x));
   if (!whole) {
-    workers = total > 0 ? min(workers, (total - 1) / max(kMinShare, longest / kMaxParts) + 1) : 0;
-    if (D == 64 && total / kFullShare < static_cast<int>(gridDim.x)) workers = min(workers, static_cast<int>(gridDim.x / 2));
+    workers = total > 0 ? min(workers, (total - 1) / max(kMinShare >> a.cost_shift, longest / kMaxParts) + 1) : 0;
+    if (D == 64 && total / (kFullShare >> a.cost_shift) < static_cast<int>(gridDim.x)) workers = min(workers, static_cast<int>(gridDim.x / 2));
   }
   const int per_xcd = (workers + 7) / 8, turn = static_cast<int>(blockIdx.x >> 3);
   const int me = static_cast<int>(blockIdx.x & 7) * per_xcd + turn;
@@ -629,14 +630,21 @@ hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream
 
 template <int D>
 hipError_t launch_for(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
-  switch (prompt_attention_tile_rows(a)) {
+  switch (a.tile_rows) {
     case 64: return launch<D, 4, 2>(a, workspace, counters, stream);
     case 128: return launch<D, 4, 1>(a, workspace, counters, stream);
     default: return launch<D, 8, 1>(a, workspace, counters, stream);
   }
 }
 
-}  // namespace
+// The most that the cost units of a call's row tiles can add up to.  With n rows a tile and rows / n = y, sequences
+// have at most y + R tiles together, tile j of each costs first + step j (tile_costs), and the sum of all j is
+// largest, below (y + 1) y / 2, where one sequence has all rows; x is y rounded down.
+int64_t most_cost(const PromptArgs& a, int n, int shift) {
+  const int64_t group = a.H / a.KV, rows = a.T * group, x = rows / n;
+  const int64_t step = ((n / (kKeys / kKeyTileCost) >> shift) + group - 1) / group, first = step + (kSetupCost >> shift);
+  return a.KV * ((x + (a.R < rows ? a.R : rows)) * first + step * ((x + 1) * (x + 2) / 2));
+}
 
 // While row tiles of 64 find a CU each, the longest of them is what takes time: with its keys split between
 // two waves, one prompt of 511 rows (32 + 8 heads of 128) takes 14.4 us instead of 16.5, one of 700 rows of 16
@@ -647,10 +655,28 @@ hipError_t launch_for(const PromptArgs& a, void* workspace, int* counters, hipSt
 // rows 2118 us instead of 2348, 2039 rows 49 instead of 52).  Four waves, two workgroups a CU, waste less on
 // short row tiles and have more of them (24 prompts of up to 120 rows 13 us instead of 23, 128 of up to 100 43
 // instead of 48, 32 of up to 200 in 16 heads of 64 19 instead of 22); about 500 rows a request are the border.
-int prompt_attention_tile_rows(const PromptArgs& a) {
+int tile_rows(const PromptArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.H;
   if (rows <= 256 * 64 && static_cast<int64_t>(a.R) * a.KV <= 256) return 64;
   return rows >= 200 * 256 && a.T / 512 >= a.R ? 256 : 128;
+}
+
+}  // namespace
+
+// The kernel counts work in 32 bits.  A step of many requests may be one long prompt and empty places, which the
+// host cannot tell from their number: where its work might pass 32 bits, it takes the form with fewer row tiles, and
+// units of up to a whole tile of keys (shares of so many are even whatever the unit).  262144 rows of 64 + 8 heads,
+// one prompt, count 2.155e9 sixteenths of a tile of keys.
+bool plan_prompt_attention(PromptArgs* a) {
+  constexpr int64_t kMost = 0x7FFFFFFF;
+  static_assert(kKeyTileCost == 16, "a tile of keys in units of cost_shift 4 is one");
+  a->tile_rows = tile_rows(*a), a->cost_shift = 0;
+  if (most_cost(*a, a->tile_rows, 0) <= kMost) return true;
+  if (a->T > kPromptStepRows) return false;
+  a->tile_rows = 256;
+  for (; a->cost_shift <= 4; ++a->cost_shift)
+    if (most_cost(*a, 256, a->cost_shift) <= kMost) return true;
+  return false;
 }
 
 size_t prompt_attention_workspace(const PromptArgs& a) {

@@ -1457,29 +1457,23 @@ int w4a16_kv_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, c
   return check_launch(w4a16::launch_qk_rope(a, static_cast<hipStream_t>(stream)), "kv append");
 }
 
-static int validate_prompts(int T, int R, int H, int KV, int D) {
+// The sizes of a prompt attention call, entered into a with what is planned from them.
+static int validate_prompts(w4a16::PromptArgs* a, int T, int R, int H, int KV, int D) {
   if (T < 0 || R < 0) return fail(W4A16_ERR_ARG, "T (%d) and R (%d) must not be negative", T, R);
   if (H <= 0 || KV <= 0 || H % KV) return fail(W4A16_ERR_SHAPE, "query heads (%d) must be a multiple of kv heads (%d)", H, KV);
   if (D != 64 && D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", D);
   if (T == 0 || R == 0) return W4A16_OK;
   if (H > 1 << 14 || static_cast<int64_t>(T) * H > 0x3FFFFFFF)
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too many for one call", T, H);
-  // The kernel counts its work in 32 bits.  With n rows a tile, tile j of a sequence's m costs 64 + s (j + 1) with
-  // s = ceil(n / 4 / group), and m <= rows / n + 1: their mean, 64 + s (m + 1) / 2, is at most
-  // T / 8 + rows / (2 n) + n / 4 + 65.
-  w4a16::PromptArgs a{};
-  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D;
-  const int64_t n = w4a16::prompt_attention_tile_rows(a);
-  const int64_t rows = static_cast<int64_t>(T) * (H / KV), tiles = rows / n + (R < rows ? R : rows);
-  if (static_cast<int64_t>(T) / 8 + rows / (2 * n) + n / 4 + 65 > 0x7FFFFFFF / tiles / KV)
+  a->T = T, a->R = R, a->H = H, a->KV = KV, a->D = D;
+  if (!w4a16::plan_prompt_attention(a))
     return fail(W4A16_ERR_SHAPE, "%d rows of %d heads are too much work for one call", T, H);
   return W4A16_OK;
 }
 
 size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D) {
-  if (validate_prompts(T, R, H, KV, D) != W4A16_OK || T == 0 || R == 0) return 0;
   w4a16::PromptArgs a{};
-  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D;
+  if (validate_prompts(&a, T, R, H, KV, D) != W4A16_OK || T == 0 || R == 0) return 0;
   return w4a16::prompt_attention_workspace(a);
 }
 
@@ -1488,7 +1482,8 @@ int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stri
                            int64_t v_stride_h, const int32_t* cu_query_lens, uint16_t* out, float scale, int T, int R,
                            int H, int KV, int D, int zero_tail, void* workspace, size_t workspace_bytes,
                            int32_t* counters, void* stream) {
-  int e = validate_prompts(T, R, H, KV, D);
+  w4a16::PromptArgs a{};
+  int e = validate_prompts(&a, T, R, H, KV, D);
   if (e != W4A16_OK) return e;
   const float scale_log2e = scale * 1.44269504088896341f;
   if (!(scale > 0.0f) || !(scale_log2e <= 3.402823466e38f))
@@ -1506,12 +1501,11 @@ int w4a16_prompt_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stri
     return fail(W4A16_ERR_SHAPE, "rows of q, k and v must be 0 to 2^22 elements apart (got %lld, %lld and %lld), a group of q's heads within 2^28",
                 static_cast<long long>(q_stride_t), static_cast<long long>(k_stride_t), static_cast<long long>(v_stride_t));
   if (!aligned(out, 16)) return fail(W4A16_ERR_ALIGN, "out must be 16-byte aligned");
-  w4a16::PromptArgs a{};
   a.q = q, a.q_stride_t = q_stride_t, a.q_stride_h = q_stride_h;
   a.k = k, a.k_stride_t = k_stride_t, a.k_stride_h = k_stride_h;
   a.v = v, a.v_stride_t = v_stride_t, a.v_stride_h = v_stride_h;
   a.cu_query_lens = cu_query_lens, a.out = out, a.scale_log2e = scale_log2e;
-  a.T = T, a.R = R, a.H = H, a.KV = KV, a.D = D, a.zero_tail = zero_tail != 0;
+  a.zero_tail = zero_tail != 0;
   // x / group as a product: with 2^l >= group the inverse's error, below 1, times x < 2^31 stays below 2^(31 + l).
   a.group = H / KV;
   int l = 0;

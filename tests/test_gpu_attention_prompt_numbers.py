@@ -5,6 +5,8 @@ import math
 import pytest
 import torch
 
+from oracle import prompt_oracle as ora
+
 pytestmark = pytest.mark.gpu
 
 attn = importlib.import_module("llm-serve_amd.layers.attention")
@@ -89,3 +91,39 @@ def test_rows_of_very_large_scores_are_alone(gpu_lib, heads, lengths):
     out = attn.attention_prompt(q, k, v, offsets)
     assert torch.equal(out[~large], want[~large]) and bool(torch.isfinite(out).all())
     assert not torch.equal(out[large], want[large])
+
+
+def check_rows(out, q, k, v, first, rows, scale):
+    """Some rows of a sequence that begins at `first`, against their 64-bit sums."""
+    group, dim = q.shape[1] // k.shape[1], q.shape[2]
+    for row in rows:
+        n = row - first + 1
+        for g in range(k.shape[1]):
+            keys, values = k[first:row + 1, g].double(), v[first:row + 1, g].double()
+            for h in range(g * group, (g + 1) * group):
+                s = (keys * q[row, h].double()).sum(-1) * scale
+                w = torch.softmax(s, 0)[:, None]
+                want, spread = (w * values).sum(0), (w * values.abs()).sum(0)
+                reach = (keys.abs() * q[row, h].double().abs()).sum(-1).amax().expand(1) * scale
+                off = (out[row, h].double() - want).abs()
+                # tiles of keys, and the additions of one of them
+                assert bool((off <= ora.prompt_tolerance(want[None], spread[None], reach, n // 64 + 64)[0]).all()), (row, h)
+
+
+@pytest.mark.parametrize("heads,kv_heads,requests", [(32, 8, 513), (64, 8, 4096)])
+def test_largest_steps_of_many_requests(gpu_lib, heads, kv_heads, requests):
+    """2^18 rows of more than a request a 512 rows: prompts of the same length, whose sequences are those of a smaller
+    call, and one prompt of all rows but one for each other request."""
+    rows = 1 << 18
+    gen = torch.Generator(device="cuda").manual_seed(10)
+    q, k, v = (torch.randn(rows, h, 128, generator=gen, device="cuda", dtype=torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+    each = rows // requests
+    even = [i * each for i in range(requests)] + [rows]
+    out = attn.attention_prompt(q, k, v, int32(even))
+    for r in (0, 1, requests // 2, requests - 1):
+        a, b = even[r], even[r + 1]
+        ora.check_prompt(out[a:b], *ora.prompt(q[a:b], k[a:b], v[a:b], [0, b - a]), b - a)
+    long = rows - (requests - 1)
+    out = attn.attention_prompt(q, k, v, int32([0] + list(range(long, rows + 1))))
+    check_rows(out, q, k, v, 0, (0, 63, 4097, 100000, long - 1), 128 ** -0.5)
+    assert torch.equal(out[long:], v[long:].repeat_interleave(heads // kv_heads, 1))

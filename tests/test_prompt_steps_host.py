@@ -1,0 +1,80 @@
+"""Which sizes prompt attention takes, on the CPU (nothing is launched): every step that ``kv_step`` makes, whatever
+its number of requests."""
+import importlib
+
+import pytest
+
+attn = importlib.import_module("llm-serve_amd.layers.attention")
+
+
+@pytest.fixture(scope="module")
+def dll(pkg):
+    return pkg.lib().dll
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(32, 8, 128), (40, 8, 128), (64, 8, 128), (128, 8, 128), (16, 16, 64), (32, 32, 64),
+                                                (16, 1, 128)])
+@pytest.mark.parametrize("requests", [1, 512, 513, 600, 1000, 4096])
+@pytest.mark.parametrize("rows", [attn.MAX_STEP_TOKENS, 240000, 180000, 131073])
+def test_steps_of_any_number_of_requests(dll, rows, requests, heads, kv_heads, dim):
+    assert requests <= attn.MAX_STEP_REQUESTS
+    assert dll.w4a16_prompt_attention_workspace(rows, requests, heads, kv_heads, dim) > 0
+
+
+def test_a_long_prompt(dll):
+    """The documented limit of one call: 350000 rows with 32 heads."""
+    assert dll.w4a16_prompt_attention_workspace(350000, 1, 32, 8, 128) > 0
+    assert dll.w4a16_prompt_attention_workspace(350000, 680, 32, 8, 128) > 0
+    assert dll.w4a16_prompt_attention_workspace(380000, 1, 32, 8, 128) == 0
+
+
+def units(lengths, group, kv_heads, n, shift):
+    """The cost units of sequences' row tiles of n rows (sixteenths of a tile of 64 keys, 2^shift of them)."""
+    step = -(-(n // 4 >> shift) // group)
+    first = step + (64 >> shift)
+    tiles = [-(-x * group // n) for x in lengths]
+    return kv_heads * sum(m * first + step * m * (m - 1) // 2 for m in tiles)
+
+
+def shares(lengths, group, kv_heads, n, shift, workers):
+    """The parts that equal shares cut the row tiles of one head into: {(sequence, tile): [(first key tile, end)]}."""
+    step = -(-(n // 4 >> shift) // group)
+    first = step + (64 >> shift)
+    total = units(lengths, group, kv_heads, n, shift)
+    borders = [w * (total // workers) + min(w, total % workers) for w in range(workers + 1)]
+    parts, at = {}, 0
+    cuts = iter(borders)
+    cut = next(cuts)
+    for r, x in enumerate(lengths):
+        for head in range(kv_heads):
+            for j in range(-(-x * group // n)):
+                cost = first + step * j
+                keys = -(-((min((j + 1) * n, x * group) - 1) // group + 1) // 64)
+                while cut <= at:
+                    cut = next(cuts)
+                inside = []
+                while cut < at + cost:
+                    inside.append(cut - at)
+                    cut = next(cuts)
+                ends = [int(c * (keys * (1.0 / cost))) for c in inside] + [keys]
+                parts[r, head, j] = list(zip([0] + ends[:-1], ends))
+                at += cost
+    assert at == total
+    return parts
+
+
+@pytest.mark.parametrize("shift", [0, 1, 4])
+def test_shares_in_coarser_units_cover_every_key_once(shift):
+    """The shares' arithmetic with units of up to a whole tile of keys: each row tile's parts follow each other from its
+    first tile of keys to its last."""
+    for lengths, group, kv_heads, n in (([9000, 0, 70, 1, 4000], 8, 2, 256), ([20000], 4, 1, 256), ([1] * 300 + [6000], 5, 2, 256)):
+        for parts in shares(lengths, group, kv_heads, n, shift, 256).values():
+            assert parts[0][0] == 0 and all(a <= b for a, b in parts) and all(x[1] == y[0] for x, y in zip(parts, parts[1:]))
+
+
+def test_counts_stay_below_32_bits():
+    """The longest prompts of a step's rows, in the form and unit that the library takes for them."""
+    most = attn.MAX_STEP_TOKENS
+    assert units([most], 4, 8, 128, 0) > 2 ** 31 > units([most], 4, 8, 256, 0)  # why 32 + 8 heads take 256 rows
+    assert units([most], 8, 8, 256, 0) > 2 ** 31 > units([most - 4095] + [1] * 4095, 8, 8, 256, 1)
+    assert units([most - 4095] + [1] * 4095, 1, 32, 256, 2) < 2 ** 31
