@@ -315,6 +315,21 @@ class _ScratchPool:
 SCRATCH = _ScratchPool()
 
 
+def _check_scale(scale: float) -> None:
+    if not 0.0 < scale < MAX_SCALE:
+        raise ValueError(f"attention scale must be positive and below {MAX_SCALE} (got {scale})")
+
+
+def _check_max_query_len(max_query_len: int) -> None:
+    if max_query_len < 1:
+        raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
+
+
+def _check_tree_mask(tree_mask: torch.Tensor, rows: int, index: int) -> None:
+    if tree_mask.dtype != torch.int64 or tree_mask.get_device() != index or tree_mask.shape != (rows,):
+        raise ValueError("tree_mask must be an int64 [rows] tensor on the cache's GPU")
+
+
 def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Tensor, seq_lens: torch.Tensor,
                    cu_query_lens: torch.Tensor, *, block_size: int, scale: float | None = None,
                    max_query_len: int | None = None, tree_mask: torch.Tensor | None = None,
@@ -354,15 +369,14 @@ def attention_int4(q: torch.Tensor, cache: torch.Tensor, block_tables: torch.Ten
     rows, heads = shape[0], shape[1]
     if scale is None:
         scale = head_dim ** -0.5
-    elif not 0.0 < scale < MAX_SCALE:
-        raise ValueError(f"attention scale must be positive and below {MAX_SCALE} (got {scale})")
+    else:
+        _check_scale(scale)
     if max_query_len is None:
         max_query_len = max(rows, 1)
-    elif max_query_len < 1:
-        raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
+    else:
+        _check_max_query_len(max_query_len)
     if tree_mask is not None:
-        if tree_mask.dtype != torch.int64 or tree_mask.get_device() != index or tree_mask.shape != (rows,):
-            raise ValueError("tree_mask must be an int64 [rows] tensor on the cache's GPU")
+        _check_tree_mask(tree_mask, rows, index)
         tree_mask = tree_mask.contiguous()
     zero_tail = out is None
     if out is None:
@@ -430,10 +444,10 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query
     rows, heads, head_dim = shape
     if scale is None:
         scale = head_dim ** -0.5
-    elif not 0.0 < scale < MAX_SCALE:
-        raise ValueError(f"attention scale must be positive and below {MAX_SCALE} (got {scale})")
-    if max_query_len is not None and max_query_len < 1:
-        raise ValueError(f"max_query_len must be at least 1 (got {max_query_len})")
+    else:
+        _check_scale(scale)
+    if max_query_len is not None:
+        _check_max_query_len(max_query_len)
     zero_tail = out is None
     if out is None:
         out = torch.empty_strided(shape, (heads * head_dim, head_dim, 1), dtype=_BF16, device=index)
@@ -523,13 +537,14 @@ class Attention(nn.Module):
 
         ``whole_prompts`` says that every request of the step is a prompt with nothing cached before it:
         its rows then attend to their own keys and values as they are, in bf16, and not to their 4-bit
-        copies in the cache."""
+        copies in the cache.  A step that the attention refuses leaves the cache as it was."""
         if self.kv_cache is None:
             raise RuntimeError("Attention.kv_cache must be set before the first step")
         if whole_prompts and tree_mask is not None:
             raise ValueError("whole prompts are causal: they take no tree_mask")
         heads, kv_heads, rows = self.num_heads, self.num_kv_heads, qkv.shape[0]
         q, k, v = qkv.view(rows, heads + 2 * kv_heads, self.head_dim).split((heads, kv_heads, kv_heads), 1)
+        self._check_attends(rows, step, whole_prompts, max_query_len, tree_mask)
         q = append_kv_int4(q, k, v, self.kv_cache, step.slots, step.positions, table, block_size=self.block_size,
                            q_weight=q_weight, k_weight=k_weight, eps=eps, return_keys=whole_prompts)
         if whole_prompts:
@@ -540,3 +555,26 @@ class Attention(nn.Module):
                                  block_size=self.block_size, scale=self.scale, max_query_len=max_query_len,
                                  tree_mask=tree_mask)
         return out.view(rows, heads * self.head_dim)
+
+    def _check_attends(self, rows: int, step: KVStep, whole_prompts: bool, max_query_len: int | None,
+                       tree_mask: torch.Tensor | None) -> None:
+        """What the attention of a step would refuse, in front of the cache's writing: a refused step leaves the
+        cache as it was."""
+        _check_scale(self.scale)
+        if max_query_len is not None:
+            _check_max_query_len(max_query_len)
+        if tree_mask is not None:
+            _check_tree_mask(tree_mask, rows, self.kv_cache.get_device())
+        requests = step.cu_query_lens.shape[0] - 1
+        if step.cu_query_lens.ndim != 1 or requests < 1:
+            raise ValueError("KV cu_query_lens must be [requests + 1], of at least one request")
+        if rows > 0:
+            sizes = (rows, requests, self.num_heads, self.num_kv_heads, self.head_dim)
+            if whole_prompts:
+                size = _prompt_workspace_bytes(*sizes)
+            else:
+                if step.block_tables.ndim != 2 or step.block_tables.shape[0] != requests:
+                    raise ValueError("KV block_tables must be [requests, width]")
+                size = _workspace_bytes(*sizes, self.block_size, step.block_tables.shape[1], max_query_len or rows)
+            if size == 0:
+                raise ValueError(f"{rows} rows of {requests} requests and {self.num_heads} heads are too many for one step")

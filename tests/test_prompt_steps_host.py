@@ -1,8 +1,9 @@
 """Which sizes prompt attention takes, on the CPU (nothing is launched): every step that ``kv_step`` makes, whatever
-its number of requests."""
+its number of requests; and steps that it refuses leave the cache as it was."""
 import importlib
 
 import pytest
+import torch
 
 attn = importlib.import_module("llm-serve_amd.layers.attention")
 
@@ -78,3 +79,49 @@ def test_counts_stay_below_32_bits():
     assert units([most], 4, 8, 128, 0) > 2 ** 31 > units([most], 4, 8, 256, 0)  # why 32 + 8 heads take 256 rows
     assert units([most], 8, 8, 256, 0) > 2 ** 31 > units([most - 4095] + [1] * 4095, 8, 8, 256, 1)
     assert units([most - 4095] + [1] * 4095, 1, 32, 256, 2) < 2 ** 31
+
+
+@pytest.fixture
+def layer(monkeypatch, pkg):
+    """A layer whose cache must not be written."""
+    def written(*args, **kwargs):
+        raise AssertionError("the cache was written")
+
+    monkeypatch.setattr(attn, "append_kv_int4", written)
+    layer = attn.Attention(32, 128, 0.1, 8, block_size=16)
+    layer.kv_cache = torch.zeros(4, 8, 16 * 136, dtype=torch.uint8)
+    return layer
+
+
+def step(rows, requests, width=2):
+    lists = torch.zeros(1, dtype=torch.int32)
+    tables = torch.zeros(1, width, dtype=torch.int32).expand(requests, width)
+    return attn.KVStep(lists.expand(requests + 1), lists.expand(requests), lists.expand(rows), lists.expand(rows), tables, lists)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+@pytest.mark.parametrize("rows,requests,change", [(400000, 1000, {}), (1 << 27, 1, {}), (8, 0, {}), (8, 2, {"max_query_len": 0}),
+                                                  (8, 2, {"scale": 0.0}), (8, 2, {"scale": float("nan")})])
+def test_a_step_that_attention_refuses_is_not_stored(layer, rows, requests, change, whole):
+    if not whole and rows == 400000:
+        rows, requests = 1 << 26, 4096  # chunks behind cached tokens have another bound
+    change = dict(change)
+    layer.scale = change.pop("scale", layer.scale)
+    qkv = torch.zeros(1, 48 * 128, dtype=torch.bfloat16).expand(rows, 48 * 128)
+    with pytest.raises(ValueError):
+        layer.forward_qkv(qkv, step(rows, requests), None, whole_prompts=whole, **change)
+
+
+@pytest.mark.parametrize("mask", [torch.zeros(8, dtype=torch.int32), torch.zeros(7, dtype=torch.int64)])
+def test_a_step_with_a_wrong_tree_mask_is_not_stored(layer, mask):
+    qkv = torch.zeros(8, 48 * 128, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="tree_mask"):
+        layer.forward_qkv(qkv, step(8, 2), None, tree_mask=mask)
+
+
+@pytest.mark.parametrize("whole", [True, False])
+def test_a_step_that_attention_takes_is_stored(layer, whole):
+    for rows, requests in ((8, 2), (attn.MAX_STEP_TOKENS, 4096) if whole else (16384, 64), (0, 2)):
+        qkv = torch.zeros(1, 48 * 128, dtype=torch.bfloat16).expand(rows, 48 * 128)
+        with pytest.raises(AssertionError, match="written"):
+            layer.forward_qkv(qkv, step(rows, requests), None, whole_prompts=whole)
