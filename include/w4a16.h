@@ -388,7 +388,7 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
  * ------------------------------------------------------------------------- */
 
 /* Per-head RMSNorm and position rotation of q [T, H, D] and k [T, KV, D] (bf16, strides as in
- * w4a16_kv_store, D in {64, 128}) into q_out and k_out (contiguous, overlapping no input).  A row x
+ * w4a16_kv_store, D in {64, 128}) into q_out and k_out (contiguous, overlapping no input), T up to 2^26 - 32.  A row x
  * becomes y = x * r * w with r = 1 / sqrt(mean(x^2) + eps) and the weight w [D] (q_weight, k_weight;
  * null: y = x), and channels i and i + rotary / 2 of y turn by the angle of the row's position:
  *   z[i] = y[i] cos - y[i + rotary / 2] sin,  z[i + rotary / 2] = y[i + rotary / 2] cos + y[i] sin;

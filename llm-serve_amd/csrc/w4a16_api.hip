@@ -1401,7 +1401,8 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
 static int validate_rope(const w4a16::QkRopeArgs& a) {
   if (a.T < 0) return fail(W4A16_ERR_ARG, "T must not be negative (got %d)", a.T);
   if (a.H <= 0 || a.KV <= 0) return fail(W4A16_ERR_ARG, "query heads (%d) and kv heads (%d) must be positive", a.H, a.KV);
-  if (a.T > 1 << 30) return fail(W4A16_ERR_SHAPE, "%d tokens are too many for one call", a.T);
+  // A launch counts its threads in 32 bits: 64 a token, the workgroups (of four tokens) a multiple of 8.
+  if (a.T > (1 << 26) - 32) return fail(W4A16_ERR_SHAPE, "%d tokens are too many for one call", a.T);
   if (a.H > 0xFFFF || a.KV > 0xFFFF) return fail(W4A16_ERR_SHAPE, "%d query heads and %d kv heads are too many", a.H, a.KV);
   if (a.D != 64 && a.D != 128) return fail(W4A16_ERR_SHAPE, "the head size must be 64 or 128 (got %d)", a.D);
   if (a.rotary <= 0 || a.rotary % 16 || a.rotary > a.D)
