@@ -94,12 +94,12 @@ struct PromptArgs {
   uint32_t group_inverse;
   int group_shift;
   bool zero_tail;
-  int tile_rows, cost_shift;  // plan_prompt_attention's
+  int tile_rows, cost_shift, part_workers;  // plan_prompt_attention's
 };
 // Steps of up to this many rows (the most that w4a16_kv_step makes) are planned whatever their number of requests.
 constexpr int kPromptStepRows = 1 << 18;
-// The rows (tokens x heads of a group) of a row tile and the unit that work is counted in, for a call of these
-// sizes (T, R, H, KV); false: its work may pass 32 bits.
+// The rows (tokens x heads of a group) of a row tile, the unit that work is counted in and the workers that may hand
+// over parts of row tiles, for a call of these sizes (T, R, H, KV, D); false: its work may pass 32 bits.
 bool plan_prompt_attention(PromptArgs* a);
 size_t prompt_attention_workspace(const PromptArgs& a);
 // counters: kKvAttentionCounters ints, zero before and after the call's kernel.

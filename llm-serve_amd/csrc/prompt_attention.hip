@@ -620,10 +620,16 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
   if (a.zero_tail) kv_zero_unowned(a, false);
 }
 
+// Workgroups of a form: row tiles of 256 rows have eight waves, others four.
+constexpr int workers(int D, int tile_rows) {
+  return 256 * 4 * (D == 64 ? kWavesPerSimd<64> : kWavesPerSimd<128>) / (tile_rows == 256 ? 8 : 4);
+}
+
 template <int D, int WAVES, int SPLIT>
 hipError_t launch(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {
-  constexpr int kWorkers = 256 * 4 * kWavesPerSimd<D> / WAVES;
-  const KvPartials part = partials_at(static_cast<char*>(workspace), counters, kWorkers, 32 * WAVES / SPLIT, D);
+  constexpr int kWorkers = workers(D, 32 * WAVES / SPLIT);
+  static_assert(kWorkers == 256 * 4 * kWavesPerSimd<D> / WAVES, "as many workgroups as the chip holds");
+  const KvPartials part = partials_at(static_cast<char*>(workspace), counters, a.part_workers, 32 * WAVES / SPLIT, D);
   prompt_attention_kernel<D, WAVES, SPLIT><<<kWorkers, 64 * WAVES, 0, stream>>>(a, part);
   return hipGetLastError();
 }
@@ -637,13 +643,25 @@ hipError_t launch_for(const PromptArgs& a, void* workspace, int* counters, hipSt
   }
 }
 
-// The most that the cost units of a call's row tiles can add up to.  With n rows a tile and rows / n = y, sequences
-// have at most y + R tiles together, tile j of each costs first + step j (tile_costs), and the sum of all j is
-// largest, below (y + 1) y / 2, where one sequence has all rows; x is y rounded down.
-int64_t most_cost(const PromptArgs& a, int n, int shift) {
+// The most row tiles of n rows that a call may have, what the longest of them may cost, and what all may.  With
+// rows / n = y, sequences have at most y + R tiles together, tile j of each costs first + step j (tile_costs), and the
+// sum of all j is largest, below (y + 1) y / 2, where one sequence has all rows; x is y rounded down.
+struct MostWork {
+  int64_t tiles, longest, total;
+};
+MostWork most_work(const PromptArgs& a, int n, int shift) {
   const int64_t group = a.H / a.KV, rows = a.T * group, x = rows / n;
   const int64_t step = ((n / (kKeys / kKeyTileCost) >> shift) + group - 1) / group, first = step + (kSetupCost >> shift);
-  return a.KV * ((x + (a.R < rows ? a.R : rows)) * first + step * ((x + 1) * (x + 2) / 2));
+  const int64_t tiles = x + (a.R < rows ? a.R : rows);
+  return {a.KV * tiles, first + step * x, a.KV * (tiles * first + step * ((x + 1) * (x + 2) / 2))};
+}
+
+// The most workers that a call may have where row tiles are cut, by the kernel's own rule; 0 where none can be.
+int part_workers(const PromptArgs& a, const MostWork& most) {
+  const int grid = workers(a.D, a.tile_rows);
+  if (most.longest <= kWholeCost >> a.cost_shift || (most.longest <= kShortCost >> a.cost_shift && most.tiles <= grid)) return 0;
+  const int64_t n = (most.total - 1) / (kMinShare >> a.cost_shift) + 1;
+  return n < grid ? static_cast<int>(n) : grid;
 }
 
 // While row tiles of 64 find a CU each, the longest of them is what takes time: with its keys split between
@@ -671,16 +689,20 @@ bool plan_prompt_attention(PromptArgs* a) {
   constexpr int64_t kMost = 0x7FFFFFFF;
   static_assert(kKeyTileCost == 16, "a tile of keys in units of cost_shift 4 is one");
   a->tile_rows = tile_rows(*a), a->cost_shift = 0;
-  if (most_cost(*a, a->tile_rows, 0) <= kMost) return true;
-  if (a->T > kPromptStepRows) return false;
-  a->tile_rows = 256;
-  for (; a->cost_shift <= 4; ++a->cost_shift)
-    if (most_cost(*a, 256, a->cost_shift) <= kMost) return true;
-  return false;
+  MostWork most = most_work(*a, a->tile_rows, 0);
+  if (most.total > kMost) {
+    if (a->T > kPromptStepRows) return false;
+    a->tile_rows = 256;
+    while ((most = most_work(*a, 256, a->cost_shift)).total > kMost)
+      if (++a->cost_shift > 4) return false;
+  }
+  a->part_workers = part_workers(*a, most);
+  return true;
 }
 
+// (Never nothing: zero bytes would read as a refusal.)
 size_t prompt_attention_workspace(const PromptArgs& a) {
-  return partials_bytes(kKvPromptWorkers * (a.D == 64 ? kWavesPerSimd<64> : kWavesPerSimd<128>) / 2, kKvPromptRows, a.D);
+  return a.part_workers ? partials_bytes(a.part_workers, a.tile_rows, a.D) : 256;
 }
 
 hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {

@@ -127,3 +127,22 @@ def test_largest_steps_of_many_requests(gpu_lib, heads, kv_heads, requests):
     out = attn.attention_prompt(q, k, v, int32([0] + list(range(long, rows + 1))))
     check_rows(out, q, k, v, 0, (0, 63, 4097, 100000, long - 1), 128 ** -0.5)
     assert torch.equal(out[long:], v[long:].repeat_interleave(heads // kv_heads, 1))
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(8, 2, 128, [1, 3]), (32, 8, 128, [511]), (32, 8, 128, [700]), (32, 8, 128, [2039]),
+                                                        (40, 8, 128, [300, 1, 0, 1111, 7]), (32, 8, 128, [50] * 40), (4, 2, 128, [3000]),
+                                                        (16, 16, 64, [1500, 1, 333]), (2, 1, 64, [2500, 900]), (1, 1, 128, [6000])])
+def test_the_workspace_is_as_large_as_a_call_needs(gpu_lib, heads, kv_heads, dim, lengths):
+    """With exactly the bytes that are asked for: the same bits, the bytes behind them as they were, counters at zero."""
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    q, k, v = (torch.randn(sum(lengths), h, dim, generator=gen, device="cuda").to(torch.bfloat16) for h in (heads, kv_heads, kv_heads))
+    offsets = int32([0] + [sum(lengths[:i + 1]) for i in range(len(lengths))])
+    want = attn.attention_prompt(q, k, v, offsets)
+    size = gpu_lib.prompt_attention_workspace(sum(lengths), len(lengths), heads, kv_heads, dim)
+    space = torch.full((size + (1 << 20),), 0x5A, dtype=torch.uint8, device="cuda")
+    counters = torch.zeros(1024, dtype=torch.int32, device="cuda")
+    for _ in range(3):
+        out = torch.full_like(want, 9.0)
+        gpu_lib.prompt_attention(q, k, v, offsets, out, dim ** -0.5, True, space[:size], counters)
+        assert torch.equal(out, want)
+        assert bool((space[size:] == 0x5A).all()) and not bool(counters.any())

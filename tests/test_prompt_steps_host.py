@@ -125,3 +125,43 @@ def test_a_step_that_attention_takes_is_stored(layer, whole):
         qkv = torch.zeros(1, 48 * 128, dtype=torch.bfloat16).expand(rows, 48 * 128)
         with pytest.raises(AssertionError, match="written"):
             layer.forward_qkv(qkv, step(rows, requests), None, whole_prompts=whole)
+
+
+def form(rows, requests, heads, kv_heads):
+    """The rows of a row tile (of calls that count in sixteenths of a tile of keys)."""
+    if rows * heads <= 256 * 64 and requests * kv_heads <= 256:
+        return 64
+    return 256 if rows * heads >= 200 * 256 and rows // 512 >= requests else 128
+
+
+def workers_with_parts(lengths, group, kv_heads, dim, n):
+    """The workers among whom the kernel deals out these sequences' row tiles, 0 where it cuts none."""
+    grid = 256 * (4 if dim == 64 else 2) * 4 // (8 if n == 256 else 4)
+    tiles = [-(-x * group // n) for x in lengths]
+    step = -(-(n // 4) // group)
+    longest = max((64 + step * m for m in tiles if m), default=0)
+    if longest <= 128 or (longest <= 256 and kv_heads * sum(tiles) <= grid):
+        return 0
+    total = units(lengths, group, kv_heads, n, 0)
+    return min(grid, (total - 1) // max(48, longest // 12) + 1)
+
+
+def test_the_workspace_holds_what_a_call_may_hand_over(dll):
+    """Room for two row tiles (a row's channels and two numbers, in fp32) of each worker that shares one, whatever the
+    requests' lengths; calls that cut none need next to nothing."""
+    import random
+
+    rng = random.Random(4)
+    for _ in range(400):
+        kv_heads, group, dim = rng.choice([1, 2, 8, 16]), rng.choice([1, 4, 5, 8, 40]), rng.choice([64, 128])
+        rows, requests = int(2 ** rng.uniform(0, 16)), int(2 ** rng.uniform(0, 8))
+        size = dll.w4a16_prompt_attention_workspace(rows, requests, kv_heads * group, kv_heads, dim)
+        n = form(rows, requests, kv_heads * group, kv_heads)
+        for lengths in ([rows], [rows // requests] * requests, [max(rows - requests + 1, 0)] + [1] * min(requests - 1, rows - 1)):
+            assert len(lengths) <= requests and sum(lengths) <= rows
+            assert 2 * workers_with_parts(lengths, group, kv_heads, dim, n) * n * (dim + 2) * 4 <= size
+
+
+@pytest.mark.parametrize("sizes", [(1, 1, 32, 8, 128), (120, 1, 32, 8, 128), (511, 1, 32, 8, 128), (16, 16, 32, 8, 128), (300, 1, 16, 16, 64)])
+def test_short_prompts_need_no_workspace_to_speak_of(dll, sizes):
+    assert 0 < dll.w4a16_prompt_attention_workspace(*sizes) <= 4096
