@@ -32,10 +32,11 @@ namespace w4a16 {
 namespace {
 
 constexpr int kKeys = 64;  // keys of a tile
-// The weights' exponents c s - m are formed without rounding c s, and m is a rounded c s: weights are larger by
-// half of m's last place at most, 2^(2^-5) below this border.  Beyond it, in rows of their own, c s is rounded as m is:
-// for scores of 2^31 and more that place is 2^7 and takes the largest weight of a row out of fp32.
-constexpr float kFarReference = 0x1p20f;
+// Whether a row's reference lies beyond the border from which c s is rounded as m is.  The weights' exponents c s - m
+// are formed without rounding c s, and m is a rounded c s: weights are larger by half of m's last place at most, which
+// is 2^-5 below the border, but 2^7 and more from scores of 2^31 on and takes the row's largest weight out of fp32.
+// Looked for in one branch with references that grow: a comparison a tile, 0 to 1.5 % of a call.
+__device__ __forceinline__ bool is_far(float m) { return (fabsf(m) > 0x1p20f) & (m != -INFINITY); }
 // Of a row tile besides its keys: finding it, queries, output take as long as four tiles of keys (with half of
 // that in the shares, nine prompts of up to 2500 rows take 313 us instead of 305).
 constexpr int kSetupCost = 4 * kKeyTileCost;
@@ -470,7 +471,8 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
       top = halves_max(top) * scale;
       // The reference follows the maximum where that leads it by more than 8: weights stay below 2^8.
       const bool grew = top - row_max > 8.0f;
-      if (__any(grew)) {
+      bool far = false;
+      if (__any(grew | is_far(row_max))) {
         const float f = grew ? __builtin_amdgcn_exp2f(row_max - top) : 1.0f;
         row_max = grew ? top : row_max;
         row_sum *= f;
@@ -478,26 +480,28 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
         for (int c = 0; c < kTiles; ++c)
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[c][i] *= f;
-      }
-      const bool my_far = (fabsf(row_max) > kFarReference) & (row_max != -INFINITY), far = __any(my_far);
-      if (__builtin_expect(far, 0)) {  // the exponents themselves, of each row as its own reference asks
-        if (my_far) {
+        far = __any(is_far(row_max));
+        if (__builtin_expect(far, 0)) {  // the exponents themselves, of each row as its own reference asks
+          if (is_far(row_max)) {
 #pragma unroll
-          for (int n = 0; n < kHalves; ++n)
+            for (int n = 0; n < kHalves; ++n)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) sc[n][i] *= scale;
+              for (int i = 0; i < 16; ++i) sc[n][i] *= scale;
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[n][i] -= row_max;
+          } else {
+            const float from = row_max == -INFINITY ? 0.0f : -row_max;
+#pragma unroll
+            for (int n = 0; n < kHalves; ++n)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[n][i] = __builtin_fmaf(sc[n][i], scale, from);
+          }
 #pragma unroll
           for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
-#pragma unroll
-          for (int n = 0; n < kHalves; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[n][i] -= row_max;
-        } else {
-          const float from = row_max == -INFINITY ? 0.0f : -row_max;
-#pragma unroll
-          for (int n = 0; n < kHalves; ++n)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) sc[n][i] = __builtin_fmaf(sc[n][i], scale, from);
         }
 #pragma unroll
         for (int n = 0; n < kHalves; ++n) asm volatile("" : "+v"(sc[n]));
