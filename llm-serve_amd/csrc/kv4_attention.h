@@ -122,8 +122,7 @@ __device__ __forceinline__ void kv_write(const KvAttentionArgs& a, int row, int 
 
 // Whether request r's offsets decrease.  Offsets that never do give requests of at most T rows in
 // all, which bounds every count of work; with others the kernels do none.
-template <class Args>
-__device__ __forceinline__ bool kv_decreases(const Args& a, int r) {
+__device__ __forceinline__ bool kv_decreases(const KvAttentionArgs& a, int r) {
   return const_ints(a.cu_query_lens)[r + 1] < const_ints(a.cu_query_lens)[r];
 }
 

@@ -10,8 +10,9 @@
 // a lane then holds 32 keys' scores of one row, its maximum and sum need one exchange with the other half of
 // the wave, and the weights, rounded to bf16, are in place as the second operand of O^T = V^T P^T.  V is read
 // by rows and turned over by ds_read_b64_tr_b16.  Weights are rounded to bf16 because the matrix cores multiply
-// bf16; their sum is of the fp32 values, so that the rounding errors average out in the quotient
-// (error against 64 bits 1.2 times that of a computation in fp32 with one rounding at the end).
+// bf16; their sum is of the fp32 values.  Errors of different weights average out in the quotient (against 64 bits 1.3
+// times the error of a computation in fp32 with one rounding at the end), those of equal ones do not: such a row may
+// be off by a rounding of bf16 besides the output's own.
 //
 // Keys and values go to LDS by loads that pass no register, a tile ahead (two stages); queries and outputs
 // go through LDS too, so that memory is read and written in whole rows.  A row's channels lie in LDS in an order
@@ -40,8 +41,10 @@ __device__ __forceinline__ bool is_far(float m) { return (fabsf(m) > 0x1p20f) & 
 // Of a row tile besides its keys: finding it, queries, output take as long as four tiles of keys (with half of
 // that in the shares, nine prompts of up to 2500 rows take 313 us instead of 305).
 constexpr int kSetupCost = 4 * kKeyTileCost;
-// A worker's least share, and the parts of the longest row tile at most: joining them costs some 3 us, and more
-// with each.
+// The share that workers are counted by where there is little work, and the number of parts of the longest row tile
+// where there is much: joining parts costs some 3 us, and more with each.  Neither is a bound: the number of workers
+// is rounded up, so that a share may be little more than half of kMinShare, and a tile that begins inside a
+// share has a part more than kMaxParts.
 constexpr int kMinShare = 3 * kKeyTileCost;
 // Workgroups beyond two waves a SIMD work from this share on: below it more joins cost what they gain (3 prompts of up
 // to 1500, 16 + 16 heads of 64, 33 us instead of 30), and a number in between leaves CUs unevenly filled (43).
@@ -123,10 +126,7 @@ __device__ __forceinline__ int swizzle(int row) {
 __device__ __forceinline__ void load_to_lds(const void* base, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset), "s"(base), "s"(to) : "m0", "memory");
 }
-template <int LATER>
-__device__ __forceinline__ void wait_loads() {  // but for the last LATER ones; loads to LDS complete in order
-  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LATER) : "memory");
-}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // A value that is no number would reach rows that do not see its key (0 * NaN in the second product).  Where a
 // tile is masked, each wave looks through its loads' part of the values (`found` in its flag) ...
@@ -396,7 +396,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
     };
 
     bf16x8_t qf[kSteps];
-    wait_loads<0>();
+    wait_loads();
     if (SPLIT > 1) barrier();
     {
       const int lane = lane_again(), c = lane & 31;
@@ -408,7 +408,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
 
     for (int kt = t0; kt < t1; ++kt) {
       const int key0 = kt * kKeys;
-      wait_loads<0>();
+      wait_loads();
       barrier();
       issue_k(kt + 1);
       issue_v(kt + 1);
@@ -620,7 +620,7 @@ __global__ __launch_bounds__(64 * WAVES, kWavesPerSimd<D>) void prompt_attention
     __syncthreads();  // all are done with this tile's LDS
     u += x1 - x0;
   }
-  wait_loads<0>();  // none may land when the workgroup's LDS is another's
+  wait_loads();  // none may land when the workgroup's LDS is another's
   if (a.zero_tail) kv_zero_unowned(a, false);
 }
 
