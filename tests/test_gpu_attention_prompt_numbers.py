@@ -1,4 +1,5 @@
-"""Prompt attention where its arithmetic is at its limits: sums over very long prompts, scores of any size."""
+"""Prompt attention where its arithmetic is at its limits: sums over very long prompts, scores of any size; its
+largest steps, and each of its forms for each size of group."""
 import importlib
 import math
 
@@ -6,6 +7,7 @@ import pytest
 import torch
 
 from oracle import prompt_oracle as ora
+from prompt_helpers import form
 
 pytestmark = pytest.mark.gpu
 
@@ -146,3 +148,19 @@ def test_the_workspace_is_as_large_as_a_call_needs(gpu_lib, heads, kv_heads, dim
         gpu_lib.prompt_attention(q, k, v, offsets, out, dim ** -0.5, True, space[:size], counters)
         assert torch.equal(out, want)
         assert bool((space[size:] == 0x5A).all()) and not bool(counters.any())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 2, 128), (40, 8, 128), (5, 1, 64), (6, 2, 128), (14, 2, 64), (16, 16, 64), (24, 2, 128)])
+@pytest.mark.parametrize("tile,least", [(64, 0), (128, 17000), (256, 52000)])
+def test_packed_lengths_in_each_form(gpu_lib, heads, kv_heads, dim, tile, least):
+    """Groups of 1 to 12 heads in each form, the last prompt as long as the form needs: with groups that do not divide
+    a tile's or a wave's rows, tokens are cut between them."""
+    lengths = [0, 129, 1, 33]
+    if tile != 64:
+        lengths.append(max(-(-least // heads) - sum(lengths), 2600 if tile == 256 else 130))
+    assert form(sum(lengths), len(lengths), heads, kv_heads) == tile
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    q, k, v = torch.randn(sum(lengths), heads + 2 * kv_heads, dim, generator=gen,
+                          device="cuda").to(torch.bfloat16).split((heads, kv_heads, kv_heads), 1)
+    offsets = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
+    ora.check_prompt(attn.attention_prompt(q, k, v, int32(offsets)), *ora.prompt(q, k, v, offsets), max(lengths))

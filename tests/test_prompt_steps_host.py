@@ -5,6 +5,8 @@ import importlib
 import pytest
 import torch
 
+from prompt_helpers import form
+
 attn = importlib.import_module("llm-serve_amd.layers.attention")
 
 
@@ -125,13 +127,6 @@ def test_a_step_that_attention_takes_is_stored(layer, whole):
         qkv = torch.zeros(1, 48 * 128, dtype=torch.bfloat16).expand(rows, 48 * 128)
         with pytest.raises(AssertionError, match="written"):
             layer.forward_qkv(qkv, step(rows, requests), None, whole_prompts=whole)
-
-
-def form(rows, requests, heads, kv_heads):
-    """The rows of a row tile (of calls that count in sixteenths of a tile of keys)."""
-    if rows * heads <= 256 * 64 and requests * kv_heads <= 256:
-        return 64
-    return 256 if rows * heads >= 200 * 256 and rows // 512 >= requests else 128
 
 
 def workers_with_parts(lengths, group, kv_heads, dim, n):
