@@ -395,7 +395,8 @@ int w4a16_kv_attention(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h
  * channels from rotary on are y.  table [table_rows, rotary] (fp32) holds a position's rotary / 2
  * cosines, then its sines; rotary is a multiple of 16 up to D.  A row whose position [T] lies outside
  * the table becomes NaN.  The sum of squares is fp64, r the nearest fp32, every other step one fp32
- * operation in the order written, and z is rounded to bf16 once.  Replaces q_norm, k_norm and
+ * operation in the order written, and z is rounded to bf16 once (a row whose mean square passes fp32's
+ * range, of sizes from 2^64 on, becomes zero).  Replaces q_norm, k_norm and
  * rotary_emb of the reference's attention (qwen3.py:87-94, rotary_embedding.py:37-48), which round
  * after each of their steps. */
 int w4a16_qk_norm_rope(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t* k,
@@ -424,7 +425,11 @@ size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D);
  * contiguous) = softmax(scale * q k^T) v with fp32 scores, statistics and sums; the weights, up to 2^8
  * of the row's largest, are rounded to bf16 for the second product (so that values beyond 2^119
  * divided by the row's number of keys may overflow in the sum).  NaN and infinities in keys and
- * values that a row does not see have no effect on it.  Rows of no sequence,
+ * values that a row does not see have no effect on it; an infinite value that it sees gives infinity in
+ * its channel, or NaN where its weight underflows.  Scores, also times scale log2(e), are fp32: a row
+ * all of whose scores are minus infinity or below that range is zero, as in w4a16_kv_attention, and one
+ * that has a score above it is NaN.  T up to 2^18 with any R, H up to 128 and H / KV up to 16; other
+ * sizes while their work counts in 32 bits (W4A16_ERR_SHAPE otherwise).  Rows of no sequence,
  * offsets that decrease, zero_tail, workspace and counters are as in w4a16_kv_attention.  out may be q
  * where that is contiguous, and overlaps no other operand.  Replaces the reference's attention of
  * prompts where nothing is cached (attention.py:118-125). */

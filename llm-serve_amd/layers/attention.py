@@ -423,7 +423,9 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_query
     A prompt's rows give what ``attention_int4`` gives over their cached copies, but for the 4 bits.
     ``scale`` defaults to 1 / sqrt(head_dim).  ``max_query_len``, the longest prompt if the caller knows it
     (as ``attention_int4`` takes it), must be positive and changes nothing here.  Sums are fp32 with weights
-    of up to 2^8: values beyond 2^119 divided by a row's number of keys may overflow in them.  Offsets that
+    of up to 2^8: values beyond 2^119 divided by a row's number of keys may overflow in them.  An infinite value
+    gives infinity in the rows that see it, or NaN where its weight underflows; a row all of whose scores are
+    minus infinity, or below fp32's range, is zero, one that has a score above that range NaN.  Offsets that
     decrease name no rows at all.  Without ``out`` (contiguous, of q's shape), rows of no request are zero; in
     ``out`` they are left as they were.
     ``out`` may be q itself, and overlaps no other operand."""

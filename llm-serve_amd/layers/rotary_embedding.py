@@ -131,7 +131,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, tabl
     ``table`` [max positions, rotary_dim] is ``rotary_table``'s; channel i turns with channel
     i + rotary_dim / 2, and channels from rotary_dim on keep their place.  A row whose position the table
     does not have becomes NaN.  All steps are fp32, each rounded by itself (the sum of squares is fp64),
-    and the result is rounded to bf16 once, where the reference rounds after each norm's step too."""
+    and the result is rounded to bf16 once, where the reference rounds after each norm's step too.  A row with
+    a weight whose mean square passes fp32's range (sizes from 2^64 on) becomes zero."""
     if not rope_ready(q, k, positions, table, q_weight, k_weight, eps):
         q, k, positions, table, q_weight, k_weight = rope_operands(q, k, positions, table, q_weight, k_weight, eps)
     shape, kshape, index = q.shape, k.shape, q.get_device()

@@ -164,3 +164,34 @@ def test_packed_lengths_in_each_form(gpu_lib, heads, kv_heads, dim, tile, least)
                           device="cuda").to(torch.bfloat16).split((heads, kv_heads, kv_heads), 1)
     offsets = [sum(lengths[:i]) for i in range(len(lengths) + 1)]
     ora.check_prompt(attn.attention_prompt(q, k, v, int32(offsets)), *ora.prompt(q, k, v, offsets), max(lengths))
+
+
+@pytest.mark.parametrize("heads,lengths", [(4, [90]), (16, [700, 400]), (32, [2039])])
+def test_scores_beyond_fp32(gpu_lib, heads, lengths):
+    """Finite queries and keys whose product passes fp32's range: above it a row is NaN, and where all of a row's
+    scores lie below it the row is zero; other rows keep their bits."""
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    q, k, v = (torch.randn(sum(lengths), h, 128, generator=gen, device="cuda").abs().add(0.5).to(torch.bfloat16) for h in (heads, 4, 4))
+    offsets = int32([0] + [sum(lengths[:i + 1]) for i in range(len(lengths))])
+    k = k * 2.0 ** 60
+    q = q * 2.0 ** -60
+    want = attn.attention_prompt(q, k, v, offsets)
+    row = torch.rand(q.shape[:2], generator=gen, device="cuda")
+    above, below = row < 0.05, row > 0.95
+    large = q * 2.0 ** 65 * 2.0 ** 65  # 2^130 itself is no fp32 number
+    q = torch.where(above[..., None], large, torch.where(below[..., None], -large, q))
+    assert bool(torch.isfinite(q).all()) and bool(torch.isfinite(k).all())
+    out = attn.attention_prompt(q, k, v, offsets)
+    assert bool(out[above].isnan().all()) and not bool(out[below].any())
+    assert torch.equal(out[~(above | below)], want[~(above | below)])
+
+
+def test_infinite_values_are_not_finite_anywhere(gpu_lib):
+    """An infinite value whose weight underflows leaves infinity or NaN in its channel, and nothing in others."""
+    q, k, v = (torch.zeros(500, 1, 64, dtype=torch.bfloat16, device="cuda") for _ in range(3))
+    q[:, 0, 0], k[:, 0, 0] = 100, 100
+    k[100, 0, 0] = k[420, 0, 0] = -100
+    v[:, 0, 1], v[100, 0, 0], v[420, 0, 0] = 1, float("inf"), float("inf")
+    out = attn.attention_prompt(q, k, v, int32([0, 500]), scale=1.0)
+    assert not bool(out[:100, 0, 0].any()) and not bool(torch.isfinite(out[100:, 0, 0]).any())
+    assert bool((out[:, 0, 1] == 1).all()) and not bool(out[:, 0, 2:].any())
