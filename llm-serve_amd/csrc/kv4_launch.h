@@ -44,7 +44,8 @@ struct KvRowsArgs {
 hipError_t launch_kv_store(const KvRowsArgs& a, hipStream_t stream);
 hipError_t launch_kv_load(const KvRowsArgs& a, hipStream_t stream);
 
-// Up to this many tokens a wave of the norm-and-rotation kernel takes one group of heads (qk_rope.hip).
+// Up to this many tokens a wave of the norm-and-rotation kernel takes one group of heads, whatever the heads
+// (qk_rope.hip has both sides measured).
 constexpr int kQkRopeFewTokens = 2048;
 
 struct QkRopeArgs {

@@ -11,9 +11,9 @@
 // of the formulas' plain operations gives the same bits.
 //
 // Bytes bound it: each row is read and written once, the table's row of a token is read once for all of
-// the token's heads that a wave takes.  16384 tokens of 32 + 8 heads of 128 channels move 335 MB in 70 us
-// (4.8 TB/s, where a large copy reaches 5.2), with the store into the cache behind it 422 MB in 76 us; few
-// tokens take the 3 us of a launch whose loads wait for each other twice (position, then table).
+// the token's heads that a wave takes.  16384 tokens of 32 + 8 heads of 128 channels move 335 MB in 68 us
+// (4.9 TB/s, where a large copy reaches 5.2), with the store into the cache behind it, keys written too, 387 MB in
+// 80 us; few tokens take the 3 us of a launch whose loads wait for each other twice (position, then table).
 #include "kv4_launch.h"
 #include "kv4_quantize.h"
 
@@ -87,12 +87,16 @@ __device__ __forceinline__ void turn_row(uint4 (&x)[2], bool norm, const uint4 (
 // with 16 channels each, so that a rotating pair lies in one lane, and HEADS groups of 64 / (D / 16)
 // rows at a time, all loaded before the first is used.
 //
-// While there are few tokens, each group of rows has a wave of its own (HEADS 1, a grid of groups): 3.0 us
-// where a wave that takes all of a token's rows, three groups at a time, needs 5.3 (8 tokens of 32 + 8
-// heads of 128 channels), 7.2 against 8.1 for 1024 tokens, 10.6 against 11.1 for 2039.  With more, the waves
-// outnumber what the chip holds, and reading weights and table once for all of a token's rows wins: 17.9
-// against 21.3 for 4096, 70 against 82 for 16384; 32.1 against 36.1 in 14 + 2 heads of 64 with the store.  One
-// group at a time instead of three takes 3 % longer there with the store, four take 4 % longer.
+// While there are few tokens, waves that take all of a token's rows, three groups at a time, are too few to hide
+// what they wait for (2048 of them are two a SIMD), and each group of rows has a wave of its own (HEADS 1, a
+// grid of groups): 3.0 us instead of 5.3 for 8 tokens of 32 + 8 heads of 128 channels, 6.0 instead of 6.8 for
+// 1024, 9.8 instead of 10.2 for 2048.  With more tokens, reading weights and table once for all of a token's
+// rows wins: 15.4 us instead of 16.4 for 4096, 66 instead of 81 for 16384.  So the border is a number of tokens,
+// whatever the heads.  Of 256 to 16384 tokens, with and without the store, one form is ahead up to 2048 and the
+// other from 4096 on, but for a few sizes in which they are within 6 %, in 64 + 8 and 8 + 2 heads of 128 (2048:
+// 15.5 and 15.9, 4.8 and 4.8; 16384: 152 and 127, 23 and 19) and in 16 + 16 and 14 + 2 of 64 (2048 with the store: 6.6
+// and 6.9, 6.3 and 7.0; 16384: 37 and 32, 30 and 27); at 3000 they are within 6 % of each other.  One group at a
+// time instead of three takes 3 % longer there with the store, four take 4 % longer.
 template <int D, int HEADS>
 __global__ __launch_bounds__(256) void qk_rope_kernel(QkRopeArgs a) {
   constexpr int kLanes = D / 16, kRows = 64 / kLanes;
