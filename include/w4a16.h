@@ -415,7 +415,8 @@ int w4a16_kv_append(const uint16_t* q, int64_t q_stride_t, int64_t q_stride_h, c
                     const uint16_t* k_weight, float eps, uint16_t* q_out, uint16_t* k_out, int T, int H,
                     int KV, int D, int num_blocks, int block_size, void* stream);
 
-/* Bytes of workspace w4a16_prompt_attention needs (as w4a16_kv_attention_workspace). */
+/* Bytes of workspace w4a16_prompt_attention needs (as w4a16_kv_attention_workspace); fewer rows and
+ * requests need no more. */
 size_t w4a16_prompt_attention_workspace(int T, int R, int H, int KV, int D);
 
 /* Causal attention of whole prompts over their own keys and values: q [T, H, D], k and v [T, KV, D]

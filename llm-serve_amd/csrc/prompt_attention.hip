@@ -27,6 +27,8 @@
 // wave priorities, or by a next row tile's first loads beside the present one's last tile (0 to 4 % slower).
 // Short prompts are bound by a chain of latencies: 1 us to find the part, 2 for queries and first tile, 0.7 to
 // 1.2 a tile, 1.2 to write.
+#include <algorithm>
+
 #include "attention_rows.h"
 
 namespace w4a16 {
@@ -677,10 +679,13 @@ int part_workers(const PromptArgs& a, const MostWork& most) {
 // rows 2118 us instead of 2348, 2039 rows 49 instead of 52).  Four waves, two workgroups a CU, waste less on
 // short row tiles and have more of them (24 prompts of up to 120 rows 13 us instead of 23, 128 of up to 100 43
 // instead of 48, 32 of up to 200 in 16 heads of 64 19 instead of 22); about 500 rows a request are the border.
+//
+// (T counts rows of no request too and R empty places, so that a request's mean length may be larger than T / R.)
+constexpr int kSplitRows = 256 * 64, kSplitTiles = 256, kLongRows = 200 * 256;
 int tile_rows(const PromptArgs& a) {
   const int64_t rows = static_cast<int64_t>(a.T) * a.H;
-  if (rows <= 256 * 64 && static_cast<int64_t>(a.R) * a.KV <= 256) return 64;
-  return rows >= 200 * 256 && a.T / 512 >= a.R ? 256 : 128;
+  if (rows <= kSplitRows && static_cast<int64_t>(a.R) * a.KV <= kSplitTiles) return 64;
+  return rows >= kLongRows && a.T / 512 >= a.R ? 256 : 128;
 }
 
 }  // namespace
@@ -704,9 +709,20 @@ bool plan_prompt_attention(PromptArgs* a) {
   return true;
 }
 
+// The most that a call of these sizes or of fewer rows or requests needs, in any form that one of them takes.
 // (Never nothing: zero bytes would read as a refusal.)
 size_t prompt_attention_workspace(const PromptArgs& a) {
-  return a.part_workers ? partials_bytes(a.part_workers, a.tile_rows, a.D) : 256;
+  size_t most = 256;
+  const auto form = [&](int n, int T, int R) {
+    PromptArgs b = a;
+    b.T = T, b.R = R, b.tile_rows = n, b.cost_shift = 0;
+    if (const int workers = part_workers(b, most_work(b, n, 0))) most = std::max(most, partials_bytes(workers, n, b.D));
+  };
+  const int64_t rows = static_cast<int64_t>(a.T) * a.H, tiles = static_cast<int64_t>(a.R) * a.KV;
+  form(64, std::min(a.T, kSplitRows / a.H), std::min(a.R, kSplitTiles / a.KV));
+  if (rows > kSplitRows || tiles > kSplitTiles) form(128, a.T, a.R);
+  if (rows >= kLongRows) form(256, a.T, a.R);
+  return most;
 }
 
 hipError_t launch_prompt_attention(const PromptArgs& a, void* workspace, int* counters, hipStream_t stream) {

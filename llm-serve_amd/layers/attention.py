@@ -567,8 +567,8 @@ class Attention(nn.Module):
             _check_max_query_len(max_query_len)
         if tree_mask is not None:
             _check_tree_mask(tree_mask, rows, self.kv_cache.get_device())
-        requests = step.cu_query_lens.shape[0] - 1
-        if step.cu_query_lens.ndim != 1 or requests < 1:
+        requests = step.cu_query_lens.shape[0] - 1 if step.cu_query_lens.ndim == 1 else 0
+        if requests < 1:
             raise ValueError("KV cu_query_lens must be [requests + 1], of at least one request")
         if rows > 0:
             sizes = (rows, requests, self.num_heads, self.num_kv_heads, self.head_dim)

@@ -160,3 +160,18 @@ def test_the_workspace_holds_what_a_call_may_hand_over(dll):
 @pytest.mark.parametrize("sizes", [(1, 1, 32, 8, 128), (120, 1, 32, 8, 128), (511, 1, 32, 8, 128), (16, 16, 32, 8, 128), (300, 1, 16, 16, 64)])
 def test_short_prompts_need_no_workspace_to_speak_of(dll, sizes):
     assert 0 < dll.w4a16_prompt_attention_workspace(*sizes) <= 4096
+
+
+def test_a_workspace_for_the_largest_step_serves_smaller_ones(dll):
+    import random
+
+    rng = random.Random(5)
+    for _ in range(3000):
+        kv_heads, group, dim = rng.choice([1, 2, 8, 16]), rng.choice([1, 4, 5, 8, 40]), rng.choice([64, 128])
+        rows, requests = int(2 ** rng.uniform(0, 17)), int(2 ** rng.uniform(0, 10))
+        most = dll.w4a16_prompt_attention_workspace(rows, requests, kv_heads * group, kv_heads, dim)
+        if most == 0:  # refused
+            continue
+        for fewer in ((rng.randint(1, rows), rng.randint(1, requests)), (max(rows - 1, 1), requests), (rows, max(requests - 1, 1)),
+                      (rows // 2 + 1, requests), (rows, requests // 2 + 1)):
+            assert dll.w4a16_prompt_attention_workspace(*fewer, kv_heads * group, kv_heads, dim) <= most, (rows, requests, fewer)
