@@ -10,23 +10,26 @@
 // a lane then holds 32 keys' scores of one row, its maximum and sum need one exchange with the other half of
 // the wave, and the weights, rounded to bf16, are in place as the second operand of O^T = V^T P^T.  V is read
 // by rows and turned over by ds_read_b64_tr_b16.  Weights are rounded to bf16 because the matrix cores multiply
-// bf16; their sum is of the fp32 values.  Errors of different weights average out in the quotient (against 64 bits 1.3
-// times the error of a computation in fp32 with one rounding at the end), those of equal ones do not: such a row may
-// be off by a rounding of bf16 besides the output's own.
+// bf16; their sum is of the fp32 values.  Errors of different weights average out in the quotient (0.0021 of the output
+// against 64 bits, where a computation in fp32 with one rounding at the end has 0.0016), those of equal ones do not: such a
+// row may be off by a rounding of bf16 besides the output's own.  Weights in two bf16 terms, with a second product
+// each, give 0.0016 and cost 10 % of short prompts' time (24 of up to 120 rows 12.7 us instead of 11.6) and a
+// third of long ones' (2039 rows 63 instead of 51, 16384 rows 2935 instead of 2189): not taken.
 //
 // Keys and values go to LDS by loads that pass no register, a tile ahead (two stages); queries and outputs
 // go through LDS too, so that memory is read and written in whole rows.  A row's channels lie in LDS in an order
 // of their own (swizzle), in which no read has a bank conflict.
 //
-// One prompt of 16384 rows, 32 + 8 heads of 128 channels (2.2 TFLOP): 2.1 to 2.2 ms, 1000 to 1050 TFLOP/s, 85 %
-// of what large library products of the same data reach (1230 to 1250).  What bounds it there is power: the
-// core clock is 1.9 to 2.0 GHz in the loop, and 2.4 with zeros in place of the data (1150 TFLOP/s).  A wave
-// needs 1024 cycles of matrix instructions for a tile and takes 2000 of a SIMD; loops that overlap one tile's
-// products with another's softmax within a wave need a sixth fewer cycles, at a lower clock: 3 % less time, which
-// they lose again at both ends of a row tile in prompts of a few thousand rows.  Nor is anything gained by waves half a tile apart, by
-// wave priorities, or by a next row tile's first loads beside the present one's last tile (0 to 4 % slower).
-// Short prompts are bound by a chain of latencies: 1 us to find the part, 2 for queries and first tile, 0.7 to
-// 1.2 a tile, 1.2 to write.
+// One prompt of 16384 rows, 32 + 8 heads of 128 channels (2.2 TFLOP): 2.1 to 2.25 ms, 980 to 1040 TFLOP/s.  On one box
+// and in turn with it, library products of 8192 x 8192 x 8192 reach 1395 TFLOP/s and this 973, 70 % of them (of five
+// boxes the library's range is 1227 to 1414).  What bounds it there is power: the core clock is 1.9 to 2.0 GHz in the
+// loop, and 2.4 with zeros in place of the data (1150 TFLOP/s).  A wave needs 1024 cycles of matrix instructions for a
+// tile and takes 2000 of a SIMD; loops that overlap one tile's products with another's softmax within a wave need a
+// sixth fewer cycles, at a lower clock: 3 % less time, which they lose again at both ends of a row tile in prompts of
+// a few thousand rows.  Nor is anything gained by waves half a tile apart, by wave priorities, or by a next row tile's
+// first loads beside the present one's last tile (0 to 4 % slower).
+// Short prompts are bound by a chain of latencies: 1 us to find the part, 2 for queries and first tile, 0.7 to 1.2 a
+// tile, 1.2 to write.
 #include <algorithm>
 
 #include "attention_rows.h"
