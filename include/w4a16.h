@@ -365,7 +365,8 @@ size_t w4a16_kv_attention_workspace(int T, int R, int H, int KV, int D, int bloc
  * taken out of each query row and of every 16 keys: a key or value whose scale is 2^-24 of the
  * largest among its 16, seen by the row or not, loses bits.  Sums are fp32 and have terms of up to
  * 143 |q| and 143 scales of values: a row with queries or values of 2^110 and more may be infinite
- * or NaN.  tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of
+ * or NaN.  A row with a score beyond 2^26 (2^30 for requests of up to 64 rows a kv head) may be NaN
+ * or zero: the exponents' own rounding leaves the weights' range there.  tree_mask (may be null) [T]: row t then sees its request's cached tokens and, instead of
  * the earlier new ones, those new ones j < 64 whose bit j is set.
  * A row that sees no key gives zeros; keys on a page id outside the cache are not seen; NaN and
  * infinities in keys that a row does not see have no effect on it.  Rows of no request (before
