@@ -175,3 +175,13 @@ def test_a_workspace_for_the_largest_step_serves_smaller_ones(dll):
         for fewer in ((rng.randint(1, rows), rng.randint(1, requests)), (max(rows - 1, 1), requests), (rows, max(requests - 1, 1)),
                       (rows // 2 + 1, requests), (rows, requests // 2 + 1)):
             assert dll.w4a16_prompt_attention_workspace(*fewer, kv_heads * group, kv_heads, dim) <= most, (rows, requests, fewer)
+
+
+@pytest.mark.parametrize("group", range(1, 17))
+def test_every_step_of_up_to_128_heads_is_taken(dll, group):
+    """The documented range: 2^18 rows, any number of requests, up to 128 heads in groups of up to 16."""
+    for kv_heads in {1, 2, 3, 8, 128 // group}:
+        if kv_heads * group <= 128:
+            for rows in (1, 1000, 16385, 60000, 131073, 200001, attn.MAX_STEP_TOKENS):
+                for requests in (1, 7, 512, 513, 4096, 1 << 18, 1 << 30):
+                    assert dll.w4a16_prompt_attention_workspace(rows, requests, kv_heads * group, kv_heads, 128) > 0
