@@ -47,7 +47,7 @@ def test_sums_of_equal_weights_over_a_long_prompt(gpu_lib):
 
 
 @pytest.mark.parametrize("heads,kv_heads,dim,lengths", [(4, 2, 128, [300]), (4, 4, 64, [100, 270]), (16, 4, 64, [1500]), (32, 8, 128, [700, 600]),
-                                                        (32, 8, 128, [2039])])
+                                                        (32, 8, 128, [2039]), (16, 4, 64, [4000])])
 @pytest.mark.parametrize("size", [2.0 ** 13, 2.0 ** 17, 2.0 ** 20, 2.0 ** 45])
 def test_rows_of_very_large_scores(gpu_lib, heads, kv_heads, dim, lengths, size):
     """Scores of 2^23 to 2^95, where a last place of fp32 is worth far more than 1: a row is the value of its
